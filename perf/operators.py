@@ -335,10 +335,10 @@ def _own(s, kind):
     if kind == "select":
         return s["pool"].select_blocks(s["q"], s["bounds"], s["tables"], s["ctx"], case["top"],
                                        case["first"], case["last"], cu_q_lens=s["cu"],
-                                       max_context_len=s["ctx_max"])
+                                       max_q_len=s["q_max"], max_context_len=s["ctx_max"])
     if kind == "attend":
         return s["pool"].sparse_attention(s["q"], s["blocks"], s["tables"], s["ctx"],
-                                          cu_q_lens=s["cu"])
+                                          cu_q_lens=s["cu"], max_q_len=s["q_max"])
     tokens, accepted = _package().verify_drafts(s["target"], s["drafts"], s["cu"], s["u"],
                                                 s["u_last"], draft_logits=s["draft"],
                                                 temperatures=s["temps"])
