@@ -36,6 +36,10 @@ SOURCES = [
     "pkv_mixed.hip",
     "pkv_rope.hip",
     "pkv_sample.hip",
+    "pkv_step.hip",
+    "pkv_select.hip",
+    "pkv_sparse.hip",
+    "pkv_verify.hip",
 ]
 
 # Packed-FP32 instructions stay off (the compiler would otherwise form

@@ -11,6 +11,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <new>
 #include <string>
 #include <vector>
@@ -1139,6 +1140,329 @@ int pkv_sample_expf(const float* in, float* out, long long n, void* stream) {
     return fail(nullptr, PKV_ERR_INVALID, "sample_expf: n %lld, NULL pointer", n);
   hipError_t e = pkv::launch_expf_glibc(in, out, n, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(nullptr, e, "sample_expf launch");
+  return PKV_OK;
+}
+
+namespace {
+bool misaligned4(std::initializer_list<const void*> ptrs) {
+  for (const void* x : ptrs)
+    if (reinterpret_cast<uintptr_t>(x) & 3u) return true;
+  return false;
+}
+
+struct Range {
+  const void* at;
+  size_t bytes;
+};
+bool overlap(const Range& a, const Range& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+}  // namespace
+
+int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
+                    const int32_t* new_lens, int n_seqs, const int32_t* block_tables,
+                    const int32_t* n_blocks, int max_blocks_per_seq, const int32_t* free_list,
+                    int free_len, const int32_t* free_count, int max_tokens,
+                    int32_t* block_tables_out, int32_t* n_blocks_out, int32_t* free_count_out,
+                    int32_t* context_lens, int32_t* cu_q_lens, int32_t* positions,
+                    int32_t* slot_mapping, int32_t* status, void* stream) {
+  g_thread_error.clear();
+  if (!is_pow2(block_size) || block_size > 256)
+    return fail(nullptr, PKV_ERR_UNSUPPORTED,
+                "step_tables: block_size %d: must be a power of two in [1, 256]", block_size);
+  if (num_blocks <= 0 || n_seqs < 0 || max_blocks_per_seq <= 0 || free_len < 0 || max_tokens < 0)
+    return fail(nullptr, PKV_ERR_INVALID,
+                "step_tables: num_blocks %d, n_seqs %d, max_blocks_per_seq %d, free_len %d, "
+                "max_tokens %d", num_blocks, n_seqs, max_blocks_per_seq, free_len, max_tokens);
+  if ((long long)num_blocks * block_size > INT32_MAX ||
+      (long long)max_blocks_per_seq * block_size > INT32_MAX)
+    return fail(nullptr, PKV_ERR_INVALID,
+                "step_tables: %d blocks, %d per sequence, of %d tokens: at most 2^31 - 1 slots",
+                num_blocks, max_blocks_per_seq, block_size);
+  if (!free_count || !free_count_out || !cu_q_lens || !status || (free_len && !free_list) ||
+      (max_tokens && (!positions || !slot_mapping)) ||
+      (n_seqs && (!seq_lens || !new_lens || !n_blocks || !block_tables || !block_tables_out ||
+                  !n_blocks_out || !context_lens)))
+    return fail(nullptr, PKV_ERR_INVALID, "step_tables: NULL argument");
+  if (misaligned4({seq_lens, new_lens, block_tables, n_blocks, free_list, free_count,
+                   block_tables_out, n_blocks_out, free_count_out, context_lens, cu_q_lens,
+                   positions, slot_mapping, status}))
+    return fail(nullptr, PKV_ERR_INVALID, "step_tables: arrays must be 4-byte aligned");
+  const size_t n = 4 * (size_t)n_seqs, tab = n * (size_t)max_blocks_per_seq;
+  const size_t tok = 4 * (size_t)max_tokens;
+  const Range in[] = {{seq_lens, n}, {new_lens, n}, {n_blocks, n}, {block_tables, tab},
+                      {free_list, 4 * (size_t)free_len}, {free_count, 4}};
+  const Range out[] = {{block_tables_out, tab}, {n_blocks_out, n}, {free_count_out, 4},
+                       {context_lens, n}, {cu_q_lens, n + 4}, {positions, tok},
+                       {slot_mapping, tok}, {status, 4}};
+  for (const Range& o : out) {
+    for (const Range& i : in)
+      if (overlap(o, i) && !(o.at == block_tables_out && i.at == o.at && i.at == block_tables))
+        return fail(nullptr, PKV_ERR_INVALID, "step_tables: an output overlaps an input");
+    for (const Range& x : out)
+      if (&x != &o && overlap(o, x))
+        return fail(nullptr, PKV_ERR_INVALID, "step_tables: outputs overlap");
+  }
+  pkv::StepArgs a{};
+  a.seq_lens = seq_lens;
+  a.new_lens = new_lens;
+  a.n_blocks = n_blocks;
+  a.tables_in = block_tables;
+  a.free_list = free_list;
+  a.free_count = free_count;
+  a.free_len = free_len;
+  a.n_seqs = n_seqs;
+  a.width = max_blocks_per_seq;
+  a.max_tokens = max_tokens;
+  while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
+  a.num_blocks = num_blocks;
+  a.tables_out = block_tables_out;
+  a.n_blocks_out = n_blocks_out;
+  a.free_count_out = free_count_out;
+  a.context_lens = context_lens;
+  a.cu_q_lens = cu_q_lens;
+  a.positions = positions;
+  a.slots = slot_mapping;
+  a.status = status;
+  hipError_t e = pkv::launch_step_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(nullptr, e, "step_tables launch");
+  return PKV_OK;
+}
+
+size_t pkv_key_bounds_bytes(const pkv_pool* p) {
+  return p ? (size_t)p->num_blocks * p->n_kv_head * 2 * p->row_bytes : 0;
+}
+
+int pkv_key_bounds(pkv_pool* p, int layer, void* bounds, const int32_t* block_tables,
+                   int max_blocks_per_seq, const int32_t* first_positions,
+                   const int32_t* context_lens, int n_seqs, int max_new_len, void* stream) {
+  CHECK_POOL(p);
+  if (int rc = check_layer(p, layer)) return rc;
+  if (n_seqs < 0) return fail(p, PKV_ERR_INVALID, "n_seqs %d < 0", n_seqs);
+  if (n_seqs == 0) return PKV_OK;
+  if (!bounds || !block_tables || !context_lens)
+    return fail(p, PKV_ERR_INVALID, "bounds, block_tables and context_lens must be non-NULL");
+  if (!aligned16(bounds)) return fail(p, PKV_ERR_INVALID, "bounds must be 16-byte aligned");
+  if (max_blocks_per_seq <= 0 || max_new_len <= 0 || max_new_len > pkv::kMaxLen)
+    return fail(p, PKV_ERR_INVALID,
+                "max_blocks_per_seq (%d) must be > 0 and max_new_len (%d) in 1 .. 2^30",
+                max_blocks_per_seq, max_new_len);
+  if (!pkv::bounds_fits(p, n_seqs, max_new_len, max_blocks_per_seq))
+    return fail(p, PKV_ERR_UNSUPPORTED, "key_bounds: %d sequences of up to %d new tokens: too many "
+                "work-items for one launch", n_seqs, max_new_len);
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_bounds(p, layer, bounds, block_tables, max_blocks_per_seq,
+                                    first_positions, context_lens, n_seqs, max_new_len,
+                                    static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "key_bounds launch");
+  return PKV_OK;
+}
+
+namespace {
+// What pkv_select_blocks and pkv_sparse_attention have in common.
+int rows_validate(pkv_pool* p, const void* q, const int32_t* blocks, int top_blocks,
+                  const int32_t* cu_q_lens, const int32_t* context_lens,
+                  const int32_t* block_tables, int max_blocks_per_seq, int n_seqs, int total_q,
+                  int max_q_len, int n_head) {
+  if (!q || !blocks || !context_lens || !block_tables)
+    return fail(p, PKV_ERR_INVALID, "q, blocks, context_lens and block_tables must be non-NULL");
+  if (!aligned16(q)) return fail(p, PKV_ERR_INVALID, "q must be 16-byte aligned");
+  if (!cu_q_lens && (total_q != n_seqs || max_q_len != 1))
+    return fail(p, PKV_ERR_INVALID,
+                "without cu_q_lens there is one row per sequence: total_q %d, n_seqs %d, "
+                "max_q_len %d", total_q, n_seqs, max_q_len);
+  if (max_blocks_per_seq <= 0 || top_blocks <= 0 || max_q_len <= 0 || max_q_len > pkv::kMaxLen)
+    return fail(p, PKV_ERR_INVALID,
+                "max_blocks_per_seq (%d) and top_blocks (%d) must be > 0 and max_q_len (%d) in "
+                "1 .. 2^30", max_blocks_per_seq, top_blocks, max_q_len);
+  if (top_blocks > pkv::kMaxLen / p->block_size)
+    return fail(p, PKV_ERR_INVALID, "top_blocks %d of %d tokens: at most 2^30 tokens", top_blocks,
+                p->block_size);
+  if (n_head <= 0 || n_head % p->n_kv_head != 0)
+    return fail(p, PKV_ERR_INVALID, "n_head %d is not a multiple of n_kv_head %d", n_head,
+                p->n_kv_head);
+  return PKV_OK;
+}
+
+int workspace_check(pkv_pool* p, const void* ws, size_t have, size_t need, const char* what) {
+  if (need && (!ws || have < need))
+    return fail(p, PKV_ERR_INVALID, "%s: the workspace needs %zu bytes, got %zu", what, need,
+                ws ? have : (size_t)0);
+  if (!aligned16(ws)) return fail(p, PKV_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+  return PKV_OK;
+}
+
+pkv::SelectArgs select_shape(int n_seqs, int total_q, int max_q_len, int max_context_len,
+                             int max_blocks_per_seq, int n_head) {
+  pkv::SelectArgs a{};
+  a.n_seqs = n_seqs;
+  a.total_q = total_q;
+  a.max_q_len = max_q_len;
+  a.max_context_len = max_context_len;
+  a.max_blocks_per_seq = max_blocks_per_seq;
+  a.n_head = n_head;
+  return a;
+}
+}  // namespace
+
+size_t pkv_select_workspace_bytes(const pkv_pool* p, int n_seqs, int total_q, int max_q_len,
+                                  int max_context_len, int max_blocks_per_seq, int n_head) {
+  if (!p || n_seqs <= 0 || total_q <= 0 || max_q_len <= 0 || max_q_len > pkv::kMaxLen ||
+      max_context_len <= 0 || max_context_len > pkv::kMaxLen || max_blocks_per_seq <= 0 ||
+      n_head < p->n_kv_head)
+    return 0;
+  return pkv::select_workspace_bytes(p, select_shape(n_seqs, total_q, max_q_len, max_context_len,
+                                                     max_blocks_per_seq, n_head));
+}
+
+int pkv_select_blocks(pkv_pool* p, const void* q, const void* bounds, int32_t* blocks,
+                      int top_blocks, int first_blocks, int last_blocks,
+                      const int32_t* cu_q_lens, const int32_t* context_lens,
+                      const int32_t* block_tables, int max_blocks_per_seq, int n_seqs,
+                      int total_q, int max_q_len, int max_context_len, int n_head,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  CHECK_POOL(p);
+  if (n_seqs < 0 || total_q < 0)
+    return fail(p, PKV_ERR_INVALID, "n_seqs %d, total_q %d < 0", n_seqs, total_q);
+  if (n_seqs == 0 || total_q == 0) return PKV_OK;
+  if (int rc = rows_validate(p, q, blocks, top_blocks, cu_q_lens, context_lens, block_tables,
+                             max_blocks_per_seq, n_seqs, total_q, max_q_len, n_head))
+    return rc;
+  if (!bounds || !aligned16(bounds))
+    return fail(p, PKV_ERR_INVALID, "bounds must be non-NULL and 16-byte aligned");
+  if (first_blocks < 0 || last_blocks < 1 || (long long)first_blocks + last_blocks > top_blocks)
+    return fail(p, PKV_ERR_INVALID,
+                "first_blocks %d >= 0 and last_blocks %d >= 1 must fit in top_blocks %d",
+                first_blocks, last_blocks, top_blocks);
+  if (max_context_len <= 0 || max_context_len > pkv::kMaxLen)
+    return fail(p, PKV_ERR_INVALID, "max_context_len (%d) must be in 1 .. 2^30", max_context_len);
+  pkv::SelectArgs a = select_shape(n_seqs, total_q, max_q_len, max_context_len,
+                                   max_blocks_per_seq, n_head);
+  a.q = q;
+  a.blocks = blocks;
+  a.top_blocks = top_blocks;
+  a.first_blocks = first_blocks;
+  a.last_blocks = last_blocks;
+  a.cu_q_lens = cu_q_lens;
+  a.context_lens = context_lens;
+  a.block_tables = block_tables;
+  if (!pkv::select_fits(p, a))
+    return fail(p, PKV_ERR_UNSUPPORTED, "select_blocks: %d sequences of up to %d rows and %d keys: "
+                "too many work-items for one launch", n_seqs, max_q_len, max_context_len);
+  if (int rc = workspace_check(p, workspace, workspace_bytes, pkv::select_workspace_bytes(p, a),
+                               "select_blocks"))
+    return rc;
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_select(p, bounds, a, static_cast<char*>(workspace),
+                                    static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "select_blocks launch");
+  return PKV_OK;
+}
+
+size_t pkv_sparse_workspace_bytes(const pkv_pool* p, int total_q, int n_head, int top_blocks) {
+  if (!p || total_q <= 0 || n_head < p->n_kv_head || top_blocks <= 0 ||
+      top_blocks > pkv::kMaxLen / p->block_size)
+    return 0;
+  pkv::SparseArgs a{};
+  a.total_q = total_q;
+  a.n_head = n_head;
+  a.top_blocks = top_blocks;
+  return pkv::sparse_workspace_bytes(p, a);
+}
+
+int pkv_sparse_attention(pkv_pool* p, int layer, const void* q, void* out, int out_dtype,
+                         const int32_t* blocks, int top_blocks, const int32_t* cu_q_lens,
+                         const int32_t* context_lens, const int32_t* block_tables,
+                         int max_blocks_per_seq, int n_seqs, int total_q, int max_q_len,
+                         int n_head, float scale, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  CHECK_POOL(p);
+  if (int rc = check_layer(p, layer)) return rc;
+  if (n_seqs < 0 || total_q < 0)
+    return fail(p, PKV_ERR_INVALID, "n_seqs %d, total_q %d < 0", n_seqs, total_q);
+  if (n_seqs == 0 || total_q == 0) return PKV_OK;
+  if (int rc = rows_validate(p, q, blocks, top_blocks, cu_q_lens, context_lens, block_tables,
+                             max_blocks_per_seq, n_seqs, total_q, max_q_len, n_head))
+    return rc;
+  if (!out || !aligned16(out))
+    return fail(p, PKV_ERR_INVALID, "out must be non-NULL and 16-byte aligned");
+  if (out_dtype != PKV_F32 && out_dtype != p->dtype)
+    return fail(p, PKV_ERR_INVALID, "out_dtype must be PKV_F32 or the pool dtype");
+  if (!(scale == scale)) return fail(p, PKV_ERR_INVALID, "scale is NaN");
+  pkv::SparseArgs a{q, out, out_dtype, blocks, top_blocks, cu_q_lens, context_lens, block_tables,
+                    max_blocks_per_seq, n_seqs, total_q, max_q_len, n_head, scale};
+  if (!pkv::sparse_fits(p, a))
+    return fail(p, PKV_ERR_UNSUPPORTED,
+                "sparse_attention: %d sequences of up to %d rows, %d blocks each: more than 2^26 "
+                "waves", n_seqs, max_q_len, top_blocks);
+  if (int rc = workspace_check(p, workspace, workspace_bytes, pkv::sparse_workspace_bytes(p, a),
+                               "sparse_attention"))
+    return rc;
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_sparse(p, layer, a, static_cast<char*>(workspace),
+                                    static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "sparse_attention launch");
+  return PKV_OK;
+}
+
+size_t pkv_verify_workspace_bytes(int batch, int total_drafts, int vocab, int has_draft_logits) {
+  if (batch <= 0 || total_drafts < 0 || total_drafts > pkv::kMaxLen || batch > pkv::kMaxLen / 2 ||
+      vocab <= 0 || vocab >= (1 << 24))
+    return 0;
+  pkv::VerifyArgs a{};
+  a.batch = batch;
+  a.total_drafts = total_drafts;
+  a.vocab = vocab;
+  a.has_draft = has_draft_logits != 0;
+  return pkv::verify_workspace_bytes(a);
+}
+
+int pkv_verify_drafts(const void* target_logits, int target_dtype, long long target_row_stride,
+                      const void* draft_logits, int draft_dtype, long long draft_row_stride,
+                      const int32_t* draft_tokens, const int32_t* cu_drafts, int batch,
+                      int total_drafts, int vocab, const float* uniforms,
+                      const float* final_uniforms, const float* temperatures,
+                      int32_t* out_tokens, int32_t* n_accepted, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  g_thread_error.clear();
+  if (batch < 0 || total_drafts < 0 || batch > pkv::kMaxLen / 2 || total_drafts > pkv::kMaxLen / 2)
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: batch %d, total_drafts %d (0 .. 2^29)",
+                batch, total_drafts);
+  if (vocab <= 0 || vocab >= (1 << 24))
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: vocab %d (1 .. 2^24 - 1)", vocab);
+  if (batch == 0) return PKV_OK;
+  for (int dt : {target_dtype, draft_logits ? draft_dtype : PKV_F32})
+    if (dt != PKV_F32 && dt != PKV_F16 && dt != PKV_BF16)
+      return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: dtype %d", dt);
+  if (!target_logits || !cu_drafts || !out_tokens || !n_accepted ||
+      (total_drafts && !draft_tokens) ||
+      (temperatures && (!final_uniforms || (total_drafts && !uniforms))))
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: NULL argument");
+  if ((total_drafts + batch > 1 && target_row_stride < vocab) ||
+      (draft_logits && total_drafts > 1 && draft_row_stride < vocab))
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: row stride %lld, %lld < vocab %d",
+                target_row_stride, draft_row_stride, vocab);
+  if (reinterpret_cast<uintptr_t>(target_logits) % pkv::dtype_bytes(target_dtype) ||
+      (draft_logits && reinterpret_cast<uintptr_t>(draft_logits) % pkv::dtype_bytes(draft_dtype)))
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: logits not aligned to the element size");
+  if (misaligned4({draft_tokens, cu_drafts, uniforms, final_uniforms, temperatures, out_tokens,
+                   n_accepted}))
+    return fail(nullptr, PKV_ERR_INVALID, "verify_drafts: arrays must be 4-byte aligned");
+  pkv::VerifyArgs a{target_logits, target_dtype, target_row_stride, draft_logits, draft_dtype,
+                    draft_row_stride, draft_tokens, cu_drafts, uniforms, final_uniforms,
+                    temperatures, batch, total_drafts, vocab, draft_logits != nullptr, out_tokens,
+                    n_accepted};
+  if (!pkv::verify_fits(a))
+    return fail(nullptr, PKV_ERR_UNSUPPORTED,
+                "verify_drafts: batch %d, total_drafts %d: too many work-items for one launch",
+                batch, total_drafts);
+  if (int rc = workspace_check(nullptr, workspace, workspace_bytes, pkv::verify_workspace_bytes(a),
+                               "verify_drafts"))
+    return rc;
+  hipError_t e = pkv::launch_verify(a, static_cast<char*>(workspace),
+                                    static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(nullptr, e, "verify_drafts launch");
   return PKV_OK;
 }
 

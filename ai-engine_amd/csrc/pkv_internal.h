@@ -234,4 +234,104 @@ hipError_t launch_mixed(const pkv_pool* p, int layer, const PrefillArgs& pa,
                         hipStream_t stream, hipEvent_t ev_begin = nullptr,
                         hipEvent_t ev_end = nullptr);
 
+// Block tables, slots and positions of a step (pkv_step.hip).
+struct StepArgs {
+  const int32_t* seq_lens;
+  const int32_t* new_lens;
+  const int32_t* n_blocks;
+  const int32_t* tables_in;
+  const int32_t* free_list;
+  const int32_t* free_count;
+  int free_len;
+  int n_seqs;
+  int width;  // table entries per request
+  int max_tokens;
+  int bs_log2;
+  int num_blocks;
+  int32_t* tables_out;
+  int32_t* n_blocks_out;
+  int32_t* free_count_out;
+  int32_t* context_lens;
+  int32_t* cu_q_lens;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* status;
+};
+hipError_t launch_step_tables(const StepArgs& a, hipStream_t stream);
+
+// Key bounds of the blocks that hold new positions (pkv_select.hip); fits:
+// the launch's grid is within HIP's limits.
+bool bounds_fits(const pkv_pool* p, int n_seqs, int max_new_len, int mbps);
+hipError_t launch_bounds(const pkv_pool* p, int layer, void* bounds, const int32_t* tables,
+                         int mbps, const int32_t* first, const int32_t* ctx, int n_seqs,
+                         int max_new_len, hipStream_t stream);
+
+// The choice of blocks (pkv_select.hip).
+struct SelectArgs {
+  const void* q;
+  int32_t* blocks;
+  int top_blocks;
+  int first_blocks;
+  int last_blocks;
+  const int32_t* cu_q_lens;  // null: one row per sequence
+  const int32_t* context_lens;
+  const int32_t* block_tables;
+  int max_blocks_per_seq;
+  int n_seqs;
+  int total_q;
+  int max_q_len;
+  int max_context_len;
+  int n_head;
+};
+size_t select_workspace_bytes(const pkv_pool* p, const SelectArgs& a);
+bool select_fits(const pkv_pool* p, const SelectArgs& a);
+hipError_t launch_select(const pkv_pool* p, const void* bounds, const SelectArgs& a, char* ws,
+                         hipStream_t stream);
+
+// Attention over chosen blocks (pkv_sparse.hip).
+struct SparseArgs {
+  const void* q;
+  void* out;
+  int out_dtype;
+  const int32_t* blocks;
+  int top_blocks;
+  const int32_t* cu_q_lens;  // null: one row per sequence
+  const int32_t* context_lens;
+  const int32_t* block_tables;
+  int max_blocks_per_seq;
+  int n_seqs;
+  int total_q;
+  int max_q_len;
+  int n_head;
+  float scale;
+};
+size_t sparse_workspace_bytes(const pkv_pool* p, const SparseArgs& a);
+bool sparse_fits(const pkv_pool* p, const SparseArgs& a);
+hipError_t launch_sparse(const pkv_pool* p, int layer, const SparseArgs& a, char* ws,
+                         hipStream_t stream);
+
+// Verification of drafted tokens (pkv_verify.hip).
+struct VerifyArgs {
+  const void* target_logits;
+  int target_dtype;
+  long long target_stride;
+  const void* draft_logits;  // or null
+  int draft_dtype;
+  long long draft_stride;
+  const int32_t* draft_tokens;
+  const int32_t* cu_drafts;
+  const float* uniforms;
+  const float* final_uniforms;
+  const float* temperatures;  // or null: greedy
+  int batch;
+  int total_drafts;
+  int vocab;
+  bool has_draft;  // draft_logits are given
+  int32_t* out_tokens;
+  int32_t* n_accepted;
+};
+size_t verify_workspace_bytes(const VerifyArgs& a);
+bool verify_fits(const VerifyArgs& a);
+hipError_t launch_verify(const VerifyArgs& a, char* ws, hipStream_t stream);
+
 }  // namespace pkv

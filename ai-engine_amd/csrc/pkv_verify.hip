@@ -1,0 +1,552 @@
+// pkv_verify.hip -- verification of drafted tokens against the target's
+// probabilities, from given random numbers (gfx950).
+//
+// A request with n drafts d_0 .. d_{n-1} has n + 1 target rows.  With p_i =
+// softmax(target row i / T) and q_i = softmax(draft row i / T) (or all of q_i on
+// d_i without draft rows), draft i is kept while u_i q_i(d_i) < p_i(d_i); at
+// the first one that is not, the next token is drawn from max(p_i - q_i, 0),
+// after the last draft from p_n: the first token whose running sum of weights
+// passes v times their total.  Greedy requests keep drafts that are the
+// row's first maximum and end with a row's first maximum.
+//
+// Every decision is that of 64-bit arithmetic: exponentials, sums and
+// comparisons are doubles.  On this GPU a double multiply-add issues at the
+// rate of a float one, and 2^x for x <= 0 is range reduction by rounding and
+// the Taylor polynomial of e^z (|z| <= ln 2 / 2, degree 12, error 2e-16),
+// some 20 operations an element against 2 or 4 bytes read.
+//
+// Three launches: statistics of every row (maximum, sum, argmax) in G chunks;
+// per request the kept drafts, and the last row's weights summed in chunks;
+// the token, found in the chunk in which the running sum passes.
+#include <algorithm>
+
+#include "pkv_device.h"
+#include "pkv_internal.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kVT = 256;  // threads
+constexpr int kVW = kVT / kWave;
+
+struct RowPart {  // of one chunk of a row
+  float m;        // largest logit (NaN aside)
+  int arg;        // its first index
+  double s;       // sum of 2^((l - m) c)
+};
+struct WeightPart {
+  double left, p;  // sums of max(p - q, 0) and of p
+};
+struct Decision {
+  double inv_p, inv_q;  // 1 / sum of the target and the draft row (0: none)
+  float m_p, m_q;
+  int row;      // target row of the next token
+  int draft;    // its draft row, or -1
+  int not_tok;  // token whose weight is taken out (no draft rows), or -1
+  int token;    // >= 0: the token itself
+  int at;       // where it goes
+  int pad;
+};
+
+struct VerifyKArgs {
+  const char* target;
+  const char* draft;  // or null
+  long long t_stride, d_stride;  // elements
+  int draft_dt;
+  const int32_t* tokens;
+  const int32_t* cu;
+  const float* u;
+  const float* u_last;
+  const float* temps;  // or null: greedy
+  int batch, total, vocab;
+  int g1, g2;  // chunks of the statistics and of the weights
+  int len1, len2;
+  RowPart* rows;      // [total + batch target rows, total draft rows][g1]
+  WeightPart* parts;  // [batch][g2]
+  Decision* decide;   // [batch]
+  int32_t* out;       // [total + batch]
+  int32_t* accepted;  // [batch]
+};
+
+// 2^t for t <= 0.
+__device__ __forceinline__ double exp2_neg(double t) {
+  const double n = __builtin_rint(t);
+  const double z = (t - n) * 0.6931471805599453094;
+  double p = 1.0 / 479001600.0;
+  p = fma(p, z, 1.0 / 39916800.0);
+  p = fma(p, z, 1.0 / 3628800.0);
+  p = fma(p, z, 1.0 / 362880.0);
+  p = fma(p, z, 1.0 / 40320.0);
+  p = fma(p, z, 1.0 / 5040.0);
+  p = fma(p, z, 1.0 / 720.0);
+  p = fma(p, z, 1.0 / 120.0);
+  p = fma(p, z, 1.0 / 24.0);
+  p = fma(p, z, 1.0 / 6.0);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)fmax(n, -1200.0));
+}
+// Weight of a logit under the row's maximum; NaN and -inf weigh nothing.
+__device__ __forceinline__ double weight(float l, float m, double c) {
+  if (!(l > -INFINITY)) return 0.0;
+  if (l == m) return 1.0;
+  return exp2_neg(fmax(((double)l - (double)m) * c, -1200.0));
+}
+
+template <int DT>
+__device__ __forceinline__ float logit(const char* row, long long i) {
+  if constexpr (DT == PKV_F32) return reinterpret_cast<const float*>(row)[i];
+  const uint16_t w = reinterpret_cast<const uint16_t*>(row)[i];
+  return DT == PKV_BF16 ? bf16lo(w) : f16lo(w);
+}
+__device__ __forceinline__ float logit_dt(int dt, const char* row, long long i) {
+  return dt == PKV_F32 ? logit<PKV_F32>(row, i)
+                       : dt == PKV_F16 ? logit<PKV_F16>(row, i) : logit<PKV_BF16>(row, i);
+}
+__device__ __forceinline__ int bytes_of(int dt) { return dt == PKV_F32 ? 4 : 2; }
+
+// c of exp(l / T) = 2^(l c); 0: greedy (T is 0, or not a positive number).
+__device__ __forceinline__ double exponent(const VerifyKArgs& a, int b) {
+  const float t = a.temps ? a.temps[b] : 0.0f;
+  return t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0;
+}
+// Drafts of request b, within the call's total.
+__device__ __forceinline__ int first_draft(const VerifyKArgs& a, int b) {
+  return min(max(a.cu[b], 0), a.total);
+}
+// Number of requests k >= 1 whose first entry cu[k] + step k is at most x: the
+// request of target row x (step 1) or of draft x (step 0).
+__device__ __forceinline__ int request_of(const VerifyKArgs& a, int x, int step) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int k0 = 1; k0 < a.batch; k0 += kWave) {
+    const int k = k0 + lane;
+    n += __popcll(__ballot(k < a.batch && first_draft(a, k) + step * k <= x));
+  }
+  return n;
+}
+
+// A chunk's running maximum, its index, and the sum below it.
+struct Stat {
+  float m;
+  int arg;
+  double s;
+};
+constexpr Stat kNoStat{-INFINITY, 0, 0.0};
+__device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
+  const float m = fmaxf(x.m, y.m);
+  if (y.m > x.m || (y.m == x.m && y.arg < x.arg)) x.arg = y.arg;
+  if (c != 0.0 && m > -INFINITY) x.s = x.s * weight(x.m, m, c) + y.s * weight(y.m, m, c);
+  x.m = m;
+}
+
+// Elements i .. i + 7 of a row as floats, i a multiple of 8; those from n on
+// are -inf.  VEC: rows start on 16 bytes.
+constexpr int kN = 8;
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const char* row, int i, int n, float (&x)[kN]) {
+  if (VEC && i + kN <= n) {
+    if constexpr (DT == PKV_F32) {
+      float y[4], z[4];
+      widen16<DT, 4>(ld16(row + (size_t)i * 4), y);
+      widen16<DT, 4>(ld16(row + (size_t)i * 4 + 16), z);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = y[e];
+        x[4 + e] = z[e];
+      }
+    } else {
+      widen16<DT, 8>(ld16(row + (size_t)i * 2), x);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kN; ++e) x[e] = i + e < n ? logit<DT>(row, i + e) : -INFINITY;
+}
+
+// Statistics of elements c0 .. c1 - 1 by the workgroup; thread 0 has them.
+template <int DT, bool VEC>
+__device__ Stat chunk_stat(const char* row, int c0, int c1, double c, Stat* lds) {
+  Stat st = kNoStat;
+  for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
+    float x[kN];
+    load8<DT, VEC>(row, i, c1, x);
+    float gm = -INFINITY;
+    int ga = 0;
+#pragma unroll
+    for (int e = 0; e < kN; ++e)
+      if (x[e] > gm) {
+        gm = x[e];
+        ga = i + e;
+      }
+    if (gm > st.m) {
+      if (c != 0.0) st.s *= weight(st.m, gm, c);
+      st.m = gm;
+      st.arg = ga;
+    }
+    if (c != 0.0) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) st.s += weight(x[e], st.m, c);
+    }
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    Stat y;
+    y.m = __shfl_xor(st.m, o, kWave);
+    y.arg = __shfl_xor(st.arg, o, kWave);
+    y.s = __shfl_xor(st.s, o, kWave);
+    join(st, y, c);
+  }
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = st;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < kVW; ++w) join(st, lds[w], c);
+  return st;
+}
+
+// Grid rows x g1: target rows first, then draft rows.  Draft rows of greedy
+// requests are not read.
+template <int DT, int DDT, bool VEC>
+__global__ void __launch_bounds__(kVT) verify_stat_kernel(VerifyKArgs a) {
+  __shared__ Stat lds[kVW];
+  const int n_target = a.total + a.batch;
+  const int r = blockIdx.x / a.g1, chunk = blockIdx.x % a.g1;
+  const bool draft = r >= n_target;
+  const int b = draft ? request_of(a, r - n_target, 0) : request_of(a, r, 1);
+  const double c = exponent(a, b);
+  if (draft && c == 0.0) return;
+  const int c0 = chunk * a.len1, c1 = min(c0 + a.len1, a.vocab);
+  const Stat st =
+      draft ? chunk_stat<DDT, VEC>(a.draft + (r - n_target) * a.d_stride * bytes_of(DDT), c0, c1, c, lds)
+            : chunk_stat<DT, VEC>(a.target + r * a.t_stride * bytes_of(DT), c0, c1, c, lds);
+  if (threadIdx.x == 0) a.rows[(size_t)r * a.g1 + chunk] = {st.m, st.arg, st.s};
+}
+
+// A row's statistics from its chunks'.
+__device__ __forceinline__ Stat row_stat(const VerifyKArgs& a, int r, double c) {
+  Stat st = kNoStat;
+  for (int k = 0; k < a.g1; ++k) {
+    const RowPart y = a.rows[(size_t)r * a.g1 + k];
+    const Stat t{y.m, y.arg, y.s};
+    if (k == 0) st = t;
+    else join(st, t, c);
+  }
+  return st;
+}
+
+// The drafts of request b that are kept and what its next token is drawn
+// from, in every thread.
+__device__ Decision decide(const VerifyKArgs& a, int b, int& kept, int* lds) {
+  const int d0 = first_draft(a, b);
+  const int n = max(first_draft(a, b + 1) - d0, 0);
+  const double c = exponent(a, b);
+  const int n_target = a.total + a.batch;
+  kept = n;
+  for (int i0 = 0; i0 < n; i0 += kVT) {  // uniform
+    const int i = i0 + (int)threadIdx.x;
+    bool keep = true;
+    if (i < n) {
+      const int d = a.tokens[d0 + i];
+      const int r = d0 + b + i;
+      const Stat p = row_stat(a, r, c);
+      if (d < 0 || d >= a.vocab) {
+        keep = false;
+      } else if (c == 0.0) {
+        keep = d == p.arg && p.m > -INFINITY;
+      } else {
+        const float lp = logit_dt(a.draft_dt >> 8, a.target + r * a.t_stride * bytes_of(a.draft_dt >> 8), d);
+        const double wp = weight(lp, p.m, c);
+        double wq = 1.0, sq = 1.0;
+        if (a.draft) {
+          const Stat q = row_stat(a, n_target + d0 + i, c);
+          const int dt = a.draft_dt & 255;
+          wq = weight(logit_dt(dt, a.draft + (d0 + i) * a.d_stride * bytes_of(dt), d), q.m, c);
+          sq = q.s;
+        }
+        // u q(d) < p(d); a draft row without weight has q = 0
+        const double qd = sq > 0.0 ? wq / sq : 0.0, pd = p.s > 0.0 ? wp / p.s : 0.0;
+        keep = (double)a.u[d0 + i] * qd < pd;
+      }
+    }
+    const unsigned long long lost = __ballot(!keep);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+      lds[threadIdx.x >> 6] = lost ? (int)threadIdx.x + __ffsll((long long)lost) - 1 : INT32_MAX;
+    __syncthreads();
+    int first = INT32_MAX;
+    for (int w = 0; w < kVW; ++w) first = min(first, lds[w]);
+    if (first != INT32_MAX) {
+      kept = i0 + first;
+      break;
+    }
+  }
+  Decision d{};
+  d.row = d0 + b + kept;
+  d.at = d.row;
+  d.draft = -1;
+  d.not_tok = -1;
+  const Stat p = row_stat(a, d.row, c);
+  d.token = c == 0.0 ? p.arg : p.s > 0.0 ? -1 : 0;
+  d.m_p = p.m;
+  d.inv_p = p.s > 0.0 ? 1.0 / p.s : 0.0;
+  if (c != 0.0 && kept < n) {
+    if (a.draft) {
+      const Stat q = row_stat(a, n_target + d0 + kept, c);
+      if (q.s > 0.0) {
+        d.draft = d0 + kept;
+        d.m_q = q.m;
+        d.inv_q = 1.0 / q.s;
+      }
+    } else {
+      d.not_tok = a.tokens[d0 + kept];
+    }
+  }
+  return d;
+}
+
+// p and max(p - q, 0) of token i.
+__device__ __forceinline__ WeightPart weigh(const Decision& d, float lp, float lq, int i, double c) {
+  const double p = weight(lp, d.m_p, c) * d.inv_p;
+  const double q = d.draft >= 0 ? weight(lq, d.m_q, c) * d.inv_q : 0.0;
+  return {i == d.not_tok ? 0.0 : fmax(p - q, 0.0), p};
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  return x;
+}
+
+// Grid batch x g2.
+template <int DT, int DDT, bool VEC>
+__global__ void __launch_bounds__(kVT) verify_weight_kernel(VerifyKArgs a) {
+  __shared__ int lds[kVW];
+  __shared__ WeightPart sum[kVW];
+  const int b = blockIdx.x / a.g2, chunk = blockIdx.x % a.g2;
+  int kept = 0;
+  const Decision d = decide(a, b, kept, lds);
+  if (chunk == 0) {
+    const int d0 = first_draft(a, b), n = max(first_draft(a, b + 1) - d0, 0);
+    if (threadIdx.x == 0) {
+      a.decide[b] = d;
+      a.accepted[b] = kept;
+    }
+    for (int i = threadIdx.x; i <= n; i += kVT)
+      a.out[d0 + b + i] = i < kept ? a.tokens[d0 + i] : i == kept ? max(d.token, 0) : -1;
+  }
+  if (d.token >= 0) return;
+  const double c = exponent(a, b);
+  const char* tr = a.target + d.row * a.t_stride * bytes_of(DT);
+  const char* dr = d.draft >= 0 ? a.draft + d.draft * a.d_stride * bytes_of(DDT) : nullptr;
+  const int c0 = chunk * a.len2, c1 = min(c0 + a.len2, a.vocab);
+  WeightPart w{0.0, 0.0};
+  for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
+    float lp[kN], lq[kN];
+    load8<DT, VEC>(tr, i, c1, lp);
+    if (dr) load8<DDT, VEC>(dr, i, c1, lq);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const WeightPart x = weigh(d, lp[e], dr ? lq[e] : 0.0f, i + e, c);
+      w.left += x.left;
+      w.p += x.p;
+    }
+  }
+  w.left = wave_sum(w.left);
+  w.p = wave_sum(w.p);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < kVW; ++k) {
+      w.left += sum[k].left;
+      w.p += sum[k].p;
+    }
+    a.parts[(size_t)b * a.g2 + chunk] = w;
+  }
+}
+
+// Grid batch: the chunk in which the running sum passes, then the token.
+template <int DT, int DDT>
+__global__ void __launch_bounds__(kVT) verify_token_kernel(VerifyKArgs a) {
+  __shared__ double sum[kVW];
+  __shared__ int found[kVW], last[kVW];
+  const int b = blockIdx.x;
+  const Decision d = a.decide[b];
+  if (d.token >= 0) return;
+  const double c = exponent(a, b);
+  const WeightPart* parts = a.parts + (size_t)b * a.g2;
+  double total = 0.0, total_p = 0.0;
+  for (int k = 0; k < a.g2; ++k) {
+    total += parts[k].left;
+    total_p += parts[k].p;
+  }
+  const bool res = total > 0.0;  // else p itself (p <= q all over, by rounding only)
+  if (!res) total = total_p;
+  const double want = (double)a.u_last[b] * total;
+  double before = 0.0;
+  int at = -1;
+  double at_before = 0.0;
+  for (int k = 0; k < a.g2; ++k) {
+    const double x = res ? parts[k].left : parts[k].p;
+    if (x > 0.0) {  // the last chunk with weight, unless one passes before
+      at = k;
+      at_before = before;
+      if (before + x > want) break;
+    }
+    before += x;
+  }
+  if (at < 0) {
+    if (threadIdx.x == 0) a.out[d.at] = 0;
+    return;
+  }
+  const char* tr = a.target + d.row * a.t_stride * bytes_of(DT);
+  const char* dr = d.draft >= 0 ? a.draft + d.draft * a.d_stride * bytes_of(DDT) : nullptr;
+  const int c0 = at * a.len2, c1 = min(c0 + a.len2, a.vocab);
+  // consecutive elements per thread
+  const int per = (c1 - c0 + kVT - 1) / kVT;
+  const int i0 = min(c0 + (int)threadIdx.x * per, c1), i1 = min(i0 + per, c1);
+  auto w = [&](int i) {
+    const WeightPart x = weigh(d, logit<DT>(tr, i), dr ? logit<DDT>(dr, i) : 0.0f, i, c);
+    return res ? x.left : x.p;
+  };
+  double mine = 0.0;
+  int final = -1;  // the thread's last token with weight
+  for (int i = i0; i < i1; ++i) {
+    const double x = w(i);
+    mine += x;
+    if (x > 0.0) final = i;
+  }
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  double incl = mine;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(incl, o, kWave);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) sum[wv] = incl;
+  __syncthreads();
+  double run = at_before + incl - mine;
+  for (int k = 0; k < wv; ++k) run += sum[k];
+  int pick = INT32_MAX;
+  if (run + mine > want) {
+    for (int i = i0; i < i1; ++i) {
+      const double x = w(i);
+      run += x;
+      if (x > 0.0 && run > want) {
+        pick = i;
+        break;
+      }
+    }
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    pick = min(pick, __shfl_xor(pick, o, kWave));
+    final = max(final, __shfl_xor(final, o, kWave));
+  }
+  if (lane == 0) {
+    found[wv] = pick;
+    last[wv] = final;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 1; k < kVW; ++k) {
+    pick = min(pick, found[k]);
+    final = max(final, last[k]);
+  }
+  a.out[d.at] = pick != INT32_MAX ? pick : final;
+}
+
+template <int DT, int DDT>
+hipError_t launch_dt(const VerifyKArgs& a, bool vec, int rows, hipStream_t s) {
+  const unsigned g1 = (unsigned)rows * a.g1, g2 = (unsigned)a.batch * a.g2;
+  if (vec) {
+    verify_stat_kernel<DT, DDT, true><<<g1, kVT, 0, s>>>(a);
+    verify_weight_kernel<DT, DDT, true><<<g2, kVT, 0, s>>>(a);
+  } else {
+    verify_stat_kernel<DT, DDT, false><<<g1, kVT, 0, s>>>(a);
+    verify_weight_kernel<DT, DDT, false><<<g2, kVT, 0, s>>>(a);
+  }
+  if (a.temps) verify_token_kernel<DT, DDT><<<a.batch, kVT, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_ddt(int ddt, const VerifyKArgs& a, bool vec, int rows, hipStream_t s) {
+  switch (ddt) {
+    case PKV_F32: return launch_dt<DT, PKV_F32>(a, vec, rows, s);
+    case PKV_F16: return launch_dt<DT, PKV_F16>(a, vec, rows, s);
+    default: return launch_dt<DT, PKV_BF16>(a, vec, rows, s);
+  }
+}
+
+struct VerifyPlan {
+  int rows, g1, len1, g2, len2;
+  size_t parts, decide, bytes;
+};
+
+// Chunks of a row: as many as give about 1024 workgroups, of 4096 elements or
+// more, a multiple of 8 long.
+void chunks(long long rows, int vocab, int& g, int& len) {
+  const int most = std::max(1, vocab / 4096);
+  g = (int)std::max<long long>(1, std::min<long long>(1024 / std::max<long long>(rows, 1), most));
+  len = ((vocab + g - 1) / g + 7) / 8 * 8;
+  g = std::max(1, (vocab + len - 1) / len);
+}
+
+VerifyPlan verify_plan(const VerifyArgs& a) {
+  VerifyPlan p{};
+  p.rows = a.total_drafts + a.batch + (a.has_draft ? a.total_drafts : 0);
+  chunks(p.rows, a.vocab, p.g1, p.len1);
+  chunks(a.batch, a.vocab, p.g2, p.len2);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  p.parts = up((size_t)p.rows * p.g1 * sizeof(RowPart));
+  p.decide = p.parts + up((size_t)a.batch * p.g2 * sizeof(WeightPart));
+  p.bytes = p.decide + up((size_t)a.batch * sizeof(Decision));
+  return p;
+}
+
+}  // namespace
+
+size_t verify_workspace_bytes(const VerifyArgs& a) { return verify_plan(a).bytes; }
+
+bool verify_fits(const VerifyArgs& a) {
+  const VerifyPlan p = verify_plan(a);
+  return grid_fits((long long)p.rows * p.g1, kVT) && grid_fits((long long)a.batch * p.g2, kVT);
+}
+
+hipError_t launch_verify(const VerifyArgs& a, char* ws, hipStream_t stream) {
+  const VerifyPlan pl = verify_plan(a);
+  VerifyKArgs k{};
+  k.target = static_cast<const char*>(a.target_logits);
+  k.draft = static_cast<const char*>(a.draft_logits);
+  k.t_stride = a.target_stride;
+  k.d_stride = a.draft_stride;
+  k.draft_dt = a.target_dtype << 8 | a.draft_dtype;
+  k.tokens = a.draft_tokens;
+  k.cu = a.cu_drafts;
+  k.u = a.uniforms;
+  k.u_last = a.final_uniforms;
+  k.temps = a.temperatures;
+  k.batch = a.batch;
+  k.total = a.total_drafts;
+  k.vocab = a.vocab;
+  k.g1 = pl.g1;
+  k.g2 = pl.g2;
+  k.len1 = pl.len1;
+  k.len2 = pl.len2;
+  k.rows = reinterpret_cast<RowPart*>(ws);
+  k.parts = reinterpret_cast<WeightPart*>(ws + pl.parts);
+  k.decide = reinterpret_cast<Decision*>(ws + pl.decide);
+  k.out = a.out_tokens;
+  k.accepted = a.n_accepted;
+  // 16-byte loads where every row starts on 16 bytes
+  auto al = [](const void* p, long long stride, int dt) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * (long long)dtype_bytes(dt))) & 15) == 0;
+  };
+  const bool vec = al(k.target, k.t_stride, a.target_dtype) &&
+                   (!k.draft || al(k.draft, k.d_stride, a.draft_dtype));
+  const int ddt = k.draft ? a.draft_dtype : a.target_dtype;
+  switch (a.target_dtype) {
+    case PKV_F32: return launch_ddt<PKV_F32>(ddt, k, vec, pl.rows, stream);
+    case PKV_F16: return launch_ddt<PKV_F16>(ddt, k, vec, pl.rows, stream);
+    default: return launch_ddt<PKV_BF16>(ddt, k, vec, pl.rows, stream);
+  }
+}
+
+}  // namespace pkv

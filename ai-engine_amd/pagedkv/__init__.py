@@ -15,6 +15,8 @@ torch tensors are used only as device memory and for the current stream.
 """
 from __future__ import annotations
 
+import collections
+import contextlib
 import ctypes
 import sys
 import math
@@ -27,7 +29,7 @@ __all__ = [
     "BlockAllocator", "BlockTable", "PagedKvCache", "KvPool", "Rope", "rope_tables_host",
     "CapacityError",
     "PagedKvError", "F32", "F16", "BF16", "lib", "LIB_PATH", "torch_dtype",
-    "pkv_dtype",
+    "pkv_dtype", "StepTables", "step_tables", "verify_drafts",
 ]
 
 
@@ -233,6 +235,150 @@ def sample_expf(x):
     check(lib().pkv_sample_expf(_dev_ptr(x), _dev_ptr(out), x.numel(),
                                 _stream_ptr(torch.cuda.current_stream(x.device))), None)
     return out
+
+
+def _device_tensor(t, name: str, device, dtype, shape=None):
+    """t, after a check that a kernel may read it as this."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise ValueError(f"{name} must be a tensor on {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _run_on(stream, device, tensors):
+    """(stream to launch on, context in which to allocate and launch).  Another
+    stream than the current one first waits for the work queued on the current
+    one, and the tensors' memory is not reused before it has run."""
+    import torch
+    cur = torch.cuda.current_stream(device)
+    if stream is None or stream == cur:
+        if torch.cuda.current_device() == device.index:
+            return cur, contextlib.nullcontext()
+        return cur, torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream must be on {device}")
+    stream.wait_stream(cur)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    return stream, torch.cuda.stream(stream)
+
+
+def _workspace(nbytes: int, device):
+    """Scratch of one call, from torch's allocator: it belongs to the call's
+    stream, and to the graph's memory while that stream is captured."""
+    import torch
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+StepTables = collections.namedtuple(
+    "StepTables", "block_tables n_blocks free_count context_lens cu_q_lens positions "
+                  "slot_mapping status")
+
+
+def step_tables(seq_lens, new_lens, block_tables, n_blocks, free_list, free_count,
+                block_size: int, num_blocks: int, max_tokens: int, stream=None) -> StepTables:
+    """Block tables, slots and positions of a step from request lengths on the
+    device (pkv_step_tables): request i, with seq_lens[i] tokens in n_blocks[i]
+    blocks, writes new_lens[i] more; blocks that it lacks come from the end of
+    free_list[: free_count] in request order (BlockAllocator.ensure_capacity).
+    seq_lens, new_lens, n_blocks: (n,) int32, block_tables: (n, width) int32,
+    free_list: (any,) int32, free_count: (1,) int32, all on one device;
+    max_tokens: length of the step's token arrays (a host bound of the new
+    tokens).  Nothing synchronises.  Returns new tensors:
+      block_tables, n_blocks, free_count  for the next step
+      context_lens (n,), cu_q_lens (n + 1,)
+      positions, slot_mapping (max_tokens,), -1 past the step's tokens
+      status (1,): 0, the number of blocks that the free list is short of, or
+        -1 for lengths out of range; unless 0 the step is empty and tables,
+        n_blocks and free_count are unchanged."""
+    import torch
+    if not isinstance(block_tables, torch.Tensor) or not block_tables.is_cuda:
+        raise ValueError("block_tables must be a device tensor")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be (n, width)")
+    dev, i32 = block_tables.device, torch.int32
+    n, width = block_tables.shape
+    bt = _device_tensor(block_tables, "block_tables", dev, i32)
+    sl = _device_tensor(seq_lens, "seq_lens", dev, i32, (n,))
+    nl = _device_tensor(new_lens, "new_lens", dev, i32, (n,))
+    nb = _device_tensor(n_blocks, "n_blocks", dev, i32, (n,))
+    fl = _device_tensor(free_list, "free_list", dev, i32)
+    fc = _device_tensor(free_count, "free_count", dev, i32, (1,))
+    s, ctx = _run_on(stream, dev, (bt, sl, nl, nb, fl, fc))
+    with ctx:
+        def new(*shape):
+            return torch.empty(shape, dtype=i32, device=dev)
+        r = StepTables(new(n, width), new(n), new(1), new(n), new(n + 1), new(max_tokens),
+                       new(max_tokens), new(1))
+        check(lib().pkv_step_tables(
+            block_size, num_blocks, _dev_ptr(sl), _dev_ptr(nl), n, _dev_ptr(bt), _dev_ptr(nb),
+            width, _dev_ptr(fl), fl.numel(), _dev_ptr(fc), max_tokens, _dev_ptr(r.block_tables),
+            _dev_ptr(r.n_blocks), _dev_ptr(r.free_count), _dev_ptr(r.context_lens),
+            _dev_ptr(r.cu_q_lens), _dev_ptr(r.positions), _dev_ptr(r.slot_mapping),
+            _dev_ptr(r.status), _stream_ptr(s)), None)
+    return r
+
+
+def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_uniforms,
+                  draft_logits=None, temperatures=None, stream=None):
+    """Keeps the drafted tokens that the target's distribution keeps and draws
+    the token after them (pkv_verify_drafts), from given random numbers.
+    target_logits: (drafts + batch, vocab) f32/f16/bf16, request b's rows (one
+    per draft and one after the last) at cu_drafts[b] + b; draft_tokens:
+    (drafts,) int32; cu_drafts: (batch + 1,) int32; uniforms: (drafts,) and
+    final_uniforms: (batch,) float32 in [0, 1); draft_logits: (drafts, vocab)
+    f32/f16/bf16, or None for drafts without a distribution; temperatures:
+    (batch,) float32, or None (all greedy; 0 is greedy).  Both logits have unit
+    stride along vocab.  Draft i is kept while u_i q_i(d_i) < p_i(d_i); the next
+    token comes from max(p - q, 0) of the first one that is not, or from p
+    after the last.  Nothing synchronises.  Returns (tokens, accepted):
+    (drafts + batch,) int32 with a request's kept drafts, next token and then
+    -1 at cu_drafts[b] + b, and (batch,) int32 with the number of kept drafts."""
+    import torch
+    if not isinstance(target_logits, torch.Tensor) or not target_logits.is_cuda:
+        raise ValueError("target_logits must be a device tensor")
+    dev, i32, f32 = target_logits.device, torch.int32, torch.float32
+    total, batch = draft_tokens.numel(), final_uniforms.numel()
+    for t, name, rows in ((target_logits, "target_logits", total + batch),
+                          (draft_logits, "draft_logits", total)):
+        if t is None:
+            continue
+        if t.device != dev or t.dim() != 2 or t.shape[0] != rows or \
+                t.shape[1] != target_logits.shape[1] or \
+                (t.numel() and t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be ({rows}, vocab) on {dev} with unit stride along "
+                             "vocab")
+    vocab = target_logits.shape[1]
+    dt = _device_tensor(draft_tokens, "draft_tokens", dev, i32, (total,))
+    cu = _device_tensor(cu_drafts, "cu_drafts", dev, i32, (batch + 1,))
+    u = _device_tensor(uniforms, "uniforms", dev, f32, (total,))
+    uf = _device_tensor(final_uniforms, "final_uniforms", dev, f32, (batch,))
+    tp = None
+    if temperatures is not None:
+        tp = _device_tensor(temperatures, "temperatures", dev, f32, (batch,))
+    has_draft = draft_logits is not None and total > 0
+    s, ctx = _run_on(stream, dev, (target_logits, draft_logits, dt, cu, u, uf, tp))
+    with ctx:
+        tokens = torch.empty(total + batch, dtype=i32, device=dev)
+        accepted = torch.empty(batch, dtype=i32, device=dev)
+        need = lib().pkv_verify_workspace_bytes(batch, total, vocab, has_draft)
+        ws = _workspace(need, dev)
+        check(lib().pkv_verify_drafts(
+            _dev_ptr(target_logits), pkv_dtype(target_logits.dtype),
+            max(target_logits.stride(0), vocab) if total + batch <= 1 else target_logits.stride(0),
+            _dev_ptr(draft_logits) if has_draft else None,
+            pkv_dtype(draft_logits.dtype) if has_draft else F32,
+            (max(draft_logits.stride(0), vocab) if total <= 1 else draft_logits.stride(0))
+            if has_draft else 0,
+            _dev_ptr(dt), _dev_ptr(cu), batch, total, vocab, _dev_ptr(u), _dev_ptr(uf),
+            _dev_ptr(tp) if tp is not None else None, _dev_ptr(tokens), _dev_ptr(accepted),
+            _dev_ptr(ws), need, _stream_ptr(s)), None)
+    return tokens, accepted
 
 
 class Rope:
@@ -712,6 +858,139 @@ class KvPool:
                                         ctypes.byref(db), H, float(scale),
                                         _stream_ptr(stream)), self._h)
         return rows["prefill"], rows["decode"]
+
+    # -- attention over chosen blocks -------------------------------------------
+    def new_key_bounds(self):
+        """Zeroed key bounds of one layer: (num_blocks, n_kv, 2, hd) in the pool
+        dtype, the smallest and the largest key element of each block."""
+        import torch
+        c = self.cache
+        return torch.zeros((c.num_blocks, c.n_kv_head, 2, c.head_dim), dtype=c.dtype,
+                           device=c.device)
+
+    def _check_bounds(self, bounds) -> None:
+        c = self.cache
+        shape = (c.num_blocks, c.n_kv_head, 2, c.head_dim)
+        if _device_tensor(bounds, "bounds", c.device, c.dtype, shape) is not bounds:
+            raise ValueError("bounds must be contiguous")
+
+    def update_key_bounds(self, bounds, block_tables, context_lens, first_positions=None,
+                          max_new_len: int | None = None, stream=None):
+        """Brings `bounds` (new_key_bounds) up to date for every block that holds
+        a position from first_positions[s] (None: 0) to context_lens[s] - 1 of
+        a sequence (pkv_key_bounds).  block_tables: (n, width) int32;
+        context_lens, first_positions: (n,) int32; max_new_len: host bound of
+        their difference (None: what the tables hold).  Returns bounds."""
+        c = self.cache
+        self._check_bounds(bounds)
+        bt, cl = _i32(block_tables, c.device), _i32(context_lens, c.device)
+        fp = _i32(first_positions, c.device) if first_positions is not None else None
+        n = cl.numel()
+        if bt.dim() != 2 or bt.shape[0] != n or (fp is not None and fp.numel() != n):
+            raise ValueError("block_tables must be (n, width), context_lens and "
+                             "first_positions (n,)")
+        if max_new_len is None:
+            max_new_len = bt.shape[1] * c.block_size
+        s, ctx = _run_on(stream, c.device, (bounds, bt, cl, fp))
+        with ctx:
+            check(lib().pkv_key_bounds(
+                self._h, self.layer_index, _dev_ptr(bounds), _dev_ptr(bt), bt.shape[1],
+                _dev_ptr(fp) if fp is not None else None, _dev_ptr(cl), n, int(max_new_len),
+                _stream_ptr(s)), self._h)
+        return bounds
+
+    def _rows(self, q, block_tables, context_lens, cu_q_lens, max_q_len):
+        """Checked row arguments of select_blocks and sparse_attention."""
+        c = self.cache
+        if q.device != c.device or q.dim() != 3 or q.shape[2] != c.head_dim:
+            raise ValueError(f"q must be (rows, n_head, {c.head_dim}) on {c.device}")
+        if q.dtype != c.dtype:
+            raise TypeError("q must have the pool dtype")
+        bt, cl = _i32(block_tables, c.device), _i32(context_lens, c.device)
+        cu = _i32(cu_q_lens, c.device) if cu_q_lens is not None else None
+        n, rows = cl.numel(), q.shape[0]
+        if bt.dim() != 2 or bt.shape[0] != n:
+            raise ValueError("block_tables must be (n, width), context_lens (n,)")
+        if cu is not None and cu.numel() != n + 1:
+            raise ValueError("cu_q_lens must be (n + 1,)")
+        if cu is None and rows != n:
+            raise ValueError("without cu_q_lens q has one row per sequence")
+        if max_q_len is None:
+            max_q_len = max(rows, 1) if cu is not None else 1
+        return q.contiguous(), bt, cl, cu, n, rows, int(max_q_len)
+
+    def select_blocks(self, q, bounds, block_tables, context_lens, top_blocks: int,
+                      first_blocks: int = 1, last_blocks: int = 1, cu_q_lens=None,
+                      max_q_len: int | None = None, max_context_len: int | None = None, out=None,
+                      stream=None):
+        """The blocks that each query row attends, per kv head (pkv_select_blocks):
+        the first and last ones of its context and, of those between, the ones
+        whose `bounds` promise the group's heads the largest score, top_blocks in
+        all.  q: (rows, H, hd) in the pool dtype, as the attention will get it;
+        context_lens: (n,) int32; block_tables: (n, width) int32; cu_q_lens: (n + 1,)
+        int32 (None: one row per sequence), row i of a chunk of m rows having
+        the keys up to position context_lens - m + i.  max_q_len, max_context_len:
+        host bounds (None: all rows, what the tables hold).  Returns
+        (rows, n_kv, top_blocks) int32, ascending indexes into the sequence's row
+        of block_tables, then -1 (into `out` if given)."""
+        import torch
+        c = self.cache
+        self._check_bounds(bounds)
+        qq, bt, cl, cu, n, rows, mq = self._rows(q, block_tables, context_lens, cu_q_lens,
+                                                 max_q_len)
+        H = qq.shape[1]
+        if max_context_len is None:
+            max_context_len = bt.shape[1] * c.block_size
+        shape = (rows, c.n_kv_head, top_blocks)
+        if out is not None and _device_tensor(out, "out", c.device, torch.int32, shape) is not out:
+            raise ValueError("out must be contiguous")
+        s, ctx = _run_on(stream, c.device, (qq, bounds, bt, cl, cu, out))
+        with ctx:
+            if out is None:
+                out = torch.empty(shape, dtype=torch.int32, device=c.device)
+            need = lib().pkv_select_workspace_bytes(self._h, n, rows, mq, int(max_context_len),
+                                                    bt.shape[1], H)
+            ws = _workspace(need, c.device)
+            check(lib().pkv_select_blocks(
+                self._h, _dev_ptr(qq), _dev_ptr(bounds), _dev_ptr(out), int(top_blocks),
+                int(first_blocks), int(last_blocks), _dev_ptr(cu) if cu is not None else None,
+                _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, int(max_context_len), H,
+                _dev_ptr(ws), need, _stream_ptr(s)), self._h)
+        return out
+
+    def sparse_attention(self, q, blocks, block_tables, context_lens, cu_q_lens=None,
+                         max_q_len: int | None = None, scale: float | None = None, out_dtype=None,
+                         out=None, stream=None):
+        """Attention of each query row over the keys of its listed blocks
+        (pkv_sparse_attention).  blocks: (rows, n_kv, top) int32, as select_blocks
+        returns them (any order, distinct; negative entries are skipped); the
+        other arguments as select_blocks'.  The rows' keys are in the pool
+        already.  Returns (rows, H * hd); a row without keys is zero."""
+        import torch
+        c = self.cache
+        qq, bt, cl, cu, n, rows, mq = self._rows(q, block_tables, context_lens, cu_q_lens,
+                                                 max_q_len)
+        H, hd = qq.shape[1], qq.shape[2]
+        if blocks.dim() != 3 or blocks.shape[:2] != (rows, c.n_kv_head):
+            raise ValueError(f"blocks must be ({rows}, {c.n_kv_head}, top)")
+        bl = _device_tensor(blocks, "blocks", c.device, torch.int32)
+        if scale is None:
+            scale = 1.0 / math.sqrt(hd)
+        if out is not None and (out.device != c.device or out.shape != (rows, H * hd)
+                                or not out.is_contiguous()):
+            raise ValueError(f"out must be contiguous ({rows}, {H * hd}) on {c.device}")
+        s, ctx = _run_on(stream, c.device, (qq, bl, bt, cl, cu, out))
+        with ctx:
+            if out is None:
+                out = torch.empty((rows, H * hd), dtype=out_dtype or c.dtype, device=c.device)
+            need = lib().pkv_sparse_workspace_bytes(self._h, rows, H, bl.shape[2])
+            ws = _workspace(need, c.device)
+            check(lib().pkv_sparse_attention(
+                self._h, self.layer_index, _dev_ptr(qq), _dev_ptr(out), pkv_dtype(out.dtype),
+                _dev_ptr(bl), bl.shape[2], _dev_ptr(cu) if cu is not None else None,
+                _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, H, float(scale),
+                _dev_ptr(ws), need, _stream_ptr(s)), self._h)
+        return out
 
     def _check_rows(self, t, name: str) -> None:
         c = self.cache

@@ -115,6 +115,19 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_sample_expf": (_I, [_P, _P, ctypes.c_longlong, _P]),
     "pkv_sample_trim": (_I, []),
     "pkv_sample_draw": (ctypes.c_float, [ctypes.c_uint64]),
+    "pkv_step_tables": (_I, [_I, _I, _P, _P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P,
+                             _P, _P, _P]),
+    "pkv_key_bounds_bytes": (_SZ, [_P]),
+    "pkv_key_bounds": (_I, [_P, _I, _P, _P, _I, _P, _P, _I, _I, _P]),
+    "pkv_select_workspace_bytes": (_SZ, [_P, _I, _I, _I, _I, _I, _I]),
+    "pkv_select_blocks": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P,
+                               _SZ, _P]),
+    "pkv_sparse_workspace_bytes": (_SZ, [_P, _I, _I, _I]),
+    "pkv_sparse_attention": (_I, [_P, _I, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I,
+                                  ctypes.c_float, _P, _SZ, _P]),
+    "pkv_verify_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "pkv_verify_drafts": (_I, [_P, _I, ctypes.c_longlong, _P, _I, ctypes.c_longlong, _P, _P, _I, _I,
+                               _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "pkv_pool_profile": (_I, [_P, _I]),
     "pkv_pool_profile_read": (_I, [_P, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I)]),
     "pkv_allocator_new": (_P, [_SZ, _SZ]),

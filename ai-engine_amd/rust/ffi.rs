@@ -272,6 +272,54 @@ extern "C" {
     pub fn pkv_sample_trim() -> c_int;
     pub fn pkv_sample_draw(seed: u64) -> f32;
 
+    // ---- speculative decoding over long contexts (no reference counterpart)
+    pub fn pkv_step_tables(
+        block_size: c_int, num_blocks: c_int, seq_lens: *const i32, new_lens: *const i32, n_seqs:
+        c_int, block_tables: *const i32, n_blocks: *const i32, max_blocks_per_seq: c_int,
+        free_list: *const i32, free_len: c_int, free_count: *const i32, max_tokens: c_int,
+        block_tables_out: *mut i32, n_blocks_out: *mut i32, free_count_out: *mut i32,
+        context_lens: *mut i32, cu_q_lens: *mut i32, positions: *mut i32, slot_mapping: *mut i32,
+        status: *mut i32, stream: *mut c_void
+    ) -> c_int;
+    pub fn pkv_key_bounds_bytes(pool: *const PkvPool) -> usize;
+    pub fn pkv_key_bounds(
+        pool: *mut PkvPool, layer: c_int, bounds: *mut c_void, block_tables: *const i32,
+        max_blocks_per_seq: c_int, first_positions: *const i32, context_lens: *const i32, n_seqs:
+        c_int, max_new_len: c_int, stream: *mut c_void
+    ) -> c_int;
+    pub fn pkv_select_workspace_bytes(
+        pool: *const PkvPool, n_seqs: c_int, total_q: c_int, max_q_len: c_int, max_context_len:
+        c_int, max_blocks_per_seq: c_int, n_head: c_int
+    ) -> usize;
+    pub fn pkv_select_blocks(
+        pool: *mut PkvPool, q: *const c_void, bounds: *const c_void, blocks: *mut i32, top_blocks:
+        c_int, first_blocks: c_int, last_blocks: c_int, cu_q_lens: *const i32, context_lens:
+        *const i32, block_tables: *const i32, max_blocks_per_seq: c_int, n_seqs: c_int, total_q:
+        c_int, max_q_len: c_int, max_context_len: c_int, n_head: c_int, workspace: *mut c_void,
+        workspace_bytes: usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn pkv_sparse_workspace_bytes(
+        pool: *const PkvPool, total_q: c_int, n_head: c_int, top_blocks: c_int
+    ) -> usize;
+    pub fn pkv_sparse_attention(
+        pool: *mut PkvPool, layer: c_int, q: *const c_void, out: *mut c_void, out_dtype: c_int,
+        blocks: *const i32, top_blocks: c_int, cu_q_lens: *const i32, context_lens: *const i32,
+        block_tables: *const i32, max_blocks_per_seq: c_int, n_seqs: c_int, total_q: c_int,
+        max_q_len: c_int, n_head: c_int, scale: f32, workspace: *mut c_void, workspace_bytes:
+        usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn pkv_verify_workspace_bytes(
+        batch: c_int, total_drafts: c_int, vocab: c_int, has_draft_logits: c_int
+    ) -> usize;
+    pub fn pkv_verify_drafts(
+        target_logits: *const c_void, target_dtype: c_int, target_row_stride: c_longlong,
+        draft_logits: *const c_void, draft_dtype: c_int, draft_row_stride: c_longlong,
+        draft_tokens: *const i32, cu_drafts: *const i32, batch: c_int, total_drafts: c_int, vocab:
+        c_int, uniforms: *const f32, final_uniforms: *const f32, temperatures: *const f32,
+        out_tokens: *mut i32, n_accepted: *mut i32, workspace: *mut c_void, workspace_bytes:
+        usize, stream: *mut c_void
+    ) -> c_int;
+
     // ---- block allocator and tables (block_table.rs:5-58)
     pub fn pkv_allocator_new(num_blocks: usize, block_size: usize) -> *mut PkvAllocator;
     pub fn pkv_allocator_free(a: *mut PkvAllocator);

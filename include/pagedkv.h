@@ -537,6 +537,154 @@ int pkv_sample_trim(void);
 /* StdRng::seed_from_u64(seed).gen::<f32>() (sample.rs:41-42; host only). */
 float pkv_sample_draw(uint64_t seed);
 
+/* ---- speculative decoding over long contexts (no reference counterpart) ------
+ * A step that drafts several tokens per request and attends to a chosen part
+ * of each context, with lengths that stay on the device between steps:
+ *   pkv_step_tables       block tables, slots and positions of the step
+ *   pkv_append            its keys and values
+ *   pkv_key_bounds        the bounds of the blocks that they filled
+ *   pkv_select_blocks     per row and kv head, the blocks to attend
+ *   pkv_sparse_attention  attention over them
+ *   pkv_verify_drafts     the drafts that are kept and the token after them
+ * All are stream-ordered, allocate nothing and can be captured in a HIP graph.
+ * Scratch is the caller's (`workspace`, 16-byte aligned, of at least the bytes
+ * that the query beside each call returns), so calls on several streams, or
+ * several graphs, do not share any unless the caller makes them. */
+
+/* Block tables, slots and positions of a step from lengths on the device: the
+ * work of BlockAllocator::ensure_capacity and locate (block_table.rs:32-58) for a
+ * whole step.  Request i has seq_lens[i] tokens in n_blocks[i] blocks
+ * (block_tables[i][0 ..]; it may hold more blocks than it has tokens for) and
+ * writes new_lens[i] more; blocks that it lacks are taken from the end of
+ * free_list[0 .. *free_count - 1] in request order, as ensure_capacity does
+ * request by request.
+ *  block_tables, block_tables_out: int32 [n_seqs][max_blocks_per_seq] (entries past
+ *      a request's blocks are written as 0); may be the same array.
+ *  n_blocks_out: int32 [n_seqs], free_count_out: int32 [1], for the next step.
+ *  context_lens: int32 [n_seqs] = seq_lens + new_lens; cu_q_lens: int32 [n_seqs + 1].
+ *  positions, slot_mapping: int32 [max_tokens], token cu_q_lens[i] + t of request
+ *      i at position seq_lens[i] + t; -1 past the step's tokens.  The slot of a
+ *      block id outside [0, num_blocks) is INT32_MAX, which pkv_append reports.
+ *  status: int32 [1].  0: done.  k > 0: the free list is k blocks short.  -1: a
+ *      length is negative, a table too narrow, n_blocks or *free_count out of
+ *      range (0 .. free_len), or the step has more than max_tokens tokens.
+ *      Unless it is 0 nothing is allocated: tables, n_blocks and free_count
+ *      are copied, context_lens = seq_lens, cu_q_lens 0, slots and positions -1.
+ * Other outputs must not overlap the inputs or each other
+ * (PKV_ERR_INVALID).  block_size: a power of two in [1, 256]; num_blocks *
+ * block_size and max_blocks_per_seq * block_size below 2^31.  Runs on the calling
+ * thread's current device. */
+int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
+                    const int32_t* new_lens, int n_seqs, const int32_t* block_tables,
+                    const int32_t* n_blocks, int max_blocks_per_seq, const int32_t* free_list,
+                    int free_len, const int32_t* free_count, int max_tokens,
+                    int32_t* block_tables_out, int32_t* n_blocks_out, int32_t* free_count_out,
+                    int32_t* context_lens, int32_t* cu_q_lens, int32_t* positions,
+                    int32_t* slot_mapping, int32_t* status, void* stream);
+
+/* Key bounds: [num_blocks][n_kv_head][2][head_dim] in the pool dtype, the
+ * elementwise smallest, then largest, key element of each block and kv head (NaN
+ * keys are passed over).  One array per layer, of pkv_key_bounds_bytes, 16-byte
+ * aligned.  pkv_key_bounds brings those of every block that holds a position
+ * from first_positions[s] (NULL: 0) to context_lens[s] - 1 of a sequence up to
+ * date, from all of the block's keys below context_lens[s].  max_new_len: host
+ * bound of context_lens[s] - first_positions[s], 1 .. 2^30.  A sequence with
+ * lengths outside 0 <= first <= context <= the table, or beyond max_new_len, is
+ * left out, as is a block id outside the pool; pkv_pool_check() reports both.
+ * A block that several sequences of a call share must have as many keys in
+ * each. */
+size_t pkv_key_bounds_bytes(const pkv_pool* pool);
+int pkv_key_bounds(pkv_pool* pool, int layer, void* bounds, const int32_t* block_tables,
+                   int max_blocks_per_seq, const int32_t* first_positions,
+                   const int32_t* context_lens, int n_seqs, int max_new_len, void* stream);
+
+/* The blocks that each query row attends, per kv head: the first first_blocks
+ * and the last last_blocks of its context and, of those between, the ones with
+ * the largest
+ *     max over the group's heads h of  sum_d max(q_hd lo_d, q_hd hi_d),
+ * an upper bound of q_h . k over the block's keys, top_blocks in all.  Exact: the
+ * sums are compared as 64-bit ones, the lower index wins among equals.  A
+ * context of at most top_blocks blocks is taken whole.
+ *  q: [total_q][n_head][head_dim], pool dtype, as the attention will get it.
+ *  cu_q_lens: int32 [n_seqs + 1], or NULL for one row per sequence (total_q ==
+ *      n_seqs); context_lens: int32 [n_seqs].  As in pkv_prefill_attention row i of
+ *      sequence s is at position context_lens[s] - q_len_s + i and has the keys
+ *      up to that position; a row without keys gets no block.
+ *  blocks: int32 [total_q][n_kv_head][top_blocks], indexes into the sequence's
+ *      row of block_tables, ascending, then -1.  Rows of no sequence are left
+ *      as they were.
+ *  max_q_len, max_context_len: host upper bounds, 1 .. 2^30 (longer rows are
+ *      left out, longer contexts cut off; pkv_pool_check() reports both).
+ *  first_blocks >= 0, last_blocks >= 1, first_blocks + last_blocks <= top_blocks.
+ * Only the bounds of blocks between the first and last ones are used, which are
+ * full: the block that a step writes to needs none.  A block with a key that is
+ * not finite, one whose products' magnitudes add up past the f32 range, and any block for a query
+ * that is not finite rank first.  Block ids outside the pool are reported by
+ * pkv_pool_check(). */
+size_t pkv_select_workspace_bytes(const pkv_pool* pool, int n_seqs, int total_q, int max_q_len,
+                                  int max_context_len, int max_blocks_per_seq, int n_head);
+int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t* blocks,
+                      int top_blocks, int first_blocks, int last_blocks,
+                      const int32_t* cu_q_lens, const int32_t* context_lens,
+                      const int32_t* block_tables, int max_blocks_per_seq, int n_seqs,
+                      int total_q, int max_q_len, int max_context_len, int n_head,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of each query row over the keys of its listed blocks:
+ * out_h = sum_k softmax_k(scale q_h . k) v_k, k over the keys of the row's context
+ * that lie in blocks[row][kv head of h], f32 accumulation and softmax.  With every
+ * block listed it is pkv_decode_attention (NULL cu_q_lens) or
+ * pkv_prefill_attention, to rounding.
+ *  q, out, out_dtype, scale (not NaN): as pkv_decode_attention; rows, cu_q_lens,
+ *      context_lens and block_tables as pkv_select_blocks.
+ *  blocks: int32 [total_q][n_kv_head][top_blocks], distinct indexes in any order;
+ *      negative entries are skipped.  An index past the row's context or a
+ *      block id outside the pool is skipped and reported by pkv_pool_check().
+ *      A row and kv head without any key is zero.
+ * total_q, n_kv_head and parts (top_blocks * block_size / 64 at most) multiply to
+ * less than 2^26 (else PKV_ERR_UNSUPPORTED). */
+size_t pkv_sparse_workspace_bytes(const pkv_pool* pool, int total_q, int n_head, int top_blocks);
+int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, int out_dtype,
+                         const int32_t* blocks, int top_blocks, const int32_t* cu_q_lens,
+                         const int32_t* context_lens, const int32_t* block_tables,
+                         int max_blocks_per_seq, int n_seqs, int total_q, int max_q_len,
+                         int n_head, float scale, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Verification of drafted tokens against the target's probabilities, from
+ * given random numbers.  Request b has n = cu_drafts[b + 1] - cu_drafts[b] drafts d_i
+ * and n + 1 target rows, rows cu_drafts[b] + b + i of target_logits; its draft rows
+ * are cu_drafts[b] + i of draft_logits.  With p_i = softmax(target row i / T) and
+ * q_i = softmax(draft row i / T), T = temperatures[b]:
+ *   draft i is kept while uniforms[cu_drafts[b] + i] * q_i(d_i) < p_i(d_i);
+ *   at the first that is not, the next token comes from max(p_i - q_i, 0), after
+ *   the last draft from p_n: the first token at which the running sum of these
+ *   weights passes final_uniforms[b] times their total.
+ * draft_logits NULL: q_i is 1 at d_i (drafts that were looked up or searched).
+ * T == 0, or temperatures NULL: greedy; a draft is kept while it is the target
+ * row's first maximum, and the next token is a row's first maximum.  Decisions are
+ * those of 64-bit arithmetic.  A distribution cut by top-k or top-p is given
+ * by its log-probabilities with -inf elsewhere, at temperature 1.
+ *  logits: rows of `vocab` values at a stride of row_stride elements, each side
+ *      PKV_F32, PKV_F16 or PKV_BF16.  -inf has probability 0, and so has NaN; +inf
+ *      takes all of it.  A target row with nothing above -inf keeps no draft
+ *      and ends with token 0.
+ *  draft_tokens: int32 [total_drafts]; one outside [0, vocab) is not kept.
+ *  cu_drafts: int32 [batch + 1], from 0 to total_drafts (a host value), nondecreasing.
+ *  uniforms: f32 [total_drafts], final_uniforms: f32 [batch], in [0, 1); not read for
+ *      greedy requests, nor the draft rows.  temperatures: f32 [batch].
+ *  out_tokens: int32 [total_drafts + batch], at cu_drafts[b] + b the request's kept
+ *      drafts, its next token, then -1.  n_accepted: int32 [batch], kept drafts.
+ * vocab 1 .. 2^24 - 1.  Runs on the calling thread's current device. */
+size_t pkv_verify_workspace_bytes(int batch, int total_drafts, int vocab, int has_draft_logits);
+int pkv_verify_drafts(const void* target_logits, int target_dtype, long long target_row_stride,
+                      const void* draft_logits, int draft_dtype, long long draft_row_stride,
+                      const int32_t* draft_tokens, const int32_t* cu_drafts, int batch,
+                      int total_drafts, int vocab, const float* uniforms,
+                      const float* final_uniforms, const float* temperatures,
+                      int32_t* out_tokens, int32_t* n_accepted, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Kernel timing (instrumentation; no reference counterpart).  While enabled,
  * every pkv_decode_attention, pkv_prefill_attention, pkv_copy_blocks and
  * pkv_compact call records HIP events, owned by the pool, on its stream right
