@@ -11,13 +11,16 @@
 //
 // Every decision is that of 64-bit arithmetic: exponentials, sums and
 // comparisons are doubles.  On this GPU a double multiply-add issues at the
-// rate of a float one, and 2^x for x <= 0 is range reduction by rounding and
-// the Taylor polynomial of e^z (|z| <= ln 2 / 2, degree 12, error 2e-16),
-// some 20 operations an element against 2 or 4 bytes read.
+// rate of a float one, so 2^x for x <= 0 is kept to such operations: x is
+// split into an integer n and z in [-1/2, 1/2] by adding and subtracting
+// 1.5 2^52, 2^z is the Taylor polynomial of degree 11 (error 6e-15 relative),
+// and n is added to the exponent field; about 20 operations an element
+// against 2 or 4 bytes read.
 //
-// Three launches: statistics of every row (maximum, sum, argmax) in G chunks;
-// per request the kept drafts, and the last row's weights summed in chunks;
-// the token, found in the chunk in which the running sum passes.
+// Three launches: statistics of every row (maximum, sum, argmax) in chunks;
+// per request the kept drafts and the last row's weights, summed in segments
+// of 512 tokens (a wave's load); the segment in which the running sum passes
+// and the token in it.
 #include <algorithm>
 
 #include "pkv_device.h"
@@ -34,9 +37,7 @@ struct RowPart {  // of one chunk of a row
   int arg;        // its first index
   double s;       // sum of 2^((l - m) c)
 };
-struct WeightPart {
-  double left, p;  // sums of max(p - q, 0) and of p
-};
+constexpr int kSeg = 512;  // tokens of a segment: 8 per lane of a wave
 struct Decision {
   double inv_p, inv_q;  // 1 / sum of the target and the draft row (0: none)
   float m_p, m_q;
@@ -59,46 +60,55 @@ struct VerifyKArgs {
   const float* u_last;
   const float* temps;  // or null: greedy
   int batch, total, vocab;
-  int g1, g2;  // chunks of the statistics and of the weights
-  int len1, len2;
+  int g1, len1;  // chunks of the statistics
+  int g2, segs;  // workgroups and segments of the weights
   RowPart* rows;      // [total + batch target rows, total draft rows][g1]
-  WeightPart* parts;  // [batch][g2]
+  double* parts;      // [batch][segs]
   Decision* decide;   // [batch]
   int32_t* out;       // [total + batch]
   int32_t* accepted;  // [batch]
 };
 
-// 2^t for t <= 0.
+// 2^t for t in [-1000, 0].
 __device__ __forceinline__ double exp2_neg(double t) {
-  const double n = __builtin_rint(t);
-  const double z = (t - n) * 0.6931471805599453094;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, z, 1.0 / 39916800.0);
-  p = fma(p, z, 1.0 / 3628800.0);
-  p = fma(p, z, 1.0 / 362880.0);
-  p = fma(p, z, 1.0 / 40320.0);
-  p = fma(p, z, 1.0 / 5040.0);
-  p = fma(p, z, 1.0 / 720.0);
-  p = fma(p, z, 1.0 / 120.0);
-  p = fma(p, z, 1.0 / 24.0);
-  p = fma(p, z, 1.0 / 6.0);
-  p = fma(p, z, 0.5);
+  const double shift = 6755399441055744.0;  // 1.5 2^52: rounds t to an integer
+  const double r = t + shift;
+  const double z = t - (r - shift);
+  // (ln 2)^k / k!
+  double p = 4.4455382718708107e-10;
+  p = fma(p, z, 7.0549116208011234e-09);
+  p = fma(p, z, 1.0178086009239697e-07);
+  p = fma(p, z, 1.3215486790144309e-06);
+  p = fma(p, z, 1.5252733804059841e-05);
+  p = fma(p, z, 1.5403530393381610e-04);
+  p = fma(p, z, 1.3333558146428443e-03);
+  p = fma(p, z, 9.6181291076284772e-03);
+  p = fma(p, z, 5.5504108664821580e-02);
+  p = fma(p, z, 2.4022650695910071e-01);
+  p = fma(p, z, 6.9314718055994531e-01);
   p = fma(p, z, 1.0);
-  p = fma(p, z, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)fmax(n, -1200.0));
+  // r's low word is the integer; 2^-1000 is still a normal number
+  const unsigned hi = (unsigned)__double2hiint(p) + ((unsigned)__double2loint(r) << 20);
+  return __hiloint2double((int)hi, __double2loint(p));
 }
-// Weight of a logit under the row's maximum; NaN and -inf weigh nothing.
+// Weight of a logit (as kept() gives it) under the row's maximum; less than
+// 2^-1000 of the maximum's is 0.
 __device__ __forceinline__ double weight(float l, float m, double c) {
-  if (!(l > -INFINITY)) return 0.0;
-  if (l == m) return 1.0;
-  return exp2_neg(fmax(((double)l - (double)m) * c, -1200.0));
+  const double t = ((double)l - (double)m) * c;
+  const double w = exp2_neg(fmax(t, -1000.0));
+  return t > -1000.0 ? w : 0.0;  // (false for NaN: -inf against -inf)
+}
+// NaN as -inf, +inf as the largest float: the maximum and all that equal it
+// weigh 1, the others nothing.
+__device__ __forceinline__ float kept(float l) {
+  return l > -INFINITY ? fminf(l, 3.402823466e+38f) : -INFINITY;
 }
 
 template <int DT>
 __device__ __forceinline__ float logit(const char* row, long long i) {
-  if constexpr (DT == PKV_F32) return reinterpret_cast<const float*>(row)[i];
+  if constexpr (DT == PKV_F32) return kept(reinterpret_cast<const float*>(row)[i]);
   const uint16_t w = reinterpret_cast<const uint16_t*>(row)[i];
-  return DT == PKV_BF16 ? bf16lo(w) : f16lo(w);
+  return kept(DT == PKV_BF16 ? bf16lo(w) : f16lo(w));
 }
 __device__ __forceinline__ float logit_dt(int dt, const char* row, long long i) {
   return dt == PKV_F32 ? logit<PKV_F32>(row, i)
@@ -137,7 +147,7 @@ constexpr Stat kNoStat{-INFINITY, 0, 0.0};
 __device__ __forceinline__ void join(Stat& x, const Stat& y, double c) {
   const float m = fmaxf(x.m, y.m);
   if (y.m > x.m || (y.m == x.m && y.arg < x.arg)) x.arg = y.arg;
-  if (c != 0.0 && m > -INFINITY) x.s = x.s * weight(x.m, m, c) + y.s * weight(y.m, m, c);
+  if (c != 0.0) x.s = x.s * weight(x.m, m, c) + y.s * weight(y.m, m, c);
   x.m = m;
 }
 
@@ -159,6 +169,8 @@ __device__ __forceinline__ void load8(const char* row, int i, int n, float (&x)[
     } else {
       widen16<DT, 8>(ld16(row + (size_t)i * 2), x);
     }
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x[e] = kept(x[e]);
     return;
   }
 #pragma unroll
@@ -304,11 +316,22 @@ __device__ Decision decide(const VerifyKArgs& a, int b, int& kept, int* lds) {
   return d;
 }
 
-// p and max(p - q, 0) of token i.
-__device__ __forceinline__ WeightPart weigh(const Decision& d, float lp, float lq, int i, double c) {
+// Weight of token i in the draw of the next token.
+__device__ __forceinline__ double weigh(const Decision& d, float lp, float lq, int i, double c) {
   const double p = weight(lp, d.m_p, c) * d.inv_p;
   const double q = d.draft >= 0 ? weight(lq, d.m_q, c) * d.inv_q : 0.0;
-  return {i == d.not_tok ? 0.0 : fmax(p - q, 0.0), p};
+  return i == d.not_tok ? 0.0 : fmax(p - q, 0.0);
+}
+// Those of tokens i .. i + 7, i a multiple of 8.
+template <int DT, int DDT, bool VEC>
+__device__ __forceinline__ void weigh8(const VerifyKArgs& a, const Decision& d, int i, double c,
+                                       double (&w)[kN]) {
+  float lp[kN], lq[kN];
+  load8<DT, VEC>(a.target + d.row * a.t_stride * bytes_of(DT), i, a.vocab, lp);
+  if (d.draft >= 0)
+    load8<DDT, VEC>(a.draft + d.draft * a.d_stride * bytes_of(DDT), i, a.vocab, lq);
+#pragma unroll
+  for (int e = 0; e < kN; ++e) w[e] = weigh(d, lp[e], d.draft >= 0 ? lq[e] : 0.0f, i + e, c);
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -316,140 +339,128 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// Grid batch x g2.
+// Grid batch x g2; a wave takes every (4 g2)-th segment.
 template <int DT, int DDT, bool VEC>
 __global__ void __launch_bounds__(kVT) verify_weight_kernel(VerifyKArgs a) {
   __shared__ int lds[kVW];
-  __shared__ WeightPart sum[kVW];
   const int b = blockIdx.x / a.g2, chunk = blockIdx.x % a.g2;
-  int kept = 0;
-  const Decision d = decide(a, b, kept, lds);
+  int n_kept = 0;
+  const Decision d = decide(a, b, n_kept, lds);
   if (chunk == 0) {
     const int d0 = first_draft(a, b), n = max(first_draft(a, b + 1) - d0, 0);
     if (threadIdx.x == 0) {
       a.decide[b] = d;
-      a.accepted[b] = kept;
+      a.accepted[b] = n_kept;
     }
     for (int i = threadIdx.x; i <= n; i += kVT)
-      a.out[d0 + b + i] = i < kept ? a.tokens[d0 + i] : i == kept ? max(d.token, 0) : -1;
+      a.out[d0 + b + i] = i < n_kept ? a.tokens[d0 + i] : i == n_kept ? max(d.token, 0) : -1;
   }
   if (d.token >= 0) return;
   const double c = exponent(a, b);
-  const char* tr = a.target + d.row * a.t_stride * bytes_of(DT);
-  const char* dr = d.draft >= 0 ? a.draft + d.draft * a.d_stride * bytes_of(DDT) : nullptr;
-  const int c0 = chunk * a.len2, c1 = min(c0 + a.len2, a.vocab);
-  WeightPart w{0.0, 0.0};
-  for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
-    float lp[kN], lq[kN];
-    load8<DT, VEC>(tr, i, c1, lp);
-    if (dr) load8<DDT, VEC>(dr, i, c1, lq);
+  const int lane = threadIdx.x & 63;
+  for (int k = chunk * kVW + (int)(threadIdx.x >> 6); k < a.segs; k += a.g2 * kVW) {
+    double w[kN], x = 0.0;
+    weigh8<DT, DDT, VEC>(a, d, k * kSeg + lane * kN, c, w);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const WeightPart x = weigh(d, lp[e], dr ? lq[e] : 0.0f, i + e, c);
-      w.left += x.left;
-      w.p += x.p;
-    }
-  }
-  w.left = wave_sum(w.left);
-  w.p = wave_sum(w.p);
-  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = w;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < kVW; ++k) {
-      w.left += sum[k].left;
-      w.p += sum[k].p;
-    }
-    a.parts[(size_t)b * a.g2 + chunk] = w;
+    for (int e = 0; e < kN; ++e) x += w[e];
+    x = wave_sum(x);
+    if (lane == 0) a.parts[(size_t)b * a.segs + k] = x;
   }
 }
 
-// Grid batch: the chunk in which the running sum passes, then the token.
-template <int DT, int DDT>
-__global__ void __launch_bounds__(kVT) verify_token_kernel(VerifyKArgs a) {
-  __shared__ double sum[kVW];
-  __shared__ int found[kVW], last[kVW];
-  const int b = blockIdx.x;
-  const Decision d = a.decide[b];
+// Inclusive running sum over the wave's lanes.
+__device__ __forceinline__ double wave_scan(double x) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, kWave);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Where the running sum of x(0), x(1), .. x(n - 1) first passes `want` (the last
+// positive one if rounding leaves it short), and the sum before it; -1 if none
+// is positive.  One wave; x is called with an index below n.
+template <class X>
+__device__ int first_past(int n, double want, double& before, X x) {
+  const int lane = threadIdx.x & 63;
+  int last = -1;
+  double last_before = 0.0, run = before;
+  for (int k0 = 0; k0 < n; k0 += kWave) {
+    const double v = k0 + lane < n ? x(k0 + lane) : 0.0;
+    const double upto = run + wave_scan(v);
+    const unsigned long long pos = __ballot(v > 0.0);
+    const unsigned long long hit = __ballot(v > 0.0 && upto > want);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      before = __shfl(upto - v, l, kWave);
+      return k0 + l;
+    }
+    if (pos) {
+      const int l = 63 - __clzll((long long)pos);
+      last = k0 + l;
+      last_before = __shfl(upto - v, l, kWave);
+    }
+    run = __shfl(upto, 63, kWave);
+  }
+  before = last_before;
+  return last;
+}
+
+// Grid batch, one wave: the segment in which the running sum passes, then the
+// token in it.
+template <int DT, int DDT, bool VEC>
+__global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  Decision d = a.decide[b];
   if (d.token >= 0) return;
   const double c = exponent(a, b);
-  const WeightPart* parts = a.parts + (size_t)b * a.g2;
-  double total = 0.0, total_p = 0.0;
-  for (int k = 0; k < a.g2; ++k) {
-    total += parts[k].left;
-    total_p += parts[k].p;
+  double* parts = a.parts + (size_t)b * a.segs;
+  auto sum_parts = [&]() {
+    double x = 0.0;
+    for (int k = lane; k < a.segs; k += kWave) x += parts[k];
+    return wave_sum(x);
+  };
+  double total = sum_parts();
+  if (!(total > 0.0) && (d.draft >= 0 || d.not_tok >= 0)) {
+    // p <= q everywhere (only by rounding, or when all of p is on the draft):
+    // the draw is from p
+    d.draft = d.not_tok = -1;
+    for (int k = 0; k < a.segs; ++k) {
+      double w[kN], x = 0.0;
+      weigh8<DT, DDT, VEC>(a, d, k * kSeg + lane * kN, c, w);
+      for (int e = 0; e < kN; ++e) x += w[e];
+      x = wave_sum(x);
+      if (lane == 0) parts[k] = x;
+    }
+    __threadfence_block();
+    __syncthreads();
+    total = sum_parts();
   }
-  const bool res = total > 0.0;  // else p itself (p <= q all over, by rounding only)
-  if (!res) total = total_p;
   const double want = (double)a.u_last[b] * total;
   double before = 0.0;
-  int at = -1;
-  double at_before = 0.0;
-  for (int k = 0; k < a.g2; ++k) {
-    const double x = res ? parts[k].left : parts[k].p;
-    if (x > 0.0) {  // the last chunk with weight, unless one passes before
-      at = k;
-      at_before = before;
-      if (before + x > want) break;
-    }
-    before += x;
-  }
-  if (at < 0) {
-    if (threadIdx.x == 0) a.out[d.at] = 0;
-    return;
-  }
-  const char* tr = a.target + d.row * a.t_stride * bytes_of(DT);
-  const char* dr = d.draft >= 0 ? a.draft + d.draft * a.d_stride * bytes_of(DDT) : nullptr;
-  const int c0 = at * a.len2, c1 = min(c0 + a.len2, a.vocab);
-  // consecutive elements per thread
-  const int per = (c1 - c0 + kVT - 1) / kVT;
-  const int i0 = min(c0 + (int)threadIdx.x * per, c1), i1 = min(i0 + per, c1);
-  auto w = [&](int i) {
-    const WeightPart x = weigh(d, logit<DT>(tr, i), dr ? logit<DDT>(dr, i) : 0.0f, i, c);
-    return res ? x.left : x.p;
-  };
-  double mine = 0.0;
-  int final = -1;  // the thread's last token with weight
-  for (int i = i0; i < i1; ++i) {
-    const double x = w(i);
-    mine += x;
-    if (x > 0.0) final = i;
-  }
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  double incl = mine;
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(incl, o, kWave);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 63) sum[wv] = incl;
-  __syncthreads();
-  double run = at_before + incl - mine;
-  for (int k = 0; k < wv; ++k) run += sum[k];
-  int pick = INT32_MAX;
-  if (run + mine > want) {
-    for (int i = i0; i < i1; ++i) {
-      const double x = w(i);
-      run += x;
-      if (x > 0.0 && run > want) {
-        pick = i;
-        break;
-      }
+  const int seg = first_past(a.segs, want, before, [&](int k) { return parts[k]; });
+  if (seg < 0) return;  // (token 0 is there)
+  double w[kN], x = 0.0;
+  weigh8<DT, DDT, VEC>(a, d, seg * kSeg + lane * kN, c, w);
+#pragma unroll
+  for (int e = 0; e < kN; ++e) x += w[e];
+  const int l = first_past(kWave, want, before, [&](int) { return x; });
+  if (lane != l) return;
+  int pick = 0;
+#pragma unroll
+  for (int e = 0; e < kN; ++e)
+    if (w[e] > 0.0) pick = e;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < kN; ++e) {
+    before += w[e];
+    if (!done && w[e] > 0.0 && before > want) {
+      pick = e;
+      done = true;
     }
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    pick = min(pick, __shfl_xor(pick, o, kWave));
-    final = max(final, __shfl_xor(final, o, kWave));
-  }
-  if (lane == 0) {
-    found[wv] = pick;
-    last[wv] = final;
-  }
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int k = 1; k < kVW; ++k) {
-    pick = min(pick, found[k]);
-    final = max(final, last[k]);
-  }
-  a.out[d.at] = pick != INT32_MAX ? pick : final;
+  a.out[d.at] = seg * kSeg + lane * kN + pick;
 }
 
 template <int DT, int DDT>
@@ -458,11 +469,12 @@ hipError_t launch_dt(const VerifyKArgs& a, bool vec, int rows, hipStream_t s) {
   if (vec) {
     verify_stat_kernel<DT, DDT, true><<<g1, kVT, 0, s>>>(a);
     verify_weight_kernel<DT, DDT, true><<<g2, kVT, 0, s>>>(a);
+    if (a.temps) verify_token_kernel<DT, DDT, true><<<a.batch, kWave, 0, s>>>(a);
   } else {
     verify_stat_kernel<DT, DDT, false><<<g1, kVT, 0, s>>>(a);
     verify_weight_kernel<DT, DDT, false><<<g2, kVT, 0, s>>>(a);
+    if (a.temps) verify_token_kernel<DT, DDT, false><<<a.batch, kWave, 0, s>>>(a);
   }
-  if (a.temps) verify_token_kernel<DT, DDT><<<a.batch, kVT, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -476,27 +488,24 @@ hipError_t launch_ddt(int ddt, const VerifyKArgs& a, bool vec, int rows, hipStre
 }
 
 struct VerifyPlan {
-  int rows, g1, len1, g2, len2;
+  int rows, g1, len1, g2, segs;
   size_t parts, decide, bytes;
 };
 
-// Chunks of a row: as many as give about 1024 workgroups, of 4096 elements or
-// more, a multiple of 8 long.
-void chunks(long long rows, int vocab, int& g, int& len) {
-  const int most = std::max(1, vocab / 4096);
-  g = (int)std::max<long long>(1, std::min<long long>(1024 / std::max<long long>(rows, 1), most));
-  len = ((vocab + g - 1) / g + 7) / 8 * 8;
-  g = std::max(1, (vocab + len - 1) / len);
-}
-
+// Rows are cut into as many chunks as give about 1024 workgroups, of 4096
+// elements or more, a multiple of 8 long; the last rows into as many workgroups,
+// a segment or more for each wave.
 VerifyPlan verify_plan(const VerifyArgs& a) {
   VerifyPlan p{};
   p.rows = a.total_drafts + a.batch + (a.has_draft ? a.total_drafts : 0);
-  chunks(p.rows, a.vocab, p.g1, p.len1);
-  chunks(a.batch, a.vocab, p.g2, p.len2);
+  const int g = std::max(1, std::min(1024 / p.rows, a.vocab / 4096));
+  p.len1 = ((a.vocab + g - 1) / g + 7) / 8 * 8;
+  p.g1 = (a.vocab + p.len1 - 1) / p.len1;
+  p.segs = (a.vocab + kSeg - 1) / kSeg;
+  p.g2 = std::max(1, std::min(1024 / a.batch, (p.segs + kVW - 1) / kVW));
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   p.parts = up((size_t)p.rows * p.g1 * sizeof(RowPart));
-  p.decide = p.parts + up((size_t)a.batch * p.g2 * sizeof(WeightPart));
+  p.decide = p.parts + up((size_t)a.batch * p.segs * sizeof(double));
   p.bytes = p.decide + up((size_t)a.batch * sizeof(Decision));
   return p;
 }
@@ -527,11 +536,11 @@ hipError_t launch_verify(const VerifyArgs& a, char* ws, hipStream_t stream) {
   k.total = a.total_drafts;
   k.vocab = a.vocab;
   k.g1 = pl.g1;
-  k.g2 = pl.g2;
   k.len1 = pl.len1;
-  k.len2 = pl.len2;
+  k.g2 = pl.g2;
+  k.segs = pl.segs;
   k.rows = reinterpret_cast<RowPart*>(ws);
-  k.parts = reinterpret_cast<WeightPart*>(ws + pl.parts);
+  k.parts = reinterpret_cast<double*>(ws + pl.parts);
   k.decide = reinterpret_cast<Decision*>(ws + pl.decide);
   k.out = a.out_tokens;
   k.accepted = a.n_accepted;
