@@ -11,16 +11,19 @@
 //
 // Every decision is that of 64-bit arithmetic: exponentials, sums and
 // comparisons are doubles.  On this GPU a double multiply-add issues at the
-// rate of a float one, so 2^x for x <= 0 is kept to such operations: x is
-// split into an integer n and z in [-1/2, 1/2] by adding and subtracting
-// 1.5 2^52, 2^z is the Taylor polynomial of degree 11 (error 6e-15 relative),
-// and n is added to the exponent field; about 20 operations an element
-// against 2 or 4 bytes read.
+// rate of a float one, so 2^x is kept to such operations: x is split into an
+// integer n and z in [-1/2, 1/2] by adding and subtracting 1.5 2^52, 2^z is a
+// polynomial of degree 10 (interpolated at the Chebyshev nodes, error 3e-16
+// relative), and n is added to the exponent field: 17 operations an element
+// against 2 or 4 bytes read.  A sum needs no maximum, only a reference near
+// the row's size, for a double holds 2^500 times its weight as well: a thread
+// keeps the largest logit of its first group and moves it only when a logit
+// is past that range.
 //
-// Three launches: statistics of every row (maximum, sum, argmax) in chunks;
-// per request the kept drafts and the last row's weights, summed in segments
-// of 512 tokens (a wave's load); the segment in which the running sum passes
-// and the token in it.
+// Three launches: statistics of every row (reference and sum, or the argmax of
+// greedy rows) in chunks; per request the kept drafts and the last row's
+// weights, summed in segments of 512 tokens (a wave's load); the segment in
+// which the running sum passes and the token in it.
 #include <algorithm>
 
 #include "pkv_device.h"
@@ -33,8 +36,8 @@ constexpr int kVT = 256;  // threads
 constexpr int kVW = kVT / kWave;
 
 struct RowPart {  // of one chunk of a row
-  float m;        // largest logit (NaN aside)
-  int arg;        // its first index
+  float m;        // a logit near its largest (greedy: the largest)
+  int arg;        // greedy: its first index
   double s;       // sum of 2^((l - m) c)
 };
 constexpr int kSeg = 512;  // tokens of a segment: 8 per lane of a wave
@@ -69,46 +72,73 @@ struct VerifyKArgs {
   int32_t* accepted;  // [batch]
 };
 
-// 2^t for t in [-1000, 0].
-__device__ __forceinline__ double exp2_neg(double t) {
+// 2^t for |t| <= 1000.
+__device__ __forceinline__ double exp2_near(double t) {
   const double shift = 6755399441055744.0;  // 1.5 2^52: rounds t to an integer
   const double r = t + shift;
   const double z = t - (r - shift);
-  // (ln 2)^k / k!
-  double p = 4.4455382718708107e-10;
-  p = fma(p, z, 7.0549116208011234e-09);
-  p = fma(p, z, 1.0178086009239697e-07);
-  p = fma(p, z, 1.3215486790144309e-06);
-  p = fma(p, z, 1.5252733804059841e-05);
-  p = fma(p, z, 1.5403530393381610e-04);
-  p = fma(p, z, 1.3333558146428443e-03);
-  p = fma(p, z, 9.6181291076284772e-03);
-  p = fma(p, z, 5.5504108664821580e-02);
-  p = fma(p, z, 2.4022650695910071e-01);
-  p = fma(p, z, 6.9314718055994531e-01);
+  double p = 7.072585949269223e-09;
+  p = fma(p, z, 1.0208690299958306e-07);
+  p = fma(p, z, 1.321544258792169e-06);
+  p = fma(p, z, 1.5252657260200837e-05);
+  p = fma(p, z, 0.0001540353044173605);
+  p = fma(p, z, 0.0013333558230164974);
+  p = fma(p, z, 0.009618129107606888);
+  p = fma(p, z, 0.05550410866444772);
+  p = fma(p, z, 0.24022650695910097);
+  p = fma(p, z, 0.69314718055995);
   p = fma(p, z, 1.0);
-  // r's low word is the integer; 2^-1000 is still a normal number
+  // r's low word is the integer
   const unsigned hi = (unsigned)__double2hiint(p) + ((unsigned)__double2loint(r) << 20);
   return __hiloint2double((int)hi, __double2loint(p));
-}
-// Weight of a logit (as kept() gives it) under the row's maximum; less than
-// 2^-1000 of the maximum's is 0.
-__device__ __forceinline__ double weight(float l, float m, double c) {
-  const double t = ((double)l - (double)m) * c;
-  const double w = exp2_neg(fmax(t, -1000.0));
-  return t > -1000.0 ? w : 0.0;  // (false for NaN: -inf against -inf)
 }
 // NaN as -inf, +inf as the largest float: the maximum and all that equal it
 // weigh 1, the others nothing.
 __device__ __forceinline__ float kept(float l) {
   return l > -INFINITY ? fminf(l, 3.402823466e+38f) : -INFINITY;
 }
+// Weight 2^((l - m) c) of a logit against reference m, at most 2^500; less
+// than 2^-1000 is 0.
+__device__ __forceinline__ double weight(float l, float m, double c) {
+  const double t = ((double)kept(l) - (double)m) * c;
+  const double w = exp2_near(fmin(fmax(t, -1000.0), 1000.0));
+  return t > -1000.0 ? w : 0.0;  // (false for NaN: -inf against -inf)
+}
+
+// A row's reference and the logits around it that need no care: [lo, hi].
+struct Ref {
+  float m, lo, hi;
+  double c, mc;
+};
+__device__ __forceinline__ void set_ref(Ref& r, float m) {
+  const float span = fminf((float)(500.0 / r.c), 1e38f);
+  r.m = m;
+  r.lo = m - span;
+  r.hi = m + span;
+  r.mc = -(double)m * r.c;
+}
+// Whether eight logits are all in the range of r (and none is NaN), and their
+// largest (NaN aside).
+__device__ __forceinline__ bool in_range(const float (&x)[8], const Ref& r, float& top) {
+  float lo = fminf(fminf(x[0], x[1]), x[2]), sum = x[0];
+  top = fmaxf(fmaxf(x[0], x[1]), x[2]);
+  lo = fminf(fminf(lo, x[3]), x[4]);
+  top = fmaxf(fmaxf(top, x[3]), x[4]);
+  lo = fminf(fminf(lo, x[5]), fminf(x[6], x[7]));
+  top = fmaxf(fmaxf(top, x[5]), fmaxf(x[6], x[7]));
+#pragma unroll
+  for (int e = 1; e < 8; ++e) sum += x[e];
+  return lo >= r.lo && top <= r.hi && sum == sum;
+}
+__device__ __forceinline__ double weight_in_range(float l, const Ref& r) {
+  return exp2_near(fma((double)l, r.c, r.mc));
+}
 
 template <int DT>
 __device__ __forceinline__ float logit(const char* row, long long i) {
-  if constexpr (DT == PKV_F32) return kept(reinterpret_cast<const float*>(row)[i]);
+  if constexpr (DT == PKV_F32) return reinterpret_cast<const float*>(row)[i];
   const uint16_t w = reinterpret_cast<const uint16_t*>(row)[i];
-  return kept(DT == PKV_BF16 ? bf16lo(w) : f16lo(w));
+  return DT == PKV_BF16 ? bf16lo(w) : f16lo(w);
 }
 __device__ __forceinline__ float logit_dt(int dt, const char* row, long long i) {
   return dt == PKV_F32 ? logit<PKV_F32>(row, i)
@@ -137,7 +167,7 @@ __device__ __forceinline__ int request_of(const VerifyKArgs& a, int x, int step)
   return n;
 }
 
-// A chunk's running maximum, its index, and the sum below it.
+// What RowPart holds, of a part of a row.
 struct Stat {
   float m;
   int arg;
@@ -169,8 +199,6 @@ __device__ __forceinline__ void load8(const char* row, int i, int n, float (&x)[
     } else {
       widen16<DT, 8>(ld16(row + (size_t)i * 2), x);
     }
-#pragma unroll
-    for (int e = 0; e < kN; ++e) x[e] = kept(x[e]);
     return;
   }
 #pragma unroll
@@ -179,28 +207,47 @@ __device__ __forceinline__ void load8(const char* row, int i, int n, float (&x)[
 
 // Statistics of elements c0 .. c1 - 1 by the workgroup; thread 0 has them.
 template <int DT, bool VEC>
-__device__ Stat chunk_stat(const char* row, int c0, int c1, double c, Stat* lds) {
+__device__ __forceinline__ Stat chunk_stat(const char* row, int c0, int c1, double c, Stat* lds) {
   Stat st = kNoStat;
-  for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
-    float x[kN];
-    load8<DT, VEC>(row, i, c1, x);
-    float gm = -INFINITY;
-    int ga = 0;
+  if (c == 0.0) {
+    for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
+      float x[kN];
+      load8<DT, VEC>(row, i, c1, x);
 #pragma unroll
-    for (int e = 0; e < kN; ++e)
-      if (x[e] > gm) {
-        gm = x[e];
-        ga = i + e;
+      for (int e = 0; e < kN; ++e)
+        if (x[e] > st.m) {
+          st.m = x[e];
+          st.arg = i + e;
+        }
+    }
+  } else {
+    Ref r;
+    r.c = c;
+    r.m = r.hi = -INFINITY;
+    r.lo = INFINITY;
+    r.mc = 0.0;
+    double sum = 0.0;
+    for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
+      float x[kN], top;
+      load8<DT, VEC>(row, i, c1, x);
+      if (!in_range(x, r, top)) {
+        top = kept(top);
+        if (top > r.hi) {  // the first group, or a logit far above the reference
+          sum *= weight(r.m, top, c);
+          set_ref(r, top);
+        }
+        if (!(top >= r.lo)) continue;  // nothing above 2^-500 of the reference
+        if (!in_range(x, r, top)) {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) sum += weight(x[e], r.m, c);
+          continue;
+        }
       }
-    if (gm > st.m) {
-      if (c != 0.0) st.s *= weight(st.m, gm, c);
-      st.m = gm;
-      st.arg = ga;
-    }
-    if (c != 0.0) {
 #pragma unroll
-      for (int e = 0; e < kN; ++e) st.s += weight(x[e], st.m, c);
+      for (int e = 0; e < kN; ++e) sum += weight_in_range(x[e], r);
     }
+    st.m = r.m;
+    st.s = sum;
   }
   for (int o = 1; o < 64; o <<= 1) {
     Stat y;
@@ -316,22 +363,49 @@ __device__ Decision decide(const VerifyKArgs& a, int b, int& kept, int* lds) {
   return d;
 }
 
-// Weight of token i in the draw of the next token.
-__device__ __forceinline__ double weigh(const Decision& d, float lp, float lq, int i, double c) {
-  const double p = weight(lp, d.m_p, c) * d.inv_p;
-  const double q = d.draft >= 0 ? weight(lq, d.m_q, c) * d.inv_q : 0.0;
-  return i == d.not_tok ? 0.0 : fmax(p - q, 0.0);
+// Probabilities of eight logits.
+__device__ __forceinline__ void probs8(const float (&x)[kN], const Ref& r, double inv, double (&p)[kN]) {
+  float top;
+  if (in_range(x, r, top)) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) p[e] = weight_in_range(x[e], r) * inv;
+  } else {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) p[e] = weight(x[e], r.m, r.c) * inv;
+  }
 }
-// Those of tokens i .. i + 7, i a multiple of 8.
+// What the next token of a request is drawn from.
+struct Draw {
+  Ref p, q;
+};
+__device__ __forceinline__ Draw draw_of(const Decision& d, double c) {
+  Draw w;
+  w.p.c = w.q.c = c;
+  set_ref(w.p, d.m_p);
+  set_ref(w.q, d.m_q);
+  return w;
+}
+// Weights of tokens i .. i + 7, i a multiple of 8.
 template <int DT, int DDT, bool VEC>
-__device__ __forceinline__ void weigh8(const VerifyKArgs& a, const Decision& d, int i, double c,
+__device__ __forceinline__ void weigh8(const VerifyKArgs& a, const Decision& d, const Draw& r, int i,
                                        double (&w)[kN]) {
   float lp[kN], lq[kN];
   load8<DT, VEC>(a.target + d.row * a.t_stride * bytes_of(DT), i, a.vocab, lp);
-  if (d.draft >= 0)
+  if (d.draft >= 0) {
     load8<DDT, VEC>(a.draft + d.draft * a.d_stride * bytes_of(DDT), i, a.vocab, lq);
+    double q[kN];
+    probs8(lq, r.q, d.inv_q, q);
+    probs8(lp, r.p, d.inv_p, w);
 #pragma unroll
-  for (int e = 0; e < kN; ++e) w[e] = weigh(d, lp[e], d.draft >= 0 ? lq[e] : 0.0f, i + e, c);
+    for (int e = 0; e < kN; ++e) w[e] = fmax(w[e] - q[e], 0.0);
+  } else {
+    probs8(lp, r.p, d.inv_p, w);
+    if ((unsigned)(d.not_tok - i) < (unsigned)kN) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (i + e == d.not_tok) w[e] = 0.0;
+    }
+  }
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -356,11 +430,11 @@ __global__ void __launch_bounds__(kVT) verify_weight_kernel(VerifyKArgs a) {
       a.out[d0 + b + i] = i < n_kept ? a.tokens[d0 + i] : i == n_kept ? max(d.token, 0) : -1;
   }
   if (d.token >= 0) return;
-  const double c = exponent(a, b);
+  const Draw r = draw_of(d, exponent(a, b));
   const int lane = threadIdx.x & 63;
   for (int k = chunk * kVW + (int)(threadIdx.x >> 6); k < a.segs; k += a.g2 * kVW) {
     double w[kN], x = 0.0;
-    weigh8<DT, DDT, VEC>(a, d, k * kSeg + lane * kN, c, w);
+    weigh8<DT, DDT, VEC>(a, d, r, k * kSeg + lane * kN, w);
 #pragma unroll
     for (int e = 0; e < kN; ++e) x += w[e];
     x = wave_sum(x);
@@ -414,7 +488,7 @@ __global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
   const int b = blockIdx.x, lane = threadIdx.x;
   Decision d = a.decide[b];
   if (d.token >= 0) return;
-  const double c = exponent(a, b);
+  const Draw r = draw_of(d, exponent(a, b));
   double* parts = a.parts + (size_t)b * a.segs;
   auto sum_parts = [&]() {
     double x = 0.0;
@@ -428,7 +502,7 @@ __global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
     d.draft = d.not_tok = -1;
     for (int k = 0; k < a.segs; ++k) {
       double w[kN], x = 0.0;
-      weigh8<DT, DDT, VEC>(a, d, k * kSeg + lane * kN, c, w);
+      weigh8<DT, DDT, VEC>(a, d, r, k * kSeg + lane * kN, w);
       for (int e = 0; e < kN; ++e) x += w[e];
       x = wave_sum(x);
       if (lane == 0) parts[k] = x;
@@ -442,7 +516,7 @@ __global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
   const int seg = first_past(a.segs, want, before, [&](int k) { return parts[k]; });
   if (seg < 0) return;  // (token 0 is there)
   double w[kN], x = 0.0;
-  weigh8<DT, DDT, VEC>(a, d, seg * kSeg + lane * kN, c, w);
+  weigh8<DT, DDT, VEC>(a, d, r, seg * kSeg + lane * kN, w);
 #pragma unroll
   for (int e = 0; e < kN; ++e) x += w[e];
   const int l = first_past(kWave, want, before, [&](int) { return x; });
@@ -492,13 +566,13 @@ struct VerifyPlan {
   size_t parts, decide, bytes;
 };
 
-// Rows are cut into as many chunks as give about 1024 workgroups, of 4096
+// Rows are cut into as many chunks as give about 4096 workgroups, of 4096
 // elements or more, a multiple of 8 long; the last rows into as many workgroups,
 // a segment or more for each wave.
 VerifyPlan verify_plan(const VerifyArgs& a) {
   VerifyPlan p{};
   p.rows = a.total_drafts + a.batch + (a.has_draft ? a.total_drafts : 0);
-  const int g = std::max(1, std::min(1024 / p.rows, a.vocab / 4096));
+  const int g = std::max(1, std::min(4096 / p.rows, a.vocab / 4096));
   p.len1 = ((a.vocab + g - 1) / g + 7) / 8 * 8;
   p.g1 = (a.vocab + p.len1 - 1) / p.len1;
   p.segs = (a.vocab + kSeg - 1) / kSeg;
