@@ -133,6 +133,20 @@ __device__ __forceinline__ bool in_range(const float (&x)[8], const Ref& r, floa
 __device__ __forceinline__ double weight_in_range(float l, const Ref& r) {
   return exp2_near(fma((double)l, r.c, r.mc));
 }
+// A term of a sum: logits below the range count as its lower end, 2^-500, those
+// above it as its upper end.  (One instruction; min and max of unpacked words
+// cost another each, to quiet NaN.)
+__device__ __forceinline__ double weight_clamped(float l, const Ref& r) {
+  float x;
+  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(l), "v"(r.lo), "v"(r.hi));
+  return weight_in_range(x, r);
+}
+__device__ __forceinline__ float largest(const float (&x)[8]) {
+  float top = kept(x[0]);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) top = fmaxf(top, kept(x[e]));
+  return top;
+}
 
 template <int DT>
 __device__ __forceinline__ float logit(const char* row, long long i) {
@@ -165,6 +179,11 @@ __device__ __forceinline__ int request_of(const VerifyKArgs& a, int x, int step)
     n += __popcll(__ballot(k < a.batch && first_draft(a, k) + step * k <= x));
   }
   return n;
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  return x;
 }
 
 // What RowPart holds, of a part of a row.
@@ -223,39 +242,55 @@ __device__ __forceinline__ Stat chunk_stat(const char* row, int c0, int c1, doub
   } else {
     Ref r;
     r.c = c;
-    r.m = r.hi = -INFINITY;
-    r.lo = INFINITY;
-    r.mc = 0.0;
-    double sum = 0.0;
-    for (int i = c0 + (int)threadIdx.x * kN; i < c1; i += kVT * kN) {
-      float x[kN], top;
+    const int step = kVT * kN;
+    float x[kN];
+    // the reference: the largest of the first group with anything in it
+    int i = c0 + (int)threadIdx.x * kN;
+    float top = -INFINITY;
+    for (; i < c1; i += step) {
       load8<DT, VEC>(row, i, c1, x);
-      if (!in_range(x, r, top)) {
-        top = kept(top);
-        if (top > r.hi) {  // the first group, or a logit far above the reference
+      top = largest(x);
+      if (top > -INFINITY) break;
+    }
+    set_ref(r, top);
+    double sum = 0.0;
+    while (i < c1) {
+      float y[kN];  // the next group, on its way
+      if (i + step < c1) load8<DT, VEC>(row, i + step, c1, y);
+      double g = 0.0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) g += weight_clamped(x[e], r);
+      if (g < 0x1p499) {
+        sum += g;
+      } else {  // a logit at the range's upper end, or NaN
+        top = largest(x);
+        if (top > r.hi) {
           sum *= weight(r.m, top, c);
           set_ref(r, top);
         }
-        if (!(top >= r.lo)) continue;  // nothing above 2^-500 of the reference
-        if (!in_range(x, r, top)) {
 #pragma unroll
-          for (int e = 0; e < kN; ++e) sum += weight(x[e], r.m, c);
-          continue;
-        }
+        for (int e = 0; e < kN; ++e) sum += weight(x[e], r.m, c);
       }
+      i += step;
 #pragma unroll
-      for (int e = 0; e < kN; ++e) sum += weight_in_range(x[e], r);
+      for (int e = 0; e < kN; ++e) x[e] = y[e];
     }
     st.m = r.m;
     st.s = sum;
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    Stat y;
-    y.m = __shfl_xor(st.m, o, kWave);
-    y.arg = __shfl_xor(st.arg, o, kWave);
-    y.s = __shfl_xor(st.s, o, kWave);
-    join(st, y, c);
+  // over the wave: the largest reference, and every sum against it once
+  float m = st.m;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+  if (c == 0.0) {
+    int arg = st.m == m ? st.arg : INT32_MAX;  // (0 where nothing is above -inf)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) arg = min(arg, __shfl_xor(arg, o, kWave));
+    st.arg = arg;
+  } else {
+    st.s = wave_sum(st.s * weight(st.m, m, c));
   }
+  st.m = m;
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = st;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -406,11 +441,6 @@ __device__ __forceinline__ void weigh8(const VerifyKArgs& a, const Decision& d, 
         if (i + e == d.not_tok) w[e] = 0.0;
     }
   }
-}
-
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
-  return x;
 }
 
 // Grid batch x g2; a wave takes every (4 g2)-th segment.
