@@ -258,21 +258,6 @@ __device__ __forceinline__ int clamp_ctx(const DecodeKArgs& a, int ctx, int BS) 
   return ctx < 0 ? 0 : min(ctx, min(a.max_context_len, a.mbps * BS));
 }
 
-// Inclusive prefix sum across the 64 lanes of a wave in lane order, on DPP:
-// shifts by 1, 2, 4 and 8 lanes within each 16-lane row (lanes shifted in
-// from outside the row add 0), then lane 15's sum broadcast into rows 1 and
-// 3 and lane 31's into rows 2 and 3 (no LDS round trips).
-__device__ __forceinline__ int wave_incl_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
-  return x;
-}
-
-
 // Keys row b attends: context_lens[b] (ctx_raw), bounded by positions[b] + 1
 // when positions are given -- build_mask's two bounds k < seq_lens[b] and
 // k <= q_positions[b] (attention.rs:22).  A negative position attends

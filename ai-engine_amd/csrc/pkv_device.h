@@ -110,6 +110,20 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
+// Inclusive prefix sum across the 64 lanes of a wave in lane order, on DPP:
+// shifts by 1, 2, 4 and 8 lanes within each 16-lane row (lanes shifted in
+// from outside the row add 0), then lane 15's sum broadcast into rows 1 and
+// 3 and lane 31's into rows 2 and 3 (no LDS round trips).
+__device__ __forceinline__ int wave_incl_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
 __device__ __forceinline__ float readlane_f(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }

@@ -330,7 +330,9 @@ __global__ void __launch_bounds__(256) score_kernel(SelectKArgs a) {
 // ---- choice ------------------------------------------------------------------
 
 constexpr int kSelThreads = 256;
+constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kSelLds = 8192;  // scores of a row kept in LDS
+constexpr int kNear = 64;      // blocks near the border ranked by one wave
 
 // Order-preserving integers: larger value, larger key; +inf the largest.
 __device__ __forceinline__ uint32_t key32(float x) {
@@ -347,102 +349,158 @@ __device__ __forceinline__ unsigned long long key64(double x) {
 
 struct SelSmem {
   float score[kSelLds];
-  int hist[256];
-  int part[kSelThreads / kWave];
-  unsigned long long bound[2][kSelThreads / kWave];
+  int hist[2][256];
+  int part[2][kSelWaves];
+  unsigned long long bound[2][kSelWaves];
+  float emax[kSelWaves];
   int digit, above;
+  int list[kNear];
+  double sum[kNear];
 };
 
-// Sum of x over the workgroup's threads before this one, and over all.
-__device__ __forceinline__ int wg_scan(int x, int* part, int& all) {
+// Sums of x and y over the workgroup's threads before this one, and over all.
+struct Scan {
+  int x, y, all_x, all_y;
+};
+__device__ __forceinline__ Scan wg_scan(int x, int y, SelSmem& sm) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int incl = x;
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o, kWave);
-    if (lane >= o) incl += y;
+  const int ix = wave_incl_scan(x), iy = wave_incl_scan(y);
+  __syncthreads();
+  if (lane == 63) {
+    sm.part[0][w] = ix;
+    sm.part[1][w] = iy;
   }
   __syncthreads();
-  if (lane == 63) part[w] = incl;
-  __syncthreads();
-  int before = 0;
-  all = 0;
+  Scan s{ix - x, iy - y, 0, 0};
 #pragma unroll
-  for (int i = 0; i < kSelThreads / kWave; ++i) {
-    if (i < w) before += part[i];
-    all += part[i];
+  for (int i = 0; i < kSelWaves; ++i) {
+    if (i < w) {
+      s.x += sm.part[0][i];
+      s.y += sm.part[1][i];
+    }
+    s.all_x += sm.part[0][i];
+    s.all_y += sm.part[1][i];
   }
-  return before + incl - x;
+  return s;
 }
 
-// The want-th largest key (1 <= want <= number of keys) of those that
-// get(i, key) admits, i < n, and how many are larger: digits of 8 bits from
-// the highest in which the keys differ.
-template <class Key, class Get>
-__device__ Key kth_largest(int n, int want, Get get, SelSmem& sm, int& larger) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  Key lo = ~(Key)0, hi = 0;
-  for (int i = tid; i < n; i += kSelThreads) {
-    Key k;
-    if (get(i, k)) {
-      lo = k < lo ? k : lo;
-      hi = k > hi ? k : hi;
-    }
-  }
-  unsigned long long l = lo, h = hi;
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned long long l2 = __shfl_xor(l, o, kWave), h2 = __shfl_xor(h, o, kWave);
+// The smallest and largest of the threads' l and h, in every thread; `em` as
+// well becomes the largest.  Ends with a barrier's worth of order: what was
+// stored to LDS before is visible after.
+template <class Key>
+__device__ __forceinline__ void wg_extremes(Key& l, Key& h, float& em, SelSmem& sm) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const Key l2 = __shfl_xor(l, o, kWave), h2 = __shfl_xor(h, o, kWave);
     l = l2 < l ? l2 : l;
     h = h2 > h ? h2 : h;
+    em = fmaxf(em, __shfl_xor(em, o, kWave));
   }
   __syncthreads();
   if (lane == 0) {
     sm.bound[0][w] = l;
     sm.bound[1][w] = h;
+    sm.emax[w] = em;
   }
   __syncthreads();
-  for (int i = 0; i < kSelThreads / kWave; ++i) {
-    l = sm.bound[0][i] < l ? sm.bound[0][i] : l;
-    h = sm.bound[1][i] > h ? sm.bound[1][i] : h;
+#pragma unroll
+  for (int i = 0; i < kSelWaves; ++i) {
+    l = sm.bound[0][i] < l ? (Key)sm.bound[0][i] : l;
+    h = sm.bound[1][i] > h ? (Key)sm.bound[1][i] : h;
+    em = fmaxf(em, sm.emax[i]);
   }
+}
+
+// The want-th largest key (1 <= want <= number of keys) of those that
+// get(i, key) admits, i < n, and how many are larger, given the smallest and
+// largest: digits of 8 bits from the highest in which the keys differ, two
+// barriers each.
+template <class Key, class Get>
+__device__ Key kth_largest(int n, int want, Key lo, Key hi, Get get, SelSmem& sm, int& larger) {
+  constexpr int kBits = (int)sizeof(Key) * 8;
+  const int tid = threadIdx.x, lane = tid & 63;
   larger = 0;
-  if (l == h) return (Key)h;
-  int bits = 64 - __clzll((long long)(l ^ h));  // the keys agree above these
-  Key prefix = bits >= (int)sizeof(Key) * 8 ? 0 : (Key)(h >> bits);
-  while (bits > 0) {
+  if (lo == hi) return hi;
+  int bits = 64 - __clzll((long long)((unsigned long long)lo ^ hi));  // the keys agree above these
+  Key prefix = bits >= kBits ? 0 : (Key)(hi >> bits);
+  sm.hist[0][tid] = 0;
+  __syncthreads();
+  for (int pass = 0; bits > 0; ++pass) {
+    int* hist = sm.hist[pass & 1];
     const int take = bits < 8 ? bits : 8;
     const int shift = bits - take;
-    sm.hist[tid] = 0;
-    __syncthreads();
+    sm.hist[~pass & 1][tid] = 0;  // the next pass's
     for (int i = tid; i < n; i += kSelThreads) {
       Key k;
-      if (get(i, k) && (bits >= (int)sizeof(Key) * 8 || (Key)(k >> bits) == prefix))
-        atomicAdd(&sm.hist[(int)((k >> shift) & ((1 << take) - 1))], 1);
+      if (get(i, k) && (bits >= kBits || (Key)(k >> bits) == prefix))
+        atomicAdd(&hist[(int)((k >> shift) & ((1 << take) - 1))], 1);
     }
     __syncthreads();
-    // from the largest digit down: the one in which the want-th key is
-    const int c = sm.hist[255 - tid];
-    int all;
-    const int before = wg_scan(c, sm.part, all);
-    if (before < want - larger && before + c >= want - larger) {
-      sm.digit = 255 - tid;
-      sm.above = before;
+    if (tid < kWave) {  // from the largest digit down, four a lane
+      int c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += c[j] = hist[255 - 4 * lane - j];
+      int before = wave_incl_scan(sum) - sum;
+      if (before < want - larger && before + sum >= want - larger) {
+        int j = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (j == i && before + c[i] < want - larger) {
+            before += c[i];
+            j = i + 1;
+          }
+        sm.digit = 255 - 4 * lane - j;
+        sm.above = before;
+      }
     }
     __syncthreads();
     larger += sm.above;
     prefix = (Key)(prefix << take) | (Key)sm.digit;
     bits = shift;
-    __syncthreads();
   }
   return prefix;
+}
+
+// The score of a block in 64 bits, by a wave: 16 lanes a query head, four heads
+// at a time, 16 bytes of a row per lane and step.  Every lane has the result.
+template <int DT, int HD>
+__device__ __forceinline__ double score64(const char* q, const char* bound, int heads) {
+  constexpr int EPL = DT == PKV_F32 ? 4 : 8;
+  constexpr int RB = HD * (DT == PKV_F32 ? 4 : 2);
+  const int lane = threadIdx.x & 63;
+  double best = -INFINITY;
+  for (int h0 = 0; h0 < heads; h0 += 4) {
+    const int h = min(h0 + (lane >> 4), heads - 1);
+    double t = 0.0;
+#pragma unroll
+    for (int o = (lane & 15) * 16; o < RB; o += 256) {
+      float x[EPL], lo[EPL], hi[EPL];
+      widen16<DT, EPL>(ld16(q + (size_t)h * RB + o), x);
+      widen16<DT, EPL>(ld16(bound + o), lo);
+      widen16<DT, EPL>(ld16(bound + RB + o), hi);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)
+        t = fma((double)x[e], (double)(x[e] > 0.0f ? hi[e] : lo[e]), t);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o, kWave);
+    best = t > best ? t : best;
+  }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    const double y = __shfl_xor(best, o, kWave);
+    best = y > best ? y : best;
+  }
+  return best;
 }
 
 // One workgroup per query row and kv head.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
-  constexpr int E = DT == PKV_F32 ? 4 : 2;
-  constexpr int RB = HD * E;
+  constexpr int RB = HD * (DT == PKV_F32 ? 4 : 2);
   __shared__ SelSmem sm;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = blockIdx.x % a.kvh;
   const int slot = blockIdx.x / a.kvh;  // (sequence, row of it)
   const int s = slot / a.max_q, i = slot % a.max_q;
@@ -468,23 +526,21 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
 
   const float* score = a.score + row * a.nb_max + a.n_first;
   const bool in_lds = n <= kSelLds;
-  if (in_lds)
-    for (int k = tid; k < n; k += kSelThreads) sm.score[k] = score[k];
+  uint32_t klo = ~0u, khi = 0;
+  for (int k = tid; k < n; k += kSelThreads) {
+    const float x = score[k];
+    if (in_lds) sm.score[k] = x;
+    klo = min(klo, key32(x));
+    khi = max(khi, key32(x));
+  }
   float em = 0.0f;
   for (int k = tid; k < a.chunks; k += kSelThreads) em = fmaxf(em, a.emax[row * a.chunks + k]);
-  for (int o = 1; o < 64; o <<= 1) em = fmaxf(em, shfl_xor_f(em, o));
-  __syncthreads();
-  if (lane == 0) sm.hist[tid >> 6] = __float_as_int(em);
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelThreads / kWave; ++w) em = fmaxf(em, __int_as_float(sm.hist[w]));
+  wg_extremes(klo, khi, em, sm);
   const double E2 = 2.0 * (HD + 16) * 0x1p-23 * (double)em;
   auto at = [&](int k) { return in_lds ? sm.score[k] : score[k]; };
-  __syncthreads();
-
   int larger = 0;
   const uint32_t tkey = kth_largest<uint32_t>(
-      n, want, [&](int k, uint32_t& key) { key = key32(at(k)); return true; }, sm, larger);
+      n, want, klo, khi, [&](int k, uint32_t& key) { key = key32(at(k)); return true; }, sm, larger);
   const float tau = unkey32(tkey);
   // 2: taken, 1: within the bound of the border, 0: not taken.  An infinite
   // score is what it is.
@@ -494,90 +550,116 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
     const double d = (double)x - (double)tau;
     return d > E2 ? 2 : d >= -E2 ? 1 : 0;
   };
+  // consecutive blocks per thread, so one scan gives every place in index order
+  const int per = (n + kSelThreads - 1) / kSelThreads;
+  const int k0 = min(tid * per, n), k1 = min(k0 + per, n);
   int n2 = 0, n1 = 0;
-  for (int k = tid; k < n; k += kSelThreads) {
+  for (int k = k0; k < k1; ++k) {
     const int c = cls(k);
     n2 += c == 2;
     n1 += c == 1;
   }
-  int sure, near;
-  wg_scan(n2, sm.part, sure);
-  wg_scan(n1, sm.part, near);
-  const int need = want - sure;  // of the near ones
-  // When not all of them are needed they are ranked by their sums in 64 bits
-  // (the 32-bit ones are exact where the bound is 0 or tau infinite).
-  const bool rank = near > need;
+  const Scan sc = wg_scan(n2, n1, sm);
+  const int need = want - sc.all_x, near = sc.all_y;  // of the near ones, `need` are taken
+  // All of them, or the first ones where they are equal (the 32-bit sums are
+  // exact where the bound is 0 or tau infinite); else by their 64-bit sums.
+  const bool sum64 = near > need && E2 > 0.0 && tau < INFINITY;
+  if (!sum64 || near <= kNear) {
+    unsigned long long mask = ~0ull;  // near ones taken (while there are up to 64)
+    if (sum64) {
+      int j = sc.y;
+      for (int k = k0; k < k1; ++k)
+        if (cls(k) == 1) sm.list[j++] = k;
+      __syncthreads();
+      const char* q = a.q + row * a.rtot * (size_t)RB;
+      const int32_t* tab = a.tables + (size_t)s * a.mbps + a.n_first;
+      for (int e = wave; e < near; e += kSelWaves) {
+        int id = tab[sm.list[e]];
+        if (id < 0 || id >= a.num_blocks) id = 0;  // as its score (reported there)
+        const double t =
+            score64<DT, HD>(q, a.bounds + ((size_t)id * a.kvh + g) * 2 * RB, a.rtot);
+        if (lane == 0) sm.sum[e] = t;
+      }
+      __syncthreads();
+      const double mine = lane < near ? sm.sum[lane] : -INFINITY;
+      int rank = 0;
+      for (int e = 0; e < near; ++e) {
+        const double y = sm.sum[e];
+        rank += y > mine || (y == mine && e < lane);
+      }
+      mask = __ballot(lane < near && rank < need);
+    }
+    int p2 = sc.x, p1 = sc.y;  // taken for sure, and near, before block k
+    for (int k = k0; k < k1; ++k) {
+      const int c = cls(k);
+      bool take = c == 2;
+      int before = min(p1, need);
+      if (sum64) {
+        before = __popcll(p1 < 64 ? mask & ((1ull << p1) - 1) : mask);
+        if (c == 1) take = mask >> p1 & 1;
+      } else if (c == 1) {
+        take = p1 < need;
+      }
+      if (take) out[a.n_first + p2 + before] = a.n_first + k;
+      p2 += c == 2;
+      p1 += c == 1;
+    }
+    return;
+  }
+  // many near ones: their sums go to the workspace, and a second search
   double* again = a.again + row * a.nb_max;
-  const bool sum64 = rank && E2 > 0.0 && tau < INFINITY;
-  if (sum64) {
-    const char* q = a.q + (row * a.rtot) * (size_t)RB;
+  {
+    const char* q = a.q + row * a.rtot * (size_t)RB;
     const int32_t* tab = a.tables + (size_t)s * a.mbps + a.n_first;
-    const int w = tid >> 6;
-    for (int k0 = w * 64; k0 < n; k0 += kSelThreads) {
-      unsigned long long todo = __ballot(k0 + lane < n && cls(min(k0 + lane, n - 1)) == 1);
+    for (int b0 = wave * kWave; b0 < n; b0 += kSelThreads) {
+      unsigned long long todo = __ballot(b0 + lane < n && cls(min(b0 + lane, n - 1)) == 1);
       while (todo) {  // wave-uniform
-        const int k = k0 + __ffsll((long long)todo) - 1;
+        const int k = b0 + __ffsll((long long)todo) - 1;
         todo &= todo - 1;
         int id = tab[k];
-        if (id < 0 || id >= a.num_blocks) id = 0;  // as its score (reported there)
-        const char* b = a.bounds + ((size_t)id * a.kvh + g) * 2 * RB;
-        double best = -INFINITY;
-        for (int h = 0; h < a.rtot; ++h) {
-          double t = 0.0;
-          for (int d = lane; d < HD; d += kWave) {
-            auto el = [&](const char* r) -> double {
-              if constexpr (DT == PKV_F32) return reinterpret_cast<const float*>(r)[d];
-              const uint16_t u = reinterpret_cast<const uint16_t*>(r)[d];
-              return DT == PKV_BF16 ? bf16lo(u) : f16lo(u);
-            };
-            const double x = el(q + (size_t)h * RB);
-            t += x * (x > 0.0 ? el(b + RB) : el(b));
-          }
-          for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, kWave);
-          best = t > best ? t : best;
-        }
-        if (lane == 0) again[k] = best;
+        if (id < 0 || id >= a.num_blocks) id = 0;
+        const double t =
+            score64<DT, HD>(q, a.bounds + ((size_t)id * a.kvh + g) * 2 * RB, a.rtot);
+        if (lane == 0) again[k] = t;
       }
     }
-    __syncthreads();  // (drains the stores: read back by this workgroup only)
+    __syncthreads();  // (read back by this workgroup only)
   }
-  unsigned long long kappa = 0;
-  int ties = near;  // near blocks with this key that are taken, lowest index first
-  if (sum64) {
-    int more = 0;
-    kappa = kth_largest<unsigned long long>(
-        n, need, [&](int k, unsigned long long& key) {
-          if (cls(k) != 1) return false;
-          key = key64(again[k]);
-          return true;
-        }, sm, more);
-    ties = need - more;
-  } else if (rank) {
-    // equal 32-bit values are ties; with a bound of 0 near means equal
-    ties = need;
-  }
-  // in index order
-  int done = 0, tied = 0;
-  for (int k0 = 0; k0 < n; k0 += kSelThreads) {
-    const int k = k0 + tid;
-    const int c = k < n ? cls(k) : 0;
-    bool take = c == 2, tie = false;
-    if (c == 1) {
-      if (sum64) {
-        const unsigned long long key = key64(again[k]);
-        take = key > kappa;
-        tie = key == kappa;
-      } else {
-        tie = true;
-      }
+  auto get = [&](int k, unsigned long long& key) {
+    if (cls(k) != 1) return false;
+    key = key64(again[k]);
+    return true;
+  };
+  unsigned long long lo64 = ~0ull, hi64 = 0;
+  for (int k = tid; k < n; k += kSelThreads) {
+    unsigned long long key;
+    if (get(k, key)) {
+      lo64 = key < lo64 ? key : lo64;
+      hi64 = key > hi64 ? key : hi64;
     }
-    int all;
-    const int tr = tied + wg_scan(tie, sm.part, all);
-    tied += all;
-    if (tie && tr < ties) take = true;
-    const int pos = done + wg_scan(take, sm.part, all);
-    done += all;
-    if (take && pos < want) out[a.n_first + pos] = a.n_first + k;
+  }
+  wg_extremes(lo64, hi64, em, sm);
+  int more = 0;
+  const unsigned long long kappa =
+      kth_largest<unsigned long long>(n, need, lo64, hi64, get, sm, more);
+  const int ties = need - more;  // of those equal to kappa, lowest index first
+  int taken = 0, equal = 0;
+  for (int k = k0; k < k1; ++k) {
+    unsigned long long key;
+    const int c = cls(k);
+    taken += c == 2 || (c == 1 && get(k, key) && key > kappa);
+    equal += c == 1 && get(k, key) && key == kappa;
+  }
+  const Scan s2 = wg_scan(taken, equal, sm);
+  int p2 = s2.x, p1 = s2.y;
+  for (int k = k0; k < k1; ++k) {
+    unsigned long long key = 0;
+    const int c = cls(k);
+    if (c == 1) (void)get(k, key);
+    const bool eq = c == 1 && key == kappa, sure = c == 2 || (c == 1 && key > kappa);
+    if (sure || (eq && p1 < ties)) out[a.n_first + p2 + min(p1, ties)] = a.n_first + k;
+    p2 += sure;
+    p1 += eq;
   }
 }
 
