@@ -142,7 +142,8 @@ struct SelectKArgs {
   int tiles;   // row tiles per sequence
   int chunks;  // waves along the blocks
   int per;     // blocks per wave (a multiple of 16)
-  int nb_max;  // pitch of score
+  int nb_max;  // blocks of a row at most
+  int pitch;   // of score and again: nb_max in whole lines
   int num_blocks;
   int bs_log2;
   int kvh;
@@ -151,9 +152,9 @@ struct SelectKArgs {
   int n_first;
   int n_last;
   int max_q;
-  float* score;  // [total_q][kvh][nb_max]
+  float* score;  // [total_q][kvh][pitch]
   float* emax;   // [total_q][kvh][chunks]
-  double* again; // [total_q][kvh][nb_max], written where a sum is made again
+  double* again; // [total_q][kvh][pitch], written where a sum is made again
   int32_t* out;  // [total_q][kvh][top]
   uint32_t* err;
 };
@@ -205,13 +206,22 @@ __device__ __forceinline__ u32x4 magnitude(const u32x4& w) {
 // matrix operand, R heads each) against `per` blocks of one kv head, 16 at a
 // time.  Lane l supplies 16-byte pieces of block l % 16's bound rows, as the
 // K fragments of the decode kernel; S~ takes 2 NF matrix instructions, the
-// two halves of T as many.
+// two halves of T as many.  Bound by HBM: 360 MB of bounds (64 contexts of
+// 12-32k tokens, 8 kv heads of 128) in 80 us, reads of the same rows
+// alone in 74; scores leave through LDS in whole lines, for 64 bytes at a time
+// (16 blocks) made it 83.  More loads in flight (the next 16 blocks' beside
+// these: 85-117 us), non-temporal ones (93) and longer runs per wave (87 with
+// 256 blocks) are slower.
+constexpr int kFlush = 64;  // blocks whose scores a wave gathers
+
 template <int DT, int HD, int R>
 __global__ void __launch_bounds__(256) score_kernel(SelectKArgs a) {
   constexpr int E = DT == PKV_F32 ? 4 : 2;
   constexpr int RB = HD * E;
   constexpr int NF = RB / 64;
   constexpr int RP = 16 / R;  // query rows per tile
+  __shared__ float buf_all[4][RP][kFlush];
+  auto& buf = buf_all[threadIdx.x >> 6];
   const int lane = threadIdx.x & 63;
   const int G = lane >> 4, col = lane & 15;
   const long long wave = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -313,11 +323,19 @@ __global__ void __launch_bounds__(256) score_kernel(SelectKArgs a) {
       for (int i = 0; i < 4; i += (R < 4 ? R : 4)) {
         const int m = 4 * G + i;
         const int qr = m / R;
-        if (m % R == 0 && qr < nrow && in) {
-          float* o = a.score + ((size_t)(sr.r0 + i0 + qr) * a.kvh + g) * a.nb_max + j + col;
-          *o = h0 ? fmaxf(*o, sc[i]) : sc[i];
-        }
+        if (m % R == 0 && qr < nrow) buf[qr][(j + col) % kFlush] = sc[i];
         if (in) etop = fmaxf(etop, er[i]);
+      }
+      // every kFlush blocks, and at the end: the scores so far, lane by lane
+      if ((j + 16) % kFlush == 0 || j + 16 >= j1) {
+        const int k = (j / kFlush) * kFlush + lane;
+        __builtin_amdgcn_wave_barrier();
+        for (int qr = 0; qr < nrow; ++qr)
+          if (k >= max(j0, a.n_first) && k < j1) {
+            float* o = a.score + ((size_t)(sr.r0 + i0 + qr) * a.kvh + g) * a.pitch + k;
+            *o = h0 ? fmaxf(*o, buf[qr][lane]) : buf[qr][lane];
+          }
+        __builtin_amdgcn_wave_barrier();
       }
     }
   }
@@ -524,7 +542,7 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
     out[a.top - a.n_last + k] = nb - a.n_last + k;
   if (want == 0) return;
 
-  const float* score = a.score + row * a.nb_max + a.n_first;
+  const float* score = a.score + row * a.pitch + a.n_first;
   const bool in_lds = n <= kSelLds;
   uint32_t klo = ~0u, khi = 0;
   for (int k = tid; k < n; k += kSelThreads) {
@@ -536,7 +554,8 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
   float em = 0.0f;
   for (int k = tid; k < a.chunks; k += kSelThreads) em = fmaxf(em, a.emax[row * a.chunks + k]);
   wg_extremes(klo, khi, em, sm);
-  const double E2 = 2.0 * (HD + 16) * 0x1p-23 * (double)em;
+  // twice the row's bound, and a little for the border's own rounding below
+  const float E2 = 2.02f * (HD + 16) * 0x1p-23f * em;
   auto at = [&](int k) { return in_lds ? sm.score[k] : score[k]; };
   int larger = 0;
   const uint32_t tkey = kth_largest<uint32_t>(
@@ -544,11 +563,10 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
   const float tau = unkey32(tkey);
   // 2: taken, 1: within the bound of the border, 0: not taken.  An infinite
   // score is what it is.
+  const float above = tau < INFINITY ? tau + E2 : tau, below = tau < INFINITY ? tau - E2 : tau;
   auto cls = [&](int k) {
     const float x = at(k);
-    if (x == INFINITY || tau == INFINITY) return x > tau ? 2 : x == tau ? 1 : 0;
-    const double d = (double)x - (double)tau;
-    return d > E2 ? 2 : d >= -E2 ? 1 : 0;
+    return x > above ? 2 : x >= below ? 1 : 0;
   };
   // consecutive blocks per thread, so one scan gives every place in index order
   const int per = (n + kSelThreads - 1) / kSelThreads;
@@ -563,7 +581,7 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
   const int need = want - sc.all_x, near = sc.all_y;  // of the near ones, `need` are taken
   // All of them, or the first ones where they are equal (the 32-bit sums are
   // exact where the bound is 0 or tau infinite); else by their 64-bit sums.
-  const bool sum64 = near > need && E2 > 0.0 && tau < INFINITY;
+  const bool sum64 = near > need && E2 > 0.0f && tau < INFINITY;
   if (!sum64 || near <= kNear) {
     unsigned long long mask = ~0ull;  // near ones taken (while there are up to 64)
     if (sum64) {
@@ -607,7 +625,7 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
     return;
   }
   // many near ones: their sums go to the workspace, and a second search
-  double* again = a.again + row * a.nb_max;
+  double* again = a.again + row * a.pitch;
   {
     const char* q = a.q + row * a.rtot * (size_t)RB;
     const int32_t* tab = a.tables + (size_t)s * a.mbps + a.n_first;
@@ -709,7 +727,7 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Layout of a call's workspace.
 struct SelectPlan {
-  int R, tiles, per, chunks, nb_max;
+  int R, tiles, per, chunks, nb_max, pitch;
   long long waves;
   size_t score, emax, again, bytes;
 };
@@ -729,9 +747,10 @@ SelectPlan select_plan(const pkv_pool* p, const SelectArgs& a) {
   pl.waves = rows * pl.chunks;
   const size_t pairs = (size_t)a.total_q * p->n_kv_head;
   pl.score = 0;
-  pl.emax = round256(pairs * pl.nb_max * 4);
+  pl.pitch = (pl.nb_max + kFlush - 1) / kFlush * kFlush;
+  pl.emax = round256(pairs * pl.pitch * 4);
   pl.again = pl.emax + round256(pairs * pl.chunks * 4);
-  pl.bytes = pl.again + round256(pairs * pl.nb_max * 8);
+  pl.bytes = pl.again + round256(pairs * pl.pitch * 8);
   return pl;
 }
 
@@ -762,6 +781,7 @@ hipError_t launch_select(const pkv_pool* p, const void* bounds, const SelectArgs
   k.chunks = pl.chunks;
   k.per = pl.per;
   k.nb_max = pl.nb_max;
+  k.pitch = pl.pitch;
   k.num_blocks = p->num_blocks;
   k.bs_log2 = log2_of(p->block_size);
   k.kvh = p->n_kv_head;
