@@ -239,40 +239,51 @@ def sample_expf(x):
 
 def _device_tensor(t, name: str, device, dtype, shape=None):
     """t, after a check that a kernel may read it as this."""
-    import torch
-    if not isinstance(t, torch.Tensor) or t.device != device:
+    if getattr(t, "device", None) != device:
         raise ValueError(f"{name} must be a tensor on {device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     return t.contiguous()
 
 
-def _run_on(stream, device, tensors):
-    """(stream to launch on, context in which to allocate and launch).  Another
-    stream than the current one first waits for the work queued on the current
-    one, and the tensors' memory is not reused before it has run."""
+def _i32_on(x, device):
+    """_i32, at once for what is one already."""
     import torch
+    if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device:
+        return x.contiguous()
+    return _i32(x, device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _run_on(stream, device, tensors):
+    """(raw stream to launch on, context in which to allocate and launch).
+    Another stream than the current one first waits for the work queued on the
+    current one, and the tensors' memory is not reused before it has run."""
+    import torch
+    if stream is None and torch.cuda.current_device() == device.index:
+        # the handle alone: a Stream object costs 2 us of a 10 us call
+        return torch._C._cuda_getCurrentRawStream(device.index) or None, _HERE
     cur = torch.cuda.current_stream(device)
     if stream is None or stream == cur:
-        if torch.cuda.current_device() == device.index:
-            return cur, contextlib.nullcontext()
-        return cur, torch.cuda.device(device)
+        return _stream_ptr(cur), torch.cuda.device(device)
     if stream.device != device:
         raise ValueError(f"stream must be on {device}")
     stream.wait_stream(cur)
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
-    return stream, torch.cuda.stream(stream)
+    return _stream_ptr(stream), torch.cuda.stream(stream)
 
 
 def _workspace(nbytes: int, device):
     """Scratch of one call, from torch's allocator: it belongs to the call's
     stream, and to the graph's memory while that stream is captured."""
     import torch
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
 StepTables = collections.namedtuple(
@@ -311,16 +322,18 @@ def step_tables(seq_lens, new_lens, block_tables, n_blocks, free_list, free_coun
     fc = _device_tensor(free_count, "free_count", dev, i32, (1,))
     s, ctx = _run_on(stream, dev, (bt, sl, nl, nb, fl, fc))
     with ctx:
-        def new(*shape):
-            return torch.empty(shape, dtype=i32, device=dev)
-        r = StepTables(new(n, width), new(n), new(1), new(n), new(n + 1), new(max_tokens),
-                       new(max_tokens), new(1))
+        tables = torch.empty((n, width), dtype=i32, device=dev)
+        # the small arrays share one allocation
+        small = torch.empty(3 * n + 3 + 2 * max_tokens, dtype=i32, device=dev)
+        r = StepTables(tables, *small.split((n, 1, n, n + 1, max_tokens, max_tokens, 1)))
+        p = _dev_ptr(small)
+        ctx_at = p + 4 * n + 4
+        pos_at = ctx_at + 8 * n + 4
+        slot_at = pos_at + 4 * max_tokens
         check(lib().pkv_step_tables(
             block_size, num_blocks, _dev_ptr(sl), _dev_ptr(nl), n, _dev_ptr(bt), _dev_ptr(nb),
-            width, _dev_ptr(fl), fl.numel(), _dev_ptr(fc), max_tokens, _dev_ptr(r.block_tables),
-            _dev_ptr(r.n_blocks), _dev_ptr(r.free_count), _dev_ptr(r.context_lens),
-            _dev_ptr(r.cu_q_lens), _dev_ptr(r.positions), _dev_ptr(r.slot_mapping),
-            _dev_ptr(r.status), _stream_ptr(s)), None)
+            width, _dev_ptr(fl), fl.numel(), _dev_ptr(fc), max_tokens, _dev_ptr(tables), p,
+            p + 4 * n, ctx_at, ctx_at + 4 * n, pos_at, slot_at, slot_at + 4 * max_tokens, s), None)
     return r
 
 
@@ -364,8 +377,8 @@ def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_unifor
     has_draft = draft_logits is not None and total > 0
     s, ctx = _run_on(stream, dev, (target_logits, draft_logits, dt, cu, u, uf, tp))
     with ctx:
-        tokens = torch.empty(total + batch, dtype=i32, device=dev)
-        accepted = torch.empty(batch, dtype=i32, device=dev)
+        tokens, accepted = torch.empty(total + 2 * batch, dtype=i32, device=dev).split(
+            (total + batch, batch))
         need = lib().pkv_verify_workspace_bytes(batch, total, vocab, has_draft)
         ws = _workspace(need, dev)
         check(lib().pkv_verify_drafts(
@@ -377,7 +390,7 @@ def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_unifor
             if has_draft else 0,
             _dev_ptr(dt), _dev_ptr(cu), batch, total, vocab, _dev_ptr(u), _dev_ptr(uf),
             _dev_ptr(tp) if tp is not None else None, _dev_ptr(tokens), _dev_ptr(accepted),
-            _dev_ptr(ws), need, _stream_ptr(s)), None)
+            _dev_ptr(ws), need, s), None)
     return tokens, accepted
 
 
@@ -883,8 +896,8 @@ class KvPool:
         their difference (None: what the tables hold).  Returns bounds."""
         c = self.cache
         self._check_bounds(bounds)
-        bt, cl = _i32(block_tables, c.device), _i32(context_lens, c.device)
-        fp = _i32(first_positions, c.device) if first_positions is not None else None
+        bt, cl = _i32_on(block_tables, c.device), _i32_on(context_lens, c.device)
+        fp = _i32_on(first_positions, c.device) if first_positions is not None else None
         n = cl.numel()
         if bt.dim() != 2 or bt.shape[0] != n or (fp is not None and fp.numel() != n):
             raise ValueError("block_tables must be (n, width), context_lens and "
@@ -895,8 +908,8 @@ class KvPool:
         with ctx:
             check(lib().pkv_key_bounds(
                 self._h, self.layer_index, _dev_ptr(bounds), _dev_ptr(bt), bt.shape[1],
-                _dev_ptr(fp) if fp is not None else None, _dev_ptr(cl), n, int(max_new_len),
-                _stream_ptr(s)), self._h)
+                _dev_ptr(fp) if fp is not None else None, _dev_ptr(cl), n, int(max_new_len), s),
+                self._h)
         return bounds
 
     def _rows(self, q, block_tables, context_lens, cu_q_lens, max_q_len):
@@ -906,8 +919,8 @@ class KvPool:
             raise ValueError(f"q must be (rows, n_head, {c.head_dim}) on {c.device}")
         if q.dtype != c.dtype:
             raise TypeError("q must have the pool dtype")
-        bt, cl = _i32(block_tables, c.device), _i32(context_lens, c.device)
-        cu = _i32(cu_q_lens, c.device) if cu_q_lens is not None else None
+        bt, cl = _i32_on(block_tables, c.device), _i32_on(context_lens, c.device)
+        cu = _i32_on(cu_q_lens, c.device) if cu_q_lens is not None else None
         n, rows = cl.numel(), q.shape[0]
         if bt.dim() != 2 or bt.shape[0] != n:
             raise ValueError("block_tables must be (n, width), context_lens (n,)")
@@ -955,7 +968,7 @@ class KvPool:
                 self._h, _dev_ptr(qq), _dev_ptr(bounds), _dev_ptr(out), int(top_blocks),
                 int(first_blocks), int(last_blocks), _dev_ptr(cu) if cu is not None else None,
                 _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, int(max_context_len), H,
-                _dev_ptr(ws), need, _stream_ptr(s)), self._h)
+                _dev_ptr(ws), need, s), self._h)
         return out
 
     def sparse_attention(self, q, blocks, block_tables, context_lens, cu_q_lens=None,
@@ -989,7 +1002,7 @@ class KvPool:
                 self._h, self.layer_index, _dev_ptr(qq), _dev_ptr(out), pkv_dtype(out.dtype),
                 _dev_ptr(bl), bl.shape[2], _dev_ptr(cu) if cu is not None else None,
                 _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, H, float(scale),
-                _dev_ptr(ws), need, _stream_ptr(s)), self._h)
+                _dev_ptr(ws), need, s), self._h)
         return out
 
     def _check_rows(self, t, name: str) -> None:
