@@ -75,7 +75,12 @@ struct SparseSmem {
 };
 
 // SB: block_size below 16, the tokens of a sub-tile span several blocks.
-template <int DT, int HD, int R, bool SB>
+// ONCE: one row per sequence, so no other wave reads a block's rows of a head,
+// and the loads say so.  The rows of a chunk choose much the same blocks: their
+// loads stay in the caches (42 rows of 12 chunks, 64 heads of 128, 75 blocks
+// each: 40 us against 50 with such loads; the other way 64 single rows of 128
+// blocks, 32 heads: 98 against 86).
+template <int DT, int HD, int R, bool SB, bool ONCE>
 __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKArgs a) {
   using C = DCfg<DT, HD, R, false>;
   __shared__ SparseSmem<DT, HD, R> sm;
@@ -166,6 +171,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
   const char* kh = a.k_pool + head_off;
   const char* vh = a.v_pool + head_off;
   const size_t blk_stride = (size_t)BS * slot_stride;
+  auto ld = [](const char* x) { return ONCE ? ld16_stream(x) : ld16(x); };
   auto lane_of = [&](int v, int t) {
     return __builtin_amdgcn_ds_bpermute(((t + o0) >> lg) << 2, v);
   };
@@ -216,10 +222,10 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
   for (int st = 0; st < C::NST; ++st) {
     const char* r = k_row(0, st);
 #pragma unroll
-    for (int f = 0; f < C::NF; ++f) kf[st][f] = ld16_stream(r + 64 * f);
+    for (int f = 0; f < C::NF; ++f) kf[st][f] = ld(r + 64 * f);
   }
 #pragma unroll
-  for (int k = 0; k < C::NV; ++k) vf[k] = ld16_stream(v_chunk(0, k));
+  for (int k = 0; k < C::NV; ++k) vf[k] = ld(v_chunk(0, k));
 
   // One tile, the next one's loads issued as the registers come free.
   auto tile_body = [&](const int tile_base, auto prefetch) {
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
       if constexpr (PF) {
         const char* r = k_row(next, st);
 #pragma unroll
-        for (int f = 0; f < C::NF; ++f) kf[st][f] = ld16_stream(r + 64 * f);
+        for (int f = 0; f < C::NF; ++f) kf[st][f] = ld(r + 64 * f);
       }
     }
     float sc[C::NST][4];
@@ -270,11 +276,14 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
             f32x4{sc[st][0], sc[st][1], sc[st][2], sc[st][3]};
     }
     __builtin_amdgcn_wave_barrier();
+    // the running sums follow a new maximum (after the first tiles seldom)
+    if (__any(alpha[0] != 1.0f || alpha[1] != 1.0f || alpha[2] != 1.0f || alpha[3] != 1.0f)) {
 #pragma unroll
-    for (int h = 0; h < R; ++h) {
-      const float ah = readlane_f(alpha[h & 3], 16 * (h >> 2));
+      for (int h = 0; h < R; ++h) {
+        const float ah = readlane_f(alpha[h & 3], 16 * (h >> 2));
 #pragma unroll
-      for (int e = 0; e < C::EPL; ++e) o[h][e] *= ah;
+        for (int e = 0; e < C::EPL; ++e) o[h][e] *= ah;
+      }
     }
 #pragma unroll
     for (int k = 0; k < C::NV; ++k) {
@@ -295,7 +304,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
       }
       float x[C::EPL];
       widen16<DT, C::EPL>(vf[k], x);
-      if constexpr (PF) vf[k] = ld16_stream(v_chunk(next, k));
+      if constexpr (PF) vf[k] = ld(v_chunk(next, k));
 #pragma unroll
       for (int h = 0; h < R; ++h)
 #pragma unroll
@@ -354,13 +363,14 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
 
 // Joins the parts: M = max m_p, L = sum l_p 2^(m_p - M), O = sum O_p 2^(m_p - M) / L;
 // L = 0 (no key at all) gives a zero row.  One wave per query head: HD / 4
-// lanes read a partial row, 64 / (HD / 4) rows per load, 4 loads in flight.
+// lanes read a partial row, 64 / (HD / 4) rows per load, U loads in flight; the
+// first ones and the (m, l) pairs of up to 64 parts go out together.
 template <int HD>
 __global__ void __launch_bounds__(kWavesPerBlock * kWave)
     sparse_merge_kernel(SparseKArgs a, int R, int dt) {
   constexpr int LPR = HD / 4;
   constexpr int PPI = kWave / LPR;
-  constexpr int U = 4;
+  constexpr int U = HD == 64 ? 4 : 8;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const unsigned qh = blockIdx.x * kWavesPerBlock + wave;
@@ -377,31 +387,45 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
   const int q = lane / LPR, c = lane % LPR;
   const float* po = a.part_o + (pair * a.parts * R + h) * HD + 4 * c;
   const size_t row = (size_t)R * HD;
-  float M = kLowest;
-  for (int p = lane; p < a.parts; p += kWave) M = fmaxf(M, ml[(size_t)p * kMlFloats]);
+  f32x4 ov[U];
+  auto load = [&](int p0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      ov[u] = *reinterpret_cast<const f32x4*>(po + (size_t)min(p0 + u * PPI + q, a.parts - 1) * row);
+  };
+  load(0);
+  float m0 = kLowest, l0 = 0.0f;  // part `lane`
+  if (lane < a.parts) {
+    m0 = ml[(size_t)lane * kMlFloats];
+    l0 = ml[(size_t)lane * kMlFloats + 1];
+  }
+  float M = m0;
+  for (int p = kWave + lane; p < a.parts; p += kWave) M = fmaxf(M, ml[(size_t)p * kMlFloats]);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, shfl_xor_f(M, x));
-  float L = 0.0f;
-  for (int p = lane; p < a.parts; p += kWave)
+  const float w0 = fast_exp2(m0 - M);
+  float L = w0 * l0;
+  for (int p = kWave + lane; p < a.parts; p += kWave)
     L += fast_exp2(ml[(size_t)p * kMlFloats] - M) * ml[(size_t)p * kMlFloats + 1];
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) L += shfl_xor_f(L, x);
   f32x4 acc = {0, 0, 0, 0};
   for (int p0 = 0; p0 < a.parts; p0 += PPI * U) {
-    f32x4 ov[U];
-    float w[U];
+    if (p0) load(p0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int p = p0 + u * PPI + q;
-      // a part without a key wrote no rows
-      const bool ok = p < a.parts && ml[(size_t)p * kMlFloats + 1] != 0.0f;
-      ov[u] = ok ? *reinterpret_cast<const f32x4*>(po + (size_t)p * row) : f32x4{0, 0, 0, 0};
-      w[u] = ok ? fast_exp2(ml[(size_t)p * kMlFloats] - M) : 0.0f;
+      // weight and l of the part; one without a key (l = 0) wrote no rows
+      float w = __int_as_float(__builtin_amdgcn_ds_bpermute((p & 63) << 2, __float_as_int(w0)));
+      float l = __int_as_float(__builtin_amdgcn_ds_bpermute((p & 63) << 2, __float_as_int(l0)));
+      if (p >= kWave && p < a.parts) {
+        w = fast_exp2(ml[(size_t)p * kMlFloats] - M);
+        l = ml[(size_t)p * kMlFloats + 1];
+      }
+      if (p < a.parts && l != 0.0f)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = fmaf(w, ov[u][k], acc[k]);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = fmaf(w[u], ov[u][k], acc[k]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -431,8 +455,10 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
 
 template <int DT, int HD, int R>
 void launch_main(const SparseKArgs& k, unsigned grid, hipStream_t s) {
-  if (k.bs_log2 < 4) sparse_kernel<DT, HD, R, true><<<grid, kWavesPerBlock * kWave, 0, s>>>(k);
-  else sparse_kernel<DT, HD, R, false><<<grid, kWavesPerBlock * kWave, 0, s>>>(k);
+  constexpr int kThreads = kWavesPerBlock * kWave;
+  if (k.bs_log2 < 4) sparse_kernel<DT, HD, R, true, false><<<grid, kThreads, 0, s>>>(k);
+  else if (k.max_q > 1) sparse_kernel<DT, HD, R, false, false><<<grid, kThreads, 0, s>>>(k);
+  else sparse_kernel<DT, HD, R, false, true><<<grid, kThreads, 0, s>>>(k);
 }
 
 template <int DT, int HD>
@@ -462,7 +488,11 @@ struct SparsePlan {
 };
 
 // Parts of 1024 tokens, halved (down to 64) while the call has fewer than
-// 2048 waves, and while a part has more than the 64 list entries of a wave.
+// 1024 waves, one per SIMD, and while a part has more than the 64 list entries of
+// a wave.  Eight heads and more keep a wave at P.V for longer, so they get half
+// as many waves again.  (us, main kernel and merge, parts of 128 / 256 / 512 /
+// 1024: 64 rows of 2048 tokens, 32 heads on 8 of 128: 112 / 101 / 95 / 91; 42 rows
+// of 1200, 64 heads: 64 / 57 / 80 / 87.)
 SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   SparsePlan pl{};
   while ((1 << pl.bs_log2) < p->block_size) ++pl.bs_log2;
@@ -470,7 +500,7 @@ SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   const long long len = (long long)a.top_blocks << pl.bs_log2;
   const long long pairs = (long long)a.total_q * p->n_kv_head;
   int pt = 1024;
-  while (pt > 64 && pairs * ((len + pt - 1) / pt) < 2048) pt >>= 1;
+  while (pt > 64 && pairs * ((len + pt - 1) / pt) < (pl.R < 8 ? 1024 : 1536)) pt >>= 1;
   while (pt > 64 && (pt >> pl.bs_log2) > 64) pt >>= 1;
   pl.part_tokens = pt;
   pl.parts = (int)((len + pt - 1) / pt);
