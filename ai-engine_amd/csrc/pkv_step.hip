@@ -27,56 +27,63 @@ namespace {
 
 constexpr int kStepThreads = 256;
 
-// Sum over the workgroup, in every thread.
-__device__ __forceinline__ long long wg_sum(long long x, long long* lds) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
-  __syncthreads();  // the previous sum has been read
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-  __syncthreads();
-  long long s = 0;
+constexpr int kStepWaves = kStepThreads / kWave;
+constexpr int kSums = 5;
+
+// Sums over the workgroup, in every thread, behind one barrier.
+__device__ __forceinline__ void wg_sums(long long (&x)[kSums], long long (&lds)[kSums][kStepWaves]) {
 #pragma unroll
-  for (int w = 0; w < kStepThreads / kWave; ++w) s += lds[w];
-  return s;
+  for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) x[k] += __shfl_xor(x[k], o, kWave);
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) lds[k][threadIdx.x >> 6] = x[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+    x[k] = 0;
+#pragma unroll
+    for (int w = 0; w < kStepWaves; ++w) x[k] += lds[k][w];
+  }
 }
 
 __global__ void __launch_bounds__(kStepThreads) step_tables_kernel(StepArgs a) {
-  __shared__ long long red[kStepThreads / kWave];
+  __shared__ long long red[kSums][kStepWaves];
   const int me = blockIdx.x;
   const int tid = threadIdx.x;
   const int bsl = a.bs_log2, bs = 1 << bsl;
   // counts of the requests before this one and of all; a request whose
   // lengths its table cannot hold makes the step invalid
-  long long need_b = 0, need_t = 0, new_b = 0, new_t = 0, bad = 0;
+  enum { kNeedBefore, kNeed, kNewBefore, kNew, kBad };
+  long long sum[kSums] = {};
   for (int i = tid; i < a.n_seqs; i += kStepThreads) {
     const long long seq = a.seq_lens[i], nw = a.new_lens[i], have = a.n_blocks[i];
     const long long upto = (seq + nw + bs - 1) >> bsl;
     if (seq < 0 || nw < 0 || have < 0 || have > a.width || upto > a.width) {
-      bad = 1;
+      sum[kBad] = 1;
       continue;
     }
     const long long need = upto > have ? upto - have : 0;
-    need_t += need;
-    new_t += nw;
-    if (i < me) {
-      need_b += need;
-      new_b += nw;
-    }
+    sum[kNeed] += need;
+    sum[kNew] += nw;
+    sum[kNeedBefore] += i < me ? need : 0;
+    sum[kNewBefore] += i < me ? nw : 0;
   }
   const int count = *a.free_count;
-  need_t = wg_sum(need_t, red);
-  need_b = wg_sum(need_b, red);
-  new_t = wg_sum(new_t, red);
-  new_b = wg_sum(new_b, red);
-  bad = wg_sum(bad, red);
-  if (count < 0 || count > a.free_len || new_t > a.max_tokens) bad = 1;
-  const long long lacking = need_t - count;
-  const bool ok = !bad && lacking <= 0;
-
   // (a step without requests still has its buffers filled)
   const bool any = me < a.n_seqs;
   const int seq = any ? a.seq_lens[me] : 0, have_raw = any ? a.n_blocks[me] : 0;
+  const int new_raw = any ? a.new_lens[me] : 0;
+  wg_sums(sum, red);
+  const long long need_b = sum[kNeedBefore], need_t = sum[kNeed];
+  const long long new_b = sum[kNewBefore], new_t = sum[kNew];
+  const bool bad = sum[kBad] || count < 0 || count > a.free_len || new_t > a.max_tokens;
+  const long long lacking = need_t - count;
+  const bool ok = !bad && lacking <= 0;
+
   const int have = min(max(have_raw, 0), a.width);
-  const int nw = ok && any ? a.new_lens[me] : 0;
+  const int nw = ok ? new_raw : 0;
   const int total = ok ? (int)new_t : 0;
   const int upto = ok ? (int)(((long long)seq + nw + bs - 1) >> bsl) : 0;
   const int blocks = max(have, upto);
