@@ -105,33 +105,21 @@ __device__ __forceinline__ double weight(float l, float m, double c) {
   return t > -1000.0 ? w : 0.0;  // (false for NaN: -inf against -inf)
 }
 
-// A row's reference and the logits around it that need no care: [lo, hi].
+// A row's reference and the logits around it whose weights are 2^-500 to 2^500:
+// [lo, hi].  far: these are not to be told from m itself (m is a type's lowest
+// value, say), every logit needs care.
 struct Ref {
   float m, lo, hi;
-  double c, mc;
+  bool far;
+  double c, m64;
 };
 __device__ __forceinline__ void set_ref(Ref& r, float m) {
   const float span = fminf((float)(500.0 / r.c), 1e38f);
   r.m = m;
+  r.far = !(span > fabsf(m) * 0x1p-20f);
   r.lo = m - span;
   r.hi = m + span;
-  r.mc = -(double)m * r.c;
-}
-// Whether eight logits are all in the range of r (and none is NaN), and their
-// largest (NaN aside).
-__device__ __forceinline__ bool in_range(const float (&x)[8], const Ref& r, float& top) {
-  float lo = fminf(fminf(x[0], x[1]), x[2]), sum = x[0];
-  top = fmaxf(fmaxf(x[0], x[1]), x[2]);
-  lo = fminf(fminf(lo, x[3]), x[4]);
-  top = fmaxf(fmaxf(top, x[3]), x[4]);
-  lo = fminf(fminf(lo, x[5]), fminf(x[6], x[7]));
-  top = fmaxf(fmaxf(top, x[5]), fmaxf(x[6], x[7]));
-#pragma unroll
-  for (int e = 1; e < 8; ++e) sum += x[e];
-  return lo >= r.lo && top <= r.hi && sum == sum;
-}
-__device__ __forceinline__ double weight_in_range(float l, const Ref& r) {
-  return exp2_near(fma((double)l, r.c, r.mc));
+  r.m64 = m;
 }
 // A term of a sum: logits below the range count as its lower end, 2^-500, those
 // above it as its upper end.  (One instruction; min and max of unpacked words
@@ -139,7 +127,8 @@ __device__ __forceinline__ double weight_in_range(float l, const Ref& r) {
 __device__ __forceinline__ double weight_clamped(float l, const Ref& r) {
   float x;
   asm("v_med3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(l), "v"(r.lo), "v"(r.hi));
-  return weight_in_range(x, r);
+  // (a product and one addition would be off by the rounding of m c)
+  return exp2_near(((double)x - r.m64) * r.c);
 }
 __device__ __forceinline__ float largest(const float (&x)[8]) {
   float top = kept(x[0]);
@@ -260,7 +249,7 @@ __device__ __forceinline__ Stat chunk_stat(const char* row, int c0, int c1, doub
       double g = 0.0;
 #pragma unroll
       for (int e = 0; e < kN; ++e) g += weight_clamped(x[e], r);
-      if (g < 0x1p499) {
+      if (g < 0x1p499 && !r.far) {
         sum += g;
       } else {  // a logit at the range's upper end, or NaN
         top = largest(x);
@@ -398,13 +387,19 @@ __device__ Decision decide(const VerifyKArgs& a, int b, int& kept, int* lds) {
   return d;
 }
 
+// Probabilities below this count as 0 in a draw: the weight of a logit below
+// the reference's range is 2^-500, not 0.
+constexpr double kNothing = 0x1p-400;
+
 // Probabilities of eight logits.
 __device__ __forceinline__ void probs8(const float (&x)[kN], const Ref& r, double inv, double (&p)[kN]) {
-  float top;
-  if (in_range(x, r, top)) {
+  float sum = x[0];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) p[e] = weight_in_range(x[e], r) * inv;
-  } else {
+  for (int e = 1; e < kN; ++e) sum += x[e];
+  if (sum == sum && !r.far) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) p[e] = weight_clamped(x[e], r) * inv;
+  } else {  // NaN, or both infinities
 #pragma unroll
     for (int e = 0; e < kN; ++e) p[e] = weight(x[e], r.m, r.c) * inv;
   }
@@ -483,32 +478,37 @@ __device__ __forceinline__ double wave_scan(double x) {
 }
 
 // Where the running sum of x(0), x(1), .. x(n - 1) first passes `want` (the last
-// positive one if rounding leaves it short), and the sum before it; -1 if none
-// is positive.  One wave; x is called with an index below n.
+// that counts if rounding leaves it short), and the sum before it; -1 if none
+// counts.  One wave, consecutive numbers per lane.
 template <class X>
 __device__ int first_past(int n, double want, double& before, X x) {
   const int lane = threadIdx.x & 63;
-  int last = -1;
-  double last_before = 0.0, run = before;
-  for (int k0 = 0; k0 < n; k0 += kWave) {
-    const double v = k0 + lane < n ? x(k0 + lane) : 0.0;
-    const double upto = run + wave_scan(v);
-    const unsigned long long pos = __ballot(v > 0.0);
-    const unsigned long long hit = __ballot(v > 0.0 && upto > want);
-    if (hit) {
-      const int l = __ffsll((long long)hit) - 1;
-      before = __shfl(upto - v, l, kWave);
-      return k0 + l;
-    }
-    if (pos) {
-      const int l = 63 - __clzll((long long)pos);
-      last = k0 + l;
-      last_before = __shfl(upto - v, l, kWave);
-    }
-    run = __shfl(upto, 63, kWave);
+  const int per = (n + kWave - 1) / kWave;
+  const int k0 = min(lane * per, n), k1 = min(k0 + per, n);
+  double mine = 0.0;
+  bool some = false;
+  for (int k = k0; k < k1; ++k) {
+    const double v = x(k);
+    mine += v;
+    some |= v > kNothing;
   }
-  before = last_before;
-  return last;
+  const double upto = before + wave_scan(mine);
+  const unsigned long long hit = __ballot(some && upto > want), any = __ballot(some);
+  if (!any) return -1;
+  const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)any);
+  double run = upto - mine, at = run;
+  int pick = -1;
+  for (int k = k0; k < k1; ++k) {
+    const double v = x(k);
+    if (v > kNothing) {
+      pick = k;
+      at = run;
+      if (run + v > want) break;
+    }
+    run += v;
+  }
+  before = __shfl(at, l, kWave);
+  return __shfl(pick, l, kWave);
 }
 
 // Grid batch, one wave: the segment in which the running sum passes, then the
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
     return wave_sum(x);
   };
   double total = sum_parts();
-  if (!(total > 0.0) && (d.draft >= 0 || d.not_tok >= 0)) {
+  if (!(total > kNothing) && (d.draft >= 0 || d.not_tok >= 0)) {
     // p <= q everywhere (only by rounding, or when all of p is on the draft):
     // the draw is from p
     d.draft = d.not_tok = -1;
@@ -554,12 +554,12 @@ __global__ void __launch_bounds__(kWave) verify_token_kernel(VerifyKArgs a) {
   int pick = 0;
 #pragma unroll
   for (int e = 0; e < kN; ++e)
-    if (w[e] > 0.0) pick = e;
+    if (w[e] > kNothing) pick = e;
   bool done = false;
 #pragma unroll
   for (int e = 0; e < kN; ++e) {
     before += w[e];
-    if (!done && w[e] > 0.0 && before > want) {
+    if (!done && w[e] > kNothing && before > want) {
       pick = e;
       done = true;
     }

@@ -601,7 +601,7 @@ def test_verify_greedy_without_temperatures(gpu):
 
 
 @pytest.mark.parametrize("what", ["masked", "empty", "nan", "inf", "tokens", "edges", "same", "flat",
-                                  "cold", "emptydraft"])
+                                  "cold", "emptydraft", "lowest", "huge", "offset"])
 @pytest.mark.parametrize("draft", [True, False])
 def test_verify_odd_values(gpu, what, draft):
     x, d, cu, u, ul, y, temps = verify_case(17, 24, 4700, 4, "f32", "f32")
@@ -631,6 +631,17 @@ def test_verify_odd_values(gpu, what, draft):
             y[cu[b]:cu[b + 1]] = x[cu[b] + b:cu[b + 1] + b]
     elif what == "flat":
         x[:], y[:] = 0.0, 1.0
+    elif what == "lowest":  # masked by the type's lowest value, whole stretches of a row
+        low = np.finfo(np.float32).min
+        x[:, :3000], y[:, 200:] = low, low
+        x[::2, 3500:], y[::3, :190] = low, low
+    elif what == "huge":
+        x *= 1e37
+        y *= 1e30
+    elif what == "offset":  # all of a row far from 0
+        x += np.where(np.arange(len(x)) % 2, 1e9, -3e5)[:, None]
+        y -= 1e7
+        x, y = x.astype(np.float32).astype(np.float64), y.astype(np.float32).astype(np.float64)
     else:
         temps[:] = np.where(temps > 0, np.float32(0.01), 0)
     y = y if draft else None
