@@ -305,86 +305,95 @@ __global__ void __launch_bounds__(kVT) verify_stat_kernel(VerifyKArgs a) {
   if (threadIdx.x == 0) a.rows[(size_t)r * a.g1 + chunk] = {st.m, st.arg, st.s};
 }
 
-// A row's statistics from its chunks'.
+// A row's statistics from its chunks', four at a time side by side.
 __device__ __forceinline__ Stat row_stat(const VerifyKArgs& a, int r, double c) {
+  constexpr int U = 4;
   Stat st = kNoStat;
-  for (int k = 0; k < a.g1; ++k) {
-    const RowPart y = a.rows[(size_t)r * a.g1 + k];
-    const Stat t{y.m, y.arg, y.s};
-    if (k == 0) st = t;
-    else join(st, t, c);
+  for (int k0 = 0; k0 < a.g1; k0 += U) {
+    RowPart y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      y[u] = a.rows[(size_t)r * a.g1 + min(k0 + u, a.g1 - 1)];
+      if (k0 + u >= a.g1) y[u].m = -INFINITY;
+    }
+    Stat x = kNoStat;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (y[u].m > x.m) {
+        x.m = y[u].m;
+        x.arg = y[u].arg;
+      }
+    if (c != 0.0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) x.s += y[u].s * weight(y[u].m, x.m, c);
+    }
+    if (k0 == 0) st = x;
+    else join(st, x, c);
   }
   return st;
 }
 
 // The drafts of request b that are kept and what its next token is drawn
-// from, in every thread.
-__device__ Decision decide(const VerifyKArgs& a, int b, int& kept, int* lds) {
+// from, in every thread.  Thread i has draft i and its rows; one past the last
+// draft stands for the request's end.
+__device__ __forceinline__ Decision decide(const VerifyKArgs& a, int b, int& n, int& kept, int* lds,
+                                           Decision& shared) {
   const int d0 = first_draft(a, b);
-  const int n = max(first_draft(a, b + 1) - d0, 0);
+  n = max(first_draft(a, b + 1) - d0, 0);
   const double c = exponent(a, b);
   const int n_target = a.total + a.batch;
-  kept = n;
-  for (int i0 = 0; i0 < n; i0 += kVT) {  // uniform
+  const int tdt = a.draft_dt >> 8, ddt = a.draft_dt & 255;
+  for (int i0 = 0;; i0 += kVT) {  // uniform, ends at i = n
     const int i = i0 + (int)threadIdx.x;
     bool keep = true;
-    if (i < n) {
-      const int d = a.tokens[d0 + i];
+    Decision d{};
+    if (i <= n) {
       const int r = d0 + b + i;
+      const bool some = i < n, drawn = some && c != 0.0 && a.draft;
+      const int tok = some ? a.tokens[d0 + i] : -1;
+      const double u = some && c != 0.0 ? (double)a.u[d0 + i] : 0.0;
+      const bool known = tok >= 0 && tok < a.vocab;
+      float lp = 0.0f, lq = 0.0f;
+      if (known && c != 0.0) {
+        lp = logit_dt(tdt, a.target + r * a.t_stride * bytes_of(tdt), tok);
+        if (drawn) lq = logit_dt(ddt, a.draft + (d0 + i) * a.d_stride * bytes_of(ddt), tok);
+      }
       const Stat p = row_stat(a, r, c);
-      if (d < 0 || d >= a.vocab) {
+      const Stat q = drawn ? row_stat(a, n_target + d0 + i, c) : kNoStat;
+      if (!known) {
         keep = false;
       } else if (c == 0.0) {
-        keep = d == p.arg && p.m > -INFINITY;
+        keep = tok == p.arg && p.m > -INFINITY;
       } else {
-        const float lp = logit_dt(a.draft_dt >> 8, a.target + r * a.t_stride * bytes_of(a.draft_dt >> 8), d);
-        const double wp = weight(lp, p.m, c);
-        double wq = 1.0, sq = 1.0;
-        if (a.draft) {
-          const Stat q = row_stat(a, n_target + d0 + i, c);
-          const int dt = a.draft_dt & 255;
-          wq = weight(logit_dt(dt, a.draft + (d0 + i) * a.d_stride * bytes_of(dt), d), q.m, c);
-          sq = q.s;
-        }
         // u q(d) < p(d); a draft row without weight has q = 0
-        const double qd = sq > 0.0 ? wq / sq : 0.0, pd = p.s > 0.0 ? wp / p.s : 0.0;
-        keep = (double)a.u[d0 + i] * qd < pd;
+        const double pd = p.s > 0.0 ? weight(lp, p.m, c) / p.s : 0.0;
+        const double qd = !a.draft ? 1.0 : q.s > 0.0 ? weight(lq, q.m, c) / q.s : 0.0;
+        keep = u * qd < pd;
       }
+      d.row = d.at = r;
+      d.draft = drawn && q.s > 0.0 ? d0 + i : -1;
+      d.not_tok = some && c != 0.0 && !a.draft ? tok : -1;
+      d.token = c == 0.0 ? p.arg : p.s > 0.0 ? -1 : 0;
+      d.m_p = p.m;
+      d.inv_p = p.s > 0.0 ? 1.0 / p.s : 0.0;
+      d.m_q = d.draft >= 0 ? q.m : 0.0f;
+      d.inv_q = d.draft >= 0 ? 1.0 / q.s : 0.0;
     }
     const unsigned long long lost = __ballot(!keep);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0)
       lds[threadIdx.x >> 6] = lost ? (int)threadIdx.x + __ffsll((long long)lost) - 1 : INT32_MAX;
     __syncthreads();
     int first = INT32_MAX;
+#pragma unroll
     for (int w = 0; w < kVW; ++w) first = min(first, lds[w]);
     if (first != INT32_MAX) {
       kept = i0 + first;
-      break;
+      if ((int)threadIdx.x == first) shared = d;
+      __syncthreads();
+      return shared;
     }
+    __syncthreads();
   }
-  Decision d{};
-  d.row = d0 + b + kept;
-  d.at = d.row;
-  d.draft = -1;
-  d.not_tok = -1;
-  const Stat p = row_stat(a, d.row, c);
-  d.token = c == 0.0 ? p.arg : p.s > 0.0 ? -1 : 0;
-  d.m_p = p.m;
-  d.inv_p = p.s > 0.0 ? 1.0 / p.s : 0.0;
-  if (c != 0.0 && kept < n) {
-    if (a.draft) {
-      const Stat q = row_stat(a, n_target + d0 + kept, c);
-      if (q.s > 0.0) {
-        d.draft = d0 + kept;
-        d.m_q = q.m;
-        d.inv_q = 1.0 / q.s;
-      }
-    } else {
-      d.not_tok = a.tokens[d0 + kept];
-    }
-  }
-  return d;
 }
 
 // Probabilities below this count as 0 in a draw: the weight of a logit below
@@ -442,11 +451,12 @@ __device__ __forceinline__ void weigh8(const VerifyKArgs& a, const Decision& d, 
 template <int DT, int DDT, bool VEC>
 __global__ void __launch_bounds__(kVT) verify_weight_kernel(VerifyKArgs a) {
   __shared__ int lds[kVW];
+  __shared__ Decision shared;
   const int b = blockIdx.x / a.g2, chunk = blockIdx.x % a.g2;
-  int n_kept = 0;
-  const Decision d = decide(a, b, n_kept, lds);
+  int n = 0, n_kept = 0;
+  const Decision d = decide(a, b, n, n_kept, lds, shared);
   if (chunk == 0) {
-    const int d0 = first_draft(a, b), n = max(first_draft(a, b + 1) - d0, 0);
+    const int d0 = d.row - b - n_kept;
     if (threadIdx.x == 0) {
       a.decide[b] = d;
       a.accepted[b] = n_kept;
