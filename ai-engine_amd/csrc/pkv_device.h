@@ -124,6 +124,30 @@ __device__ __forceinline__ int wave_incl_scan(int x) {
   return x;
 }
 
+// The same for doubles, whose words move apart: a DPP step's source lanes
+// outside the row give 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_d(double x) {
+  return __hiloint2double(
+      __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xf, false),
+      __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ double wave_incl_scan(double x) {
+  x += dpp_d<0x111, 0xf>(x);  // row_shr:1
+  x += dpp_d<0x112, 0xf>(x);  // row_shr:2
+  x += dpp_d<0x114, 0xf>(x);  // row_shr:4
+  x += dpp_d<0x118, 0xf>(x);  // row_shr:8
+  x += dpp_d<0x142, 0xa>(x);  // row_bcast:15
+  x += dpp_d<0x143, 0xc>(x);  // row_bcast:31
+  return x;
+}
+// Sum over the wave, in every lane.
+__device__ __forceinline__ double wave_sum(double x) {
+  x = wave_incl_scan(x);
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), 63),
+                          __builtin_amdgcn_readlane(__double2loint(x), 63));
+}
+
 __device__ __forceinline__ float readlane_f(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }

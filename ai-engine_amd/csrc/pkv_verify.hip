@@ -170,11 +170,6 @@ __device__ __forceinline__ int request_of(const VerifyKArgs& a, int x, int step)
   return n;
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
-  return x;
-}
-
 // What RowPart holds, of a part of a row.
 struct Stat {
   float m;
@@ -477,16 +472,6 @@ __global__ void __launch_bounds__(kVT) verify_weight_kernel(VerifyKArgs a) {
   }
 }
 
-// Inclusive running sum over the wave's lanes.
-__device__ __forceinline__ double wave_scan(double x) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o, kWave);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
 // Where the running sum of x(0), x(1), .. x(n - 1) first passes `want` (the last
 // that counts if rounding leaves it short), and the sum before it; -1 if none
 // counts.  One wave, consecutive numbers per lane.
@@ -502,7 +487,7 @@ __device__ int first_past(int n, double want, double& before, X x) {
     mine += v;
     some |= v > kNothing;
   }
-  const double upto = before + wave_scan(mine);
+  const double upto = before + wave_incl_scan(mine);
   const unsigned long long hit = __ballot(some && upto > want), any = __ballot(some);
   if (!any) return -1;
   const int l = hit ? __ffsll((long long)hit) - 1 : 63 - __clzll((long long)any);
