@@ -545,14 +545,20 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
   const float* score = a.score + row * a.pitch + a.n_first;
   const bool in_lds = n <= kSelLds;
   uint32_t klo = ~0u, khi = 0;
-  for (int k = tid; k < n; k += kSelThreads) {
-    const float x = score[k];
-    if (in_lds) sm.score[k] = x;
-    klo = min(klo, key32(x));
-    khi = max(khi, key32(x));
-  }
   float em = 0.0f;
   for (int k = tid; k < a.chunks; k += kSelThreads) em = fmaxf(em, a.emax[row * a.chunks + k]);
+  constexpr int U = 8;  // loads in flight
+  for (int k = tid; k < n; k += U * kSelThreads) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = score[min(k + u * kSelThreads, n - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (the last one again changes nothing)
+      if (in_lds) sm.score[min(k + u * kSelThreads, n - 1)] = x[u];
+      klo = min(klo, key32(x[u]));
+      khi = max(khi, key32(x[u]));
+    }
+  }
   wg_extremes(klo, khi, em, sm);
   // twice the row's bound, and a little for the border's own rounding below
   const float E2 = 2.02f * (HD + 16) * 0x1p-23f * em;
