@@ -158,16 +158,19 @@ __device__ __forceinline__ double exponent(const VerifyKArgs& a, int b) {
 __device__ __forceinline__ int first_draft(const VerifyKArgs& a, int b) {
   return min(max(a.cu[b], 0), a.total);
 }
-// Number of requests k >= 1 whose first entry cu[k] + step k is at most x: the
-// request of target row x (step 1) or of draft x (step 0).
+// The last request k with cu[k] + step k <= x (0 if none has): the request of
+// target row x (step 1) or of draft x (step 0).  64 at a time, a wave's ballot.
 __device__ __forceinline__ int request_of(const VerifyKArgs& a, int x, int step) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int k0 = 1; k0 < a.batch; k0 += kWave) {
-    const int k = k0 + lane;
-    n += __popcll(__ballot(k < a.batch && first_draft(a, k) + step * k <= x));
+  int first = 0, n = a.batch;
+  while (n > 1) {
+    const int stride = (n + kWave - 1) / kWave;
+    const int k = first + lane * stride;
+    const bool ok = lane * stride < n && first_draft(a, k) + step * k <= x;
+    first += max(__popcll(__ballot(ok)) - 1, 0) * stride;
+    n = min(stride, a.batch - first);
   }
-  return n;
+  return first;
 }
 
 // What RowPart holds, of a part of a row.

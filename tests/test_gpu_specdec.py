@@ -578,7 +578,7 @@ def same_verify(got, want):
     ("bf16", "bf16", 5, 1000, 4, 0), ("f32", "f32", 3, 5001, 5, 0), ("f16", "f32", 9, 77, 3, 3),
     ("bf16", "f16", 1, 40000, 8, 8), ("f32", "bf16", 70, 33, 6, 1), ("f16", "f16", 4, 1, 3, 0),
     ("bf16", "f32", 2, 2, 2, 0), ("f32", "f32", 2, 20000, 300, 4), ("bf16", "bf16", 300, 130, 2, 6),
-    ("f16", "bf16", 1, 9000, 1, 0)])
+    ("f16", "bf16", 1, 9000, 1, 0), ("bf16", "bf16", 4500, 12, 2, 0), ("f32", "f32", 65, 40, 1, 0)])
 def test_verify(gpu, dt, ddt, batch, vocab, k, stride, draft):
     a = verify_case(batch * 31 + vocab, batch, vocab, k, dt, ddt)
     x, d, cu, u, ul, y, temps = a
