@@ -99,6 +99,29 @@ __device__ __forceinline__ float swap32_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Max over the four lane groups (rows of 16 lanes) holding one score row:
+// permlane16_swap pairs rows 0/1 and 2/3, permlane32_swap the two halves.
+__device__ __forceinline__ float row_group_max(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Two floats to packed 16-bit (round to nearest even, v_cvt_pk_*_f32).
+template <int DT>
+__device__ __forceinline__ uint32_t cvt_pk16(float x0, float x1) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 v = {x0, x1};
+  if constexpr (DT == PKV_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+  }
+}
+
 // Sum of x over the lanes l' with l' % CH == l % CH (CH a power of two in
 // [4, 64]); every lane receives the sum.
 template <int CH>

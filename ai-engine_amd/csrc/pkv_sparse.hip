@@ -8,8 +8,7 @@
 // Bound by HBM: every listed block's K and V rows of a head (2 bs hd
 // elements) are read once for the group's query heads.  The list is laid out
 // as one run of tokens and cut into parts, a wavefront each, as the decode
-// kernel cuts a context; a wave's tiles, matrix instructions, online softmax
-// and P.V are those of pkv_decode.hip.  What differs is where a token is:
+// kernel cuts a context.  What differs is where a token is:
 //  - a wave reads its slice of the list, then the table entries of those
 //    blocks (two dependent loads in place of one), and moves the valid ones
 //    to the front, so an entry that is no block costs nothing;
@@ -17,6 +16,10 @@
 //    of them: tokens past it read the block's last key with weight 0.
 // Every row's list is equally long, so parts are the same for all rows and
 // need no context lengths in the merge.
+//
+// Both products of 16-bit pools run on the matrix cores, the heads as the 16
+// columns: S^T = K Q^T, O^T = V^T P^T (sparse16_kernel).  f32 pools take the
+// decode kernel's way, P.V in f32 multiply-adds (sparse32_kernel).
 #include <algorithm>
 
 #include "pkv_decode_dev.h"
@@ -48,7 +51,8 @@ struct SparseKArgs {
   float* part_ml;
   float* part_o;
   uint32_t* err;
-  int rq;  // query heads of this launch per group, h0 .. h0 + rq - 1 of rtot
+  int width;  // heads a partial has room for
+  int rq;     // query heads of this launch per group, h0 .. h0 + rq - 1 of rtot
   int rtot;
   int h0;
 };
@@ -68,140 +72,359 @@ __device__ __forceinline__ RowAt row_at(const SparseKArgs& a, int s, int i) {
   return {r0 + i, (int)(keys > 0 ? keys : 0)};
 }
 
-template <int DT, int HD, int R>
-struct SparseSmem {
-  using C = DCfg<DT, HD, R, false>;
-  float p[kWavesPerBlock][C::TILE * C::PP];
+// What a wave computes: part p of the list of (row, kv head g).
+struct Part {
+  int s, row, keys, g, p;
+  size_t pair;  // row * kvh + g
+  int o0;       // offset in its first block (parts shorter than a block)
+  int T;        // tokens 0 .. T - 1; token t is at offset (t + o0) % bs of entry (t + o0) / bs
+  int id, lim;  // lane e: block and number of keys of entry e
 };
 
-// SB: block_size below 16, the tokens of a sub-tile span several blocks.
-// ONCE: one row per sequence, so no other wave reads a block's rows of a head,
-// and the loads say so.  The rows of a chunk choose much the same blocks: their
-// loads stay in the caches (42 rows of 12 chunks, 64 heads of 128, 75 blocks
-// each: 40 us against 50 with such loads; the other way 64 single rows of 128
-// blocks, 32 heads: 98 against 86).
-template <int DT, int HD, int R, bool SB, bool ONCE>
-__global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKArgs a) {
-  using C = DCfg<DT, HD, R, false>;
-  __shared__ SparseSmem<DT, HD, R> sm;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  float* p_lds = sm.p[wave];
-  const int H = a.kvh * a.rtot;
-  const int lg = a.bs_log2, BS = 1 << lg, tmask = BS - 1;
-  // item = ((sequence, row of it), part, kv head), the head fastest
-  const unsigned item = blockIdx.x * kWavesPerBlock + wave;
+// Item = ((sequence, row of it), part, kv head), the head fastest.
+__device__ __forceinline__ bool locate(const SparseKArgs& a, unsigned item, Part& w) {
   const unsigned rest = item / (unsigned)a.kvh;
-  const int g = (int)(item - rest * (unsigned)a.kvh);
+  w.g = (int)(item - rest * (unsigned)a.kvh);
   const unsigned slot = rest / (unsigned)a.parts;
-  const int p = (int)(rest - slot * (unsigned)a.parts);
-  const unsigned s = slot / (unsigned)a.max_q;
-  const int i = (int)(slot - s * (unsigned)a.max_q);
-  if (s >= (unsigned)a.n_seqs) return;
-  const RowAt at = row_at(a, (int)s, i);
-  if (at.row < 0) return;
-  const int b = at.row;
-  const size_t pair = (size_t)b * a.kvh + g;
+  w.p = (int)(rest - slot * (unsigned)a.parts);
+  w.s = (int)(slot / (unsigned)a.max_q);
+  if (w.s >= a.n_seqs) return false;
+  const RowAt at = row_at(a, w.s, (int)(slot - (unsigned)w.s * (unsigned)a.max_q));
+  w.row = at.row;
+  w.keys = at.keys;
+  w.pair = (size_t)w.row * a.kvh + w.g;
+  return at.row >= 0;
+}
 
-  const int G = lane >> 4, col = lane & 15;
-  const int c = lane % C::CH;   // 16-byte chunk of a row (PV / output mapping)
-  const int tg = lane / C::CH;  // token group of a V load
-  const int PT = a.part_tokens;
-  const int u0 = p * PT;
-  const int e0 = u0 >> lg;    // the part's first list entry
-  const int o0 = u0 & tmask;  // and offset in it (parts shorter than a block)
+// The part's list entries, the valid ones first.  T = 0: no key.
+__device__ __forceinline__ void take_list(const SparseKArgs& a, int lane, Part& w) {
+  const int lg = a.bs_log2, BS = 1 << lg, tmask = BS - 1, PT = a.part_tokens;
+  const int u0 = w.p * PT;
+  const int e0 = u0 >> lg;  // the part's first list entry
+  w.o0 = u0 & tmask;
   const int span = PT >> lg > 1 ? PT >> lg : 1;  // entries, at most 64
   int sel = -1;
-  if (lane < span && e0 + lane < a.top) sel = a.blocks[pair * a.top + e0 + lane];
-  u32x4 qf[C::NF];
-  {
-    const char* qrow = a.q + ((size_t)b * H + g * a.rtot + a.h0 + (col < a.rq ? col : 0)) * C::RB;
-#pragma unroll
-    for (int f = 0; f < C::NF; ++f)
-      qf[f] = col < a.rq ? ld16(qrow + 64 * f + 16 * G) : u32x4{0, 0, 0, 0};
-  }
-  const bool too_long = (long long)at.keys > (long long)a.mbps << lg;
-  const int keys = too_long ? a.mbps << lg : at.keys;
+  if (lane < span && e0 + lane < a.top) sel = a.blocks[w.pair * a.top + e0 + lane];
+  const bool too_long = (long long)w.keys > (long long)a.mbps << lg;
+  const int keys = too_long ? a.mbps << lg : w.keys;
   const int nb = (int)(((long long)keys + tmask) >> lg);
   bool valid = sel >= 0 && sel < nb;
   bool odd = sel >= nb;  // no block of this context
   int id = 0;
   if (valid) {
-    id = a.tables[(size_t)s * a.mbps + sel];
+    id = a.tables[(size_t)w.s * a.mbps + sel];
     if (id < 0 || id >= a.num_blocks) valid = false, odd = true;
   }
   if (odd) atomicOr(a.err, PKV_EBIT_BLOCK);
   if (too_long && lane == 0) atomicOr(a.err, PKV_EBIT_LENGTH);
   int lim = valid ? min(BS, keys - (sel << lg)) : 0;  // the block's keys
-  valid = lim > o0;
+  valid = lim > w.o0;
   const unsigned long long have = __ballot(valid);
   const int nv = __popcll(have);
+  const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32),
+                                              __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
+  const int to = (valid ? below : nv + lane - below) << 2;
+  w.id = __builtin_amdgcn_ds_permute(to, id);
+  w.lim = __builtin_amdgcn_ds_permute(to, lim);
+  w.T = nv == 0                ? 0
+        : w.o0 || PT < BS      ? min(PT, readlane_i(w.lim, 0) - w.o0)
+                               : ((nv - 1) << lg) + readlane_i(w.lim, nv - 1);
+}
 
-  // where the part's result goes
-  float* ml = a.part_ml + (pair * a.parts + p) * kMlFloats;
-  float* po = a.part_o + (pair * a.parts + p) * R * HD;
-  if (nv == 0) {
-    if (a.parts > 1) {  // (the merge reads no rows of a part whose l is 0)
-      if (lane < kMlFloats) ml[lane] = lane & 1 ? 0.0f : kLowest;
-    } else if (lane < C::CH) {
-      float z[C::EPL];
+// A part without keys: zero rows, or l = 0 for the merge (which reads no rows
+// of such a part).
+__device__ __forceinline__ void store_nothing(const SparseKArgs& a, const Part& w, int lane, int hd) {
+  if (a.parts > 1) {
+    float* ml = a.part_ml + (w.pair * a.parts + w.p) * kMlFloats;
+    if (lane < kMlFloats) ml[lane] = lane & 1 ? 0.0f : kLowest;
+    return;
+  }
+  const size_t at = (w.pair * a.rtot + a.h0) * hd;
+  for (int i = lane; i < a.rq * hd; i += kWave) {
+    if (a.out_f32) reinterpret_cast<float*>(a.out)[at + i] = 0.0f;
+    else reinterpret_cast<uint16_t*>(a.out)[at + i] = 0;
+  }
+}
+
+// Rows of a part's tokens in a pool of one kv head.  SB: block_size below 16,
+// so the tokens of a sub-tile span several blocks.
+template <bool SB>
+struct Rows {
+  const Part& w;
+  int lg, tmask;
+  size_t slot_stride, blk_stride;
+  __device__ __forceinline__ Rows(const SparseKArgs& a, const Part& p, int row_bytes)
+      : w(p), lg(a.bs_log2), tmask((1 << a.bs_log2) - 1), slot_stride((size_t)a.kvh * row_bytes),
+        blk_stride(slot_stride << a.bs_log2) {}
+  __device__ __forceinline__ int lane_of(int v, int t) const {
+    return __builtin_amdgcn_ds_bpermute(((t + w.o0) >> lg) << 2, v);
+  }
+  // Row of token t; t0: a wave-uniform token of the same block.  Tokens past
+  // the block's keys give its last one.
+  __device__ __forceinline__ const char* row(const char* pool, int t0, int t) const {
+    const int off = (t + w.o0) & tmask;
+    if constexpr (SB)
+      return pool + (size_t)lane_of(w.id, t) * blk_stride +
+             (uint32_t)(min(off, lane_of(w.lim, t) - 1) * slot_stride);
+    const int e = (t0 + w.o0) >> lg;
+    return pool + (size_t)readlane_i(w.id, e) * blk_stride +
+           (uint32_t)(min(off, readlane_i(w.lim, e) - 1) * slot_stride);
+  }
+  // Row of token base + i of a run of up to 16, in one block without SB.
+  __device__ __forceinline__ const char* run(const char* pool, int base, int i) const {
+    return row(pool, min(base, w.T - 1), min(base + i, w.T - 1));
+  }
+  // How many tokens of the 16 from t0 on are attended (not SB).
+  __device__ __forceinline__ int live16(int t0) const {
+    const int at = t0 + w.o0;
+    return t0 < w.T ? min(w.T - t0, readlane_i(w.lim, at >> lg) - (at & tmask)) : 0;
+  }
+  __device__ __forceinline__ bool live(int t) const {
+    const int lim = lane_of(w.lim, min(t, w.T - 1));
+    return t < w.T && ((t + w.o0) & tmask) < lim;
+  }
+};
+
+// ONCE: one row per sequence, so no other wave reads a block's rows of a head,
+// and the loads say so.  The rows of a chunk choose much the same blocks: their
+// loads stay in the caches (42 rows of 12 chunks, 64 heads of 128, 75 blocks
+// each: 40 us against 50 with such loads; the other way 64 single rows of 128
+// blocks, 32 heads: 98 against 86).
+template <bool ONCE>
+__device__ __forceinline__ u32x4 ld_row(const char* x) {
+  return ONCE ? ld16_stream(x) : ld16(x);
+}
+
+// ---- 16-bit pools ------------------------------------------------------------
+
+template <int HD>
+struct Cfg16 {
+  static constexpr int RB = HD * 2;
+  static constexpr int NF = RB / 64;   // 16-byte fragments per lane of a row
+  static constexpr int CH = RB / 16;   // 16-byte chunks of a row
+  static constexpr int TPL = 64 / CH;  // tokens per V load
+  static constexpr int TILE = 32;      // tokens: two sub-tiles of S^T, one k-step of O^T
+  static constexpr int NV = TILE / TPL;
+  static constexpr int ND = HD / 16;   // 16-dim tiles of O^T
+  static constexpr int VP = RB + 32;   // pitch of a V row in LDS
+};
+
+// Weights above 2^kRise raise the running maximum: until then the sums need no
+// rescaling.  f16 weights carry 2^kLift more, out of the range of its subnormals.
+constexpr float kRise = 8.0f, kLift = 7.0f;
+
+// One wave, 32 tokens a tile.
+//  S^T = K Q^T: K fragments from the pool are the A operand (lane: token lane %
+//   16, 64 contiguous bytes of a row per four lanes), the heads' Q the B
+//   operand, so lane (G, c) gets head c's scores of tokens 4 G .. 4 G + 3 of each
+//   sub-tile: the softmax state of a head sits in its column's four lanes.
+//  O^T = V^T P^T: those scores are the lane's slice of the B operand as they
+//   are, with the k-step's tokens taken in that order; V goes through the wave's
+//   LDS and is read transposed.  P enters as the sum of three bf16 parts (24
+//   bits) or two f16 ones (22), so the weights lose nothing: error against 64
+//   bits as with P.V in f32 multiply-adds, which took 1020 vector instructions a
+//   tile at 8 heads of 128.
+// The next tile's K is loaded when this one's scores are there, its V when this
+// one's is in LDS.
+template <int DT, int HD, bool SB, bool ONCE>
+__global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(SparseKArgs a) {
+  using C = Cfg16<HD>;
+  __shared__ alignas(16) char v_lds_all[kWavesPerBlock][C::TILE * C::VP];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int G = lane >> 4, col = lane & 15;
+  char* v_lds = v_lds_all[wave];
+  Part w;
+  if (!locate(a, blockIdx.x * kWavesPerBlock + wave, w)) return;
+  u32x4 qf[C::NF];
+  {
+    const char* qrow = a.q + (w.pair * a.rtot + a.h0 + (col < a.rq ? col : 0)) * C::RB;
 #pragma unroll
-      for (int e = 0; e < C::EPL; ++e) z[e] = 0.0f;
-      for (int h = 0; h < a.rq; ++h)
-        store_out<C::EPL>(a.out, ((size_t)b * H + g * a.rtot + a.h0 + h) * HD + c * C::EPL,
-                          a.out_f32, DT, z);
+    for (int f = 0; f < C::NF; ++f)
+      qf[f] = col < a.rq ? ld16(qrow + 64 * f + 16 * G) : u32x4{0, 0, 0, 0};
+  }
+  take_list(a, lane, w);
+  if (w.T == 0) {
+    store_nothing(a, w, lane, HD);
+    return;
+  }
+  const Rows<SB> rows(a, w, C::RB);
+  const char* kh = a.k_pool + (size_t)w.g * C::RB + 16 * G;
+  const int c = lane % C::CH, tg = lane / C::CH;
+  const char* vh = a.v_pool + (size_t)w.g * C::RB + 16 * c;
+
+  u32x4 kf[2][C::NF], vf[C::NV];
+  auto load_k = [&](int base) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const char* r = rows.run(kh, base + 16 * st, col);
+#pragma unroll
+      for (int f = 0; f < C::NF; ++f) kf[st][f] = ld_row<ONCE>(r + 64 * f);
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < C::NV; ++i) vf[i] = ld_row<ONCE>(rows.run(vh, base + i * C::TPL, tg));
+  };
+  float m = kLowest, l = 0.0f;
+  f32x4 o[C::ND];
+#pragma unroll
+  for (int d = 0; d < C::ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  load_k(0);
+  load_v(0);
+
+  for (int base = 0; base < w.T; base += C::TILE) {
+    const bool more = base + C::TILE < w.T;
+    f32x4 sc[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      sc[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int f = 0; f < C::NF; ++f) mfma_frag<DT>(kf[st][f], qf[f], sc[st]);
+    }
+    // V rows to LDS: token i TPL + tg of the tile
+#pragma unroll
+    for (int i = 0; i < C::NV; ++i) st16(v_lds + (i * C::TPL + tg) * C::VP + 16 * c, vf[i]);
+    __builtin_amdgcn_wave_barrier();
+    if (more) {
+      load_v(base + C::TILE);
+      load_k(base + C::TILE);
+    }
+    // scores in the exp2 domain, tokens that are not attended at -inf
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int t0 = base + 16 * st;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[st][j] *= a.scale_log2;
+      if constexpr (SB) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!rows.live(t0 + 4 * G + j)) sc[st][j] = -INFINITY;
+      } else {
+        const int n = rows.live16(t0);
+        if (n < 16) {  // wave-uniform
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (4 * G + j >= n) sc[st][j] = -INFINITY;
+        }
+      }
+    }
+    float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+    top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    if (__any(top > m + kRise)) {  // the first tile, and seldom after it
+      top = row_group_max(top);
+      if (top > m + kRise) {
+        const float alpha = fast_exp2(m - top);
+        m = top;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < C::ND; ++d) o[d] *= alpha;
+      }
+    }
+    const float shift = DT == PKV_F16 ? kLift - m : -m;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = fast_exp2(sc[i >> 2][i & 3] + shift);
+      l += p[i];
+    }
+    // the weights' parts as B operands
+    constexpr int NP = DT == PKV_BF16 ? 3 : 2;
+    u32x4 part[NP];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x0 = p[2 * i], x1 = p[2 * i + 1];
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const uint32_t b = cvt_pk16<DT>(x0, x1);
+        part[k][i] = b;
+        x0 -= DT == PKV_BF16 ? bf16lo(b) : f16lo(b);
+        x1 -= DT == PKV_BF16 ? bf16hi(b) : f16hi(b);
+      }
+    }
+    // A operand: lane (dim 16 d + col, group G) needs tokens 4 G .. 4 G + 3 of
+    // both sub-tiles.  ds_read_b64_tr_b16 gives lane i of a 16-lane group, element
+    // j, the (i & 3)-th value at the address of lane 4 j + (i >> 2).
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    const char* vt = v_lds + (4 * G + (col >> 2)) * C::VP + 8 * (col & 3);
+#pragma unroll
+    for (int d = 0; d < C::ND; ++d) {
+      const uint2 lo = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + 32 * d)));
+      const uint2 hi = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vt + 32 * d + 16 * C::VP)));
+      const u32x4 va{lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int k = 0; k < NP; ++k) mfma_frag<DT>(va, part[k], o[d]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  l = swap32_sum(swap16_sum(l));
+
+  // lane: head col, dims 16 d + 4 G .. + 3
+  if (a.parts > 1) {
+    float* ml = a.part_ml + (w.pair * a.parts + w.p) * kMlFloats;
+    float* po = a.part_o + ((w.pair * a.parts + w.p) * a.width + col) * HD + 4 * G;
+    if (G == 0) {
+      ml[2 * col] = m;
+      ml[2 * col + 1] = l;
+    }
+    if (col < a.rq) {
+#pragma unroll
+      for (int d = 0; d < C::ND; ++d) *reinterpret_cast<f32x4*>(po + 16 * d) = o[d];
     }
     return;
   }
-  // valid entries to the front, the others behind them
-  {
-    const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32),
-                                                __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
-    const int to = (valid ? below : nv + lane - below) << 2;
-    id = __builtin_amdgcn_ds_permute(to, id);
-    lim = __builtin_amdgcn_ds_permute(to, lim);
-  }
-  // tokens 0 .. T - 1 of the part: token t is at offset (t + o0) % BS of entry
-  // (t + o0) / BS
-  const int T = o0 || PT < BS ? min(PT, readlane_i(lim, 0) - o0)
-                              : ((nv - 1) << lg) + readlane_i(lim, nv - 1);
-
-  const size_t head_off = (size_t)g * C::RB;
-  const size_t slot_stride = (size_t)a.kvh * C::RB;
-  const char* kh = a.k_pool + head_off;
-  const char* vh = a.v_pool + head_off;
-  const size_t blk_stride = (size_t)BS * slot_stride;
-  auto ld = [](const char* x) { return ONCE ? ld16_stream(x) : ld16(x); };
-  auto lane_of = [&](int v, int t) {
-    return __builtin_amdgcn_ds_bpermute(((t + o0) >> lg) << 2, v);
-  };
-  // Row of token t in `pool`; t0: a wave-uniform token of the same block.
-  auto row_of = [&](const char* pool, int t0, int t) {
-    const int off = (t + o0) & tmask;
-    if constexpr (SB)
-      return pool + (size_t)lane_of(id, t) * blk_stride +
-             (uint32_t)(min(off, lane_of(lim, t) - 1) * slot_stride);
-    const int e = (t0 + o0) >> lg;
-    return pool + (size_t)readlane_i(id, e) * blk_stride +
-           (uint32_t)(min(off, readlane_i(lim, e) - 1) * slot_stride);
-  };
-  auto k_row = [&](int tile_base, int st) {
-    const int t0 = min(tile_base + 16 * st, T - 1);
-    return row_of(kh, t0, min(tile_base + 16 * st + col, T - 1)) + 16 * G;
-  };
-  auto v_chunk = [&](int tile_base, int k) {
-    const int t0 = min(tile_base + k * C::TPL, T - 1);
-    return row_of(vh, t0, min(tile_base + k * C::TPL + tg, T - 1)) + 16 * c;
-  };
-  // whether token t (sub-tile token t0 + col) is attended
-  auto live = [&](int t0, int t) {
-    const int off = (t + o0) & tmask;
-    if constexpr (SB) {
-      const int l = lane_of(lim, min(t, T - 1));
-      return t < T && off < l;
+  if (col >= a.rq) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const size_t at = (w.pair * a.rtot + a.h0 + col) * HD + 4 * G;
+#pragma unroll
+  for (int d = 0; d < C::ND; ++d) {
+    const f32x4 x = o[d] * inv;
+    if (a.out_f32) {
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) + at + 16 * d) = x;
+    } else {
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at + 16 * d) =
+          uint2{cvt_pk16<DT>(x[0], x[1]), cvt_pk16<DT>(x[2], x[3])};
     }
-    return t < T && off < readlane_i(lim, (min(t0, T - 1) + o0) >> lg);
-  };
+  }
+}
+
+// ---- f32 pools ---------------------------------------------------------------
+
+// The decode kernel's tile: scores on v_mfma_f32_16x16x4f32, P.V in f32
+// multiply-adds with the weights handed over through LDS.
+template <int HD, int R, bool SB, bool ONCE>
+__global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse32_kernel(SparseKArgs a) {
+  constexpr int DT = PKV_F32;
+  using C = DCfg<DT, HD, R, false>;
+  __shared__ float p_lds_all[kWavesPerBlock][C::TILE * C::PP];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  float* p_lds = p_lds_all[wave];
+  const int G = lane >> 4, col = lane & 15;
+  Part w;
+  if (!locate(a, blockIdx.x * kWavesPerBlock + wave, w)) return;
+  u32x4 qf[C::NF];
+  {
+    const char* qrow = a.q + (w.pair * a.rtot + a.h0 + (col < a.rq ? col : 0)) * C::RB;
+#pragma unroll
+    for (int f = 0; f < C::NF; ++f)
+      qf[f] = col < a.rq ? ld16(qrow + 64 * f + 16 * G) : u32x4{0, 0, 0, 0};
+  }
+  take_list(a, lane, w);
+  if (w.T == 0) {
+    store_nothing(a, w, lane, HD);
+    return;
+  }
+  const Rows<SB> rows(a, w, C::RB);
+  const int c = lane % C::CH;   // 16-byte chunk of a row (PV / output mapping)
+  const int tg = lane / C::CH;  // token group of a V load
+  const char* kh = a.k_pool + (size_t)w.g * C::RB + 16 * G;
+  const char* vh = a.v_pool + (size_t)w.g * C::RB + 16 * c;
+  auto k_row = [&](int base, int st) { return rows.run(kh, base + 16 * st, col); };
+  auto v_chunk = [&](int base, int k) { return rows.run(vh, base + k * C::TPL, tg); };
 
   float m[4], lsum[4];
 #pragma unroll
@@ -215,17 +438,17 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
 #pragma unroll
     for (int e = 0; e < C::EPL; ++e) o[h][e] = 0.0f;
 
-  const int ntiles = (T + C::TILE - 1) / C::TILE;
+  const int ntiles = (w.T + C::TILE - 1) / C::TILE;
   u32x4 kf[C::NST][C::NF];
   u32x4 vf[C::NV];
 #pragma unroll
   for (int st = 0; st < C::NST; ++st) {
     const char* r = k_row(0, st);
 #pragma unroll
-    for (int f = 0; f < C::NF; ++f) kf[st][f] = ld(r + 64 * f);
+    for (int f = 0; f < C::NF; ++f) kf[st][f] = ld_row<ONCE>(r + 64 * f);
   }
 #pragma unroll
-  for (int k = 0; k < C::NV; ++k) vf[k] = ld(v_chunk(0, k));
+  for (int k = 0; k < C::NV; ++k) vf[k] = ld_row<ONCE>(v_chunk(0, k));
 
   // One tile, the next one's loads issued as the registers come free.
   auto tile_body = [&](const int tile_base, auto prefetch) {
@@ -240,14 +463,14 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
       if constexpr (PF) {
         const char* r = k_row(next, st);
 #pragma unroll
-        for (int f = 0; f < C::NF; ++f) kf[st][f] = ld(r + 64 * f);
+        for (int f = 0; f < C::NF; ++f) kf[st][f] = ld_row<ONCE>(r + 64 * f);
       }
     }
     float sc[C::NST][4];
 #pragma unroll
     for (int st = 0; st < C::NST; ++st) {
       const int t0 = tile_base + 16 * st;
-      const bool ok = live(t0, t0 + col);
+      const bool ok = SB ? rows.live(t0 + col) : col < rows.live16(t0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) sc[st][j] = ok ? acc[st][j] * a.scale_log2 : -INFINITY;
     }
@@ -304,7 +527,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
       }
       float x[C::EPL];
       widen16<DT, C::EPL>(vf[k], x);
-      if constexpr (PF) vf[k] = ld(v_chunk(next, k));
+      if constexpr (PF) vf[k] = ld_row<ONCE>(v_chunk(next, k));
 #pragma unroll
       for (int h = 0; h < R; ++h)
 #pragma unroll
@@ -323,41 +546,25 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
   for (int h = 0; h < R; ++h)
 #pragma unroll
     for (int e = 0; e < C::EPL; ++e) o[h][e] = group_sum<C::CH>(o[h][e]);
-  float mh[R], lh[R];
+  float* ml = a.part_ml + (w.pair * a.parts + w.p) * kMlFloats;
+  float* po = a.part_o + (w.pair * a.parts + w.p) * a.width * HD;
 #pragma unroll
   for (int h = 0; h < R; ++h) {
-    mh[h] = readlane_f(m[h & 3], 16 * (h >> 2));
-    lh[h] = readlane_f(lsum[h & 3], 16 * (h >> 2));
-  }
-  if (a.parts == 1) {
-#pragma unroll
-    for (int h = 0; h < R; ++h) {
-      if (h % NG != tg || h >= a.rq) continue;
-      const float inv = lh[h] == 0.0f ? 0.0f : 1.0f / lh[h];
-      float x[C::EPL];
-#pragma unroll
-      for (int e = 0; e < C::EPL; ++e) x[e] = o[h][e] * inv;
-      store_out<C::EPL>(a.out, ((size_t)b * H + g * a.rtot + a.h0 + h) * HD + c * C::EPL,
-                        a.out_f32, DT, x);
+    const float mh = readlane_f(m[h & 3], 16 * (h >> 2));
+    const float lh = readlane_f(lsum[h & 3], 16 * (h >> 2));
+    if (a.parts > 1 && lane == 0) {
+      ml[2 * h] = mh;
+      ml[2 * h + 1] = lh;
     }
-    return;
-  }
-  // partials in whole lines, as the decode kernel's: quad j of a lane's
-  // elements goes to float 4 CH j + 4 c of the head's partial row
-#pragma unroll
-  for (int h = 0; h < R; ++h) {
     if (h % NG != tg || h >= a.rq) continue;
-#pragma unroll
-    for (int e = 0; e < C::EPL; e += 4)
-      __builtin_nontemporal_store(f32x4{o[h][e], o[h][e + 1], o[h][e + 2], o[h][e + 3]},
-                                  reinterpret_cast<f32x4*>(po + h * HD + C::CH * e + 4 * c));
-  }
-  if (lane < kMlFloats) {
-    float v = 0.0f;
-#pragma unroll
-    for (int h = 0; h < R; ++h)
-      if ((lane >> 1) == h) v = (lane & 1) ? lh[h] : mh[h];
-    __builtin_nontemporal_store(v, ml + lane);
+    f32x4 x{o[h][0], o[h][1], o[h][2], o[h][3]};
+    if (a.parts > 1) {
+      *reinterpret_cast<f32x4*>(po + h * HD + 4 * c) = x;
+    } else {
+      x *= lh == 0.0f ? 0.0f : 1.0f / lh;
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) +
+                                (w.pair * a.rtot + a.h0 + h) * HD + 4 * c) = x;
+    }
   }
 }
 
@@ -367,7 +574,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse_kernel(SparseKA
 // first ones and the (m, l) pairs of up to 64 parts go out together.
 template <int HD>
 __global__ void __launch_bounds__(kWavesPerBlock * kWave)
-    sparse_merge_kernel(SparseKArgs a, int R, int dt) {
+    sparse_merge_kernel(SparseKArgs a, int dt) {
   constexpr int LPR = HD / 4;
   constexpr int PPI = kWave / LPR;
   constexpr int U = HD == 64 ? 4 : 8;
@@ -385,8 +592,8 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
   const size_t pair = (size_t)at.row * a.kvh + g;
   const float* ml = a.part_ml + pair * a.parts * kMlFloats + 2 * h;
   const int q = lane / LPR, c = lane % LPR;
-  const float* po = a.part_o + (pair * a.parts * R + h) * HD + 4 * c;
-  const size_t row = (size_t)R * HD;
+  const float* po = a.part_o + (pair * a.parts * a.width + h) * HD + 4 * c;
+  const size_t row = (size_t)a.width * HD;
   f32x4 ov[U];
   auto load = [&](int p0) {
 #pragma unroll
@@ -434,11 +641,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
   }
   if (lane >= LPR) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  // chunk c of a partial row holds elements (c % CH) EPL + 4 (c / CH) ..
-  const int epl = dt == PKV_F32 ? 4 : 8;
-  const int chs = HD / epl;
-  const size_t eo = ((size_t)at.row * a.kvh * a.rtot + g * a.rtot + a.h0 + h) * HD +
-                    (c % chs) * epl + 4 * (c / chs);
+  const size_t eo = (pair * a.rtot + a.h0 + h) * HD + 4 * c;
   if (a.out_f32) {
     *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) + eo) =
         f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
@@ -453,33 +656,45 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
   }
 }
 
-template <int DT, int HD, int R>
-void launch_main(const SparseKArgs& k, unsigned grid, hipStream_t s) {
-  constexpr int kThreads = kWavesPerBlock * kWave;
-  if (k.bs_log2 < 4) sparse_kernel<DT, HD, R, true, false><<<grid, kThreads, 0, s>>>(k);
-  else if (k.max_q > 1) sparse_kernel<DT, HD, R, false, false><<<grid, kThreads, 0, s>>>(k);
-  else sparse_kernel<DT, HD, R, false, true><<<grid, kThreads, 0, s>>>(k);
-}
+constexpr int kThreads = kWavesPerBlock * kWave;
 
 template <int DT, int HD>
-hipError_t launch_r(int R, const SparseKArgs& k, unsigned grid, hipStream_t s) {
-  switch (R) {
-    case 1: launch_main<DT, HD, 1>(k, grid, s); break;
-    case 2: launch_main<DT, HD, 2>(k, grid, s); break;
-    case 4: launch_main<DT, HD, 4>(k, grid, s); break;
-    case 8: launch_main<DT, HD, 8>(k, grid, s); break;
-    default: launch_main<DT, HD, 16>(k, grid, s); break;
-  }
-  return hipGetLastError();
+void launch16(const SparseKArgs& k, unsigned grid, hipStream_t s) {
+  if (k.bs_log2 < 4) sparse16_kernel<DT, HD, true, false><<<grid, kThreads, 0, s>>>(k);
+  else if (k.max_q > 1) sparse16_kernel<DT, HD, false, false><<<grid, kThreads, 0, s>>>(k);
+  else sparse16_kernel<DT, HD, false, true><<<grid, kThreads, 0, s>>>(k);
 }
 
-template <int DT>
-hipError_t launch_hd(int HD, int R, const SparseKArgs& k, unsigned grid, hipStream_t s) {
-  switch (HD) {
-    case 64: return launch_r<DT, 64>(R, k, grid, s);
-    case 128: return launch_r<DT, 128>(R, k, grid, s);
-    default: return launch_r<DT, 256>(R, k, grid, s);
+template <int HD, int R>
+void launch32_r(const SparseKArgs& k, unsigned grid, hipStream_t s) {
+  if (k.bs_log2 < 4) sparse32_kernel<HD, R, true, false><<<grid, kThreads, 0, s>>>(k);
+  else if (k.max_q > 1) sparse32_kernel<HD, R, false, false><<<grid, kThreads, 0, s>>>(k);
+  else sparse32_kernel<HD, R, false, true><<<grid, kThreads, 0, s>>>(k);
+}
+
+template <int HD>
+void launch32(const SparseKArgs& k, unsigned grid, hipStream_t s) {
+  switch (k.width) {
+    case 1: launch32_r<HD, 1>(k, grid, s); break;
+    case 2: launch32_r<HD, 2>(k, grid, s); break;
+    case 4: launch32_r<HD, 4>(k, grid, s); break;
+    case 8: launch32_r<HD, 8>(k, grid, s); break;
+    default: launch32_r<HD, 16>(k, grid, s); break;
   }
+}
+
+template <int HD>
+hipError_t launch_hd(int dt, const SparseKArgs& k, unsigned grid, unsigned merge_grid,
+                     hipStream_t s) {
+  switch (dt) {
+    case PKV_F32: launch32<HD>(k, grid, s); break;
+    case PKV_F16: launch16<PKV_F16, HD>(k, grid, s); break;
+    default: launch16<PKV_BF16, HD>(k, grid, s); break;
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || k.parts == 1) return e;
+  sparse_merge_kernel<HD><<<merge_grid, kThreads, 0, s>>>(k, dt);
+  return hipGetLastError();
 }
 
 struct SparsePlan {
@@ -487,12 +702,13 @@ struct SparsePlan {
   size_t ml, bytes;
 };
 
-// Parts of 1024 tokens, halved (down to 64) while the call has fewer than
-// 1024 waves, one per SIMD, and while a part has more than the 64 list entries of
-// a wave.  Eight heads and more keep a wave at P.V for longer, so they get half
-// as many waves again.  (us, main kernel and merge, parts of 128 / 256 / 512 /
-// 1024: 64 rows of 2048 tokens, 32 heads on 8 of 128: 112 / 101 / 95 / 91; 42 rows
-// of 1200, 64 heads: 64 / 57 / 80 / 87.)
+// Parts of 1024 tokens, halved (down to 64) while a part has more than the 64
+// list entries of a wave, and while the call has fewer than 1024 waves, one per
+// SIMD; 2048 for chunks, whose rows hit the caches and are bound by the waves'
+// own steps.  (us, main kernel and merge, from 1024 / 2048 waves, bf16: 42 chunk rows
+// of 1200 tokens, 64 heads on 8 of 128: 53 / 38; single rows: 64 of 2048 tokens, 32
+// heads: 93 / 90; 32 of 2048, 64 heads: 49 / 53; 32 of 1600, 16 heads of 256 (f16):
+// 81 / 93.)
 SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   SparsePlan pl{};
   while ((1 << pl.bs_log2) < p->block_size) ++pl.bs_log2;
@@ -500,7 +716,7 @@ SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   const long long len = (long long)a.top_blocks << pl.bs_log2;
   const long long pairs = (long long)a.total_q * p->n_kv_head;
   int pt = 1024;
-  while (pt > 64 && pairs * ((len + pt - 1) / pt) < (pl.R < 8 ? 1024 : 1536)) pt >>= 1;
+  while (pt > 64 && pairs * ((len + pt - 1) / pt) < (a.max_q_len > 1 ? 2048 : 1024)) pt >>= 1;
   while (pt > 64 && (pt >> pl.bs_log2) > 64) pt >>= 1;
   pl.part_tokens = pt;
   pl.parts = (int)((len + pt - 1) / pt);
@@ -518,7 +734,11 @@ long long sparse_items(const pkv_pool* p, const SparseArgs& a, int parts) {
 }  // namespace
 
 size_t sparse_workspace_bytes(const pkv_pool* p, const SparseArgs& a) {
-  return sparse_plan(p, a).bytes;
+  SparseArgs x = a;  // of single rows and of chunks, whichever is more
+  size_t most = 0;
+  for (x.max_q_len = 1; x.max_q_len <= 2; ++x.max_q_len)
+    most = std::max(most, sparse_plan(p, x).bytes);
+  return most;
 }
 
 bool sparse_fits(const pkv_pool* p, const SparseArgs& a) {
@@ -554,28 +774,22 @@ hipError_t launch_sparse(const pkv_pool* p, int layer, const SparseArgs& a, char
   k.part_ml = reinterpret_cast<float*>(ws);
   k.part_o = reinterpret_cast<float*>(ws + pl.ml);
   k.err = p->err;
+  k.width = pl.R;
   k.rtot = a.n_head / p->n_kv_head;
   const unsigned grid =
       (unsigned)((sparse_items(p, a, pl.parts) + kWavesPerBlock - 1) / kWavesPerBlock);
   // slices of at most 16 query heads per group share the workspace in turn
   for (k.h0 = 0; k.h0 < k.rtot; k.h0 += 16) {
     k.rq = std::min(k.rtot - k.h0, pl.R);
+    const unsigned merge_grid =
+        (unsigned)((sparse_items(p, a, k.rq) + kWavesPerBlock - 1) / kWavesPerBlock);
     hipError_t e;
-    switch (p->dtype) {
-      case PKV_F32: e = launch_hd<PKV_F32>(p->head_dim, pl.R, k, grid, stream); break;
-      case PKV_F16: e = launch_hd<PKV_F16>(p->head_dim, pl.R, k, grid, stream); break;
-      default: e = launch_hd<PKV_BF16>(p->head_dim, pl.R, k, grid, stream); break;
+    switch (p->head_dim) {
+      case 64: e = launch_hd<64>(p->dtype, k, grid, merge_grid, stream); break;
+      case 128: e = launch_hd<128>(p->dtype, k, grid, merge_grid, stream); break;
+      default: e = launch_hd<256>(p->dtype, k, grid, merge_grid, stream); break;
     }
     if (e != hipSuccess) return e;
-    if (pl.parts == 1) continue;
-    const unsigned mgrid =
-        (unsigned)((sparse_items(p, a, k.rq) + kWavesPerBlock - 1) / kWavesPerBlock);
-    switch (p->head_dim) {
-      case 64: sparse_merge_kernel<64><<<mgrid, kWavesPerBlock * kWave, 0, stream>>>(k, pl.R, p->dtype); break;
-      case 128: sparse_merge_kernel<128><<<mgrid, kWavesPerBlock * kWave, 0, stream>>>(k, pl.R, p->dtype); break;
-      default: sparse_merge_kernel<256><<<mgrid, kWavesPerBlock * kWave, 0, stream>>>(k, pl.R, p->dtype); break;
-    }
-    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
 }
