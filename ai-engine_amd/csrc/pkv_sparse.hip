@@ -52,6 +52,7 @@ struct SparseKArgs {
   float* part_o;
   uint32_t* err;
   int width;  // heads a partial has room for
+  int joined;  // 16-bit pools: a workgroup's waves are the parts of one (row, kv head)
   int rq;     // query heads of this launch per group, h0 .. h0 + rq - 1 of rtot
   int rtot;
   int h0;
@@ -81,12 +82,14 @@ struct Part {
   int id, lim;  // lane e: block and number of keys of entry e
 };
 
-// Item = ((sequence, row of it), part, kv head), the head fastest.
-__device__ __forceinline__ bool locate(const SparseKArgs& a, unsigned item, Part& w) {
+// Item = ((sequence, row of it), part, kv head), the head fastest; joined: the
+// workgroup's ((sequence, row), kv head) and the wave's part.
+__device__ __forceinline__ bool locate(const SparseKArgs& a, int wave, Part& w) {
+  const unsigned item = a.joined ? blockIdx.x : blockIdx.x * kWavesPerBlock + wave;
   const unsigned rest = item / (unsigned)a.kvh;
   w.g = (int)(item - rest * (unsigned)a.kvh);
-  const unsigned slot = rest / (unsigned)a.parts;
-  w.p = (int)(rest - slot * (unsigned)a.parts);
+  const unsigned slot = a.joined ? rest : rest / (unsigned)a.parts;
+  w.p = a.joined ? wave : (int)(rest - slot * (unsigned)a.parts);
   w.s = (int)(slot / (unsigned)a.max_q);
   if (w.s >= a.n_seqs) return false;
   const RowAt at = row_at(a, w.s, (int)(slot - (unsigned)w.s * (unsigned)a.max_q));
@@ -207,6 +210,10 @@ struct Cfg16 {
   static constexpr int NV = TILE / TPL;
   static constexpr int ND = HD / 16;   // 16-dim tiles of O^T
   static constexpr int VP = RB + 32;   // pitch of a V row in LDS
+  static constexpr int LDS = TILE * VP;  // of a wave: its V tile, later its O
+  // Most waves of a workgroup: their registers fit with 4, 2 and 1 per SIMD.
+  static constexpr int WAVES = HD == 64 ? 16 : HD == 128 ? 8 : 4;
+  static_assert(16 * HD * 4 <= LDS, "O of 16 heads");
 };
 
 // Weights above 2^kRise raise the running maximum: until then the sums need no
@@ -224,18 +231,21 @@ constexpr float kRise = 8.0f, kLift = 7.0f;
 //   bits) or two f16 ones (22), so the weights lose nothing: error against 64
 //   bits as with P.V in f32 multiply-adds, which took 1020 vector instructions a
 //   tile at 8 heads of 128.
-// The next tile's K is loaded when this one's scores are there, its V when this
-// one's is in LDS.
+// The next tile's rows are loaded when this one's scores are there and its V is
+// in LDS.
+//  Joined: the parts of a (row, kv head), equally long, are one workgroup, and
+//   their results meet in LDS: one launch, and no partial leaves the CU.
 template <int DT, int HD, bool SB, bool ONCE>
-__global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(SparseKArgs a) {
+__global__ void __launch_bounds__(Cfg16<HD>::WAVES * kWave) sparse16_kernel(SparseKArgs a) {
   using C = Cfg16<HD>;
-  __shared__ alignas(16) char v_lds_all[kWavesPerBlock][C::TILE * C::VP];
+  extern __shared__ __attribute__((aligned(16))) char v_lds_all[];  // LDS bytes a wave
+  __shared__ float ml_lds[C::WAVES][kMlFloats];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int G = lane >> 4, col = lane & 15;
-  char* v_lds = v_lds_all[wave];
+  char* v_lds = v_lds_all + wave * C::LDS;
   Part w;
-  if (!locate(a, blockIdx.x * kWavesPerBlock + wave, w)) return;
+  if (!locate(a, wave, w)) return;
   u32x4 qf[C::NF];
   {
     const char* qrow = a.q + (w.pair * a.rtot + a.h0 + (col < a.rq ? col : 0)) * C::RB;
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(Sparse
       qf[f] = col < a.rq ? ld16(qrow + 64 * f + 16 * G) : u32x4{0, 0, 0, 0};
   }
   take_list(a, lane, w);
-  if (w.T == 0) {
+  if (w.T == 0 && !a.joined) {
     store_nothing(a, w, lane, HD);
     return;
   }
@@ -270,8 +280,10 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(Sparse
   f32x4 o[C::ND];
 #pragma unroll
   for (int d = 0; d < C::ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  load_k(0);
-  load_v(0);
+  if (w.T > 0) {
+    load_k(0);
+    load_v(0);
+  }
 
   for (int base = 0; base < w.T; base += C::TILE) {
     const bool more = base + C::TILE < w.T;
@@ -363,6 +375,37 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(Sparse
   l = swap32_sum(swap16_sum(l));
 
   // lane: head col, dims 16 d + 4 G .. + 3
+  auto store = [&](size_t at, const f32x4& x) {
+    if (a.out_f32)
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) + at) = x;
+    else
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at) =
+          uint2{cvt_pk16<DT>(x[0], x[1]), cvt_pk16<DT>(x[2], x[3])};
+  };
+  const size_t out0 = (w.pair * a.rtot + a.h0) * HD;
+  if (a.joined) {
+    float* mine = reinterpret_cast<float*>(v_lds) + col * HD + 4 * G;
+#pragma unroll
+    for (int d = 0; d < C::ND; ++d) *reinterpret_cast<f32x4*>(mine + 16 * d) = o[d];
+    if (G == 0) {
+      ml_lds[wave][2 * col] = m;
+      ml_lds[wave][2 * col + 1] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.rq * (HD / 4); i += a.parts * kWave) {
+      const int h = i / (HD / 4);
+      float M = kLowest, L = 0.0f;
+      for (int p = 0; p < a.parts; ++p) M = fmaxf(M, ml_lds[p][2 * h]);
+      f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int p = 0; p < a.parts; ++p) {
+        const float f = fast_exp2(ml_lds[p][2 * h] - M);
+        L += f * ml_lds[p][2 * h + 1];
+        acc += f * *reinterpret_cast<const f32x4*>(v_lds_all + p * C::LDS + i * 16);
+      }
+      store(out0 + 4 * i, acc * (L == 0.0f ? 0.0f : 1.0f / L));
+    }
+    return;
+  }
   if (a.parts > 1) {
     float* ml = a.part_ml + (w.pair * a.parts + w.p) * kMlFloats;
     float* po = a.part_o + ((w.pair * a.parts + w.p) * a.width + col) * HD + 4 * G;
@@ -378,17 +421,8 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse16_kernel(Sparse
   }
   if (col >= a.rq) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const size_t at = (w.pair * a.rtot + a.h0 + col) * HD + 4 * G;
 #pragma unroll
-  for (int d = 0; d < C::ND; ++d) {
-    const f32x4 x = o[d] * inv;
-    if (a.out_f32) {
-      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) + at + 16 * d) = x;
-    } else {
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at + 16 * d) =
-          uint2{cvt_pk16<DT>(x[0], x[1]), cvt_pk16<DT>(x[2], x[3])};
-    }
-  }
+  for (int d = 0; d < C::ND; ++d) store(out0 + col * HD + 16 * d + 4 * G, o[d] * inv);
 }
 
 // ---- f32 pools ---------------------------------------------------------------
@@ -405,7 +439,7 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave) sparse32_kernel(Sparse
   float* p_lds = p_lds_all[wave];
   const int G = lane >> 4, col = lane & 15;
   Part w;
-  if (!locate(a, blockIdx.x * kWavesPerBlock + wave, w)) return;
+  if (!locate(a, wave, w)) return;
   u32x4 qf[C::NF];
   {
     const char* qrow = a.q + (w.pair * a.rtot + a.h0 + (col < a.rq ? col : 0)) * C::RB;
@@ -660,9 +694,11 @@ constexpr int kThreads = kWavesPerBlock * kWave;
 
 template <int DT, int HD>
 void launch16(const SparseKArgs& k, unsigned grid, hipStream_t s) {
-  if (k.bs_log2 < 4) sparse16_kernel<DT, HD, true, false><<<grid, kThreads, 0, s>>>(k);
-  else if (k.max_q > 1) sparse16_kernel<DT, HD, false, false><<<grid, kThreads, 0, s>>>(k);
-  else sparse16_kernel<DT, HD, false, true><<<grid, kThreads, 0, s>>>(k);
+  const int waves = k.joined ? k.parts : kWavesPerBlock;
+  const int threads = waves * kWave, lds = waves * Cfg16<HD>::LDS;
+  if (k.bs_log2 < 4) sparse16_kernel<DT, HD, true, false><<<grid, threads, lds, s>>>(k);
+  else if (k.max_q > 1) sparse16_kernel<DT, HD, false, false><<<grid, threads, lds, s>>>(k);
+  else sparse16_kernel<DT, HD, false, true><<<grid, threads, lds, s>>>(k);
 }
 
 template <int HD, int R>
@@ -692,15 +728,24 @@ hipError_t launch_hd(int dt, const SparseKArgs& k, unsigned grid, unsigned merge
     default: launch16<PKV_BF16, HD>(k, grid, s); break;
   }
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || k.parts == 1) return e;
+  if (e != hipSuccess || k.parts == 1 || k.joined) return e;
   sparse_merge_kernel<HD><<<merge_grid, kThreads, 0, s>>>(k, dt);
   return hipGetLastError();
 }
 
+constexpr int kJoinTokens = 256, kJoinPairs = 160;
+
 struct SparsePlan {
   int bs_log2, part_tokens, parts, R;
+  bool joined;
   size_t ml, bytes;
 };
+
+int most_waves(int head_dim) {
+  return head_dim == 64    ? Cfg16<64>::WAVES
+         : head_dim == 128 ? Cfg16<128>::WAVES
+                           : Cfg16<256>::WAVES;
+}
 
 // Parts of 1024 tokens, halved (down to 64) while a part has more than the 64
 // list entries of a wave, and while the call has fewer than 1024 waves, one per
@@ -709,18 +754,36 @@ struct SparsePlan {
 // of 1200 tokens, 64 heads on 8 of 128: 53 / 38; single rows: 64 of 2048 tokens, 32
 // heads: 93 / 90; 32 of 2048, 64 heads: 49 / 53; 32 of 1600, 16 heads of 256 (f16):
 // 81 / 93.)
+// The parts of a row and kv head of a 16-bit pool are joined in one workgroup if
+// there are four or more and these workgroups cover most CUs (parts too many
+// for one are lengthened for it, up to 256 tokens).  A call, joined / with the
+// merge, us: 256 pairs of chunk rows, heads of 64, 1600 tokens: 14 / 23; 344 of 1200,
+// heads of 128: 33 / 38; 160 single rows of 1600, 64: 20 / 24; 256 of 1600, 256: 70 / 82;
+// 256 of 2048, 128, four parts: 50 / 49; but 512 of two parts: 96 / 87, and 128 pairs
+// of 2048, 128: 41 / 28, 64 of 1536: 30 / 19.
 SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   SparsePlan pl{};
   while ((1 << pl.bs_log2) < p->block_size) ++pl.bs_log2;
   pl.R = group_width(a.n_head / p->n_kv_head);
   const long long len = (long long)a.top_blocks << pl.bs_log2;
   const long long pairs = (long long)a.total_q * p->n_kv_head;
+  auto parts = [&](int pt) { return (len + pt - 1) / pt; };
   int pt = 1024;
-  while (pt > 64 && pairs * ((len + pt - 1) / pt) < (a.max_q_len > 1 ? 2048 : 1024)) pt >>= 1;
+  while (pt > 64 && pairs * parts(pt) < (a.max_q_len > 1 ? 2048 : 1024)) pt >>= 1;
   while (pt > 64 && (pt >> pl.bs_log2) > 64) pt >>= 1;
+  if (p->dtype != PKV_F32 && pairs >= kJoinPairs) {
+    const int most = most_waves(p->head_dim);
+    int longer = pt;
+    while (parts(longer) > most && longer < kJoinTokens && (2 * longer >> pl.bs_log2) <= 64)
+      longer <<= 1;
+    if (parts(longer) <= most && parts(longer) >= 4) {
+      pt = longer;
+      pl.joined = true;
+    }
+  }
   pl.part_tokens = pt;
-  pl.parts = (int)((len + pt - 1) / pt);
-  if (pl.parts > 1) {
+  pl.parts = (int)parts(pt);
+  if (pl.parts > 1 && !pl.joined) {
     pl.ml = ((size_t)pairs * pl.parts * kMlFloats * 4 + 255) / 256 * 256;
     pl.bytes = pl.ml + (size_t)pairs * pl.parts * pl.R * p->head_dim * 4;
   }
@@ -776,8 +839,10 @@ hipError_t launch_sparse(const pkv_pool* p, int layer, const SparseArgs& a, char
   k.err = p->err;
   k.width = pl.R;
   k.rtot = a.n_head / p->n_kv_head;
-  const unsigned grid =
-      (unsigned)((sparse_items(p, a, pl.parts) + kWavesPerBlock - 1) / kWavesPerBlock);
+  k.joined = pl.joined;
+  const unsigned grid = (unsigned)(
+      pl.joined ? sparse_items(p, a, 1)
+                : (sparse_items(p, a, pl.parts) + kWavesPerBlock - 1) / kWavesPerBlock);
   // slices of at most 16 query heads per group share the workspace in turn
   for (k.h0 = 0; k.h0 < k.rtot; k.h0 += 16) {
     k.rq = std::min(k.rtot - k.h0, pl.R);

@@ -997,12 +997,12 @@ class KvPool:
             if out is None:
                 out = torch.empty((rows, H * hd), dtype=out_dtype or c.dtype, device=c.device)
             need = lib().pkv_sparse_workspace_bytes(self._h, rows, H, bl.shape[2])
-            ws = _workspace(need, c.device)
+            ws = _workspace(need, c.device) if need else None
             check(lib().pkv_sparse_attention(
                 self._h, self.layer_index, _dev_ptr(qq), _dev_ptr(out), pkv_dtype(out.dtype),
                 _dev_ptr(bl), bl.shape[2], _dev_ptr(cu) if cu is not None else None,
                 _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, H, float(scale),
-                _dev_ptr(ws), need, s), self._h)
+                _dev_ptr(ws) if need else None, need, s), self._h)
         return out
 
     def _check_rows(self, t, name: str) -> None:

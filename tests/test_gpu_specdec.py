@@ -439,6 +439,30 @@ def test_sparse_attention_of_chunks(gpu, dt, H, kv, hd, bs):
     cache.close()
 
 
+@pytest.mark.parametrize("chunks", [False, True])
+@pytest.mark.parametrize("dt,H,kv,hd,bs,top,out_dt", [
+    ("bf16", 8, 8, 128, 16, 30, "f32"), ("f16", 16, 8, 64, 16, 61, "f16"),
+    ("bf16", 24, 8, 256, 16, 17, "bf16"), ("f16", 8, 8, 128, 8, 45, "f32"),
+    ("bf16", 160, 8, 64, 32, 20, "f32"), ("f32", 8, 8, 64, 16, 30, "f32")])
+def test_sparse_attention_of_many_rows(gpu, dt, H, kv, hd, bs, top, out_dt, chunks):
+    # enough (row, kv head) pairs for a workgroup each; some have few blocks or none
+    rng = np.random.default_rng(hd + top)
+    ctx = rng.integers(1, 2 * top * bs, 24)
+    ctx[::6] = rng.integers(0, 2 * bs, 4)
+    m = rng.integers(0, 4, 24) if chunks else None
+    cu = np.concatenate(([0], np.cumsum(m))) if chunks else None
+    tables, nb, _ = place(rng, ctx, bs)
+    k, v = (rounded(rng.normal(size=(nb, bs, kv, hd)), dt) for _ in range(2))
+    cache, pool = to_pool(dt, k, v, bs)
+    q = rounded(rng.normal(size=(cu[-1] if chunks else 24, H, hd)), dt)
+    blocks = choose(rng, ref.rows_of(cu, ctx), kv, top, bs, "holes")
+    blocks[::2] = choose(rng, ref.rows_of(cu, ctx), kv, top, bs, "select")[::2]
+    want, bound = ref.sparse_attention(q, k, v, blocks, tables, cu, ctx, bs, hd ** -0.5)
+    got = run_sparse(gpu, dt, cache, pool, q, blocks, tables, cu, ctx, out_dtype=TD[out_dt])
+    within(got, want, bound, out_dt)
+    cache.close()
+
+
 @pytest.mark.parametrize("dt,H,kv,hd", [("bf16", 32, 8, 128), ("f16", 7, 1, 64)])
 def test_all_blocks_is_decode_and_prefill_attention(gpu, dt, H, kv, hd):
     rng = np.random.default_rng(hd)
