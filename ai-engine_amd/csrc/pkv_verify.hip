@@ -149,7 +149,7 @@ __device__ __forceinline__ float logit_dt(int dt, const char* row, long long i) 
 }
 __device__ __forceinline__ int bytes_of(int dt) { return dt == PKV_F32 ? 4 : 2; }
 
-// c of exp(l / T) = 2^(l c); 0: greedy (T is 0, or not a positive number).
+// c of exp(l / T) = 2^(l c); 0: greedy (T is not positive or not finite: 1 / inf is 0).
 __device__ __forceinline__ double exponent(const VerifyKArgs& a, int b) {
   const float t = a.temps ? a.temps[b] : 0.0f;
   return t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0;

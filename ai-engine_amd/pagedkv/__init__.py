@@ -346,7 +346,8 @@ def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_unifor
     (drafts,) int32; cu_drafts: (batch + 1,) int32; uniforms: (drafts,) and
     final_uniforms: (batch,) float32 in [0, 1); draft_logits: (drafts, vocab)
     f32/f16/bf16, or None for drafts without a distribution; temperatures:
-    (batch,) float32, or None (all greedy; 0 is greedy).  Both logits have unit
+    (batch,) float32, or None (all greedy; so is one that is not positive
+    or not finite).  Both logits have unit
     stride along vocab.  Draft i is kept while u_i q_i(d_i) < p_i(d_i); the next
     token comes from max(p - q, 0) of the first one that is not, or from p
     after the last.  Nothing synchronises.  Returns (tokens, accepted):

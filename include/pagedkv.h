@@ -661,9 +661,10 @@ int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, in
  *   the last draft from p_n: the first token at which the running sum of these
  *   weights passes final_uniforms[b] times their total.
  * draft_logits NULL: q_i is 1 at d_i (drafts that were looked up or searched).
- * T == 0, or temperatures NULL: greedy; a draft is kept while it is the target
- * row's first maximum, and the next token is a row's first maximum.  Decisions are
- * those of 64-bit arithmetic.  A distribution cut by top-k or top-p is given
+ * T not positive or not finite, or temperatures NULL: greedy; a draft is kept
+ * while it is the target row's first maximum, and the next token is a row's first
+ * maximum.  Decisions are those of 64-bit arithmetic; in a draw a probability
+ * below 2^-400 counts as 0.  A distribution cut by top-k or top-p is given
  * by its log-probabilities with -inf elsewhere, at temperature 1.
  *  logits: rows of `vocab` values at a stride of row_stride elements, each side
  *      PKV_F32, PKV_F16 or PKV_BF16.  -inf has probability 0, and so has NaN; +inf

@@ -624,6 +624,17 @@ def test_verify_greedy_without_temperatures(gpu):
     same_verify(run_verify(gpu, "bf16", "bf16", x, d, cu, u, ul, y, np.zeros(20, np.float32)), want)
 
 
+@pytest.mark.parametrize("t", [-1.0, -0.0, np.nan, np.inf, -np.inf])
+def test_verify_temperatures_that_are_greedy(gpu, t):
+    # every third request has such a temperature; the others draw
+    x, d, cu, u, ul, y, temps = verify_case(11, 21, 700, 4, "f32", "bf16")
+    temps = np.maximum(temps, np.float32(0.3))
+    zero, given = temps.copy(), temps.copy()
+    zero[::3], given[::3] = 0.0, t
+    want = ref.verify(x, d, cu, u, ul, y, zero)
+    same_verify(run_verify(gpu, "f32", "bf16", x, d, cu, u, ul, y, given), want)
+
+
 @pytest.mark.parametrize("what", ["masked", "empty", "nan", "inf", "tokens", "edges", "same", "flat",
                                   "cold", "emptydraft", "lowest", "huge", "offset"])
 @pytest.mark.parametrize("draft", [True, False])
