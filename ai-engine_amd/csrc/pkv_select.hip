@@ -21,7 +21,9 @@
 // mostly nothing or a few blocks.
 //
 // A block with a key that is not finite (or a score past the f32 range)
-// scores +inf, and so does every block for such a query.
+// scores +inf, and so does every block for such a query.  E leaves out what
+// falls below the f32 range: scores that differ by less than some hd 2^-126 may
+// be taken for equal or in either order.
 #include <algorithm>
 
 #include "pkv_device.h"
@@ -178,7 +180,7 @@ __device__ __forceinline__ int row_blocks(const SeqRows& r, int i, int bsl, int 
 
 constexpr int group_width_of(int r) { return r >= 16 ? 16 : r > 8 ? 16 : r > 4 ? 8 : r > 2 ? 4 : r; }
 
-// max(x, 0) and min(x, 0) of the elements of a 16-byte chunk; NaN stays in both.
+// max(x, 0) and min(x, 0) of the elements of a 16-byte chunk; NaN stays in one.
 template <int DT>
 __device__ __forceinline__ void split_sign(const u32x4& w, u32x4& p, u32x4& m) {
 #pragma unroll
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(256) score_kernel(SelectKArgs a) {
   };
 
   // slices of 16 heads (one for ratios up to 16)
-  float etop = 0.0f;  // per query row, see below
+  float etop = 0.0f;  // the largest T
   for (int h0 = 0; h0 < a.rtot; h0 += 16) {
     const int rq = min(a.rtot - h0, R);
     // operand row m = (query row m / R, head m % R)

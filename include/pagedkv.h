@@ -618,9 +618,11 @@ int pkv_key_bounds(pkv_pool* pool, int layer, void* bounds, const int32_t* block
  *  first_blocks >= 0, last_blocks >= 1, first_blocks + last_blocks <= top_blocks.
  * Only the bounds of blocks between the first and last ones are used, which are
  * full: the block that a step writes to needs none.  A block with a key that is
- * not finite, one whose products' magnitudes add up past the f32 range, and any block for a query
- * that is not finite rank first.  Block ids outside the pool are reported by
- * pkv_pool_check(). */
+ * not finite, one whose products' magnitudes add up past the f32 range, and any
+ * block for a query that is not finite rank first.  Scores
+ * that differ by less than about head_dim * 2^-126 may be ranked either way.
+ * Block ids outside the pool are reported by pkv_pool_check().  Workspace: about
+ * 12 bytes per row, kv head and block of max_context_len. */
 size_t pkv_select_workspace_bytes(const pkv_pool* pool, int n_seqs, int total_q, int max_q_len,
                                   int max_context_len, int max_blocks_per_seq, int n_head);
 int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t* blocks,
@@ -640,7 +642,8 @@ int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t
  *  blocks: int32 [total_q][n_kv_head][top_blocks], distinct indexes in any order;
  *      negative entries are skipped.  An index past the row's context or a
  *      block id outside the pool is skipped and reported by pkv_pool_check().
- *      A row and kv head without any key is zero.
+ *      A row and kv head without any key is zero.  Attended keys and values are
+ *      to be finite: with others that row and kv head may come out as NaN.
  * total_q, n_kv_head and parts (top_blocks * block_size / 64 at most) multiply to
  * less than 2^26 (else PKV_ERR_UNSUPPORTED). */
 size_t pkv_sparse_workspace_bytes(const pkv_pool* pool, int total_q, int n_head, int top_blocks);

@@ -443,7 +443,8 @@ def test_sparse_attention_of_chunks(gpu, dt, H, kv, hd, bs):
 @pytest.mark.parametrize("dt,H,kv,hd,bs,top,out_dt", [
     ("bf16", 8, 8, 128, 16, 30, "f32"), ("f16", 16, 8, 64, 16, 61, "f16"),
     ("bf16", 24, 8, 256, 16, 17, "bf16"), ("f16", 8, 8, 128, 8, 45, "f32"),
-    ("bf16", 160, 8, 64, 32, 20, "f32"), ("f32", 8, 8, 64, 16, 30, "f32")])
+    ("bf16", 160, 8, 64, 32, 20, "f32"), ("f32", 8, 8, 64, 16, 30, "f32"),
+    ("bf16", 24, 8, 256, 16, 16, "bf16")])
 def test_sparse_attention_of_many_rows(gpu, dt, H, kv, hd, bs, top, out_dt, chunks):
     # enough (row, kv head) pairs for a workgroup each; some have few blocks or none
     rng = np.random.default_rng(hd + top)
@@ -460,6 +461,24 @@ def test_sparse_attention_of_many_rows(gpu, dt, H, kv, hd, bs, top, out_dt, chun
     want, bound = ref.sparse_attention(q, k, v, blocks, tables, cu, ctx, bs, hd ** -0.5)
     got = run_sparse(gpu, dt, cache, pool, q, blocks, tables, cu, ctx, out_dtype=TD[out_dt])
     within(got, want, bound, out_dt)
+    cache.close()
+
+
+def test_sparse_attention_of_rows_in_sixteen_parts(gpu):
+    # 21 chunk rows, 8 kv heads, 1024 tokens listed: parts of 64 in one workgroup
+    rng = np.random.default_rng(77)
+    bs, kv, hd, top, m = 16, 8, 64, 64, np.full(7, 3)
+    ctx = rng.integers(1100, 3000, 7)
+    cu = np.concatenate(([0], np.cumsum(m)))
+    tables, nb, _ = place(rng, ctx, bs)
+    k, v = (rounded(rng.normal(size=(nb, bs, kv, hd)), "f16") for _ in range(2))
+    cache, pool = to_pool("f16", k, v, bs)
+    q = rounded(rng.normal(size=(21, 16, hd)) * 2, "f16")
+    blocks = choose(rng, ref.rows_of(cu, ctx), kv, top, bs, "select")
+    want, bound = ref.sparse_attention(q, k, v, blocks, tables, cu, ctx, bs, hd ** -0.5)
+    got = run_sparse(gpu, "f16", cache, pool, q, blocks, tables, cu, ctx, out_dtype=torch.float32,
+                     max_q_len=3)
+    within(got, want, bound, "f32")
     cache.close()
 
 
