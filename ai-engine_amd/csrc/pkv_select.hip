@@ -20,7 +20,7 @@
 // so one with S~ > tau + 2E is.  Only what lies between is summed again in 64 bits,
 // mostly nothing or a few blocks.
 //
-// A block with a key that is not finite (or a score past the f32 range)
+// A block with a bound that is not finite (or a score past the f32 range)
 // scores +inf, and so does every block for such a query.  E leaves out what
 // falls below the f32 range: scores that differ by less than some hd 2^-126 may
 // be taken for equal or in either order.

@@ -584,8 +584,8 @@ int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
 
 /* Key bounds: [num_blocks][n_kv_head][2][head_dim] in the pool dtype, the
  * elementwise smallest, then largest, key element of each block and kv head (NaN
- * keys are passed over).  One array per layer, of pkv_key_bounds_bytes, 16-byte
- * aligned.  pkv_key_bounds brings those of every block that holds a position
+ * elements are passed over; +inf, then -inf, where all are NaN).  One array per
+ * layer, of pkv_key_bounds_bytes, 16-byte aligned.  pkv_key_bounds brings those of every block that holds a position
  * from first_positions[s] (NULL: 0) to context_lens[s] - 1 of a sequence up to
  * date, from all of the block's keys below context_lens[s].  max_new_len: host
  * bound of context_lens[s] - first_positions[s], 1 .. 2^30.  A sequence with
@@ -617,12 +617,13 @@ int pkv_key_bounds(pkv_pool* pool, int layer, void* bounds, const int32_t* block
  *      left out, longer contexts cut off; pkv_pool_check() reports both).
  *  first_blocks >= 0, last_blocks >= 1, first_blocks + last_blocks <= top_blocks.
  * Only the bounds of blocks between the first and last ones are used, which are
- * full: the block that a step writes to needs none.  A block with a key that is
+ * full: the block that a step writes to needs none.  A block whose bounds are
  * not finite, one whose products' magnitudes add up past the f32 range, and any
- * block for a query that is not finite rank first.  Scores
- * that differ by less than about head_dim * 2^-126 may be ranked either way.
- * Block ids outside the pool are reported by pkv_pool_check().  Workspace: about
- * 12 bytes per row, kv head and block of max_context_len. */
+ * block for a query that is not finite rank first (a NaN key that the bounds
+ * passed over does not show).  Scores that differ by less than about
+ * head_dim * 2^-126 may be ranked either way.  Block ids outside the pool are
+ * reported by pkv_pool_check().  Workspace: about 12 bytes per row, kv head and
+ * block of max_context_len. */
 size_t pkv_select_workspace_bytes(const pkv_pool* pool, int n_seqs, int total_q, int max_q_len,
                                   int max_context_len, int max_blocks_per_seq, int n_head);
 int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t* blocks,

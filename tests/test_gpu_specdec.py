@@ -272,6 +272,24 @@ def test_select_for_chunks(gpu, dt, H, kv, hd, near):
                                      max_q_len=17, max_context_len=1500), want)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_key_bounds_pass_over_nan(gpu, dt):
+    # an element that is NaN in some keys of a block, in all of them, and infinite ones
+    rng = np.random.default_rng(5)
+    bs, kv, hd = 16, 2, 64
+    k = rounded(rng.normal(size=(3, bs, kv, hd)), dt)
+    k[0, 3:9, 1, 7] = np.nan
+    k[1, :, 0, 5] = np.nan
+    k[2, 4, 1, 2], k[2, 5, 1, 2] = np.inf, -np.inf
+    cache, pool = to_pool(dt, k, k, bs)
+    bounds = pool.update_key_bounds(pool.new_key_bounds(), i32([[0, 1, 2]], gpu), i32([48], gpu))
+    cache.check()
+    want = np.stack([np.fmin.reduce(k, axis=1), np.fmax.reduce(k, axis=1)], axis=2)
+    want[1, 0, 0, 5], want[1, 0, 1, 5] = np.inf, -np.inf
+    assert np.array_equal(bounds.double().cpu().numpy(), want)
+    cache.close()
+
+
 @pytest.mark.parametrize("what", ["zero", "equal", "inf", "nan", "query", "huge", "negative"])
 def test_select_ties_and_values_that_are_not_finite(gpu, what):
     rng = np.random.default_rng(4)
