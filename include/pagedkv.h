@@ -585,12 +585,13 @@ int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
 /* Key bounds: [num_blocks][n_kv_head][2][head_dim] in the pool dtype, the
  * elementwise smallest, then largest, key element of each block and kv head (NaN
  * elements are passed over; +inf, then -inf, where all are NaN).  One array per
- * layer, of pkv_key_bounds_bytes, 16-byte aligned.  pkv_key_bounds brings those of every block that holds a position
- * from first_positions[s] (NULL: 0) to context_lens[s] - 1 of a sequence up to
- * date, from all of the block's keys below context_lens[s].  max_new_len: host
- * bound of context_lens[s] - first_positions[s], 1 .. 2^30.  A sequence with
- * lengths outside 0 <= first <= context <= the table, or beyond max_new_len, is
- * left out, as is a block id outside the pool; pkv_pool_check() reports both.
+ * layer, of pkv_key_bounds_bytes, 16-byte aligned.  pkv_key_bounds brings those
+ * of every block that holds a position from first_positions[s] (NULL: 0) to
+ * context_lens[s] - 1 of a sequence up to date, from all of the block's keys below
+ * context_lens[s].  max_new_len: host bound of context_lens[s] -
+ * first_positions[s], 1 .. 2^30.  A sequence with lengths outside 0 <= first <=
+ * context <= the table, or beyond max_new_len, is left out, as is a block id
+ * outside the pool; pkv_pool_check() reports both.
  * A block that several sequences of a call share must have as many keys in
  * each. */
 size_t pkv_key_bounds_bytes(const pkv_pool* pool);
