@@ -101,7 +101,7 @@ __device__ __forceinline__ double exp2_near(double t) {
 __device__ __forceinline__ float kept(float l) {
   return l > -INFINITY ? fminf(l, 3.402823466e+38f) : -INFINITY;
 }
-// Weight 2^((l - m) c) of a logit against reference m, at most 2^500; less
+// Weight 2^((l - m) c) of a logit against reference m, at most 2^532; less
 // than 2^-1000 is 0.
 __device__ __forceinline__ double weight(float l, float m, double c) {
   const double t = ((double)kept(l) - (double)m) * c;
@@ -109,9 +109,11 @@ __device__ __forceinline__ double weight(float l, float m, double c) {
   return t > -1000.0 ? w : 0.0;  // (false for NaN: -inf against -inf)
 }
 
-// A row's reference and the logits around it whose weights are 2^-500 to 2^500:
-// [lo, hi].  far: these are not to be told from m itself (m is a type's lowest
-// value, say), every logit needs care.
+// A row's reference and the logits around it whose weights are about 2^-500 to
+// 2^500: [lo, hi].  far: these are not to be told from m itself (m is a type's
+// lowest value, say), every logit needs care.  Else |m| < 2^20 span, so rounding
+// m +- span to 32 bits moves either end by at most (2^-4 + 2^-24) span: the
+// weights of lo and hi are 2^-532 .. 2^-468 and 2^468 .. 2^532.
 struct Ref {
   float m, lo, hi;
   bool far;
@@ -125,8 +127,8 @@ __device__ __forceinline__ void set_ref(Ref& r, float m) {
   r.hi = m + span;
   r.m64 = m;
 }
-// A term of a sum: logits below the range count as its lower end, 2^-500, those
-// above it as its upper end.  (One instruction; min and max of unpacked words
+// A term of a sum: logits below the range count as its lower end, those above it
+// as its upper end.  (One instruction; min and max of unpacked words
 // cost another each, to quiet NaN.)
 __device__ __forceinline__ double weight_clamped(float l, const Ref& r) {
   float x;
@@ -134,6 +136,8 @@ __device__ __forceinline__ double weight_clamped(float l, const Ref& r) {
   // (a product and one addition would be off by the rounding of m c)
   return exp2_near(((double)x - r.m64) * r.c);
 }
+// Below the weight of any hi: a group whose sum is less has no logit past hi.
+constexpr double kNearEnd = 0x1p460;
 __device__ __forceinline__ float largest(const float (&x)[8]) {
   float top = kept(x[0]);
 #pragma unroll
@@ -251,9 +255,9 @@ __device__ __forceinline__ Stat chunk_stat(const char* row, int c0, int c1, doub
       double g = 0.0;
 #pragma unroll
       for (int e = 0; e < kN; ++e) g += weight_clamped(x[e], r);
-      if (g < 0x1p499 && !r.far) {
+      if (g < kNearEnd && !r.far) {
         sum += g;
-      } else {  // a logit at the range's upper end, or NaN
+      } else {  // a logit near the range's upper end or past it, or NaN
         top = largest(x);
         if (top > r.hi) {
           sum *= weight(r.m, top, c);
@@ -399,7 +403,7 @@ __device__ __forceinline__ Decision decide(const VerifyKArgs& a, int b, int& n, 
 }
 
 // Probabilities below this count as 0 in a draw: the weight of a logit below
-// the reference's range is 2^-500, not 0.
+// the reference's range is that of its lower end, 2^-468 at most, not 0.
 constexpr double kNothing = 0x1p-400;
 
 // Probabilities of eight logits.

@@ -754,6 +754,52 @@ def test_verify_odd_values(gpu, what, draft):
         assert (want[1] == np.diff(cu))[temps > 0].all()
 
 
+def masked_case(seed, dt, mask, temps, vocab=9000):
+    """Requests of one to three live tokens a row, all others at `mask`; the live
+    ones lie beyond the first tokens that a thread meets (2048) of a chunk."""
+    rng = np.random.default_rng(seed)
+    batch, k = 4 * len(temps), 2
+    cu = np.arange(batch + 1) * k
+    x, y = np.full((batch * (k + 1), vocab), mask), np.full((batch * k, vocab), mask)
+    at = np.concatenate((np.arange(2050, 4300), np.arange(6700, 8900)))
+    d = np.zeros(batch * k, np.int64)
+    for r in range(len(x)):
+        b, i = divmod(r, k + 1)
+        live = rng.choice(at, 1 + r % 3, replace=False)
+        x[r, live] = rng.normal(size=len(live)) * 2
+        if i < k:
+            y[b * k + i, live] = rng.normal(size=len(live)) * 2
+            y[b * k + i, rng.choice(at)] = 1.0
+            d[b * k + i] = rng.choice(live) if r % 5 else rng.choice(at)
+    u, ul = (rng.random(n).astype(np.float32) for n in (batch * k, batch))
+    return rounded(x, dt), d, cu, u, ul, rounded(y, dt), np.tile(np.float32(temps), 4)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("dt,mask", [(t, m) for t in ("f32", "bf16") for m in (
+    -1e4, -1e7, -2e7, -5e7, -8e7, -1e8, -1.2e8, -2e8, -3e8, -1e9)] + [("f16", -65504.0)])
+def test_verify_logits_masked_by_a_finite_value(gpu, dt, mask, draft):
+    temps = [1e-3, 3e-3, 0.01, 0.2, 0.3, 0.35, 0.5, 0.7, 0.8, 0.9, 1.0, 1.2]
+    x, d, cu, u, ul, y, temps = masked_case(7, dt, mask, temps)
+    y = y if draft else None
+    want = ref.verify(x, d, cu, u, ul, y, temps)
+    same_verify(run_verify(gpu, dt, dt, x, d, cu, u, ul, y, temps), want)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_verify_temperatures_near_zero(gpu, dt, draft):
+    x, d, cu, u, ul, y, temps = verify_case(29, 24, 9000, 4, dt, dt)
+    x[1::2], y[1::2] = rounded(x[1::2] + 64, dt), rounded(y[1::2] + 10, dt)
+    temps = np.tile(np.float32([1e-5, 1e-6, 4e-7, 1e-7, 3e-8, 1e-9]), 4)
+    y = y if draft else None
+    for r in range(0, len(d), 2):  # half of the drafts are the row's maximum
+        d[r] = np.argmax(x[r + np.searchsorted(cu[1:], r, side="right")])
+    want = ref.verify(x, d, cu, u, ul, y, temps)
+    assert 0 < want[1].sum() < len(d)
+    same_verify(run_verify(gpu, dt, dt, x, d, cu, u, ul, y, temps), want)
+
+
 def test_verify_without_any_draft(gpu):
     x, d, cu, u, ul, y, temps = verify_case(23, 6, 500, 0, "bf16", "bf16")
     want = ref.verify(x, d, cu, u, ul, None, temps)
