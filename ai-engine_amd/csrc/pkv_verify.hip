@@ -111,7 +111,8 @@ __device__ __forceinline__ double weight(float l, float m, double c) {
 
 // A row's reference and the logits around it whose weights are about 2^-500 to
 // 2^500: [lo, hi].  far: these are not to be told from m itself (m is a type's
-// lowest value, say), every logit needs care.  Else |m| < 2^20 span, so rounding
+// lowest value, say) or end past the largest float (temperatures from 1e35 on),
+// every logit needs care.  Else |m| < 2^20 span, so rounding
 // m +- span to 32 bits moves either end by at most (2^-4 + 2^-24) span: the
 // weights of lo and hi are 2^-532 .. 2^-468 and 2^468 .. 2^532.
 struct Ref {
@@ -120,9 +121,9 @@ struct Ref {
   double c, m64;
 };
 __device__ __forceinline__ void set_ref(Ref& r, float m) {
-  const float span = fminf((float)(500.0 / r.c), 1e38f);
+  const float span = (float)(500.0 / r.c);
   r.m = m;
-  r.far = !(span > fabsf(m) * 0x1p-20f);
+  r.far = !(span > fabsf(m) * 0x1p-20f && span + fabsf(m) < 3.4e38f);
   r.lo = m - span;
   r.hi = m + span;
   r.m64 = m;

@@ -673,7 +673,7 @@ int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, in
  * by its log-probabilities with -inf elsewhere, at temperature 1.
  *  logits: rows of `vocab` values at a stride of row_stride elements, each side
  *      PKV_F32, PKV_F16 or PKV_BF16.  -inf has probability 0, and so has NaN; +inf
- *      takes all of it.  A target row with nothing above -inf keeps no draft
+ *      counts as the largest f32 value.  A target row with nothing above -inf keeps no draft
  *      and ends with token 0.
  *  draft_tokens: int32 [total_drafts]; one outside [0, vocab) is not kept.
  *  cu_drafts: int32 [batch + 1], from 0 to total_drafts (a host value), nondecreasing.

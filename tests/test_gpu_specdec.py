@@ -800,6 +800,23 @@ def test_verify_temperatures_near_zero(gpu, dt, draft):
     same_verify(run_verify(gpu, dt, dt, x, d, cu, u, ul, y, temps), want)
 
 
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("t", [2.5e35, 4e35, 1e37, 3e38])
+def test_verify_enormous_temperatures(gpu, t, draft):
+    # every token that is not at -inf is as likely, the others have probability 0
+    x, d, cu, u, ul, y, _ = verify_case(31, 24, 4700, 4, "f32", "f32")
+    rng = np.random.default_rng(2)
+    x[rng.random(x.shape) < 0.6] = -np.inf
+    y[rng.random(y.shape) < 0.4] = -np.inf
+    x[::4, 100] = 1e38
+    x[1::4, 5:2000] = -np.finfo(np.float32).max
+    y[::3, 7] = -3e38
+    y = y if draft else None
+    temps = np.full(24, t, np.float32)
+    want = ref.verify(x, d, cu, u, ul, y, temps)
+    same_verify(run_verify(gpu, "f32", "f32", x, d, cu, u, ul, y, temps), want)
+
+
 def test_verify_without_any_draft(gpu):
     x, d, cu, u, ul, y, temps = verify_case(23, 6, 500, 0, "bf16", "bf16")
     want = ref.verify(x, d, cu, u, ul, None, temps)
