@@ -1158,6 +1158,15 @@ bool overlap(const Range& a, const Range& b) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
   return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
+// a and any of `rows` rows of `bytes` bytes, `stride` bytes apart (stride >= bytes
+// where there are several), from `at` on: what lies between rows is not theirs.
+bool overlap_rows(const Range& a, const void* at, size_t bytes, size_t stride, size_t rows) {
+  if (!a.bytes || !rows || !overlap(a, {at, (rows - 1) * stride + bytes})) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(at);
+  if (x < y || rows == 1) return true;
+  const size_t r = (x - y) / stride, off = (x - y) % stride;
+  return off < bytes || (r + 1 < rows && a.bytes > stride - off);
+}
 }  // namespace
 
 int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
@@ -1460,6 +1469,27 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
   if (int rc = workspace_check(nullptr, workspace, workspace_bytes, pkv::verify_workspace_bytes(a),
                                "verify_drafts"))
     return rc;
+  // Workgroups of a request read its inputs while another writes its outputs.
+  const size_t nb = 4 * (size_t)batch, nd = 4 * (size_t)total_drafts;
+  const bool drawn = temperatures != nullptr;  // (the rest is not read for greedy calls)
+  const Range out[] = {{out_tokens, nd + nb}, {n_accepted, nb},
+                       {workspace, pkv::verify_workspace_bytes(a)}};
+  const Range in[] = {{draft_tokens, nd}, {cu_drafts, nb + 4}, {uniforms, drawn ? nd : 0},
+                      {final_uniforms, drawn ? nb : 0}, {temperatures, drawn ? nb : 0}};
+  const size_t te = pkv::dtype_bytes(target_dtype);
+  for (const Range& o : out) {
+    bool bad = overlap_rows(o, target_logits, te * vocab, te * (size_t)target_row_stride,
+                            (size_t)total_drafts + batch);
+    if (draft_logits && drawn) {
+      const size_t de = pkv::dtype_bytes(draft_dtype);
+      bad |= overlap_rows(o, draft_logits, de * vocab, de * (size_t)draft_row_stride, total_drafts);
+    }
+    for (const Range& i : in) bad |= overlap(o, i);
+    for (const Range& x : out) bad |= &x != &o && overlap(o, x);
+    if (bad)
+      return fail(nullptr, PKV_ERR_INVALID,
+                  "verify_drafts: outputs or workspace overlap an input or each other");
+  }
   hipError_t e = pkv::launch_verify(a, static_cast<char*>(workspace),
                                     static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(nullptr, e, "verify_drafts launch");

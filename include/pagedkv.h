@@ -681,7 +681,9 @@ int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, in
  *      greedy requests, nor the draft rows.  temperatures: f32 [batch].
  *  out_tokens: int32 [total_drafts + batch], at cu_drafts[b] + b the request's kept
  *      drafts, its next token, then -1.  n_accepted: int32 [batch], kept drafts.
- * vocab 1 .. 2^24 - 1.  Runs on the calling thread's current device. */
+ * Outputs and workspace must not overlap the inputs or each other
+ * (PKV_ERR_INVALID).  vocab 1 .. 2^24 - 1.  Runs on the calling thread's current
+ * device. */
 size_t pkv_verify_workspace_bytes(int batch, int total_drafts, int vocab, int has_draft_logits);
 int pkv_verify_drafts(const void* target_logits, int target_dtype, long long target_row_stride,
                       const void* draft_logits, int draft_dtype, long long draft_row_stride,

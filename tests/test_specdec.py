@@ -132,6 +132,23 @@ def test_verify_drafts_refuses(over):
     assert pagedkv.lib().pkv_last_error(None)
 
 
+@pytest.mark.parametrize("over", [
+    # workgroups of a request read what another of them would write
+    dict(out_tokens=3 << 20), dict(out_tokens=(3 << 20) - 32), dict(out_tokens=(3 << 20) + 20),
+    dict(n_accepted=4 << 20), dict(n_accepted=(5 << 20) + 20), dict(out_tokens=(6 << 20) + 8),
+    dict(n_accepted=7 << 20), dict(n_accepted=8 << 20), dict(workspace=8 << 20),
+    dict(workspace=(9 << 20) - 16), dict(workspace=1 << 20), dict(workspace=2 << 20),
+    # rows of logits: the last one's last elements, and any row of a strided array
+    dict(n_accepted=(1 << 20) + 9 * 200 - 4), dict(out_tokens=(2 << 20) + 6 * 400 - 4),
+    dict(target_row_stride=120, n_accepted=(1 << 20) + 240 * 3 - 4),
+    dict(target_row_stride=120, n_accepted=(1 << 20) + 240 * 3 + 196),
+    dict(target_row_stride=101, out_tokens=(1 << 20) + 200),
+])
+def test_verify_drafts_refuses_overlapping_arrays(over):
+    assert _verify(**over) == _lib.PKV_ERR_INVALID
+    assert b"overlap" in pagedkv.lib().pkv_last_error(None)
+
+
 def test_empty_calls_and_queries():
     L = pagedkv.lib()
     assert _verify(batch=0) == 0
