@@ -1416,8 +1416,8 @@ int pkv_sparse_attention(pkv_pool* p, int layer, const void* q, void* out, int o
 }
 
 size_t pkv_verify_workspace_bytes(int batch, int total_drafts, int vocab, int has_draft_logits) {
-  if (batch <= 0 || total_drafts < 0 || total_drafts > pkv::kMaxLen || batch > pkv::kMaxLen / 2 ||
-      vocab <= 0 || vocab >= (1 << 24))
+  if (batch <= 0 || total_drafts < 0 || total_drafts > pkv::kMaxLen / 2 ||
+      batch > pkv::kMaxLen / 2 || vocab <= 0 || vocab >= (1 << 24))
     return 0;
   pkv::VerifyArgs a{};
   a.batch = batch;

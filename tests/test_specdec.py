@@ -165,6 +165,15 @@ def test_empty_calls_and_queries():
         assert fn(*args) == _lib.PKV_ERR_INVALID, name
 
 
+def test_verify_workspace_query_has_the_calls_limits():
+    query, most = pagedkv.lib().pkv_verify_workspace_bytes, 1 << 29
+    # (drafts and their rows: 3 2^29 rows still count in 32 bits)
+    assert query(most, most, 1, 1) > query(most, most, 1, 0) > 0
+    for batch, drafts in ((1, most + 1), (1, 1 << 30), (most + 1, 0), (1 << 30, 1 << 30)):
+        assert query(batch, drafts, 100, 1) == query(batch, drafts, 100, 0) == 0
+        assert _verify(batch=batch, total_drafts=drafts) == _lib.PKV_ERR_INVALID
+
+
 def test_python_refuses_host_tensors():
     z = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError):
