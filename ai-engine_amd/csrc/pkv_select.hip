@@ -575,8 +575,10 @@ __global__ void __launch_bounds__(kSelThreads) choose_kernel(SelectKArgs a) {
       n, want, klo, khi, [&](int k, uint32_t& key) { key = key32(at(k)); return true; }, sm, larger);
   const float tau = unkey32(tkey);
   // 2: taken, 1: within the bound of the border, 0: not taken.  An infinite
-  // score is what it is.
-  const float above = tau < INFINITY ? tau + E2 : tau, below = tau < INFINITY ? tau - E2 : tau;
+  // score is what it is: above any finite border, also one whose bound is past
+  // the largest float.
+  const float above = tau < INFINITY ? fminf(tau + E2, 3.402823466e+38f) : tau;
+  const float below = tau < INFINITY ? tau - E2 : tau;
   auto cls = [&](int k) {
     const float x = at(k);
     return x > above ? 2 : x >= below ? 1 : 0;

@@ -333,6 +333,27 @@ def test_select_ties_and_values_that_are_not_finite(gpu, what):
     assert np.array_equal(run_select(gpu, dt, q, bounds, tables, None, ctx, bs, top, 1, 2), want)
 
 
+def test_select_scores_at_the_end_of_the_f32_range(gpu):
+    # blocks that are not finite rank first also where the border between taken
+    # and left blocks plus its error bound is past the largest float
+    kv, hd, bs, top, n = 2, 64, 16, 12, 100
+    rng = np.random.default_rng(12)
+    ctx = np.array([n * bs, n * bs])
+    tables, nb, _ = place(rng, ctx, bs)
+    bounds = np.zeros((nb, kv, 2, hd))
+    big = float(np.float32(3.4028e38))
+    bounds[:, :, 1, 0] = 1e38
+    # want is 9: six blocks at the range's end and five that are not finite
+    bounds[tables[:, 20:32:2], :, 1, 0] = big
+    bounds[tables[:, [50, 60, 70]], :, 0, 5] = np.nan
+    bounds[tables[:, [80, 90]], :, 1, 9] = np.inf
+    q = np.zeros((2, 4, hd))
+    q[:, :, 0] = 1.0
+    want = ref.select(q, bounds, tables, None, ctx, bs, top, 1, 2)
+    assert set([50, 60, 70, 80, 90]) < set(want[0, 0])
+    assert np.array_equal(run_select(gpu, "f32", q, bounds, tables, None, ctx, bs, top, 1, 2), want)
+
+
 def test_select_more_blocks_than_fit_in_lds(gpu):
     rng = np.random.default_rng(6)
     ctx = np.array([20000, 9000])
