@@ -92,7 +92,12 @@ __device__ __forceinline__ bool locate(const SparseKArgs& a, int wave, Part& w) 
   w.p = a.joined ? wave : (int)(rest - slot * (unsigned)a.parts);
   w.s = (int)(slot / (unsigned)a.max_q);
   if (w.s >= a.n_seqs) return false;
-  const RowAt at = row_at(a, w.s, (int)(slot - (unsigned)w.s * (unsigned)a.max_q));
+  const int i = (int)(slot - (unsigned)w.s * (unsigned)a.max_q);
+  const RowAt at = row_at(a, w.s, i);
+  // a chunk beyond max_q: its first wave sees a row past the launch's last
+  if (i == 0 && w.g == 0 && w.p == 0 && a.cu && (threadIdx.x & 63) == 0 &&
+      row_at(a, w.s, a.max_q).row >= 0)
+    atomicOr(a.err, PKV_EBIT_LENGTH);
   w.row = at.row;
   w.keys = at.keys;
   w.pair = (size_t)w.row * a.kvh + w.g;

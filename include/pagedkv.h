@@ -640,7 +640,8 @@ int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t
  * block listed it is pkv_decode_attention (NULL cu_q_lens) or
  * pkv_prefill_attention, to rounding.
  *  q, out, out_dtype, scale (not NaN): as pkv_decode_attention; rows, cu_q_lens,
- *      context_lens and block_tables as pkv_select_blocks.
+ *      context_lens, block_tables and max_q_len as pkv_select_blocks (rows of no
+ *      sequence and those beyond max_q_len are left as they were).
  *  blocks: int32 [total_q][n_kv_head][top_blocks], distinct indexes in any order;
  *      negative entries are skipped.  An index past the row's context or a
  *      block id outside the pool is skipped and reported by pkv_pool_check().

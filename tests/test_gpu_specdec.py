@@ -578,6 +578,33 @@ def test_sparse_attention_skips_and_reports_bad_entries(gpu, what):
     cache.close()
 
 
+@pytest.mark.parametrize("dt,H,kv,rows", [("bf16", 4, 2, 5), ("f32", 4, 2, 5), ("bf16", 32, 8, 40)])
+def test_sparse_attention_reports_chunks_beyond_max_q_len(gpu, dt, H, kv, rows):
+    # the rows up to the bound are computed, those beyond it left as they were
+    rng = np.random.default_rng(13)
+    bs, hd, top = 16, 64, 16
+    cu = np.array([0, 1, 1 + rows])
+    ctx = np.array([300, 400])
+    tables, nb, _ = place(rng, ctx, bs)
+    k, v = (rounded(rng.normal(size=(nb, bs, kv, hd)), dt) for _ in range(2))
+    cache, pool = to_pool(dt, k, v, bs)
+    q = rounded(rng.normal(size=(1 + rows, H, hd)), dt)
+    blocks = choose(rng, ref.rows_of(cu, ctx), kv, top, bs, "select")
+    want, bound = ref.sparse_attention(q, k, v, blocks, tables, cu, ctx, bs, hd ** -0.5)
+    out = torch.full((1 + rows, H * hd), 5.0, dtype=torch.float32, device=gpu)
+    pool.sparse_attention(torch.tensor(q).to(TD[dt]).to(gpu), i32(blocks, gpu), tables, ctx,
+                          cu_q_lens=i32(cu, gpu), max_q_len=rows - 1, out=out)
+    with pytest.raises(pagedkv.PagedKvError, match="length"):
+        cache.check()
+    got = out.double().cpu().numpy().reshape(q.shape)
+    within(got[:-1], want[:-1], bound[:-1], "f32")
+    assert (got[-1] == 5.0).all()
+    out.fill_(5.0)
+    got = run_sparse(gpu, dt, cache, pool, q, blocks, tables, cu, ctx, max_q_len=rows, out=out)
+    within(got, want, bound, "f32")
+    cache.close()
+
+
 def test_offsets_past_32_bits(gpu):
     # 2.1 million slots of 2 KiB rows: the last blocks lie beyond 4 GiB
     bs, kv, hd, nb = 256, 8, 128, 9000
