@@ -66,7 +66,7 @@ struct RowAt {
   int row, keys;  // row < 0: none
 };
 __device__ __forceinline__ RowAt row_at(const SparseKArgs& a, int s, int i) {
-  if (!a.cu) return {s, a.ctx[s]};
+  if (!a.cu) return {s, max(a.ctx[s], 0)};
   const int r0 = min(max(a.cu[s], 0), a.total_q), r1 = min(max(a.cu[s + 1], r0), a.total_q);
   if (i >= r1 - r0) return {-1, 0};
   const long long keys = (long long)a.ctx[s] - (r1 - r0) + i + 1;

@@ -605,6 +605,18 @@ def test_sparse_attention_reports_chunks_beyond_max_q_len(gpu, dt, H, kv, rows):
     cache.close()
 
 
+def test_sparse_attention_of_a_negative_context(gpu):
+    # no keys: a zero row, and nothing to report while its list is empty
+    cache = pagedkv.PagedKvCache(1, 10, 16, 2, 64, torch.bfloat16)
+    q = torch.ones((3, 4, 64), dtype=torch.bfloat16, device=gpu)
+    blocks = torch.full((3, 2, 4), -1, dtype=torch.int32, device=gpu)
+    tables = torch.zeros((3, 8), dtype=torch.int32, device=gpu)
+    out = cache.layer(0).sparse_attention(q, blocks, tables, i32([-40, 0, -2 ** 31], gpu))
+    cache.check()
+    assert (out == 0).all()
+    cache.close()
+
+
 def test_offsets_past_32_bits(gpu):
     # 2.1 million slots of 2 KiB rows: the last blocks lie beyond 4 GiB
     bs, kv, hd, nb = 256, 8, 128, 9000
