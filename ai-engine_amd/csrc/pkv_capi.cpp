@@ -1403,8 +1403,8 @@ int pkv_sparse_attention(pkv_pool* p, int layer, const void* q, void* out, int o
                     max_blocks_per_seq, n_seqs, total_q, max_q_len, n_head, scale};
   if (!pkv::sparse_fits(p, a))
     return fail(p, PKV_ERR_UNSUPPORTED,
-                "sparse_attention: %d sequences of up to %d rows, %d blocks each: more than 2^26 "
-                "waves", n_seqs, max_q_len, top_blocks);
+                "sparse_attention: %d sequences of up to max_q_len %d rows, %d blocks each: 2^26 "
+                "waves or more", n_seqs, max_q_len, top_blocks);
   if (int rc = workspace_check(p, workspace, workspace_bytes, pkv::sparse_workspace_bytes(p, a),
                                "sparse_attention"))
     return rc;

@@ -814,7 +814,9 @@ size_t sparse_workspace_bytes(const pkv_pool* p, const SparseArgs& a) {
 
 bool sparse_fits(const pkv_pool* p, const SparseArgs& a) {
   const SparsePlan pl = sparse_plan(p, a);
-  const int heads = std::min(a.n_head / p->n_kv_head, 16);
+  // a wave per part, and one per query head where the parts are merged
+  const bool merged = pl.parts > 1 && !pl.joined;
+  const int heads = merged ? std::min(a.n_head / p->n_kv_head, 16) : 1;
   return sparse_items(p, a, std::max(pl.parts, heads)) < (1LL << 26) - 4;
 }
 

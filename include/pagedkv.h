@@ -647,8 +647,10 @@ int pkv_select_blocks(pkv_pool* pool, const void* q, const void* bounds, int32_t
  *      block id outside the pool is skipped and reported by pkv_pool_check().
  *      A row and kv head without any key is zero.  Attended keys and values are
  *      to be finite: with others that row and kv head may come out as NaN.
- * total_q, n_kv_head and parts (top_blocks * block_size / 64 at most) multiply to
- * less than 2^26 (else PKV_ERR_UNSUPPORTED). */
+ * The launch has n_seqs * max_q_len row places, so max_q_len should be tight:
+ * these, n_kv_head and the larger of parts (1 to top_blocks * block_size / 64) and,
+ * where parts are merged by a second kernel, query heads per kv head (16 at most)
+ * multiply to less than 2^26 (else PKV_ERR_UNSUPPORTED). */
 size_t pkv_sparse_workspace_bytes(const pkv_pool* pool, int total_q, int n_head, int top_blocks);
 int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, int out_dtype,
                          const int32_t* blocks, int top_blocks, const int32_t* cu_q_lens,

@@ -617,6 +617,33 @@ def test_sparse_attention_of_a_negative_context(gpu):
     cache.close()
 
 
+def test_sparse_attention_of_a_ragged_batch_without_max_q_len(gpu):
+    # 1024 requests, 4224 rows, 16 heads: as a launch of 4224 rows a request this is
+    # 4.3 million (row, kv head) items; no part is joined, so heads do not count
+    rng = np.random.default_rng(14)
+    bs, kv, hd, H, n = 16, 1, 64, 16, 1024
+    m = np.ones(n, np.int64)
+    m[0] = 3201
+    cu = np.concatenate(([0], np.cumsum(m)))
+    ctx = np.full(n, 60)
+    ctx[0] = 3201
+    cache = pagedkv.PagedKvCache(1, 300, bs, kv, hd, torch.bfloat16)
+    pool = cache.layer(0)
+    slots = torch.arange(300 * bs, dtype=torch.int32, device=gpu)
+    k, v = (torch.tensor(rng.normal(size=(300 * bs, kv, hd))).bfloat16().to(gpu) for _ in range(2))
+    pool.append(k, v, slots)
+    tables = i32(rng.integers(0, 300, (n, 201)), gpu)
+    rows = ref.rows_of(cu, ctx)
+    blocks = i32(choose(rng, rows, kv, 4, bs, "select"), gpu)
+    q = torch.tensor(rng.normal(size=(len(rows), H, hd))).bfloat16().to(gpu)
+    args = (q, blocks, tables, i32(ctx, gpu), i32(cu, gpu))
+    got = pool.sparse_attention(*args)
+    want = pool.sparse_attention(*args, max_q_len=3201)
+    cache.check()
+    assert torch.equal(got, want)
+    cache.close()
+
+
 def test_offsets_past_32_bits(gpu):
     # 2.1 million slots of 2 KiB rows: the last blocks lie beyond 4 GiB
     bs, kv, hd, nb = 256, 8, 128, 9000
