@@ -915,6 +915,7 @@ class KvPool:
 
     def _rows(self, q, block_tables, context_lens, cu_q_lens, max_q_len):
         """Checked row arguments of select_blocks and sparse_attention."""
+        import torch
         c = self.cache
         if q.device != c.device or q.dim() != 3 or q.shape[2] != c.head_dim:
             raise ValueError(f"q must be (rows, n_head, {c.head_dim}) on {c.device}")
@@ -930,7 +931,11 @@ class KvPool:
         if cu is None and rows != n:
             raise ValueError("without cu_q_lens q has one row per sequence")
         if max_q_len is None:
-            max_q_len = max(rows, 1) if cu is not None else 1
+            max_q_len = 1
+            if cu is not None and getattr(cu_q_lens, "is_cuda", False):
+                max_q_len = max(rows, 1)  # (a bound without a synchronisation)
+            elif cu is not None and n:
+                max_q_len = max(int(torch.as_tensor(cu_q_lens, dtype=torch.int64).diff().max()), 1)
         return q.contiguous(), bt, cl, cu, n, rows, int(max_q_len)
 
     def select_blocks(self, q, bounds, block_tables, context_lens, top_blocks: int,
@@ -943,10 +948,13 @@ class KvPool:
         all.  q: (rows, H, hd) in the pool dtype, as the attention will get it;
         context_lens: (n,) int32; block_tables: (n, width) int32; cu_q_lens: (n + 1,)
         int32 (None: one row per sequence), row i of a chunk of m rows having
-        the keys up to position context_lens - m + i.  max_q_len, max_context_len:
-        host bounds (None: all rows, what the tables hold).  Returns
-        (rows, n_kv, top_blocks) int32, ascending indexes into the sequence's row
-        of block_tables, then -1 (into `out` if given)."""
+        the keys up to position context_lens - m + i.  max_context_len: host bound
+        (None: what the tables hold).  max_q_len: host bound of the chunks (None:
+        the longest one if cu_q_lens is on the host, else all rows).  The launch
+        has n * max_q_len row places, so a batch whose cu_q_lens is on the device
+        should pass it: many requests under a loose bound cost time or are
+        refused.  Returns (rows, n_kv, top_blocks) int32, ascending indexes into
+        the sequence's row of block_tables, then -1 (into `out` if given)."""
         import torch
         c = self.cache
         self._check_bounds(bounds)
@@ -978,8 +986,9 @@ class KvPool:
         """Attention of each query row over the keys of its listed blocks
         (pkv_sparse_attention).  blocks: (rows, n_kv, top) int32, as select_blocks
         returns them (any order, distinct; negative entries are skipped); the
-        other arguments as select_blocks'.  The rows' keys are in the pool
-        already.  Returns (rows, H * hd); a row without keys is zero."""
+        other arguments as select_blocks' (whether max_q_len is 1 or more also
+        decides how lists are cut, so it may change last bits).  The rows' keys
+        are in the pool already.  Returns (rows, H * hd); a row without keys is zero."""
         import torch
         c = self.cache
         qq, bt, cl, cu, n, rows, mq = self._rows(q, block_tables, context_lens, cu_q_lens,

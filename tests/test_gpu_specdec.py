@@ -644,6 +644,30 @@ def test_sparse_attention_of_a_ragged_batch_without_max_q_len(gpu):
     cache.close()
 
 
+@pytest.mark.parametrize("on_host", [list, np.asarray, torch.tensor])
+def test_bound_of_chunks_on_the_host_is_the_longest(gpu, on_host):
+    # 4096 requests, one of two rows: all rows as the bound of each would be refused
+    rng = np.random.default_rng(15)
+    bs, kv, hd, H, n = 16, 4, 64, 4, 4096
+    m = np.ones(n, np.int64)
+    m[7], m[9] = 2, 0
+    cu = np.concatenate(([0], np.cumsum(m)))
+    ctx = rng.integers(2, 200, n)
+    cache, pool = to_pool("bf16", *rng.normal(size=(2, 50, bs, kv, hd)), bs)
+    tables = i32(rng.integers(0, 50, (n, 13)), gpu)
+    bounds = pool.update_key_bounds(pool.new_key_bounds(), i32(np.arange(50)[None], gpu),
+                                    i32([50 * bs], gpu))
+    q = torch.tensor(rng.normal(size=(cu[-1], H, hd))).bfloat16().to(gpu)
+    args, given = (tables, i32(ctx, gpu)), dict(cu_q_lens=i32(cu, gpu), max_q_len=2)
+    cu = on_host(cu.tolist())
+    want = pool.select_blocks(q, bounds, *args, 5, 1, 2, **given)
+    assert torch.equal(pool.select_blocks(q, bounds, *args, 5, 1, 2, cu_q_lens=cu), want)
+    assert torch.equal(pool.sparse_attention(q, want, *args, cu_q_lens=cu),
+                       pool.sparse_attention(q, want, *args, **given))
+    cache.check()
+    cache.close()
+
+
 def test_offsets_past_32_bits(gpu):
     # 2.1 million slots of 2 KiB rows: the last blocks lie beyond 4 GiB
     bs, kv, hd, nb = 256, 8, 128, 9000
