@@ -352,7 +352,8 @@ def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_unifor
     token comes from max(p - q, 0) of the first one that is not, or from p
     after the last.  Nothing synchronises.  Returns (tokens, accepted):
     (drafts + batch,) int32 with a request's kept drafts, next token and then
-    -1 at cu_drafts[b] + b, and (batch,) int32 with the number of kept drafts."""
+    -1 at cu_drafts[b] + b, and (batch,) int32 with the number of kept drafts.
+    cu_drafts runs from 0 to drafts; what no request covers is not written."""
     import torch
     if not isinstance(target_logits, torch.Tensor) or not target_logits.is_cuda:
         raise ValueError("target_logits must be a device tensor")
@@ -954,7 +955,9 @@ class KvPool:
         has n * max_q_len row places, so a batch whose cu_q_lens is on the device
         should pass it: many requests under a loose bound cost time or are
         refused.  Returns (rows, n_kv, top_blocks) int32, ascending indexes into
-        the sequence's row of block_tables, then -1 (into `out` if given)."""
+        the sequence's row of block_tables, then -1 (into `out` if given).  Rows of
+        no sequence and those of a chunk beyond max_q_len are not written: as they
+        were in `out`, uninitialised without it."""
         import torch
         c = self.cache
         self._check_bounds(bounds)
@@ -988,7 +991,8 @@ class KvPool:
         returns them (any order, distinct; negative entries are skipped); the
         other arguments as select_blocks' (whether max_q_len is 1 or more also
         decides how lists are cut, so it may change last bits).  The rows' keys
-        are in the pool already.  Returns (rows, H * hd); a row without keys is zero."""
+        are in the pool already.  Returns (rows, H * hd); a row without keys is
+        zero, one that select_blocks would not write is not written."""
         import torch
         c = self.cache
         qq, bt, cl, cu, n, rows, mq = self._rows(q, block_tables, context_lens, cu_q_lens,
