@@ -160,10 +160,8 @@ struct DecodeSmem {
   alignas(16) char nl[kWavesPerBlock][2 * C::RB];
 };
 
-// Host side (pkv_decode.hip).  Group width of the kernel instantiated for a
-// GQA ratio: the ratio itself or the next of 1, 2, 4, 8, 16.
-int group_width(int r);
-// Kernel arguments of slice h0 (query heads h0 .. h0 + 15 of every group)
+// Host side (pkv_decode.hip).  Kernel arguments of slice h0 (query heads h0 ..
+// h0 + 15 of every group)
 // of a decode launch whose partials go to `partials`; items = waves.
 DecodeKArgs decode_kargs(const pkv_pool* p, int layer, const DecodeArgs& a, char* partials,
                          int h0, long long* items);

@@ -259,6 +259,10 @@ struct StepArgs {
 };
 hipError_t launch_step_tables(const StepArgs& a, hipStream_t stream);
 
+// Group width of the kernel instantiated for a GQA ratio: the ratio itself or
+// the next of 1, 2, 4, 8, 16 (pkv_decode.hip).
+int group_width(int r);
+
 // Key bounds of the blocks that hold new positions (pkv_select.hip); fits:
 // the launch's grid is within HIP's limits.
 bool bounds_fits(const pkv_pool* p, int n_seqs, int max_new_len, int mbps);

@@ -182,8 +182,6 @@ __device__ __forceinline__ int row_blocks(const SeqRows& r, int i, int bsl, int 
   return (int)(nb < nb_max ? nb : nb_max);
 }
 
-constexpr int group_width_of(int r) { return r >= 16 ? 16 : r > 8 ? 16 : r > 4 ? 8 : r > 2 ? 4 : r; }
-
 // max(x, 0) and min(x, 0) of the elements of a 16-byte chunk; NaN stays in one.
 template <int DT>
 __device__ __forceinline__ void split_sign(const u32x4& w, u32x4& p, u32x4& m) {
@@ -750,7 +748,7 @@ struct SelectPlan {
 SelectPlan select_plan(const pkv_pool* p, const SelectArgs& a) {
   SelectPlan pl{};
   const int bsl = log2_of(p->block_size);
-  pl.R = group_width_of(a.n_head / p->n_kv_head);
+  pl.R = group_width(a.n_head / p->n_kv_head);
   pl.tiles = (a.max_q_len + 16 / pl.R - 1) / (16 / pl.R);
   pl.nb_max = (int)std::min<long long>(((long long)a.max_context_len + p->block_size - 1) >> bsl,
                                        a.max_blocks_per_seq);
