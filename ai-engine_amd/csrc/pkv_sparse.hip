@@ -195,7 +195,7 @@ struct Rows {
 
 // ONCE: one row per sequence, so no other wave reads a block's rows of a head,
 // and the loads say so.  The rows of a chunk choose much the same blocks: their
-// loads stay in the caches (42 rows of 12 chunks, 64 heads of 128, 75 blocks
+// loads stay in the caches (43 rows of 12 chunks, 64 heads of 128, 75 blocks
 // each: 35 us against 47 with such loads; the other way 64 single rows of 128
 // blocks, 32 heads: 95 against 84).
 template <bool ONCE>
@@ -241,7 +241,7 @@ constexpr float kRise = 8.0f, kLift = 7.0f;
 //  Joined: the parts of a (row, kv head), equally long, are one workgroup, and
 //   their results meet in LDS: one launch, and no partial leaves the CU.
 // 64 single rows of 2048 tokens, 32 heads on 8 of 128: 84 us (537 MB, 6.4 TB/s, bound
-// by HBM) and the merge 4.7; 42 chunk rows of 1200, 64 heads: 35 us joined, bound by
+// by HBM) and the merge 4.7; 43 chunk rows of 1200, 64 heads: 35 us joined, bound by
 // the waves' own steps; 8 rows of 1000, 8 kv heads of 64: 7.2 + 3.4, round trips.
 template <int DT, int HD, bool SB, bool ONCE>
 __global__ void __launch_bounds__(Cfg16<HD>::WAVES * kWave) sparse16_kernel(SparseKArgs a) {
@@ -741,7 +741,7 @@ hipError_t launch_hd(int dt, const SparseKArgs& k, unsigned grid, unsigned merge
   return hipGetLastError();
 }
 
-constexpr int kJoinTokens = 256, kJoinPairs = 160;
+constexpr int kJoinTokens = 256, kJoinPairs = 160, kJoinSinglePairs = 256;
 
 struct SparsePlan {
   int bs_log2, part_tokens, parts, R;
@@ -758,17 +758,32 @@ int most_waves(int head_dim) {
 // Parts of 1024 tokens, halved (down to 64) while a part has more than the 64
 // list entries of a wave, and while the call has fewer than 1024 waves, one per
 // SIMD; 2048 for chunks, whose rows hit the caches and are bound by the waves'
-// own steps.  (us, main kernel and merge, from 1024 / 2048 waves, bf16: 42 chunk rows
+// own steps.  (us, main kernel and merge, from 1024 / 2048 waves, bf16: 43 chunk rows
 // of 1200 tokens, 64 heads on 8 of 128: 53 / 38; single rows: 64 of 2048 tokens, 32
 // heads: 93 / 90; 32 of 2048, 64 heads: 49 / 53; 32 of 1600, 16 heads of 256 (f16):
 // 81 / 93.)
 // The parts of a row and kv head of a 16-bit pool are joined in one workgroup if
-// there are four or more and these workgroups cover most CUs (parts too many
-// for one are lengthened for it, up to 256 tokens).  A call, joined / with the
-// merge, us: 256 pairs of chunk rows, heads of 64, 1600 tokens: 14 / 23; 344 of 1200,
-// heads of 128: 33 / 38; 160 single rows of 1600, 64: 20 / 24; 256 of 1600, 256: 70 / 82;
-// 256 of 2048, 128, four parts: 50 / 49; but 512 of two parts: 96 / 87, and 128 pairs
-// of 2048, 128: 41 / 28, 64 of 1536: 30 / 19.
+// there are four or more, a workgroup can have that many and the workgroups cover
+// most CUs.  Chunks and heads of 256: parts too many for a workgroup are lengthened
+// for it, up to 256 tokens.  Single rows with smaller heads read their blocks from
+// HBM whichever way and gain only the merge's launch; they are joined while the
+// workgroups are one a CU at most and have five to seven waves.  A call, joined /
+// with the merge, us, bf16, 8 kv heads, 4 query heads each (2 at heads of 256):
+//   pairs, tokens      chunks 64   chunks 128   chunks 256   single 64    single 128
+//   160    768         9.0/10.8    13.3/15.3    26/26        14.0/11.9 x  20.5/19.1 x
+//   160    1600        13/20       22/32        55/56        24.9/24.1    36.8/40.7
+//   256    768         9.3/13.1    13.6/20.6    36/36        14.8/17.0    22.8/26.7
+//   256    1024        10.0/13.9   16.6/20.3    27/35        18.6/18.3 x  28.3/28.2 x
+//   256    1200        12/17       18/30        53/53        21/25        33/42
+//   256    1600        13/25       22/42        81/80        26.4/27.8 x  41.4/44.6 x
+//   256    2048        15/19       26/30        53/53        32/29 x      52/49 x
+//   288    768         15.1/14.6   24.6/23.4    44/44        23/18 x      39/28 x
+//   320    2048        25.5/24.2   47/39        75/75        54/43 x      87/79 x
+//   384    1600        23/33       41/62        105/105      45/44 x      72/77 x
+//   512    1600        23/28       38/48        84/92        49/48 x      86/86 x
+// (x: not joined; single rows of heads of 256: 160 of 1024 40/47, 256 of 1600 71/84, 320
+// of 1600 121/140, 512 of 2048 185/177, as chunks else.)  Fewer pairs, joined / with
+// the merge: 128 of 2048, 128: 41 / 28, 64 of 1536: 30 / 19.
 SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   SparsePlan pl{};
   while ((1 << pl.bs_log2) < p->block_size) ++pl.bs_log2;
@@ -781,12 +796,14 @@ SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
   while (pt > 64 && (pt >> pl.bs_log2) > 64) pt >>= 1;
   if (p->dtype != PKV_F32 && pairs >= kJoinPairs) {
     const int most = most_waves(p->head_dim);
-    int longer = pt;
-    while (parts(longer) > most && longer < kJoinTokens && (2 * longer >> pl.bs_log2) <= 64)
-      longer <<= 1;
-    if (parts(longer) <= most && parts(longer) >= 4) {
-      pt = longer;
-      pl.joined = true;
+    if (a.max_q_len > 1 || p->head_dim == 256) {
+      int longer = pt;
+      while (parts(longer) > most && longer < kJoinTokens && (2 * longer >> pl.bs_log2) <= 64)
+        longer <<= 1;
+      pl.joined = parts(longer) >= 4 && parts(longer) <= most;
+      if (pl.joined) pt = longer;
+    } else {
+      pl.joined = pairs <= kJoinSinglePairs && parts(pt) >= 5 && parts(pt) <= 7;
     }
   }
   pl.part_tokens = pt;
