@@ -766,20 +766,26 @@ int most_waves(int head_dim) {
 // there are four or more, a workgroup can have that many and the workgroups cover
 // most CUs.  Chunks and heads of 256: parts too many for a workgroup are lengthened
 // for it, up to 256 tokens.  Single rows with smaller heads read their blocks from
-// HBM whichever way and gain only the merge's launch; they are joined while the
-// workgroups are one a CU at most and have five to seven waves.  A call, joined /
-// with the merge, us, bf16, 8 kv heads, 4 query heads each (2 at heads of 256):
+// HBM whichever way and gain only the merge's launch; they are joined with five to
+// seven parts while the workgroups are one a CU at most, and with four whose last
+// is half full at most (with more in it the merge is level or ahead).  A call,
+// joined / with the merge, us, bf16, 8 kv heads, 4 query heads each (2 at heads of
+// 256):
 //   pairs, tokens      chunks 64   chunks 128   chunks 256   single 64    single 128
 //   160    768         9.0/10.8    13.3/15.3    26/26        14.0/11.9 x  20.5/19.1 x
 //   160    1600        13/20       22/32        55/56        24.9/24.1    36.8/40.7
+//   192    1312                                              21.2/24.0    32.8/40.4
 //   256    768         9.3/13.1    13.6/20.6    36/36        14.8/17.0    22.8/26.7
 //   256    1024        10.0/13.9   16.6/20.3    27/35        18.6/18.3 x  28.3/28.2 x
 //   256    1200        12/17       18/30        53/53        21/25        33/42
-//   256    1600        13/25       22/42        81/80        26.4/27.8 x  41.4/44.6 x
+//   256    1600        13/25       22/42        81/80        26.4/27.8    41.4/44.6
+//   256    1920                                              31/29 x      49/48 x
 //   256    2048        15/19       26/30        53/53        32/29 x      52/49 x
 //   288    768         15.1/14.6   24.6/23.4    44/44        23/18 x      39/28 x
+//   320    1568                                              42.3/41.5    68/74
 //   320    2048        25.5/24.2   47/39        75/75        54/43 x      87/79 x
-//   384    1600        23/33       41/62        105/105      45/44 x      72/77 x
+//   384    1600        23/33       41/62        105/105      45.1/44.3    72/77
+//   448    832                                               26.3/26.6    43/47
 //   512    1600        23/28       38/48        84/92        49/48 x      86/86 x
 // (x: not joined; single rows of heads of 256: 160 of 1024 40/47, 256 of 1600 71/84, 320
 // of 1600 121/140, 512 of 2048 185/177, as chunks else.)  Fewer pairs, joined / with
@@ -803,7 +809,9 @@ SparsePlan sparse_plan(const pkv_pool* p, const SparseArgs& a) {
       pl.joined = parts(longer) >= 4 && parts(longer) <= most;
       if (pl.joined) pt = longer;
     } else {
-      pl.joined = pairs <= kJoinSinglePairs && parts(pt) >= 5 && parts(pt) <= 7;
+      const long long last = len % pt;
+      pl.joined = parts(pt) == 4 ? last && last <= pt / 2
+                                 : pairs <= kJoinSinglePairs && parts(pt) >= 5 && parts(pt) <= 7;
     }
   }
   pl.part_tokens = pt;
