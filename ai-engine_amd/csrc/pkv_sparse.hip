@@ -63,19 +63,22 @@ struct SparseKArgs {
 constexpr float kLowest = -3.0e38f;
 
 struct RowAt {
-  int row, keys;  // row < 0: none
+  int row, keys;  // row < 0: none; keys < 0: none (bounded where it is used: the
+                  // list's loads do not wait for the context)
+  bool over;      // its chunk has more rows than max_q
 };
 __device__ __forceinline__ RowAt row_at(const SparseKArgs& a, int s, int i) {
-  if (!a.cu) return {s, max(a.ctx[s], 0)};
+  if (!a.cu) return {s, a.ctx[s], false};
   const int r0 = min(max(a.cu[s], 0), a.total_q), r1 = min(max(a.cu[s + 1], r0), a.total_q);
-  if (i >= r1 - r0) return {-1, 0};
+  if (i >= r1 - r0) return {-1, 0, false};
   const long long keys = (long long)a.ctx[s] - (r1 - r0) + i + 1;
-  return {r0 + i, (int)(keys > 0 ? keys : 0)};
+  return {r0 + i, (int)(keys > 0 ? keys : 0), r1 - r0 > a.max_q};
 }
 
 // What a wave computes: part p of the list of (row, kv head g).
 struct Part {
   int s, row, keys, g, p;
+  bool over;    // its chunk has more rows than max_q
   size_t pair;  // row * kvh + g
   int o0;       // offset in its first block (parts shorter than a block)
   int T;        // tokens 0 .. T - 1; token t is at offset (t + o0) % bs of entry (t + o0) / bs
@@ -92,14 +95,10 @@ __device__ __forceinline__ bool locate(const SparseKArgs& a, int wave, Part& w) 
   w.p = a.joined ? wave : (int)(rest - slot * (unsigned)a.parts);
   w.s = (int)(slot / (unsigned)a.max_q);
   if (w.s >= a.n_seqs) return false;
-  const int i = (int)(slot - (unsigned)w.s * (unsigned)a.max_q);
-  const RowAt at = row_at(a, w.s, i);
-  // a chunk beyond max_q: its first wave sees a row past the launch's last
-  if (i == 0 && w.g == 0 && w.p == 0 && a.cu && (threadIdx.x & 63) == 0 &&
-      row_at(a, w.s, a.max_q).row >= 0)
-    atomicOr(a.err, PKV_EBIT_LENGTH);
+  const RowAt at = row_at(a, w.s, (int)(slot - (unsigned)w.s * (unsigned)a.max_q));
   w.row = at.row;
   w.keys = at.keys;
+  w.over = at.over;
   w.pair = (size_t)w.row * a.kvh + w.g;
   return at.row >= 0;
 }
@@ -114,7 +113,7 @@ __device__ __forceinline__ void take_list(const SparseKArgs& a, int lane, Part& 
   int sel = -1;
   if (lane < span && e0 + lane < a.top) sel = a.blocks[w.pair * a.top + e0 + lane];
   const bool too_long = (long long)w.keys > (long long)a.mbps << lg;
-  const int keys = too_long ? a.mbps << lg : w.keys;
+  const int keys = too_long ? a.mbps << lg : max(w.keys, 0);
   const int nb = (int)(((long long)keys + tmask) >> lg);
   bool valid = sel >= 0 && sel < nb;
   bool odd = sel >= nb;  // no block of this context
@@ -124,7 +123,7 @@ __device__ __forceinline__ void take_list(const SparseKArgs& a, int lane, Part& 
     if (id < 0 || id >= a.num_blocks) valid = false, odd = true;
   }
   if (odd) atomicOr(a.err, PKV_EBIT_BLOCK);
-  if (too_long && lane == 0) atomicOr(a.err, PKV_EBIT_LENGTH);
+  if ((too_long || w.over) && lane == 0) atomicOr(a.err, PKV_EBIT_LENGTH);
   int lim = valid ? min(BS, keys - (sel << lg)) : 0;  // the block's keys
   valid = lim > w.o0;
   const unsigned long long have = __ballot(valid);
