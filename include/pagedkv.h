@@ -671,8 +671,9 @@ int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, in
  * draft_logits NULL: q_i is 1 at d_i (drafts that were looked up or searched).
  * T not positive or not finite, or temperatures NULL: greedy; a draft is kept
  * while it is the target row's first maximum, and the next token is a row's first
- * maximum.  Decisions are those of 64-bit arithmetic; in a draw a probability
- * below 2^-400 counts as 0.  A distribution cut by top-k or top-p is given
+ * maximum.  Decisions are those of 64-bit arithmetic in which probabilities below
+ * about 2^-1000 are 0; in a draw those below 2^-400 count as 0, and where nothing
+ * is left of max(p_i - q_i, 0) the token comes from p_i.  A distribution cut by top-k or top-p is given
  * by its log-probabilities with -inf elsewhere, at temperature 1.
  *  logits: rows of `vocab` values at a stride of row_stride elements, each side
  *      PKV_F32, PKV_F16 or PKV_BF16.  -inf has probability 0, and so has NaN; +inf
