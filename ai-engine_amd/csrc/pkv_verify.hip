@@ -111,10 +111,10 @@ __device__ __forceinline__ double weight(float l, float m, double c) {
 
 // A row's reference and the logits around it whose weights are about 2^-500 to
 // 2^500: [lo, hi].  far: these are not to be told from m itself (m is a type's
-// lowest value, say) or end past the largest float (temperatures from 1e35 on),
-// every logit needs care.  Else |m| < 2^20 span, so rounding
-// m +- span to 32 bits moves either end by at most (2^-4 + 2^-24) span: the
-// weights of lo and hi are 2^-532 .. 2^-468 and 2^468 .. 2^532.
+// lowest value, say) or end past the largest float (temperatures from 1e35 on), so
+// every logit needs care.  Else |m| < 2^20 span, so rounding m +- span to 32 bits
+// moves either end by at most (2^-4 + 2^-24) span: the weights of lo and hi are
+// 2^-532 .. 2^-468 and 2^468 .. 2^532.
 struct Ref {
   float m, lo, hi;
   bool far;
@@ -129,8 +129,8 @@ __device__ __forceinline__ void set_ref(Ref& r, float m) {
   r.m64 = m;
 }
 // A term of a sum: logits below the range count as its lower end, those above it
-// as its upper end.  (One instruction; min and max of unpacked words
-// cost another each, to quiet NaN.)
+// as its upper end.  (One instruction; min and max of unpacked words cost another
+// each, to quiet NaN.)
 __device__ __forceinline__ double weight_clamped(float l, const Ref& r) {
   float x;
   asm("v_med3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(l), "v"(r.lo), "v"(r.hi));

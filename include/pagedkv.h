@@ -673,12 +673,13 @@ int pkv_sparse_attention(pkv_pool* pool, int layer, const void* q, void* out, in
  * while it is the target row's first maximum, and the next token is a row's first
  * maximum.  Decisions are those of 64-bit arithmetic in which probabilities below
  * about 2^-1000 are 0; in a draw those below 2^-400 count as 0, and where nothing
- * is left of max(p_i - q_i, 0) the token comes from p_i.  A distribution cut by top-k or top-p is given
- * by its log-probabilities with -inf elsewhere, at temperature 1.
+ * is left of max(p_i - q_i, 0) the token comes from p_i.  A distribution cut by
+ * top-k or top-p is given by its log-probabilities with -inf elsewhere, at
+ * temperature 1.
  *  logits: rows of `vocab` values at a stride of row_stride elements, each side
  *      PKV_F32, PKV_F16 or PKV_BF16.  -inf has probability 0, and so has NaN; +inf
- *      counts as the largest f32 value.  A target row with nothing above -inf keeps no draft
- *      and ends with token 0.
+ *      counts as the largest f32 value.  A target row with nothing above -inf
+ *      keeps no draft and ends with token 0.
  *  draft_tokens: int32 [total_drafts]; one outside [0, vocab) is not kept.
  *  cu_drafts: int32 [batch + 1], from 0 to total_drafts (a host value), nondecreasing.
  *  uniforms: f32 [total_drafts], final_uniforms: f32 [batch], in [0, 1); not read for
