@@ -40,6 +40,10 @@ SOURCES = [
     "pkv_select.hip",
     "pkv_sparse.hip",
     "pkv_verify.hip",
+    "pkv_q4.hip",
+    "pkv_q4_attn.hip",
+    "pkv_prompt.hip",
+    "pkv_logits.hip",
 ]
 
 # Packed-FP32 instructions stay off (the compiler would otherwise form

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -64,6 +65,13 @@ struct DeviceGuard {
   do {                                                                  \
     if (!(p)) return fail(nullptr, PKV_ERR_INVALID, "pool is NULL");    \
     (p)->last_error.clear();                                            \
+  } while (0)
+
+// Calls that read or write elements of the pool take those of F32, F16 and BF16.
+#define REFUSE_Q4(p, what)                                                       \
+  do {                                                                           \
+    if ((p)->dtype == PKV_Q4)                                                    \
+      return fail(p, PKV_ERR_UNSUPPORTED, what ": not for a pool of dtype PKV_Q4"); \
   } while (0)
 
 // hipMalloc on the current device, without the scratch that sampling keeps
@@ -160,12 +168,16 @@ int pkv_pool_create(pkv_pool** out, int n_layers, int num_blocks,
                 "block_size %d: must be a power of two in [1, 256]", block_size);
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(nullptr, PKV_ERR_UNSUPPORTED, "head_dim %d: must be 64, 128 or 256", head_dim);
-  if (dtype != PKV_F32 && dtype != PKV_F16 && dtype != PKV_BF16)
+  if (dtype != PKV_F32 && dtype != PKV_F16 && dtype != PKV_BF16 && dtype != PKV_Q4)
     return fail(nullptr, PKV_ERR_INVALID, "dtype %d unknown", dtype);
+  if (dtype == PKV_Q4 && block_size < 16)
+    return fail(nullptr, PKV_ERR_UNSUPPORTED, "block_size %d: at least 16 for PKV_Q4", block_size);
+  const size_t row_bytes =
+      dtype == PKV_Q4 ? pkv::q4_row_bytes(head_dim) : (size_t)head_dim * pkv::dtype_bytes(dtype);
   {
     // the kernels count a block's (and a token row's) 16-byte chunks in
     // 32-bit ints, and the slab's size must not wrap
-    const unsigned __int128 row = (unsigned __int128)head_dim * pkv::dtype_bytes(dtype);
+    const unsigned __int128 row = row_bytes;
     const unsigned __int128 blk = row * (unsigned)block_size * (unsigned)n_kv_head;
     const unsigned __int128 tot = blk * (unsigned)num_blocks * 2u * (unsigned)n_layers;
     if (n_kv_head > 1024 || blk / 16 > (unsigned __int128)INT32_MAX ||
@@ -187,8 +199,8 @@ int pkv_pool_create(pkv_pool** out, int n_layers, int num_blocks,
   p->head_dim = head_dim;
   p->dtype = dtype;
   p->device = device;
-  p->elem_bytes = pkv::dtype_bytes(dtype);
-  p->row_bytes = (size_t)head_dim * p->elem_bytes;
+  p->elem_bytes = dtype == PKV_Q4 ? 0 : pkv::dtype_bytes(dtype);
+  p->row_bytes = row_bytes;
   p->block_bytes = (size_t)block_size * n_kv_head * p->row_bytes;
   p->layer_bytes = (size_t)num_blocks * p->block_bytes;
   size_t total = p->layer_bytes * 2 * (size_t)n_layers;
@@ -331,6 +343,7 @@ int pkv_pool_write(pkv_pool* p, int layer, int which, size_t off, const void* ho
 
 int pkv_pool_fill_normal(pkv_pool* p, uint64_t seed, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "fill_normal");
   DeviceGuard dg(p->device);
   hipError_t e = pkv::launch_fill_normal(p, seed, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(p, e, "fill_normal launch");
@@ -355,6 +368,7 @@ int pkv_pool_read_blocks(pkv_pool* p, const int32_t* blocks, int n, uint64_t* su
 int pkv_pool_verify_normal(pkv_pool* p, uint64_t seed, const int32_t* blocks,
                            const int32_t* origin, int n, uint64_t* mismatches, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "verify_normal");
   if (!mismatches) return fail(p, PKV_ERR_INVALID, "mismatches is NULL");
   *mismatches = 0;
   if (n < 0) return fail(p, PKV_ERR_INVALID, "n %d < 0", n);
@@ -377,6 +391,7 @@ int pkv_pool_verify_normal(pkv_pool* p, uint64_t seed, const int32_t* blocks,
 int pkv_append(pkv_pool* p, int layer, const void* k, const void* v,
                const int32_t* slot_mapping, int n_tokens, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "append");
   if (int rc = check_layer(p, layer)) return rc;
   if (n_tokens < 0) return fail(p, PKV_ERR_INVALID, "n_tokens %d < 0", n_tokens);
   if (n_tokens == 0) return PKV_OK;
@@ -394,6 +409,7 @@ int pkv_append_rope(pkv_pool* p, int layer, const pkv_rope* rope, const int32_t*
                     int in_dtype, const void* k, const void* v, const int32_t* slot_mapping,
                     int n_tokens, const void* q, void* q_out, int n_head, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "append_rope");
   if (int rc = check_layer(p, layer)) return rc;
   if (!rope) return fail(p, PKV_ERR_INVALID, "rope is NULL");
   if (rope->rope_dim != p->head_dim)
@@ -426,6 +442,7 @@ int pkv_append_rope(pkv_pool* p, int layer, const pkv_rope* rope, const int32_t*
 int pkv_gather_seq(pkv_pool* p, int layer, const int32_t* block_table, int len,
                    void* out_k, void* out_v, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "gather_seq");
   if (int rc = check_layer(p, layer)) return rc;
   if (len < 0) return fail(p, PKV_ERR_INVALID, "len %d < 0", len);
   if (len == 0) return PKV_OK;
@@ -444,6 +461,7 @@ int pkv_gather_varlen(pkv_pool* p, int layer, const int32_t* block_tables,
                       int max_blocks_per_seq, const int32_t* cu_lens, int batch, int total_rows,
                       void* out_k, void* out_v, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "gather_varlen");
   if (int rc = check_layer(p, layer)) return rc;
   if (batch < 0 || total_rows < 0)
     return fail(p, PKV_ERR_INVALID, "batch %d, total_rows %d", batch, total_rows);
@@ -564,12 +582,14 @@ int pkv_compact(pkv_pool* p, const int32_t* src_host, const int32_t* dst_host, i
 }
 
 size_t pkv_decode_workspace_bytes(const pkv_pool* p, int batch, int n_head, int max_context_len) {
-  if (!p || batch <= 0 || n_head <= 0 || max_context_len > pkv::kMaxLen) return 0;
+  if (!p || p->dtype == PKV_Q4 || batch <= 0 || n_head <= 0 || max_context_len > pkv::kMaxLen)
+    return 0;
   return pkv::decode_workspace_bytes(p, batch, n_head, max_context_len);
 }
 
 int pkv_pool_reserve_decode(pkv_pool* p, int batch, int n_head, int max_context_len) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "reserve_decode");
   if (batch <= 0 || n_head <= 0 || max_context_len <= 0 || max_context_len > pkv::kMaxLen ||
       n_head % p->n_kv_head != 0)
     return fail(p, PKV_ERR_INVALID, "reserve_decode: bad shape (batch %d, n_head %d, max_context_len %d)",
@@ -638,6 +658,7 @@ static int decode_validate(pkv_pool* p, const pkv::DecodeArgs& a) {
 // allocated (no workspace growth, no profile events).
 static int decode_call(pkv_pool* p, int layer, pkv::DecodeArgs& a, void* stream,
                        bool noalloc = false) {
+  REFUSE_Q4(p, "decode");
   if (int rc = check_layer(p, layer)) return rc;
   if (a.batch < 0) return fail(p, PKV_ERR_INVALID, "batch %d < 0", a.batch);
   if (a.batch == 0) return PKV_OK;
@@ -762,6 +783,7 @@ int prefill_call(pkv_pool* p, int layer, const void* q, void* out, int out_dtype
                  int max_context_len, int n_head, float scale, const void* k_new,
                  const void* v_new, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "prefill");
   if (int rc = check_layer(p, layer)) return rc;
   if (n_seqs < 0) return fail(p, PKV_ERR_INVALID, "n_seqs %d < 0", n_seqs);
   if (n_seqs == 0 || max_q_len == 0) return PKV_OK;
@@ -812,8 +834,8 @@ int pkv_prefill_attention_append(pkv_pool* p, int layer, const void* q, void* ou
 
 size_t pkv_prefill_workspace_bytes(const pkv_pool* p, int n_seqs, int n_head, int max_q_len,
                                    int max_context_len) {
-  if (!p || n_seqs <= 0 || max_q_len <= 0 || n_head <= 0 || n_head % p->n_kv_head ||
-      max_q_len > pkv::kMaxLen || max_context_len > pkv::kMaxLen)
+  if (!p || p->dtype == PKV_Q4 || n_seqs <= 0 || max_q_len <= 0 || n_head <= 0 ||
+      n_head % p->n_kv_head || max_q_len > pkv::kMaxLen || max_context_len > pkv::kMaxLen)
     return 0;
   int pk = 0, mp = 0;
   size_t need = 0;
@@ -824,6 +846,7 @@ size_t pkv_prefill_workspace_bytes(const pkv_pool* p, int n_seqs, int n_head, in
 int pkv_pool_reserve_prefill(pkv_pool* p, int n_seqs, int n_head, int max_q_len,
                              int max_context_len) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "reserve_prefill");
   if (n_seqs < 0 || max_q_len < 0 || n_head <= 0 || n_head % p->n_kv_head ||
       max_q_len > pkv::kMaxLen || max_context_len > pkv::kMaxLen)
     return fail(p, PKV_ERR_INVALID, "reserve_prefill: n_seqs %d, max_q_len %d, n_head %d, "
@@ -851,7 +874,7 @@ void mixed_ws(const pkv_pool* p, int n_head, const pkv_prefill_batch& pb,
 
 size_t pkv_mixed_workspace_bytes(const pkv_pool* p, int n_head, const pkv_prefill_batch* pb,
                                  const pkv_decode_batch* db) {
-  if (!p || n_head <= 0 || n_head % p->n_kv_head) return 0;
+  if (!p || p->dtype == PKV_Q4 || n_head <= 0 || n_head % p->n_kv_head) return 0;
   if ((pb && (pb->max_q_len > pkv::kMaxLen || pb->max_context_len > pkv::kMaxLen)) ||
       (db && db->max_context_len > pkv::kMaxLen))
     return 0;
@@ -871,6 +894,7 @@ size_t pkv_mixed_workspace_bytes(const pkv_pool* p, int n_head, const pkv_prefil
 int pkv_mixed_attention(pkv_pool* p, int layer, const pkv_prefill_batch* pb,
                         const pkv_decode_batch* db, int n_head, float scale, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "mixed");
   if (int rc = check_layer(p, layer)) return rc;
   // negative counts are refused before either batch is enqueued
   if (pb && pb->n_seqs < 0) return fail(p, PKV_ERR_INVALID, "n_seqs %d < 0", pb->n_seqs);
@@ -1240,13 +1264,14 @@ int pkv_step_tables(int block_size, int num_blocks, const int32_t* seq_lens,
 }
 
 size_t pkv_key_bounds_bytes(const pkv_pool* p) {
-  return p ? (size_t)p->num_blocks * p->n_kv_head * 2 * p->row_bytes : 0;
+  return p && p->dtype != PKV_Q4 ? (size_t)p->num_blocks * p->n_kv_head * 2 * p->row_bytes : 0;
 }
 
 int pkv_key_bounds(pkv_pool* p, int layer, void* bounds, const int32_t* block_tables,
                    int max_blocks_per_seq, const int32_t* first_positions,
                    const int32_t* context_lens, int n_seqs, int max_new_len, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "key_bounds");
   if (int rc = check_layer(p, layer)) return rc;
   if (n_seqs < 0) return fail(p, PKV_ERR_INVALID, "n_seqs %d < 0", n_seqs);
   if (n_seqs == 0) return PKV_OK;
@@ -1317,8 +1342,8 @@ pkv::SelectArgs select_shape(int n_seqs, int total_q, int max_q_len, int max_con
 
 size_t pkv_select_workspace_bytes(const pkv_pool* p, int n_seqs, int total_q, int max_q_len,
                                   int max_context_len, int max_blocks_per_seq, int n_head) {
-  if (!p || n_seqs <= 0 || total_q <= 0 || max_q_len <= 0 || max_q_len > pkv::kMaxLen ||
-      max_context_len <= 0 || max_context_len > pkv::kMaxLen || max_blocks_per_seq <= 0 ||
+  if (!p || p->dtype == PKV_Q4 || n_seqs <= 0 || total_q <= 0 || max_q_len <= 0 ||
+      max_q_len > pkv::kMaxLen || max_context_len <= 0 || max_context_len > pkv::kMaxLen || max_blocks_per_seq <= 0 ||
       n_head < p->n_kv_head)
     return 0;
   return pkv::select_workspace_bytes(p, select_shape(n_seqs, total_q, max_q_len, max_context_len,
@@ -1332,6 +1357,7 @@ int pkv_select_blocks(pkv_pool* p, const void* q, const void* bounds, int32_t* b
                       int total_q, int max_q_len, int max_context_len, int n_head,
                       void* workspace, size_t workspace_bytes, void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "select_blocks");
   if (n_seqs < 0 || total_q < 0)
     return fail(p, PKV_ERR_INVALID, "n_seqs %d, total_q %d < 0", n_seqs, total_q);
   if (n_seqs == 0 || total_q == 0) return PKV_OK;
@@ -1370,7 +1396,7 @@ int pkv_select_blocks(pkv_pool* p, const void* q, const void* bounds, int32_t* b
 }
 
 size_t pkv_sparse_workspace_bytes(const pkv_pool* p, int total_q, int n_head, int top_blocks) {
-  if (!p || total_q <= 0 || n_head < p->n_kv_head || top_blocks <= 0 ||
+  if (!p || p->dtype == PKV_Q4 || total_q <= 0 || n_head < p->n_kv_head || top_blocks <= 0 ||
       top_blocks > pkv::kMaxLen / p->block_size)
     return 0;
   pkv::SparseArgs a{};
@@ -1387,6 +1413,7 @@ int pkv_sparse_attention(pkv_pool* p, int layer, const void* q, void* out, int o
                          int n_head, float scale, void* workspace, size_t workspace_bytes,
                          void* stream) {
   CHECK_POOL(p);
+  REFUSE_Q4(p, "sparse_attention");
   if (int rc = check_layer(p, layer)) return rc;
   if (n_seqs < 0 || total_q < 0)
     return fail(p, PKV_ERR_INVALID, "n_seqs %d, total_q %d < 0", n_seqs, total_q);
@@ -1493,6 +1520,270 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
   hipError_t e = pkv::launch_verify(a, static_cast<char*>(workspace),
                                     static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(nullptr, e, "verify_drafts launch");
+  return PKV_OK;
+}
+
+// ---- a cache held in 4 bits ------------------------------------------------
+namespace {
+bool is_elem(int dt) { return dt == PKV_F32 || dt == PKV_F16 || dt == PKV_BF16; }
+
+// Rows of `row` elements of dt at a token stride that 16-byte loads can take.
+bool stride_ok(long long stride, long long row, int dt, long long n) {
+  const long long e = (long long)pkv::dtype_bytes(dt);
+  return stride >= row && stride <= (1LL << 40) && (stride * e) % 16 == 0 &&
+         (n <= 1 || stride <= (LLONG_MAX / 16) / n);
+}
+// Bytes from the first to past the last of n rows.
+size_t rows_bytes(long long stride, long long row, int dt, long long n) {
+  return n <= 0 ? 0 : (size_t)((n - 1) * stride + row) * pkv::dtype_bytes(dt);
+}
+
+int q4_pool(pkv_pool* p, const char* what) {
+  if (p->dtype != PKV_Q4)
+    return fail(p, PKV_ERR_UNSUPPORTED, "%s: for pools of dtype PKV_Q4 only", what);
+  return PKV_OK;
+}
+}  // namespace
+
+int pkv_q4_append(pkv_pool* p, int layer, const void* k, const void* v, int dtype,
+                  long long k_token_stride, long long v_token_stride,
+                  const int32_t* slot_mapping, int n_tokens, void* stream) {
+  CHECK_POOL(p);
+  if (int rc = q4_pool(p, "q4_append")) return rc;
+  if (int rc = check_layer(p, layer)) return rc;
+  if (n_tokens < 0) return fail(p, PKV_ERR_INVALID, "n_tokens %d < 0", n_tokens);
+  if (!is_elem(dtype)) return fail(p, PKV_ERR_INVALID, "q4_append: dtype %d", dtype);
+  if (n_tokens == 0) return PKV_OK;
+  if (!k || !v || !slot_mapping)
+    return fail(p, PKV_ERR_INVALID, "k, v and slot_mapping must be non-NULL");
+  if (!aligned16(k) || !aligned16(v) || misaligned4({slot_mapping}))
+    return fail(p, PKV_ERR_INVALID, "k and v must be 16-byte aligned, slot_mapping 4-byte");
+  const long long row = (long long)p->n_kv_head * p->head_dim;
+  if (!stride_ok(k_token_stride, row, dtype, n_tokens) ||
+      !stride_ok(v_token_stride, row, dtype, n_tokens))
+    return fail(p, PKV_ERR_INVALID,
+                "q4_append: token strides %lld and %lld: at least %lld elements, a multiple of 16 "
+                "bytes", k_token_stride, v_token_stride, row);
+  if (!pkv::q4_rows_fit(p, n_tokens))
+    return fail(p, PKV_ERR_UNSUPPORTED, "q4_append: %d tokens: too many work-items for one launch",
+                n_tokens);
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_q4_append(p, layer, k, v, dtype, k_token_stride, v_token_stride,
+                                       slot_mapping, n_tokens, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "q4_append launch");
+  return PKV_OK;
+}
+
+int pkv_q4_gather(pkv_pool* p, int layer, const int32_t* slot_mapping, int n, void* out_k,
+                  void* out_v, int out_dtype, void* stream) {
+  CHECK_POOL(p);
+  if (int rc = q4_pool(p, "q4_gather")) return rc;
+  if (int rc = check_layer(p, layer)) return rc;
+  if (n < 0) return fail(p, PKV_ERR_INVALID, "n %d < 0", n);
+  if (!is_elem(out_dtype)) return fail(p, PKV_ERR_INVALID, "q4_gather: out_dtype %d", out_dtype);
+  if (n == 0) return PKV_OK;
+  if (!slot_mapping || !out_k || !out_v)
+    return fail(p, PKV_ERR_INVALID, "slot_mapping, out_k and out_v must be non-NULL");
+  if (!aligned16(out_k) || !aligned16(out_v) || misaligned4({slot_mapping}))
+    return fail(p, PKV_ERR_INVALID, "out_k and out_v must be 16-byte aligned, slot_mapping 4-byte");
+  if (!pkv::q4_rows_fit(p, n))
+    return fail(p, PKV_ERR_UNSUPPORTED, "q4_gather: %d tokens: too many work-items for one launch",
+                n);
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_q4_gather(p, layer, slot_mapping, n, out_k, out_v, out_dtype,
+                                       static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "q4_gather launch");
+  return PKV_OK;
+}
+
+size_t pkv_q4_workspace_bytes(const pkv_pool* p, int n_seqs, int total_q, int max_q_len,
+                              int max_context_len, int n_head) {
+  if (!p || p->dtype != PKV_Q4 || n_seqs <= 0 || total_q <= 0 || max_q_len <= 0 ||
+      max_q_len > pkv::kMaxLen || max_context_len <= 0 || max_context_len > pkv::kMaxLen ||
+      n_head <= 0 || n_head % p->n_kv_head)
+    return 0;
+  pkv::Q4Args a{};
+  a.n_seqs = n_seqs;
+  a.total_q = total_q;
+  a.max_q_len = max_q_len;
+  a.max_context_len = max_context_len;
+  a.n_head = n_head;
+  return pkv::q4_workspace_bytes(p, a);
+}
+
+int pkv_q4_attention(pkv_pool* p, int layer, const void* q, int q_dtype,
+                     long long q_token_stride, void* out, int out_dtype,
+                     const int32_t* cu_q_lens, const int32_t* context_lens,
+                     const int32_t* block_tables, int max_blocks_per_seq, int n_seqs,
+                     int total_q, int max_q_len, int max_context_len, int n_head, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  CHECK_POOL(p);
+  if (int rc = q4_pool(p, "q4_attention")) return rc;
+  if (int rc = check_layer(p, layer)) return rc;
+  if (n_seqs < 0 || total_q < 0)
+    return fail(p, PKV_ERR_INVALID, "n_seqs %d, total_q %d < 0", n_seqs, total_q);
+  if (!is_elem(q_dtype) || (out_dtype != PKV_F32 && out_dtype != q_dtype))
+    return fail(p, PKV_ERR_INVALID, "q4_attention: q_dtype %d, out_dtype %d (PKV_F32 or q_dtype)",
+                q_dtype, out_dtype);
+  if (n_seqs == 0 || total_q == 0) return PKV_OK;
+  if (!q || !out || !context_lens || !block_tables)
+    return fail(p, PKV_ERR_INVALID, "q, out, context_lens and block_tables must be non-NULL");
+  if (!aligned16(q) || !aligned16(out) || misaligned4({cu_q_lens, context_lens, block_tables}))
+    return fail(p, PKV_ERR_INVALID, "q and out must be 16-byte aligned, index arrays 4-byte");
+  if (!cu_q_lens && (total_q != n_seqs || max_q_len != 1))
+    return fail(p, PKV_ERR_INVALID,
+                "without cu_q_lens there is one row per sequence: total_q %d, n_seqs %d, "
+                "max_q_len %d", total_q, n_seqs, max_q_len);
+  if (max_blocks_per_seq <= 0 || max_q_len <= 0 || max_q_len > pkv::kMaxLen ||
+      max_context_len <= 0 || max_context_len > pkv::kMaxLen)
+    return fail(p, PKV_ERR_INVALID,
+                "max_blocks_per_seq (%d) must be > 0, max_q_len (%d) and max_context_len (%d) in "
+                "1 .. 2^30", max_blocks_per_seq, max_q_len, max_context_len);
+  if (n_head <= 0 || n_head % p->n_kv_head != 0)
+    return fail(p, PKV_ERR_INVALID, "n_head %d is not a multiple of n_kv_head %d", n_head,
+                p->n_kv_head);
+  const long long row = (long long)n_head * p->head_dim;
+  if (!stride_ok(q_token_stride, row, q_dtype, total_q))
+    return fail(p, PKV_ERR_INVALID,
+                "q4_attention: q_token_stride %lld: at least %lld elements, a multiple of 16 bytes",
+                q_token_stride, row);
+  if (!std::isfinite(scale)) return fail(p, PKV_ERR_INVALID, "scale must be finite");
+  if (overlap({out, rows_bytes(row, row, out_dtype, total_q)},
+              {q, rows_bytes(q_token_stride, row, q_dtype, total_q)}))
+    return fail(p, PKV_ERR_INVALID, "q4_attention: out overlaps q");
+  pkv::Q4Args a{q, q_dtype, q_token_stride, out, out_dtype, cu_q_lens, context_lens, block_tables,
+                max_blocks_per_seq, n_seqs, total_q, max_q_len, max_context_len, n_head, scale};
+  if (!pkv::q4_fits(p, a))
+    return fail(p, PKV_ERR_UNSUPPORTED,
+                "q4_attention: %d sequences of up to max_q_len %d rows and %d keys: too many "
+                "work-items for one launch", n_seqs, max_q_len, max_context_len);
+  const size_t need = pkv::q4_workspace_bytes(p, a);
+  if (int rc = workspace_check(p, workspace, workspace_bytes, need, "q4_attention")) return rc;
+  if (overlap({workspace, need}, {out, rows_bytes(row, row, out_dtype, total_q)}) ||
+      overlap({workspace, need}, {q, rows_bytes(q_token_stride, row, q_dtype, total_q)}))
+    return fail(p, PKV_ERR_INVALID, "q4_attention: the workspace overlaps q or out");
+  DeviceGuard dg(p->device);
+  hipError_t e = pkv::launch_q4_attention(p, layer, a, static_cast<char*>(workspace),
+                                          static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(p, e, "q4_attention launch");
+  return PKV_OK;
+}
+
+int pkv_prompt_attention(const void* q, const void* k, const void* v, int dtype,
+                         long long q_token_stride, long long k_token_stride,
+                         long long v_token_stride, void* out, int out_dtype,
+                         const int32_t* cu_lens, int n_seqs, int total, int max_len, int n_head,
+                         int n_kv_head, int head_dim, float scale, void* stream) {
+  g_thread_error.clear();
+  if (n_seqs < 0 || total < 0)
+    return fail(nullptr, PKV_ERR_INVALID, "prompt_attention: n_seqs %d, total %d", n_seqs, total);
+  if (!is_elem(dtype) || (out_dtype != PKV_F32 && out_dtype != dtype))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "prompt_attention: dtype %d, out_dtype %d (PKV_F32 or dtype)", dtype, out_dtype);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(nullptr, PKV_ERR_UNSUPPORTED,
+                "prompt_attention: head_dim %d: must be 64, 128 or 256", head_dim);
+  if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head != 0 || n_head > (1 << 20))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "prompt_attention: n_head %d is not a multiple of n_kv_head %d (at most 2^20 heads)",
+                n_head, n_kv_head);
+  if (max_len <= 0 || max_len > pkv::kMaxLen)
+    return fail(nullptr, PKV_ERR_INVALID, "prompt_attention: max_len %d (1 .. 2^30)", max_len);
+  if (!std::isfinite(scale))
+    return fail(nullptr, PKV_ERR_INVALID, "prompt_attention: scale must be finite");
+  if (n_seqs == 0 || total == 0) return PKV_OK;
+  if (!q || !k || !v || !out || !cu_lens)
+    return fail(nullptr, PKV_ERR_INVALID, "prompt_attention: NULL argument");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || misaligned4({cu_lens}))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "prompt_attention: q, k, v and out must be 16-byte aligned, cu_lens 4-byte");
+  const long long qr = (long long)n_head * head_dim, kr = (long long)n_kv_head * head_dim;
+  if (!stride_ok(q_token_stride, qr, dtype, total) || !stride_ok(k_token_stride, kr, dtype, total) ||
+      !stride_ok(v_token_stride, kr, dtype, total))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "prompt_attention: token strides %lld, %lld, %lld: at least %lld, %lld, %lld "
+                "elements, multiples of 16 bytes", q_token_stride, k_token_stride, v_token_stride,
+                qr, kr, kr);
+  const Range o = {out, rows_bytes(qr, qr, out_dtype, total)};
+  if (overlap(o, {q, rows_bytes(q_token_stride, qr, dtype, total)}) ||
+      overlap(o, {k, rows_bytes(k_token_stride, kr, dtype, total)}) ||
+      overlap(o, {v, rows_bytes(v_token_stride, kr, dtype, total)}))
+    return fail(nullptr, PKV_ERR_INVALID, "prompt_attention: out overlaps q, k or v");
+  pkv::PromptArgs a{q, k, v, dtype, q_token_stride, k_token_stride, v_token_stride, out, out_dtype,
+                    cu_lens, n_seqs, total, max_len, n_head, n_kv_head, head_dim, scale};
+  if (!pkv::prompt_fits(a))
+    return fail(nullptr, PKV_ERR_UNSUPPORTED,
+                "prompt_attention: %d prompts of up to max_len %d, %d heads: too many work-items for "
+                "one launch", n_seqs, max_len, n_head);
+  hipError_t e = pkv::launch_prompt(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(nullptr, e, "prompt_attention launch");
+  return PKV_OK;
+}
+
+int pkv_adjust_logits(const void* logits, void* out, int dtype, long long row_stride,
+                      long long out_row_stride, int batch, int vocab, const int32_t* tokens,
+                      const int32_t* cu_tokens, int total_tokens, const int32_t* prompt_lens,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const int32_t* bias_tokens, const float* bias_values,
+                      const int32_t* cu_bias, int total_bias, const uint32_t* mask, int n_masks,
+                      int mask_row_words, const int32_t* mask_rows, void* stream) {
+  g_thread_error.clear();
+  if (batch < 0 || batch > pkv::kMaxLen || vocab <= 0 || vocab >= (1 << 24))
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: batch %d, vocab %d (1 .. 2^24 - 1)",
+                batch, vocab);
+  if (!is_elem(dtype)) return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: dtype %d", dtype);
+  if (total_tokens < 0 || total_bias < 0 || total_tokens > pkv::kMaxLen ||
+      total_bias > pkv::kMaxLen)
+    return fail(nullptr, PKV_ERR_INVALID,
+                "adjust_logits: total_tokens %d, total_bias %d (0 .. 2^30)", total_tokens,
+                total_bias);
+  if (batch == 0) return PKV_OK;
+  if (!logits || !out) return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: NULL logits or out");
+  if ((cu_tokens && total_tokens && !tokens) || (!cu_tokens && total_tokens))
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: tokens and cu_tokens: both or neither");
+  if ((cu_bias && total_bias && (!bias_tokens || !bias_values)) || (!cu_bias && total_bias))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "adjust_logits: bias_tokens, bias_values and cu_bias: all or none");
+  const size_t e = pkv::dtype_bytes(dtype);
+  if (batch > 1 && (row_stride < vocab || out_row_stride < vocab || row_stride > (1LL << 40) ||
+                    out_row_stride > (1LL << 40)))
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: row strides %lld, %lld < vocab %d",
+                row_stride, out_row_stride, vocab);
+  if (batch == 1) row_stride = out_row_stride = vocab;
+  if (reinterpret_cast<uintptr_t>(logits) % e || reinterpret_cast<uintptr_t>(out) % e)
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: logits not aligned to the element size");
+  if (misaligned4({tokens, cu_tokens, prompt_lens, repetition, presence, frequency, bias_tokens,
+                   bias_values, cu_bias, mask, mask_rows}))
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: arrays must be 4-byte aligned");
+  if (mask && (n_masks <= 0 || mask_row_words < (vocab + 31) / 32 || (!mask_rows && n_masks < batch)))
+    return fail(nullptr, PKV_ERR_INVALID,
+                "adjust_logits: %d mask rows of %d words: at least %d words, and without mask_rows a "
+                "row per request", n_masks, mask_row_words, (vocab + 31) / 32);
+  // Rows are read and written by the same threads, so out may be logits.
+  const bool in_place = logits == out;
+  if (in_place && row_stride != out_row_stride)
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: in place, strides %lld and %lld differ",
+                row_stride, out_row_stride);
+  const Range o = {out, rows_bytes(out_row_stride, vocab, dtype, batch)};
+  if (!in_place && overlap(o, {logits, rows_bytes(row_stride, vocab, dtype, batch)}))
+    return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: out overlaps logits");
+  const size_t nb = 4 * (size_t)batch;
+  const Range in[] = {{tokens, 4 * (size_t)total_tokens}, {cu_tokens, nb + 4}, {prompt_lens, nb},
+                      {repetition, nb}, {presence, nb}, {frequency, nb},
+                      {bias_tokens, 4 * (size_t)total_bias}, {bias_values, 4 * (size_t)total_bias},
+                      {cu_bias, nb + 4}, {mask, 4 * (size_t)n_masks * (size_t)mask_row_words},
+                      {mask_rows, nb}};
+  for (const Range& i : in)
+    if (i.at && overlap_rows(i, out, e * vocab, e * (size_t)out_row_stride, (size_t)batch))
+      return fail(nullptr, PKV_ERR_INVALID, "adjust_logits: out overlaps an input");
+  pkv::LogitsArgs a{logits, out, dtype, row_stride, out_row_stride, batch, vocab, tokens, cu_tokens,
+                    total_tokens, prompt_lens, repetition, presence, frequency, bias_tokens,
+                    bias_values, cu_bias, total_bias, mask, n_masks, mask_row_words, mask_rows};
+  if (!pkv::logits_fits(a))
+    return fail(nullptr, PKV_ERR_UNSUPPORTED,
+                "adjust_logits: batch %d of %d: too many work-items for one launch", batch, vocab);
+  hipError_t err = pkv::launch_logits(a, static_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return hip_fail(nullptr, err, "adjust_logits launch");
   return PKV_OK;
 }
 

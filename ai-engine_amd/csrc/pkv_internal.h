@@ -85,6 +85,10 @@ namespace pkv {
 
 inline size_t dtype_bytes(int dt) { return dt == PKV_F32 ? 4 : 2; }
 
+// Bytes of a token's row in one kv head of a PKV_Q4 pool: 4 bits an element, and two
+// f16 for each group of 32.
+inline size_t q4_row_bytes(int head_dim) { return (size_t)head_dim * 5 / 8; }
+
 // Token selection (pkv_sample.hip): the fixed draw r of a seed, and the
 // launcher of the per-row argmax / sample kernel.
 float sample_draw(uint64_t seed);
@@ -337,5 +341,84 @@ struct VerifyArgs {
 size_t verify_workspace_bytes(const VerifyArgs& a);
 bool verify_fits(const VerifyArgs& a);
 hipError_t launch_verify(const VerifyArgs& a, char* ws, hipStream_t stream);
+
+// A cache held in 4 bits: the store and the values back (pkv_q4.hip) ...
+bool q4_rows_fit(const pkv_pool* p, int n_tokens);
+hipError_t launch_q4_append(const pkv_pool* p, int layer, const void* k, const void* v, int dtype,
+                            long long k_stride, long long v_stride, const int32_t* slots, int n,
+                            hipStream_t stream);
+hipError_t launch_q4_gather(const pkv_pool* p, int layer, const int32_t* slots, int n,
+                            void* out_k, void* out_v, int out_dtype, hipStream_t stream);
+
+// ... and attention over it (pkv_q4_attn.hip).
+struct Q4Args {
+  const void* q;
+  int q_dtype;
+  long long q_stride;  // elements from token to token
+  void* out;
+  int out_dtype;
+  const int32_t* cu_q_lens;  // null: one row per sequence
+  const int32_t* context_lens;
+  const int32_t* block_tables;
+  int max_blocks_per_seq;
+  int n_seqs;
+  int total_q;
+  int max_q_len;
+  int max_context_len;
+  int n_head;
+  float scale;
+};
+size_t q4_workspace_bytes(const pkv_pool* p, const Q4Args& a);
+bool q4_fits(const pkv_pool* p, const Q4Args& a);
+hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, char* ws,
+                               hipStream_t stream);
+
+// Attention of whole prompts over their own rows (pkv_prompt.hip).
+struct PromptArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  int dtype;
+  long long q_stride, k_stride, v_stride;  // elements from token to token
+  void* out;
+  int out_dtype;
+  const int32_t* cu_lens;
+  int n_seqs;
+  int total;
+  int max_len;
+  int n_head;
+  int n_kv_head;
+  int head_dim;
+  float scale;
+};
+bool prompt_fits(const PromptArgs& a);
+hipError_t launch_prompt(const PromptArgs& a, hipStream_t stream);
+
+// Penalties, biases and masks on logits (pkv_logits.hip).
+struct LogitsArgs {
+  const void* logits;
+  void* out;
+  int dtype;
+  long long row_stride, out_row_stride;
+  int batch;
+  int vocab;
+  const int32_t* tokens;
+  const int32_t* cu_tokens;
+  int total_tokens;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  const int32_t* cu_bias;
+  int total_bias;
+  const uint32_t* mask;
+  int n_masks;
+  int mask_row_words;
+  const int32_t* mask_rows;
+};
+bool logits_fits(const LogitsArgs& a);
+hipError_t launch_logits(const LogitsArgs& a, hipStream_t stream);
 
 }  // namespace pkv

@@ -22,14 +22,15 @@ import sys
 import math
 from typing import Sequence
 
-from ._lib import (BF16, F16, F32, K, V, CapacityError, PagedKvError, check, lib,
+from ._lib import (BF16, F16, F32, K, Q4, V, CapacityError, PagedKvError, check, lib,
                    LIB_PATH)
 
 __all__ = [
     "BlockAllocator", "BlockTable", "PagedKvCache", "KvPool", "Rope", "rope_tables_host",
     "CapacityError",
-    "PagedKvError", "F32", "F16", "BF16", "lib", "LIB_PATH", "torch_dtype",
-    "pkv_dtype", "StepTables", "step_tables", "verify_drafts",
+    "PagedKvError", "F32", "F16", "BF16", "Q4", "lib", "LIB_PATH", "torch_dtype",
+    "pkv_dtype", "StepTables", "step_tables", "verify_drafts", "prompt_attention",
+    "adjust_logits",
 ]
 
 
@@ -396,6 +397,149 @@ def verify_drafts(target_logits, draft_tokens, cu_drafts, uniforms, final_unifor
     return tokens, accepted
 
 
+def _rows_view(t, name: str, device, dtype, heads, head_dim):
+    """t (tokens, heads, head_dim) as (tensor, elements from token to token): rows
+    that lie whole in memory, 16 bytes aligned, at any stride (the columns of a
+    projection) are taken where they are, others copied."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise ValueError(f"{name} must be a tensor on {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ValueError(f"{name} must be (tokens, {heads}, {head_dim}), got {tuple(t.shape)}")
+    row, stride, e = heads * head_dim, t.stride(0), t.element_size()
+    if (t.stride(2) != 1 and head_dim > 1) or (t.stride(1) != head_dim and heads > 1) or \
+            t.data_ptr() % 16 or (t.shape[0] > 1 and (stride < row or stride * e % 16)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        stride = row
+    return t, (stride if t.shape[0] > 1 else row)
+
+
+def _attn_out(out, rows: int, width: int, dtype, out_dtype, device):
+    """The result tensor of an attention call, given or new, in `dtype` or float32."""
+    import torch
+    if out is None:
+        out_dtype = out_dtype or dtype
+        if out_dtype not in (dtype, torch.float32):
+            raise TypeError(f"out_dtype must be {dtype} or torch.float32")
+        return torch.empty((rows, width), dtype=out_dtype, device=device)
+    if out.device != device or out.shape != (rows, width) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous ({rows}, {width}) on {device}")
+    if out.dtype not in (dtype, torch.float32) or (out_dtype or out.dtype) != out.dtype:
+        raise TypeError(f"out must be {dtype} or torch.float32, as out_dtype says")
+    return out
+
+
+def prompt_attention(q, k, v, cu_lens, max_len: int | None = None, scale: float | None = None,
+                     out_dtype=None, out=None, stream=None):
+    """Causal attention of whole prompts over their own rows (pkv_prompt_attention):
+    prompt s is rows cu_lens[s] .. cu_lens[s + 1] - 1, and each of its tokens
+    attends those up to itself.  q: (total, H, hd), k, v: (total, n_kv, hd) in one of
+    f32/f16/bf16, hd 64, 128 or 256; columns of one projection (rows at a stride) are
+    read in place.  cu_lens: (n + 1,) int32.  max_len: host bound of the lengths (None:
+    the longest one if cu_lens is on the host, else total), which sizes the
+    launch.  out_dtype: the inputs' (default) or float32.  Nothing synchronises.
+    Returns (total, H * hd); rows of no prompt are not written."""
+    import torch
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3:
+        raise ValueError("q must be a (total, n_head, head_dim) device tensor")
+    dev, (total, H, hd) = q.device, q.shape
+    if k.dim() != 3 or k.shape[0] != total or v.shape[:1] != k.shape[:1]:
+        raise ValueError("q, k and v must have a row per token")
+    kvh = k.shape[1]
+    if kvh < 1 or H % kvh:
+        raise ValueError(f"{H} query heads are not a multiple of {kvh} kv heads")
+    cu = _i32_on(cu_lens, dev)
+    n = cu.numel() - 1
+    if n < 0:
+        raise ValueError("cu_lens must be (n + 1,)")
+    if max_len is None:
+        if getattr(cu_lens, "is_cuda", False) or n < 1:
+            max_len = total
+        else:
+            max_len = int(torch.as_tensor(cu_lens, dtype=torch.int64).diff().max())
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    s, ctx = _run_on(stream, dev, (q, k, v, cu, out))
+    with ctx:
+        qq, qs = _rows_view(q, "q", dev, q.dtype, H, hd)
+        kk, ks = _rows_view(k, "k", dev, q.dtype, kvh, hd)
+        vv, vs = _rows_view(v, "v", dev, q.dtype, kvh, hd)
+        out = _attn_out(out, total, H * hd, q.dtype, out_dtype, dev)
+        check(lib().pkv_prompt_attention(
+            _dev_ptr(qq), _dev_ptr(kk), _dev_ptr(vv), pkv_dtype(q.dtype), qs, ks, vs,
+            _dev_ptr(out), pkv_dtype(out.dtype), _dev_ptr(cu), n, total, max(int(max_len), 1), H,
+            kvh, hd, float(scale), s), None)
+    return out
+
+
+def adjust_logits(logits, tokens=None, cu_tokens=None, prompt_lens=None, repetition=None,
+                  presence=None, frequency=None, bias_tokens=None, bias_values=None, cu_bias=None,
+                  mask=None, mask_rows=None, out=None, stream=None):
+    """Penalties, biases and masks on logits before a token is chosen
+    (pkv_adjust_logits).  logits: (batch, vocab) f32/f16/bf16 with unit stride along
+    vocab.  tokens: (any,) int32, request b's at cu_tokens[b] .. cu_tokens[b + 1] - 1, the first
+    prompt_lens[b] of them its prompt.  Tokens seen: logits divided (positive ones)
+    or multiplied by repetition[b]; generated ones: frequency[b] times their
+    count and presence[b] taken off.  bias_tokens (any,) int32, bias_values (any,) float32,
+    cu_bias (batch + 1,) int32: added (the last entry of a token counts).  mask: (masks,
+    words) int32, bit t % 32 of word t // 32 set where t may be chosen, the others
+    become -inf; mask_rows: (batch,) int32, a request's row of it, negative for no mask
+    (None: row b).  In 32 bits, rounded once.  repetition, presence, frequency:
+    (batch,) float32.  Everything but logits may be None.  Nothing synchronises.
+    Returns the result: `out`, logits itself for out=logits, or a new tensor."""
+    import torch
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() != 2:
+        raise ValueError("logits must be a (batch, vocab) device tensor")
+    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    B, V = logits.shape
+    for t, name in ((logits, "logits"), (out, "out")):
+        if t is not None and (t.device != dev or t.dtype != logits.dtype or t.shape != (B, V) or
+                              (V > 1 and B and t.stride(1) != 1)):
+            raise ValueError(f"{name} must be ({B}, {V}) {logits.dtype} on {dev} with unit stride "
+                             "along vocab")
+    if (tokens is None) != (cu_tokens is None) or (prompt_lens is not None and tokens is None):
+        raise ValueError("tokens and cu_tokens go together (and prompt_lens with them)")
+    if len({x is None for x in (bias_tokens, bias_values, cu_bias)}) > 1:
+        raise ValueError("bias_tokens, bias_values and cu_bias go together")
+    if mask is None and mask_rows is not None:
+        raise ValueError("mask_rows without mask")
+
+    def dev_arr(t, name, dtype, shape=None):
+        return None if t is None else _device_tensor(t, name, dev, dtype, shape)
+
+    s, ctx = _run_on(stream, dev, (logits, out, tokens, cu_tokens, prompt_lens, repetition, presence,
+                                   frequency, bias_tokens, bias_values, cu_bias, mask, mask_rows))
+    with ctx:
+        tok = dev_arr(tokens, "tokens", i32)
+        cut = dev_arr(cu_tokens, "cu_tokens", i32, (B + 1,))
+        pl = dev_arr(prompt_lens, "prompt_lens", i32, (B,))
+        rep = dev_arr(repetition, "repetition", f32, (B,))
+        pres = dev_arr(presence, "presence", f32, (B,))
+        freq = dev_arr(frequency, "frequency", f32, (B,))
+        bt = dev_arr(bias_tokens, "bias_tokens", i32)
+        bv = dev_arr(bias_values, "bias_values", f32, None if bt is None else bt.shape)
+        cb = dev_arr(cu_bias, "cu_bias", i32, (B + 1,))
+        mk = dev_arr(mask, "mask", i32)
+        mr = dev_arr(mask_rows, "mask_rows", i32, (B,))
+        if mk is not None and mk.dim() != 2:
+            raise ValueError("mask must be (masks, words)")
+        if out is None:
+            out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+
+        def at(t):
+            return None if t is None else _dev_ptr(t)
+
+        check(lib().pkv_adjust_logits(
+            _dev_ptr(logits), _dev_ptr(out), pkv_dtype(logits.dtype), logits.stride(0),
+            out.stride(0), B, V, at(tok), at(cut), 0 if tok is None else tok.numel(), at(pl),
+            at(rep), at(pres), at(freq), at(bt), at(bv), at(cb), 0 if bt is None else bt.numel(),
+            at(mk), 0 if mk is None else mk.shape[0], 0 if mk is None else mk.shape[1], at(mr), s),
+            None)
+    return out
+
+
 class Rope:
     """The reference's Rope (rope.rs:6-33): cos/sin tables in device memory;
     apply() is apply_rope (rope.rs:38-42) with per-token positions."""
@@ -450,6 +594,9 @@ class PagedKvCache:
 
     def __init__(self, n_layers: int, num_blocks: int, block_size: int, n_kv_head: int,
                  head_dim: int, dtype=None, device: int = 0) -> None:
+        """dtype: torch.float32 (default), float16, bfloat16, or pagedkv.Q4 for a pool
+        held in 4 bits (KvPool.q4_append, q4_gather and q4_attention, copy_blocks,
+        compact)."""
         import torch
         if dtype is None:
             dtype = torch.float32
@@ -459,7 +606,8 @@ class PagedKvCache:
         self.device = torch.device("cuda", device)
         h = ctypes.c_void_p()
         rc = lib().pkv_pool_create(ctypes.byref(h), n_layers, num_blocks, block_size,
-                                   n_kv_head, head_dim, pkv_dtype(dtype), device)
+                                   n_kv_head, head_dim, Q4 if dtype == Q4 else pkv_dtype(dtype),
+                                   device)
         check(rc, None)
         self._h = h
 
@@ -1017,6 +1165,102 @@ class KvPool:
                 _dev_ptr(bl), bl.shape[2], _dev_ptr(cu) if cu is not None else None,
                 _dev_ptr(cl), _dev_ptr(bt), bt.shape[1], n, rows, mq, H, float(scale),
                 _dev_ptr(ws) if need else None, need, s), self._h)
+        return out
+
+    # -- a cache held in 4 bits ---------------------------------------------------
+    def _check_q4(self, what: str) -> None:
+        if self.cache.dtype != Q4:
+            raise TypeError(f"{what} is for caches of dtype pagedkv.Q4")
+
+    def q4_append(self, k, v, slot_mapping, stream=None) -> None:
+        """Stores k, v (n, n_kv, hd), both f32, f16 or bf16, in 4 bits at the given slots
+        (pkv_q4_append; int32, negative = skip, distinct).  Rows at a stride are
+        read in place."""
+        self._check_q4("q4_append")
+        c = self.cache
+        s, ctx = _run_on(stream, c.device, (k, v, slot_mapping if hasattr(slot_mapping, "is_cuda")
+                                            and slot_mapping.is_cuda else None))
+        with ctx:
+            kk, ks = _rows_view(k, "k", c.device, k.dtype, c.n_kv_head, c.head_dim)
+            vv, vs = _rows_view(v, "v", c.device, k.dtype, c.n_kv_head, c.head_dim)
+            sm = _i32_on(slot_mapping, c.device)
+            if sm.numel() != k.shape[0] or v.shape[0] != k.shape[0]:
+                raise ValueError("slot_mapping / k / v lengths differ")
+            check(lib().pkv_q4_append(self._h, self.layer_index, _dev_ptr(kk), _dev_ptr(vv),
+                                      pkv_dtype(k.dtype), ks, vs, _dev_ptr(sm), sm.numel(), s),
+                  self._h)
+
+    def q4_gather(self, slot_mapping, out_dtype=None, stream=None):
+        """The values that the given slots' rows stand for (pkv_q4_gather): k, v
+        (n, n_kv, hd) in out_dtype (float32 by default); zeros at negative slots."""
+        import torch
+        self._check_q4("q4_gather")
+        c = self.cache
+        s, ctx = _run_on(stream, c.device, (slot_mapping if hasattr(slot_mapping, "is_cuda")
+                                            and slot_mapping.is_cuda else None,))
+        with ctx:
+            sm = _i32_on(slot_mapping, c.device)
+            ok = torch.empty((sm.numel(), c.n_kv_head, c.head_dim),
+                             dtype=out_dtype or torch.float32, device=c.device)
+            ov = torch.empty_like(ok)
+            check(lib().pkv_q4_gather(self._h, self.layer_index, _dev_ptr(sm), sm.numel(),
+                                      _dev_ptr(ok), _dev_ptr(ov), pkv_dtype(ok.dtype), s), self._h)
+        return ok, ov
+
+    def q4_attention(self, q, block_tables, context_lens, cu_q_lens=None,
+                     max_q_len: int | None = None, max_context_len: int | None = None,
+                     scale: float | None = None, out_dtype=None, out=None, stream=None):
+        """Attention over a cache held in 4 bits (pkv_q4_attention).  q: (rows, H, hd) f32,
+        f16 or bf16, at any stride between rows; block_tables: (n, width) int32;
+        context_lens: (n,) int32, the new tokens among them, which q4_append has stored;
+        cu_q_lens: (n + 1,) int32 (None: one row per sequence), row i of a chunk of m
+        rows attending the keys up to position context_lens - m + i.  max_q_len: host
+        bound of the chunks (None: the longest one if cu_q_lens is on the host, else all
+        rows: then the launch is wider than it need be); max_context_len: host bound
+        (None: what the tables hold).  out_dtype: q's (default) or float32.  Nothing
+        synchronises.  Returns (rows, H * hd); a row without keys is zero, rows of no
+        sequence, and of one beyond a bound, are not written."""
+        import torch
+        self._check_q4("q4_attention")
+        c = self.cache
+        if not isinstance(q, torch.Tensor) or q.device != c.device or q.dim() != 3 or \
+                q.shape[2] != c.head_dim:
+            raise ValueError(f"q must be (rows, n_head, {c.head_dim}) on {c.device}")
+        rows, H, hd = q.shape
+        s, ctx = _run_on(stream, c.device,
+                         [t for t in (q, block_tables, context_lens, cu_q_lens, out)
+                          if getattr(t, "is_cuda", False)])
+        with ctx:
+            bt, cl = _i32_on(block_tables, c.device), _i32_on(context_lens, c.device)
+            cu = _i32_on(cu_q_lens, c.device) if cu_q_lens is not None else None
+            n = cl.numel()
+            if bt.dim() != 2 or bt.shape[0] != n:
+                raise ValueError("block_tables must be (n, width), context_lens (n,)")
+            if cu is not None and cu.numel() != n + 1:
+                raise ValueError("cu_q_lens must be (n + 1,)")
+            if cu is None and rows != n:
+                raise ValueError("without cu_q_lens q has one row per sequence")
+            if max_q_len is None:
+                max_q_len = 1
+                if cu is not None and getattr(cu_q_lens, "is_cuda", False):
+                    max_q_len = max(rows, 1)  # (a bound without a synchronisation)
+                elif cu is not None and n:
+                    max_q_len = max(int(torch.as_tensor(cu_q_lens, dtype=torch.int64).diff().max()),
+                                    1)
+            if max_context_len is None:
+                max_context_len = bt.shape[1] * c.block_size
+            if scale is None:
+                scale = 1.0 / math.sqrt(hd)
+            qq, qs = _rows_view(q, "q", c.device, q.dtype, H, hd)
+            out = _attn_out(out, rows, H * hd, q.dtype, out_dtype, c.device)
+            need = lib().pkv_q4_workspace_bytes(self._h, n, rows, int(max_q_len),
+                                                int(max_context_len), H)
+            ws = _workspace(need, c.device) if need else None
+            check(lib().pkv_q4_attention(
+                self._h, self.layer_index, _dev_ptr(qq), pkv_dtype(q.dtype), qs, _dev_ptr(out),
+                pkv_dtype(out.dtype), _dev_ptr(cu) if cu is not None else None, _dev_ptr(cl),
+                _dev_ptr(bt), bt.shape[1], n, rows, int(max_q_len), int(max_context_len), H,
+                float(scale), _dev_ptr(ws) if need else None, need, s), self._h)
         return out
 
     def _check_rows(self, t, name: str) -> None:

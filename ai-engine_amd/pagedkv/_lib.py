@@ -20,12 +20,13 @@ PKV_ERR_UNSUPPORTED = -4
 PKV_ERR_CAPACITY = -5
 PKV_ERR_DEVICE_DATA = -6
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, Q4 = 0, 1, 2, 3
 K, V = 0, 1
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
 _I32P = ctypes.POINTER(ctypes.c_int32)
 
 
@@ -128,6 +129,15 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_verify_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "pkv_verify_drafts": (_I, [_P, _I, ctypes.c_longlong, _P, _I, ctypes.c_longlong, _P, _P, _I, _I,
                                _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "pkv_q4_append": (_I, [_P, _I, _P, _P, _I, _LL, _LL, _P, _I, _P]),
+    "pkv_q4_gather": (_I, [_P, _I, _P, _I, _P, _P, _I, _P]),
+    "pkv_q4_workspace_bytes": (_SZ, [_P, _I, _I, _I, _I, _I]),
+    "pkv_q4_attention": (_I, [_P, _I, _P, _I, _LL, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                              ctypes.c_float, _P, _SZ, _P]),
+    "pkv_prompt_attention": (_I, [_P, _P, _P, _I, _LL, _LL, _LL, _P, _I, _P, _I, _I, _I, _I, _I, _I,
+                                  ctypes.c_float, _P]),
+    "pkv_adjust_logits": (_I, [_P, _P, _I, _LL, _LL, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P,
+                               _P, _I, _P, _I, _I, _P, _P]),
     "pkv_pool_profile": (_I, [_P, _I]),
     "pkv_pool_profile_read": (_I, [_P, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I)]),
     "pkv_allocator_new": (_P, [_SZ, _SZ]),

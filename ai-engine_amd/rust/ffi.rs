@@ -22,6 +22,7 @@ pub const PKV_ERR_DEVICE_DATA: c_int = -6;
 pub const PKV_F32: c_int = 0;
 pub const PKV_F16: c_int = 1;
 pub const PKV_BF16: c_int = 2;
+pub const PKV_Q4: c_int = 3;
 pub const PKV_K: c_int = 0;
 pub const PKV_V: c_int = 1;
 
@@ -318,6 +319,42 @@ extern "C" {
         c_int, uniforms: *const f32, final_uniforms: *const f32, temperatures: *const f32,
         out_tokens: *mut i32, n_accepted: *mut i32, workspace: *mut c_void, workspace_bytes:
         usize, stream: *mut c_void
+    ) -> c_int;
+    pub fn pkv_q4_append(
+        pool: *mut PkvPool, layer: c_int, k: *const c_void, v: *const c_void, dtype: c_int,
+        k_token_stride: c_longlong, v_token_stride: c_longlong, slot_mapping: *const i32,
+        n_tokens: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn pkv_q4_gather(
+        pool: *mut PkvPool, layer: c_int, slot_mapping: *const i32, n: c_int,
+        out_k: *mut c_void, out_v: *mut c_void, out_dtype: c_int, stream: *mut c_void,
+    ) -> c_int;
+    pub fn pkv_q4_workspace_bytes(
+        pool: *const PkvPool, n_seqs: c_int, total_q: c_int, max_q_len: c_int,
+        max_context_len: c_int, n_head: c_int,
+    ) -> usize;
+    pub fn pkv_q4_attention(
+        pool: *mut PkvPool, layer: c_int, q: *const c_void, q_dtype: c_int,
+        q_token_stride: c_longlong, out: *mut c_void, out_dtype: c_int, cu_q_lens: *const i32,
+        context_lens: *const i32, block_tables: *const i32, max_blocks_per_seq: c_int,
+        n_seqs: c_int, total_q: c_int, max_q_len: c_int, max_context_len: c_int, n_head: c_int,
+        scale: f32, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
+    ) -> c_int;
+    pub fn pkv_prompt_attention(
+        q: *const c_void, k: *const c_void, v: *const c_void, dtype: c_int,
+        q_token_stride: c_longlong, k_token_stride: c_longlong, v_token_stride: c_longlong,
+        out: *mut c_void, out_dtype: c_int, cu_lens: *const i32, n_seqs: c_int, total: c_int,
+        max_len: c_int, n_head: c_int, n_kv_head: c_int, head_dim: c_int, scale: f32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn pkv_adjust_logits(
+        logits: *const c_void, out: *mut c_void, dtype: c_int, row_stride: c_longlong,
+        out_row_stride: c_longlong, batch: c_int, vocab: c_int, tokens: *const i32,
+        cu_tokens: *const i32, total_tokens: c_int, prompt_lens: *const i32,
+        repetition: *const f32, presence: *const f32, frequency: *const f32,
+        bias_tokens: *const i32, bias_values: *const f32, cu_bias: *const i32,
+        total_bias: c_int, mask: *const u32, n_masks: c_int, mask_row_words: c_int,
+        mask_rows: *const i32, stream: *mut c_void,
     ) -> c_int;
 
     // ---- block allocator and tables (block_table.rs:5-58)

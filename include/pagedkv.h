@@ -54,6 +54,7 @@ extern "C" {
 #define PKV_F32 0
 #define PKV_F16 1
 #define PKV_BF16 2
+#define PKV_Q4 3 /* of pools only: 4 bits an element and 8 for a group's scale and offset */
 
 /* ---- pool selectors ---------------------------------------------------- */
 #define PKV_K 0
@@ -72,7 +73,8 @@ const char* pkv_last_error(const pkv_pool* pool);
  * filled like Tensor::zeros in KvPool::new (attention.rs:39-55).  One handle
  * stands for the reference's Vec<KvPool> (engine.rs:70-72): layer l of the
  * handle is the reference's kv[l].  Block ids are shared by all layers.
- * dtype: PKV_F32 (the reference's own dtype), PKV_F16 or PKV_BF16.
+ * dtype: PKV_F32 (the reference's own dtype), PKV_F16, PKV_BF16, or PKV_Q4
+ * (no reference counterpart; see "a cache held in 4 bits").
  * Shape limits (PKV_ERR_UNSUPPORTED otherwise), narrower than the
  * reference's KvPool::new, which takes any sizes:
  *  - head_dim 64, 128 or 256.  The reference reads it from GGUF
@@ -697,6 +699,132 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
                       const float* final_uniforms, const float* temperatures,
                       int32_t* out_tokens, int32_t* n_accepted, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ---- a cache held in 4 bits (no reference counterpart) ------------------------
+ * A pool of dtype PKV_Q4 holds a third of what a 16-bit pool does for the same
+ * tokens.  A step of an engine over one:
+ *   pkv_prompt_attention  whole prompts over their own rows, before they are rounded
+ *   pkv_q4_append         keys and values into the pool
+ *   pkv_q4_attention      single tokens and chunks over the pool
+ *   pkv_adjust_logits     penalties, biases and masks before pkv_sample
+ * All are stream-ordered, allocate nothing and can be captured in a HIP graph;
+ * scratch is the caller's.  Pool calls that do not read or write elements take such
+ * pools too: shapes, pkv_pool_read / write / read_blocks (bytes), pkv_copy_blocks,
+ * pkv_compact, pkv_pool_check.  The others return PKV_ERR_UNSUPPORTED.
+ *
+ * What is held: 32 neighbouring channels of a token's row in one kv head are a
+ * group.  With its elements x (NaN taken as 0, others limited to +-65504), m =
+ * f16(min x) and s = f16((max x - m) / 15), the subtraction and the division in f32,
+ * an element is held as c = (x - m) / s in 64 bits, rounded to nearest even and
+ * limited to 0 .. 15 (0 where s is 0), and stands for m + s c.
+ *
+ * Layout: block_size a power of two in [16, 256], bs; hd = head_dim, G = hd / 32
+ * groups, T = hd / 16.  One layer's K (or V) is [num_blocks][n_kv_head][chunk],
+ * a chunk being bs * hd * 5 / 8 bytes:
+ *   K  codes  [bs][4][G] 32-bit words: word (token, i, g) has channels 32 g + 8 i
+ *             + e, e = 0 .. 7, in bits 4 (e / 2 + 4 (e % 2)) on
+ *      s      [bs / 4][G][4] f16 (token / 4, group, token % 4)
+ *      m      [bs][G] f16
+ *   V  codes  [16][bs][T / 2] bytes: (i, token) has channels i + 16 t, t = 0 .. T - 1,
+ *             in bits 4 t on
+ *      s, m   [bs / 4][G][4] f16 each
+ * so that a token's bytes are its own: rows are written without reading others. */
+
+/* Stores rows of k and v (dtype PKV_F32, PKV_F16 or PKV_BF16) in 4 bits: token i, at k +
+ * i * k_token_stride elements (v likewise), [n_kv_head][head_dim], goes to slot
+ * slot_mapping[i].  Slots as in pkv_append: negative ones are skipped, ones beyond
+ * the pool reported by pkv_pool_check(); distinct (two tokens for one slot race).
+ * Token strides: at least n_kv_head * head_dim, a multiple of 16 bytes.  k and v
+ * 16-byte aligned. */
+int pkv_q4_append(pkv_pool* pool, int layer, const void* k, const void* v, int dtype,
+                  long long k_token_stride, long long v_token_stride,
+                  const int32_t* slot_mapping, int n_tokens, void* stream);
+
+/* The values that slots stand for: out_k, out_v [n][n_kv_head][head_dim] in out_dtype
+ * (PKV_F32, PKV_F16 or PKV_BF16), 16-byte aligned.  A negative slot gives a zero row, one
+ * beyond the pool a zero row that pkv_pool_check() reports. */
+int pkv_q4_gather(pkv_pool* pool, int layer, const int32_t* slot_mapping, int n, void* out_k,
+                  void* out_v, int out_dtype, void* stream);
+
+/* Attention over a 4-bit pool: out_h = sum_k softmax_k(scale q_h . k) v_k over the
+ * values that the row's keys stand for, f32 accumulation and softmax.
+ *  q: token i at q + i * q_token_stride elements, [n_head][head_dim] in q_dtype
+ *      (PKV_F32, PKV_F16 or PKV_BF16); 16-byte aligned, the stride at least n_head *
+ *      head_dim and a multiple of 16 bytes.  Elements beyond 2^100 in magnitude, or
+ *      not finite, make their row's results undefined.
+ *  out: [total_q][n_head * head_dim] in out_dtype (PKV_F32 or q_dtype), 16-byte aligned.
+ *  cu_q_lens: int32 [n_seqs + 1], or NULL for one row per sequence (total_q ==
+ *      n_seqs, max_q_len == 1); context_lens: int32 [n_seqs], the new tokens
+ *      among them (appended before).  Row i of sequence s is at position context_lens[s] -
+ *      q_len_s + i and has the keys up to it; a row without keys is zero.
+ *  block_tables: int32 [n_seqs][max_blocks_per_seq].
+ *  max_q_len, max_context_len: host upper bounds, 1 .. 2^30.  A sequence with a
+ *      longer chunk or context, a context longer than its table, a negative
+ *      length, or rows outside [0, total_q) is left out: its rows are as they
+ *      were, as are rows of no sequence, and pkv_pool_check() reports it.  Keys of
+ *      block ids outside the pool are not attended, and reported.
+ *  n_head / n_kv_head: any integer.  scale finite.
+ * Workspace: 16-byte aligned, of at least pkv_q4_workspace_bytes (0: none needed). */
+size_t pkv_q4_workspace_bytes(const pkv_pool* pool, int n_seqs, int total_q, int max_q_len,
+                              int max_context_len, int n_head);
+int pkv_q4_attention(pkv_pool* pool, int layer, const void* q, int q_dtype,
+                     long long q_token_stride, void* out, int out_dtype,
+                     const int32_t* cu_q_lens, const int32_t* context_lens,
+                     const int32_t* block_tables, int max_blocks_per_seq, int n_seqs,
+                     int total_q, int max_q_len, int max_context_len, int n_head, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention of whole prompts over their own rows, packed: token i of prompt s
+ * is row cu_lens[s] + i and attends tokens 0 .. i of its prompt; out_h = sum_j
+ * softmax_j(scale q_h . k_j) v_j, f32 accumulation and softmax (for 16-bit types the
+ * weights are rounded to them before the second product).
+ *  q: token t at q + t * q_token_stride elements, [n_head][head_dim]; k, v likewise,
+ *      [n_kv_head][head_dim]; all in dtype (PKV_F32, PKV_F16 or PKV_BF16), 16-byte
+ *      aligned, strides multiples of 16 bytes that hold a row.  Query head h reads kv head
+ *      h / (n_head / n_kv_head).  head_dim 64, 128 or 256.
+ *  out: [total][n_head * head_dim] in out_dtype (PKV_F32 or dtype), 16-byte aligned; may not
+ *      overlap q, k or v.
+ *  cu_lens: int32 [n_seqs + 1], nondecreasing, within 0 .. total; a prompt that
+ *      breaks this is left out.  Rows of no prompt are left as they were.
+ *  max_len: host bound of the prompt lengths, 1 .. 2^30; longer prompts are computed too,
+ *      with fewer workgroups than they could use.  scale finite.
+ * Runs on the calling thread's current device. */
+int pkv_prompt_attention(const void* q, const void* k, const void* v, int dtype,
+                         long long q_token_stride, long long k_token_stride,
+                         long long v_token_stride, void* out, int out_dtype,
+                         const int32_t* cu_lens, int n_seqs, int total, int max_len, int n_head,
+                         int n_kv_head, int head_dim, float scale, void* stream);
+
+/* Logits before a token is chosen: with n = how often token t is among the generated
+ * tokens of request b, in f32, each operation rounded, and once to dtype at the end:
+ *   x = logits[b][t]
+ *   t among the request's tokens:  x = x > 0 ? x / r : x * r    r = repetition[b]
+ *   n > 0:                         x = x - frequency[b] * n; x = x - presence[b]
+ *   t among its biased tokens:     x = x + its bias (the last entry of t counts)
+ *   t without its mask bit:        x = -inf
+ *  logits: [batch] rows of `vocab` values at row_stride elements, PKV_F32, PKV_F16 or
+ *      PKV_BF16; out: the same type at out_row_stride; may be logits itself (with the
+ *      same stride), may not overlap it otherwise.
+ *  tokens: int32 [total_tokens], request b's at cu_tokens[b] .. cu_tokens[b + 1] - 1, the
+ *      first prompt_lens[b] of them (NULL: none) its prompt; NULL (with cu_tokens): none.
+ *  repetition, presence, frequency: f32 [batch] or NULL (1, 0, 0).  r not positive or
+ *      not finite counts as 1.
+ *  bias_tokens, bias_values: int32, f32 [total_bias], request b's at cu_bias[b] ..
+ *      cu_bias[b + 1] - 1; all three NULL: none.
+ *  mask: uint32 [n_masks][mask_row_words], bit t % 32 of word t / 32 set where t may be
+ *      chosen; NULL: none.  mask_rows: int32 [batch], the row of a request, negative: no
+ *      mask, n_masks or more: nothing may be chosen; NULL: row b.
+ * Token ids outside [0, vocab) are passed over; offsets are limited to the arrays (at
+ * most 2^30 entries) and a request whose offsets decrease has no entries.  vocab
+ * 1 .. 2^24 - 1.
+ * Runs on the calling thread's current device. */
+int pkv_adjust_logits(const void* logits, void* out, int dtype, long long row_stride,
+                      long long out_row_stride, int batch, int vocab, const int32_t* tokens,
+                      const int32_t* cu_tokens, int total_tokens, const int32_t* prompt_lens,
+                      const float* repetition, const float* presence, const float* frequency,
+                      const int32_t* bias_tokens, const float* bias_values,
+                      const int32_t* cu_bias, int total_bias, const uint32_t* mask, int n_masks,
+                      int mask_row_words, const int32_t* mask_rows, void* stream);
 
 /* Kernel timing (instrumentation; no reference counterpart).  While enabled,
  * every pkv_decode_attention, pkv_prefill_attention, pkv_copy_blocks and
