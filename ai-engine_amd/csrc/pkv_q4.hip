@@ -103,14 +103,14 @@ __global__ void __launch_bounds__(kQ4Threads)
     *reinterpret_cast<uint32_t*>(o + L::k_word(at, i, g)) = w;
     if (i == 0) {
       *reinterpret_cast<_Float16*>(o + L::s_at(bs, at, g)) = s;
-      *reinterpret_cast<_Float16*>(o + L::km_at(bs, at, g)) = m;
+      *reinterpret_cast<_Float16*>(o + L::m_at(bs, at, g)) = m;
     }
     load8<DT>(v + ((size_t)tok * v_stride + (size_t)h * HD + lane * 8) * E, x);
     quantize8(x, c, m, s);
     o = vp + chunk;
     if (i == 0) {
       *reinterpret_cast<_Float16*>(o + L::s_at(bs, at, g)) = s;
-      *reinterpret_cast<_Float16*>(o + L::vm_at(bs, at, g)) = m;
+      *reinterpret_cast<_Float16*>(o + L::m_at(bs, at, g)) = m;
     }
     // channel 8 lane + e is (i, t) = (8 (lane % 2) + e, lane / 2)
 #pragma unroll
@@ -172,12 +172,12 @@ __global__ void __launch_bounds__(kQ4Threads)
     const char* o = kp + chunk;
     const uint32_t w = *reinterpret_cast<const uint32_t*>(o + L::k_word(at, i, g));
     float s = *reinterpret_cast<const _Float16*>(o + L::s_at(bs, at, g));
-    float m = *reinterpret_cast<const _Float16*>(o + L::km_at(bs, at, g));
+    float m = *reinterpret_cast<const _Float16*>(o + L::m_at(bs, at, g));
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)((w >> q4_k_bit(e)) & 15), m);
     o = vp + chunk;
     s = *reinterpret_cast<const _Float16*>(o + L::s_at(bs, at, g));
-    m = *reinterpret_cast<const _Float16*>(o + L::vm_at(bs, at, g));
+    m = *reinterpret_cast<const _Float16*>(o + L::m_at(bs, at, g));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint8_t b = o[L::v_bytes(bs, at, 8 * (lane & 1) + e) + t / 2];

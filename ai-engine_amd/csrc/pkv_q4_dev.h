@@ -22,10 +22,7 @@ struct Q4Layout {
   static __device__ __forceinline__ int s_at(int bs, int tok, int g) {
     return bs * (HD / 2) + (((tok >> 2) * G + g) * 4 + (tok & 3)) * 2;
   }
-  static __device__ __forceinline__ int km_at(int bs, int tok, int g) {
-    return bs * (HD / 2) + bs * G * 2 + (tok * G + g) * 2;
-  }
-  static __device__ __forceinline__ int vm_at(int bs, int tok, int g) {
+  static __device__ __forceinline__ int m_at(int bs, int tok, int g) {
     return s_at(bs, tok, g) + bs * G * 2;
   }
 };

@@ -723,11 +723,9 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
  * a chunk being bs * hd * 5 / 8 bytes:
  *   K  codes  [bs][4][G] 32-bit words: word (token, i, g) has channels 32 g + 8 i
  *             + e, e = 0 .. 7, in bits 4 (e / 2 + 4 (e % 2)) on
- *      s      [bs / 4][G][4] f16 (token / 4, group, token % 4)
- *      m      [bs][G] f16
  *   V  codes  [16][bs][T / 2] bytes: (i, token) has channels i + 16 t, t = 0 .. T - 1,
  *             in bits 4 t on
- *      s, m   [bs / 4][G][4] f16 each
+ *   both then s and m, each [bs / 4][G][4] f16 (token / 4, group, token % 4)
  * so that a token's bytes are its own: rows are written without reading others. */
 
 /* Stores rows of k and v (dtype PKV_F32, PKV_F16 or PKV_BF16) in 4 bits: token i, at k +

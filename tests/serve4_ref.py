@@ -36,6 +36,12 @@ def held(x):
     return stands_for(*quantize(x))
 
 
+def held_terms(x):
+    """|m| + s c of x's elements: the two terms that an element's value is the sum of."""
+    c, m, s = quantize(x)
+    return stands_for(c, np.abs(m), s)
+
+
 def chunk_bytes(k, c, m, s, bs):
     """Bytes of one block and kv head, from codes (bs, hd), m, s (bs, G); k: keys."""
     hd = c.shape[1]
@@ -59,14 +65,16 @@ def chunk_bytes(k, c, m, s, bs):
     def quads(x):
         return x.reshape(bs // 4, 4, g).transpose(0, 2, 1).astype(np.float16).reshape(-1).view(np.uint8)
 
-    last = m.astype(np.float16).reshape(-1).view(np.uint8) if k else quads(m)
-    return np.concatenate((words, quads(s), last))
+    return np.concatenate((words, quads(s), quads(m)))
 
 
-def attention(q, keys, values, n_rows, scale):
+def attention(q, keys, values, n_rows, scale, key_terms=None, value_terms=None):
     """Rows q (m, H, hd), the last m of n tokens with keys, values (n, kv, hd): (out,
     A, B): the result, sum_k p |v| and the largest sum_d |q| |k| of the row, from
-    which bounds of f32 arithmetic are made."""
+    which bounds of f32 arithmetic are made; key_terms, value_terms: in the place of
+    |k| and |v| where these are added up from terms that may cancel."""
+    key_terms = np.abs(keys) if key_terms is None else key_terms
+    value_terms = np.abs(values) if value_terms is None else value_terms
     m, h, hd = q.shape
     n, kv, _ = keys.shape
     out, a = np.zeros((m, h, hd)), np.zeros((m, h, hd))
@@ -80,8 +88,8 @@ def attention(q, keys, values, n_rows, scale):
             x = scale * (kk @ q[i, j])
             w = np.exp(x - x.max())
             w /= w.sum()
-            out[i, j], a[i, j] = w @ vv, w @ np.abs(vv)
-            b[i, j] = abs(scale) * (np.abs(kk) @ np.abs(q[i, j])).max()
+            out[i, j], a[i, j] = w @ vv, w @ value_terms[:seen, j * kv // h]
+            b[i, j] = abs(scale) * (key_terms[:seen, j * kv // h] @ np.abs(q[i, j])).max()
     return out, a, b
 
 

@@ -14,9 +14,9 @@ pytestmark = pytest.mark.gpu
 
 TD = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step
-# what a weight is rounded by before it meets a value: attention over 4 bits takes
-# f16 (f32 in two parts), prompt attention the type of its inputs
-Q4_WEIGHT = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -11}
+# what a weight is rounded by before it meets a value: attention over 4 bits takes two
+# f16, prompt attention the type of its inputs
+Q4_WEIGHT = dict.fromkeys(TD, 2.0 ** -21)
 PROMPT_WEIGHT = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 
 
@@ -174,7 +174,8 @@ def test_rows_past_32_bit_offsets(gpu):
     q, qx = typed(rng.normal(size=(1, 32, hd)), "bf16", gpu)
     o = pool.q4_attention(q, i32(blocks[None], gpu), i32([40], gpu))
     cache.check()
-    want, a, b = ref.attention(qx, ref.held(kx), ref.held(vx), 1, hd ** -0.5)
+    want, a, b = ref.attention(qx, ref.held(kx), ref.held(vx), 1, hd ** -0.5, ref.held_terms(kx),
+                               ref.held_terms(vx))
     tol = ref.tolerance(want, a, b, 40, hd, Q4_WEIGHT["bf16"], HALF["bf16"])
     assert np.all(np.abs(host(o).reshape(want.shape) - want) <= tol)
     cache.close()
@@ -202,7 +203,7 @@ class Case:
         k, v = keys_values(rng, nb * bs, kv, hd)
         k, self.k = typed(k * k_by, dt, gpu)
         v, self.v = typed(v * v_by, dt, gpu)
-        self.k, self.v = ref.held(self.k), ref.held(self.v)
+        self.take(self.k, self.v)
         self.cache = pagedkv.PagedKvCache(1, nb, bs, kv, hd, pagedkv.Q4)
         self.pool = self.cache.layer(0)
         self.pool.q4_append(k, v, torch.arange(nb * bs, dtype=torch.int32, device=gpu))
@@ -211,10 +212,15 @@ class Case:
         self.ctx, self.bs = list(ctx), bs
         self.q, self.qx = typed(rng.normal(size=(sum(self.q_lens), h, hd)) * q_by, dt, gpu)
 
+    def take(self, k, v):
+        """k, v have been stored in all slots."""
+        self.k, self.v = ref.held(k), ref.held(v)
+        self.terms = ref.held_terms(k), ref.held_terms(v)
+
     def rows(self, s):
         pos = np.arange(self.ctx[s])
         at = self.tables[s, pos // self.bs] * self.bs + pos % self.bs
-        return self.k[at], self.v[at]
+        return (self.k[at], self.v[at]), [t[at] for t in self.terms]
 
     def run(self, **kw):
         cu = None if self.cu is None else i32(self.cu, self.gpu)
@@ -229,8 +235,8 @@ class Case:
         got = host(out).reshape(-1, self.h, self.hd)
         for s, m in enumerate(self.q_lens):
             if s not in skip and m:
-                k, v = self.rows(s)
-                want, a, b = ref.attention(self.qx[at:at + m], k, v, m, self.scale)
+                kv, terms = self.rows(s)
+                want, a, b = ref.attention(self.qx[at:at + m], *kv, m, self.scale, *terms)
                 tol = ref.tolerance(want, a, b, self.ctx[s], self.hd, Q4_WEIGHT[self.dt],
                                     HALF[out_dt or self.dt])
                 err = np.abs(got[at:at + m] - want)
@@ -300,7 +306,7 @@ def test_attention_where_scales_of_values_jump(gpu):
         v, vx = typed(c.rng.normal(size=(n, 2, 128)) * by, "bf16", gpu)
         k, kx = typed(c.rng.normal(size=(n, 2, 128)), "bf16", gpu)
         c.pool.q4_append(k, v, slot)
-        c.k, c.v = ref.held(kx), ref.held(vx)
+        c.take(kx, vx)
         c.check(c.run())
 
 
@@ -320,9 +326,9 @@ def test_attention_leaves_rows_alone_and_reports(gpu):
     got = c.run()
     with pytest.raises(pagedkv.PagedKvError, match="block-id"):
         c.cache.check()
-    k, v = (np.concatenate((x[c.tables[0, 0] * 16:][:16], x[c.tables[0, 2] * 16:][:8]))
-            for x in (c.k, c.v))
-    want, a, b = ref.attention(c.qx[:1], k, v, 1, c.scale)
+    k, v, kt, vt = (np.concatenate((x[c.tables[0, 0] * 16:][:16], x[c.tables[0, 2] * 16:][:8]))
+                    for x in (c.k, c.v, *c.terms))
+    want, a, b = ref.attention(c.qx[:1], k, v, 1, c.scale, kt, vt)
     tol = ref.tolerance(want, a, b, 40, 64, Q4_WEIGHT["bf16"], HALF["bf16"])
     assert np.all(np.abs(host(got[:1]).reshape(want.shape) - want) <= tol)
     c.tables[1, :4] = -1
@@ -617,9 +623,9 @@ def test_a_step_of_them_together(gpu):
     prompt_check(o, np.array([0, 40, 70]), [host(t[n]) for n in ("pq", "pk", "pv")], "bf16", 0.125)
     pk, pv, dk, dv, dq = (host(t[n]) for n in ("pk", "pv", "dk", "dv", "dq"))
     for i, (lo, hi) in enumerate([(0, 40), (40, 70), (0, 0)]):
-        k = ref.held(np.concatenate((pk[lo:hi], dk[i:i + 1])))
-        v = ref.held(np.concatenate((pv[lo:hi], dv[i:i + 1])))
-        want, aa, b = ref.attention(dq[i:i + 1], k, v, 1, 0.125)
+        k, v = np.concatenate((pk[lo:hi], dk[i:i + 1])), np.concatenate((pv[lo:hi], dv[i:i + 1]))
+        want, aa, b = ref.attention(dq[i:i + 1], ref.held(k), ref.held(v), 1, 0.125,
+                                    ref.held_terms(k), ref.held_terms(v))
         tol = ref.tolerance(want, aa, b, len(k), 64, Q4_WEIGHT["bf16"], HALF["bf16"])
         assert np.all(np.abs(host(a[i:i + 1]).reshape(want.shape) - want) <= tol)
     y = (a.float() @ t["w"]).cpu().numpy()

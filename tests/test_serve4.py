@@ -54,7 +54,7 @@ def test_reference_chunk_layout_is_the_headers():
     assert (int(w[3, 1, 1]) >> 16) & 15 == c[3, 32 + 8 + 1]  # e = 1 is in the upper half
     assert (int(w[3, 1, 1]) >> 4) & 15 == c[3, 32 + 8 + 2]
     rest = b[bs * hd // 2:].view(np.float16)
-    assert rest[(7 // 4 * 2 + 1) * 4 + 7 % 4] == s[7, 1] and rest[bs * 2 + 7 * 2 + 1] == m[7, 1]
+    assert rest[(7 // 4 * 2 + 1) * 4 + 7 % 4] == s[7, 1] and rest[bs * 2 + (7 // 4 * 2 + 1) * 4 + 3] == m[7, 1]
     b = ref.chunk_bytes(False, c, m, s, bs)
     v = b[:bs * hd // 2].reshape(16, bs, 2)
     assert v[5, 9, 1] >> 4 == c[9, 5 + 16 * 3]
