@@ -58,13 +58,14 @@ COMMON = [
 
 # Per-source extras.  Prefill keeps its MFMA accumulators in ordinary VGPRs
 # (no AGPR round trips for the softmax rescale; measured faster on gfx950);
-# so do the mixed launch, which runs the same prefill body, and attention over 4
-# bits.
+# so do the mixed launch, which runs the same prefill body, attention over 4 bits and
+# of whole prompts.
 EXTRA = {
     "pkv_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "pkv_prefill_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "pkv_mixed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "pkv_q4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "pkv_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 
