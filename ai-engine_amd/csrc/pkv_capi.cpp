@@ -1528,10 +1528,9 @@ namespace {
 bool is_elem(int dt) { return dt == PKV_F32 || dt == PKV_F16 || dt == PKV_BF16; }
 
 // Rows of `row` elements of dt at a token stride that 16-byte loads can take.
-bool stride_ok(long long stride, long long row, int dt, long long n) {
+bool stride_ok(long long stride, long long row, int dt) {
   const long long e = (long long)pkv::dtype_bytes(dt);
-  return stride >= row && stride <= (1LL << 40) && (stride * e) % 16 == 0 &&
-         (n <= 1 || stride <= (LLONG_MAX / 16) / n);
+  return stride >= row && stride <= (1LL << 24) && (stride * e) % 16 == 0;
 }
 // Bytes from the first to past the last of n rows.
 size_t rows_bytes(long long stride, long long row, int dt, long long n) {
@@ -1559,8 +1558,8 @@ int pkv_q4_append(pkv_pool* p, int layer, const void* k, const void* v, int dtyp
   if (!aligned16(k) || !aligned16(v) || misaligned4({slot_mapping}))
     return fail(p, PKV_ERR_INVALID, "k and v must be 16-byte aligned, slot_mapping 4-byte");
   const long long row = (long long)p->n_kv_head * p->head_dim;
-  if (!stride_ok(k_token_stride, row, dtype, n_tokens) ||
-      !stride_ok(v_token_stride, row, dtype, n_tokens))
+  if (!stride_ok(k_token_stride, row, dtype) ||
+      !stride_ok(v_token_stride, row, dtype))
     return fail(p, PKV_ERR_INVALID,
                 "q4_append: token strides %lld and %lld: at least %lld elements, a multiple of 16 "
                 "bytes", k_token_stride, v_token_stride, row);
@@ -1643,7 +1642,7 @@ int pkv_q4_attention(pkv_pool* p, int layer, const void* q, int q_dtype,
     return fail(p, PKV_ERR_INVALID, "n_head %d is not a multiple of n_kv_head %d", n_head,
                 p->n_kv_head);
   const long long row = (long long)n_head * p->head_dim;
-  if (!stride_ok(q_token_stride, row, q_dtype, total_q))
+  if (!stride_ok(q_token_stride, row, q_dtype))
     return fail(p, PKV_ERR_INVALID,
                 "q4_attention: q_token_stride %lld: at least %lld elements, a multiple of 16 bytes",
                 q_token_stride, row);
@@ -1698,8 +1697,8 @@ int pkv_prompt_attention(const void* q, const void* k, const void* v, int dtype,
     return fail(nullptr, PKV_ERR_INVALID,
                 "prompt_attention: q, k, v and out must be 16-byte aligned, cu_lens 4-byte");
   const long long qr = (long long)n_head * head_dim, kr = (long long)n_kv_head * head_dim;
-  if (!stride_ok(q_token_stride, qr, dtype, total) || !stride_ok(k_token_stride, kr, dtype, total) ||
-      !stride_ok(v_token_stride, kr, dtype, total))
+  if (!stride_ok(q_token_stride, qr, dtype) || !stride_ok(k_token_stride, kr, dtype) ||
+      !stride_ok(v_token_stride, kr, dtype))
     return fail(nullptr, PKV_ERR_INVALID,
                 "prompt_attention: token strides %lld, %lld, %lld: at least %lld, %lld, %lld "
                 "elements, multiples of 16 bytes", q_token_stride, k_token_stride, v_token_stride,

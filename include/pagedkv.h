@@ -732,8 +732,8 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
  * i * k_token_stride elements (v likewise), [n_kv_head][head_dim], goes to slot
  * slot_mapping[i].  Slots as in pkv_append: negative ones are skipped, ones beyond
  * the pool reported by pkv_pool_check(); distinct (two tokens for one slot race).
- * Token strides: at least n_kv_head * head_dim, a multiple of 16 bytes.  k and v
- * 16-byte aligned. */
+ * Token strides: at least n_kv_head * head_dim, at most 2^24, a multiple of 16
+ * bytes.  k and v 16-byte aligned. */
 int pkv_q4_append(pkv_pool* pool, int layer, const void* k, const void* v, int dtype,
                   long long k_token_stride, long long v_token_stride,
                   const int32_t* slot_mapping, int n_tokens, void* stream);
@@ -748,7 +748,7 @@ int pkv_q4_gather(pkv_pool* pool, int layer, const int32_t* slot_mapping, int n,
  * values that the row's keys stand for, f32 accumulation and softmax.
  *  q: token i at q + i * q_token_stride elements, [n_head][head_dim] in q_dtype
  *      (PKV_F32, PKV_F16 or PKV_BF16); 16-byte aligned, the stride at least n_head *
- *      head_dim and a multiple of 16 bytes.  Elements beyond 2^100 in magnitude, or
+ *      head_dim, at most 2^24 and a multiple of 16 bytes.  Elements beyond 2^100 in magnitude, or
  *      not finite, make their row's results undefined.
  *  out: [total_q][n_head * head_dim] in out_dtype (PKV_F32 or q_dtype), 16-byte aligned.
  *  cu_q_lens: int32 [n_seqs + 1], or NULL for one row per sequence (total_q ==
@@ -778,7 +778,7 @@ int pkv_q4_attention(pkv_pool* pool, int layer, const void* q, int q_dtype,
  * weights are rounded to them before the second product).
  *  q: token t at q + t * q_token_stride elements, [n_head][head_dim]; k, v likewise,
  *      [n_kv_head][head_dim]; all in dtype (PKV_F32, PKV_F16 or PKV_BF16), 16-byte
- *      aligned, strides multiples of 16 bytes that hold a row.  Query head h reads kv head
+ *      aligned, strides multiples of 16 bytes that hold a row, at most 2^24.  Query head h reads kv head
  *      h / (n_head / n_kv_head).  head_dim 64, 128 or 256.
  *  out: [total][n_head * head_dim] in out_dtype (PKV_F32 or dtype), 16-byte aligned; may not
  *      overlap q, k or v.
