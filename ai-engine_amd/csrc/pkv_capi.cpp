@@ -1607,7 +1607,10 @@ size_t pkv_q4_workspace_bytes(const pkv_pool* p, int n_seqs, int total_q, int ma
   a.max_q_len = max_q_len;
   a.max_context_len = max_context_len;
   a.n_head = n_head;
-  return pkv::q4_workspace_bytes(p, a);
+  a.q_dtype = PKV_F32;
+  const size_t wide = pkv::q4_workspace_bytes(p, a);
+  a.q_dtype = PKV_F16;
+  return std::max(wide, pkv::q4_workspace_bytes(p, a));
 }
 
 int pkv_q4_attention(pkv_pool* p, int layer, const void* q, int q_dtype,

@@ -12,7 +12,9 @@ namespace {
 
 constexpr int kQ4Threads = 256;
 
-// Eight elements of type DT from `at`, NaN as 0 and limited to the f16 range.
+// Eight elements of type DT from `at`, NaN as 0 and limited so that what they are held
+// as stays in the f16 range (m + 15 s is above the largest by 2^-11 of 15 s at most).
+constexpr float kLimit = 65024.0f;
 template <int DT>
 __device__ __forceinline__ void load8(const char* at, float (&x)[8]) {
   if constexpr (DT == PKV_F32) {
@@ -28,7 +30,7 @@ __device__ __forceinline__ void load8(const char* at, float (&x)[8]) {
     widen16<DT>(ld16(at), x);
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+  for (int e = 0; e < 8; ++e) x[e] = x[e] != x[e] ? 0.0f : fminf(fmaxf(x[e], -kLimit), kLimit);
 }
 
 // Over the four lanes of a group.

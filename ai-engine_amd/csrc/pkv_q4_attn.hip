@@ -14,7 +14,8 @@
 // just the weights that they feed into the second product as its left operand.
 // Weights are two f16 (2^-22): one would be off by 2^-11 of p s c, and where offset and
 // code nearly cancel that is several times what rounding the result to f16 costs.
-// Two kernels share this: one for few columns (decoding), one for many (chunks).
+// One kernel is for few columns (decoding), one for more; chunks of 16-bit queries have
+// one that rounds the values a tile stands for to f16 first, for 128 columns at once.
 #include <algorithm>
 
 #include "pkv_internal.h"
@@ -38,12 +39,15 @@ struct Q4KArgs {
   int r;         // query heads of a kv head
   int bs_log2;
   int num_blocks;
+  int min_cols;    // a sequence with fewer columns of a kv head, or more than max_cols, is
+  int max_cols;    // another launch's
   int cols;        // columns of a workgroup
-  int tiles;       // workgroups that a sequence's and kv head's columns take
+  int tiles;       // workgroups that a sequence's and kv head's columns take at most
   int part_keys;   // keys of a part, a multiple of kWaves * kStep
   int max_parts;
-  float* o_part;   // [row * n_head + head][part][hd]
-  float2* ml_part; // [row * n_head + head][part] (reference, sum)
+  int seq_rows;    // rows of a sequence in the partial results; 0: they are at the row's place
+  float* o_part;   // [row][head][part][hd]
+  float2* ml_part; // [row][head][part] (reference, sum)
   uint32_t* err;
 };
 
@@ -71,6 +75,12 @@ struct Item {
   int all;              // keys that every column of the share has
 };
 
+// Place of the first part of row i (row q0 + i of all) of sequence s and a head.
+__device__ __forceinline__ size_t part_at(const Q4KArgs& ka, int s, int q0, int i, int head) {
+  const size_t row = ka.seq_rows ? (size_t)s * ka.seq_rows + i : (size_t)q0 + i;
+  return (row * ka.a.n_head + head) * ka.max_parts;
+}
+
 __device__ __forceinline__ int parts_of(const Q4KArgs& ka, int col0, int cols, int rows, int ctx,
                                         int& end) {
   const int last_row = (min(col0 + ka.cols, cols) - 1) / ka.r;
@@ -92,7 +102,7 @@ __device__ __forceinline__ bool item_of(const Q4KArgs& ka, Item& it) {
     return false;
   it.cols = it.rows * ka.r;
   it.col0 = tile * ka.cols;
-  if (it.col0 >= it.cols) return false;
+  if (it.col0 >= it.cols || it.cols < ka.min_cols || it.cols > ka.max_cols) return false;
   int end;
   it.parts = parts_of(ka, it.col0, it.cols, it.rows, it.ctx, end);
   if (it.part >= it.parts) return false;
@@ -522,11 +532,12 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
       y = fmaf(sm_o[w][c][e][j & 63], by, y);
     }
     const int row = col / ka.r;
-    const size_t at = (size_t)(it.q0 + row) * a.n_head + it.g * ka.r + (col - row * ka.r);
+    const int head = it.g * ka.r + (col - row * ka.r);
     if (it.parts == 1) {
-      put(a.out, a.out_dtype, at * HD + d, sum > 0.0f ? y / sum : 0.0f);
+      put(a.out, a.out_dtype, ((size_t)(it.q0 + row) * a.n_head + head) * HD + d,
+          sum > 0.0f ? y / sum : 0.0f);
     } else {
-      const size_t pa = at * ka.max_parts + it.part;
+      const size_t pa = part_at(ka, it.s, it.q0, row, head) + it.part;
       if (d == 0) ka.ml_part[pa] = float2{m, sum};
       ka.o_part[pa * HD + d] = y;
     }
@@ -858,17 +869,379 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
       const int col = it.col0 + c * 16 + 4 * kq + i;
       if (col >= it.cols) continue;
       const int row = col / ka.r;
-      const size_t at = (size_t)(it.q0 + row) * a.n_head + it.g * ka.r + (col - row * ka.r);
+      const int head = it.g * ka.r + (col - row * ka.r);
+      const size_t at = (size_t)(it.q0 + row) * a.n_head + head;
       if (it.parts == 1) {
         const float inv = sum[c][i] > 0.0f ? 1.0f / sum[c][i] : 0.0f;
 #pragma unroll
         for (int t = 0; t < T; ++t) put(a.out, a.out_dtype, at * HD + 16 * t + n16, o[c][t][i] * inv);
       } else {
-        const size_t pa = at * ka.max_parts + it.part;
+        const size_t pa = part_at(ka, it.s, it.q0, row, head) + it.part;
         if (n16 == 0) ka.ml_part[pa] = float2{best[c][i], sum[c][i]};
 #pragma unroll
         for (int t = 0; t < T; ++t) ka.o_part[pa * HD + 16 * t + n16] = o[c][t][i];
       }
+    }
+}
+
+// ---- chunks of 16-bit queries ---------------------------------------------------
+// Four waves of 32 columns share tiles of 32 keys: every thread turns some codes into
+// f16 in LDS, so that the work on them is done once for 128 columns, and the products are
+// those of 32x32x16 matrix instructions: S^T = K Q^T leaves a column's scores in a lane
+// and the one 32 further, in the order in which they enter O^T = V^T P^T.  Values are
+// rounded to f16 (2^-11 of each, at random), as weights are.  For f16 queries, whose
+// results show more of that: keys stay codes, a product per group is scaled in the lane
+// and the offsets' products are f32 ones, and weights are two f16.
+constexpr int kTile = 32;
+constexpr float kTau = 8.0f;  // weights are at most 2^8 of their reference
+
+template <int HD>
+struct CT {
+  static constexpr int G = HD / 32, T = HD / 16;
+  static constexpr int KP = HD * 2 + 16;            // pitch of a key's row
+  static constexpr int VP = kTile * 2 + 16;         // of a channel's values
+  static constexpr int K_ITEMS = 4 * G * 8;         // (i, group, quad of keys): a word of each key
+  static constexpr int VW = T >= 8 ? T / 8 : 1;     // items of a column and quad: eight channels
+  static constexpr int V_ITEMS = 16 * 8 * VW;
+  static constexpr int NI = (K_ITEMS + V_ITEMS + 255) / 256;
+  static constexpr int GS = G < 4 ? G : 4;          // groups of a V item's channels
+  static constexpr int SM = 8 * G * 8;              // bytes of a tile's scales
+  static constexpr int STAGE = kTile * KP + HD * VP + 2 * SM + 16;
+};
+
+// Codes 4 bits apart in 16-bit halves as f16 numbers: hi: they are in bits 4 .. 7.
+__device__ __forceinline__ f16x2 code_pair(uint32_t w, bool hi) {
+  const f16x2 x = __builtin_bit_cast(f16x2, (w & (hi ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+  const f16x2 a = {(_Float16)1024.0f, (_Float16)1024.0f}, b = {(_Float16)64.0f, (_Float16)64.0f};
+  const f16x2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
+  return hi ? x * by - b : x - a;
+}
+__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float half_max(float x) {  // over a lane and the one 32 away
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int DT, int HD>
+__global__ void __launch_bounds__(kWaves * 64)
+    __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : HD == 128 ? 2 : 1))) q4_chunk_kernel(Q4KArgs ka) {
+  using L = Q4Layout<HD>;
+  using C = CT<HD>;
+  constexpr int G = C::G, T = C::T, NS = HD / 16, ND = HD / 32;
+  constexpr bool EXACT = DT == PKV_F16;  // keys as codes, weights in two parts
+  constexpr int NP = EXACT ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) char lds[2 * C::STAGE];
+  const Q4Args& a = ka.a;
+  Item it;
+  if (!item_of(ka, it)) return;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, cl = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // ---- this wave's columns' queries ----
+  const int first = it.col0 + wave * 32;
+  const bool any = first < it.cols;
+  const int col = first + cl;
+  const bool live = col < it.cols;
+  const int qi = live ? col / ka.r : 0, head = it.g * ka.r + (live ? col - qi * ka.r : 0);
+  const int lim = live ? it.ctx - it.rows + qi + 1 : 0x7fffffff;
+  // keys that all the wave's columns have, that any has
+  const int all = min(it.ctx - it.rows + first / ka.r + 1, it.k1);
+  const int most = any ? min(it.ctx - it.rows + (min(first + 32, it.cols) - 1) / ka.r + 1, it.k1) : 0;
+  u32x4 qf[NS];
+  float qs[EXACT ? (G + 1) / 2 : 1];
+  float f;
+  {
+    const char* q = static_cast<const char*>(a.q) +
+                    ((size_t)(it.q0 + qi) * a.q_stride + (size_t)head * HD + 8 * half) * 2;
+    float x[NS][8], big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      widen16<DT>(ld16(q + 32 * i), x[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!live || a.scale == 0.0f) x[i][e] = 0.0f;
+        big = fmaxf(big, fabsf(x[i][e]));
+      }
+    }
+    big = half_max(big);
+    const int ex = big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;  // below 2^14
+    f = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, (EXACT ? 24 : 0) - ex), 0x1p-126f);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = ldexpf(a.scale < 0.0f ? -x[i][e] : x[i][e], ex);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float by = EXACT && (e & 2) ? 0.0625f : 1.0f;  // (these codes are 16 times larger)
+        qf[i][e / 2] = pack_half(x[i][e] * by, x[i][e + 1] * by);
+      }
+    }
+    if constexpr (EXACT) {  // sums of groups 2 j + half
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float t = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t += x[2 * g][e] + x[2 * g + 1][e];
+        t = swap32_sum(t) * 0x1p-24f;
+        if (half == g % 2) qs[g / 2] = t;
+      }
+    }
+  }
+
+  // ---- tiles: a thread's items ----
+  const int bs = 1 << ka.bs_log2;
+  const size_t blk_stride = (size_t)ka.kvh * L::chunk(bs);
+  const char* kh = ka.k + (size_t)it.g * L::chunk(bs);
+  const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
+  const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
+  constexpr int SG = C::GS * 2;
+  struct Raw {
+    uint32_t code[4], s[SG], m[SG];
+    bool in;
+  };
+  Raw raw[C::NI];
+  // item j of this thread: of K (i, group, quad) or V (word, i, quad), wave-uniformly
+  auto kind = [&](int j) { return (tid + 256 * j) < C::K_ITEMS ? 0 : (tid + 256 * j) < C::K_ITEMS + C::V_ITEMS ? 1 : 2; };
+  auto load = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int idx = tid + 256 * j;
+      Raw& r = raw[j];
+      const int k = __builtin_amdgcn_readfirstlane(kind(j));
+      if (k == 2) continue;
+      const int x = k == 0 ? idx : idx - C::K_ITEMS;
+      const int quad = k == 0 ? x / (4 * G) : x / (16 * C::VW);
+      const int key = k0 + 4 * quad;
+      int id = -1;
+      if (key < it.k1) {
+        id = table[key >> ka.bs_log2];
+        if ((unsigned)id >= (unsigned)ka.num_blocks) {
+          atomicOr(ka.err, PKV_EBIT_BLOCK);
+          id = -1;
+        }
+      }
+      r.in = id >= 0;
+      const int at = key & (bs - 1);
+      if (k == 0) {
+        const int i = x / G % 4, g = x % G;
+        const char* p = kh + (size_t)max(id, 0) * blk_stride;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          r.code[e] = *reinterpret_cast<const uint32_t*>(p + L::k_word(at + e, i, g));
+        load_words<8>(p + L::s_at(bs, at, g), *reinterpret_cast<uint32_t(*)[2]>(r.s));
+        load_words<8>(p + L::m_at(bs, at, g), *reinterpret_cast<uint32_t(*)[2]>(r.m));
+      } else {
+        const int i = x / C::VW % 16, w = x % C::VW;
+        const char* p = vh + (size_t)max(id, 0) * blk_stride;
+        const char* c = p + L::v_bytes(bs, at, i) + 4 * w;
+        if constexpr (T == 4) {
+          load_words<8>(c, *reinterpret_cast<uint32_t(*)[2]>(r.code));
+        } else if constexpr (T == 8) {
+          load_words<16>(c, r.code);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            r.code[e] = *reinterpret_cast<const uint32_t*>(c + e * (T / 2));
+        }
+        load_words<C::GS * 8>(p + L::s_at(bs, at, 4 * w), r.s);
+        load_words<C::GS * 8>(p + L::m_at(bs, at, 4 * w), r.m);
+      }
+    }
+  };
+  auto store = [&](int b) __attribute__((always_inline)) {
+    char* kl = lds + b * C::STAGE;
+    char* vl = kl + kTile * C::KP;
+    char* sl = vl + HD * C::VP;
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int idx = tid + 256 * j;
+      const Raw& r = raw[j];
+      const int k = __builtin_amdgcn_readfirstlane(kind(j));
+      if (k == 2) continue;
+      const int x = k == 0 ? idx : idx - C::K_ITEMS;
+      const int quad = k == 0 ? x / (4 * G) : x / (16 * C::VW);
+      if (k == 0) {
+        const int i = x / G % 4, g = x % G;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u32x4 y;
+          if constexpr (EXACT) {
+            uint32_t w[4];
+            k_pairs(r.code[e], w);
+            y = u32x4{w[0], w[1], w[2], w[3]};
+          } else {
+            const f16x2 s2 = __builtin_bit_cast(f16x2, r.s[e / 2]), m2 = __builtin_bit_cast(f16x2, r.m[e / 2]);
+            const f16x2 s = {s2[e % 2], s2[e % 2]}, m = {m2[e % 2], m2[e % 2]};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const f16x2 v = code_pair(c & 2 ? r.code[e] >> 8 : r.code[e], c & 1) * s + m;
+              y[c] = __builtin_bit_cast(uint32_t, v);
+            }
+          }
+          st16(kl + (4 * quad + e) * C::KP + (32 * g + 8 * i) * 2, y);
+        }
+        if constexpr (EXACT) {
+          if (i == 0) {
+            *reinterpret_cast<uint2*>(sl + (quad * G + g) * 8) = uint2{r.s[0], r.s[1]};
+            *reinterpret_cast<uint2*>(sl + C::SM + (quad * G + g) * 8) = uint2{r.m[0], r.m[1]};
+          }
+        }
+        // whether the tile's two blocks are in the pool
+        if (i == 0 && g == 0 && quad % 4 == 0)
+          *reinterpret_cast<int*>(sl + 2 * C::SM + quad) = r.in;
+      } else {
+        // channel i + 16 t: quad 4 s + 2 b + h at (s, h, b)
+        const int i = x / C::VW % 16, w = x % C::VW;
+        const int pos = (quad >> 2) * 32 + (quad & 1) * 16 + ((quad >> 1) & 1) * 8;
+        constexpr int TC = T < 8 ? T : 8;
+#pragma unroll
+        for (int t = 0; t < TC; ++t) {
+          uint32_t y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t pair;
+            if constexpr (T == 4) pair = r.code[e];
+            else pair = __builtin_amdgcn_perm(r.code[2 * e + 1], r.code[2 * e],
+                                              t & 4 ? 0x07060302u : 0x05040100u);
+            const f16x2 s = __builtin_bit_cast(f16x2, r.s[t / 2 * 2 + e]);
+            const f16x2 m = __builtin_bit_cast(f16x2, r.m[t / 2 * 2 + e]);
+            const f16x2 v = code_pair(t & 2 ? pair >> 8 : pair, t & 1) * s + m;
+            y[e] = __builtin_bit_cast(uint32_t, v);
+          }
+          *reinterpret_cast<uint2*>(vl + (i + 16 * (t + 8 * w)) * C::VP + pos) = uint2{y[0], y[1]};
+        }
+      }
+    }
+  };
+
+  f32x16 o[ND];
+  float ref = kNone, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+
+  load(it.k0);
+  store(0);
+  load(it.k0 + kTile);
+  __syncthreads();
+  int b = 0;
+  for (int k0 = it.k0; k0 < it.k1; k0 += kTile, b ^= 1) {
+    if (k0 < most) {
+      const char* kl = lds + b * C::STAGE;
+      const char* vl = kl + kTile * C::KP;
+      const char* sl = vl + HD * C::VP;
+      f32x16 x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+      if constexpr (EXACT) {
+        // offsets: key cl of group 2 j + half
+#pragma unroll
+        for (int j = 0; j < (G + 1) / 2; ++j) {
+          const float m = *reinterpret_cast<const _Float16*>(
+              sl + C::SM + ((cl >> 2) * G + 2 * j + half) * 8 + (cl & 3) * 2);
+          x = __builtin_amdgcn_mfma_f32_32x32x2f32(m, qs[j], x, 0, 0, 0);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          f32x16 d;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d[i] = 0.0f;
+#pragma unroll
+          for (int i = 2 * g; i < 2 * g + 2; ++i)
+            d = mfma32(ld16(kl + cl * C::KP + i * 32 + half * 16), qf[i], d);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            uint32_t w[2];
+            load_words<8>(sl + ((i / 2 + half) * G + g) * 8, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] = fmaf(half_of(w[e / 2], e % 2), d[i + e], x[i + e]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          x = mfma32(ld16(kl + cl * C::KP + i * 32 + half * 16), qf[i], x);
+      }
+      const int in0 = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(sl + 2 * C::SM));
+      const int in1 = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(sl + 2 * C::SM + 4));
+      if (k0 + kTile > all || !in0 || !in1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k0 + 8 * (i / 4) + 4 * half + i % 4 >= min(lim, it.k1) || !(i < 8 ? in0 : in1))
+            x[i] = -INFINITY;
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      mx *= f;
+      if (__builtin_amdgcn_ballot_w64(mx - ref > kTau)) {
+        mx = half_max(mx);
+        if (mx - ref > kTau) {
+          const float by = fast_exp2(ref - mx);
+          ref = mx;
+          l *= by;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= by;
+        }
+      }
+      u32x4 pf[NP][2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = fast_exp2(fmaf(x[i], f, -ref));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        l += x[2 * e];
+        l += x[2 * e + 1];
+        if constexpr (EXACT) {
+          uint32_t hi, lo;
+          split_half(x[2 * e], x[2 * e + 1], hi, lo);
+          pf[0][e / 4][e % 4] = hi;
+          pf[1][e / 4][e % 4] = lo;
+        } else {
+          pf[0][e / 4][e % 4] = pack_half(x[2 * e], x[2 * e + 1]);
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const u32x4 vf = ld16(vl + (32 * d + cl) * C::VP + 32 * ks + 16 * half);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) o[d] = mfma32(vf, pf[p][ks], o[d]);
+        }
+    }
+    store(b ^ 1);
+    load(k0 + 2 * kTile);
+    __syncthreads();
+  }
+
+  // lane: column cl, channels 32 d + 8 (i / 4) + 4 half + i % 4
+  l = swap32_sum(l);
+  if (!live) return;
+  const size_t at = (size_t)(it.q0 + qi) * a.n_head + head;
+  const size_t pa = part_at(ka, it.s, it.q0, qi, head) + it.part;
+  const float by = it.parts > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+  if (it.parts > 1 && half == 0) ka.ml_part[pa] = float2{ref, l};
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ch = 32 * d + 8 * i + 4 * half;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = o[d][4 * i + e] * by;
+      if (it.parts > 1)
+        *reinterpret_cast<f32x4*>(ka.o_part + pa * HD + ch) = f32x4{y[0], y[1], y[2], y[3]};
+      else if (a.out_dtype == PKV_F32)
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at * HD + ch) = f32x4{y[0], y[1], y[2], y[3]};
+      else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * HD + ch) =
+            uint2{cvt_pk16<DT>(y[0], y[1]), cvt_pk16<DT>(y[2], y[3])};
     }
 }
 
@@ -885,13 +1258,16 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4KArgs ka) {
   u /= a.max_q_len;
   if (u >= a.n_seqs) return;
   int q0, rows, ctx, end;
-  if (!sequence(ka, (int)u, false, q0, rows, ctx) || i >= rows) return;
+  if (!sequence(ka, (int)u, false, q0, rows, ctx) || i >= rows || rows * ka.r < ka.min_cols ||
+      rows * ka.r > ka.max_cols)
+    return;
   const int col = i * ka.r + h % ka.r;
   const int parts = parts_of(ka, col / ka.cols * ka.cols, rows * ka.r, rows, ctx, end);
   if (parts == 1) return;
   const size_t at = (size_t)(q0 + i) * a.n_head + h;
-  const float2* ml = ka.ml_part + at * ka.max_parts;
-  const float* o = ka.o_part + at * ka.max_parts * HD + lane * PER;
+  const size_t pa = part_at(ka, (int)u, q0, i, h);
+  const float2* ml = ka.ml_part + pa;
+  const float* o = ka.o_part + pa * HD + lane * PER;
   float m = kNone;
   for (int p = lane; p < parts; p += 64) m = fmaxf(m, ml[p].x);
   m = row_group_max(row_max16(m));
@@ -908,49 +1284,89 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4KArgs ka) {
   for (int j = 0; j < PER; ++j) put(a.out, a.out_dtype, at * HD + lane * PER + j, x[j] * inv);
 }
 
+// A call is one launch, or two: sequences of few columns a kv head, and chunks.
+enum Kind { kFew, kMany, kChunk };
+struct Launch {
+  Kind kind;
+  int nt, min_cols, max_cols, cols, tiles, part_keys, max_parts, seq_rows;
+  size_t part_rows;  // rows that partial results are kept of
+};
 struct Plan {
-  bool few;
-  int nt, cols, tiles, part_keys, max_parts;
+  Launch at[2];
+  int n;
 };
 
-Plan plan_of(const pkv_pool* p, const Q4Args& a) {
-  Plan pl;
-  const int c = 16 / (p->head_dim / 32);  // query columns of a tile for few
-  const long long cols = (long long)a.max_q_len * (a.n_head / p->n_kv_head);
-  pl.few = cols <= 2 * c;
-  pl.nt = pl.few ? (cols > c ? 2 : 1) : p->head_dim <= 128 && cols > 16 ? 2 : 1;
-  pl.cols = pl.nt * (pl.few ? c : 16);
-  pl.tiles = (int)std::min((cols + pl.cols - 1) / pl.cols, (long long)INT32_MAX);
-  const long long items = (long long)a.n_seqs * p->n_kv_head * pl.tiles;
+Launch launch_of(const pkv_pool* p, const Q4Args& a, Kind kind, int nt, int min_cols, int max_cols,
+                 int cols) {
+  Launch l{kind, nt, min_cols, max_cols, cols, 0, 0, 0, 0, (size_t)a.total_q};
+  if (max_cols < INT32_MAX && (size_t)a.n_seqs * (max_cols / (a.n_head / p->n_kv_head)) < l.part_rows) {
+    l.seq_rows = max_cols / (a.n_head / p->n_kv_head);
+    l.part_rows = (size_t)a.n_seqs * l.seq_rows;
+  }
+  const long long most = std::min((long long)a.max_q_len * (a.n_head / p->n_kv_head), (long long)max_cols);
+  l.tiles = (int)std::min((most + cols - 1) / cols, (long long)INT32_MAX);
+  const long long items = (long long)a.n_seqs * p->n_kv_head * l.tiles;
   // enough workgroups to fill the GPU several times over; a part is worth its join
-  // from 256 keys on
-  const long long want = std::max(1LL, 2048 / std::max(items, 1LL));
+  // from 256 keys on, and for 128 columns from 1024
+  const long long want = std::max(1LL, (kind == kChunk ? 768 : 2048) / std::max(items, 1LL));
   const int unit = kWaves * kStep;
   long long keys = (a.max_context_len + want - 1) / want;
-  keys = std::max(256LL, (keys + unit - 1) / unit * unit);
-  pl.part_keys = (int)keys;
-  pl.max_parts = (int)((a.max_context_len + keys - 1) / keys);
+  keys = std::max(kind == kChunk ? 1024LL : 256LL, (keys + unit - 1) / unit * unit);
+  l.part_keys = (int)keys;
+  l.max_parts = (int)((a.max_context_len + keys - 1) / keys);
+  return l;
+}
+
+Plan plan_of(const pkv_pool* p, const Q4Args& a) {
+  Plan pl{};
+  const int c = 16 / (p->head_dim / 32);  // query columns of a tile for few
+  const long long cols = (long long)a.max_q_len * (a.n_head / p->n_kv_head);
+  if (cols <= 2 * c) {
+    const int nt = cols > c ? 2 : 1;
+    pl.at[pl.n++] = launch_of(p, a, kFew, nt, 0, INT32_MAX, nt * c);
+  } else if (cols <= 32 || a.q_dtype == PKV_F32) {
+    const int nt = p->head_dim <= 128 && cols > 16 ? 2 : 1;
+    pl.at[pl.n++] = launch_of(p, a, kMany, nt, 0, INT32_MAX, nt * 16);
+  } else {
+    if (a.n_head / p->n_kv_head <= 2 * c) {  // (some sequences may have few)
+      const int nt = 2;
+      pl.at[pl.n++] = launch_of(p, a, kFew, nt, 0, 2 * c, nt * c);
+      pl.at[pl.n++] = launch_of(p, a, kChunk, 1, 2 * c + 1, INT32_MAX, 128);
+    } else {
+      pl.at[pl.n++] = launch_of(p, a, kChunk, 1, 0, INT32_MAX, 128);
+    }
+  }
   return pl;
 }
 
-size_t part_rows(const Q4Args& a, const Plan& pl) {
-  return (size_t)a.total_q * a.n_head * pl.max_parts;
+// (row, head, part) places of a call's partial results, which its launches use in turn.
+size_t part_places(const Q4Args& a, const Plan& pl) {
+  size_t n = 0;
+  for (int i = 0; i < pl.n; ++i)
+    if (pl.at[i].max_parts > 1)
+      n = std::max(n, pl.at[i].part_rows * a.n_head * pl.at[i].max_parts);
+  return n;
 }
 
 template <int DT, int HD>
-void attend(const Q4KArgs& ka, const Plan& pl, unsigned blocks, hipStream_t stream) {
+void attend(const Q4KArgs& ka, const Launch& l, unsigned blocks, hipStream_t stream) {
   constexpr int T = kWaves * 64;
-  if (pl.few && pl.nt == 1) q4_few_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
-  else if (pl.few) q4_few_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
-  else if (pl.nt == 1) q4_many_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
-  else if constexpr (HD <= 128) q4_many_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
+  if (l.kind == kFew) {
+    if (l.nt == 1) q4_few_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
+    else q4_few_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
+  } else if (l.kind == kMany) {
+    if (l.nt == 1) q4_many_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
+    else if constexpr (HD <= 128) q4_many_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
+  } else if constexpr (DT != PKV_F32) {
+    q4_chunk_kernel<DT, HD><<<blocks, T, 0, stream>>>(ka);
+  }
 }
 
 template <int DT>
-void attend_dt(const Q4KArgs& ka, int hd, const Plan& pl, unsigned blocks, hipStream_t stream) {
-  if (hd == 256) attend<DT, 256>(ka, pl, blocks, stream);
-  else if (hd == 128) attend<DT, 128>(ka, pl, blocks, stream);
-  else attend<DT, 64>(ka, pl, blocks, stream);
+void attend_dt(const Q4KArgs& ka, int hd, const Launch& l, unsigned blocks, hipStream_t stream) {
+  if (hd == 256) attend<DT, 256>(ka, l, blocks, stream);
+  else if (hd == 128) attend<DT, 128>(ka, l, blocks, stream);
+  else attend<DT, 64>(ka, l, blocks, stream);
 }
 
 long long join_blocks(const Q4Args& a) {
@@ -960,18 +1376,20 @@ long long join_blocks(const Q4Args& a) {
 }  // namespace
 
 size_t q4_workspace_bytes(const pkv_pool* p, const Q4Args& a) {
-  const Plan pl = plan_of(p, a);
-  return pl.max_parts == 1 ? 0 : part_rows(a, pl) * (p->head_dim + 2) * 4;
+  return part_places(a, plan_of(p, a)) * (p->head_dim + 2) * 4;
 }
 
 bool q4_fits(const pkv_pool* p, const Q4Args& a) {
-  const Plan pl = plan_of(p, a);
   if ((long long)a.max_q_len * a.n_head > INT32_MAX / 2) return false;
   const long long pairs = (long long)a.n_seqs * p->n_kv_head;
-  if (pairs > (1LL << 40) / pl.tiles) return false;
-  const long long items = pairs * pl.tiles;
-  return items <= (1LL << 40) / pl.max_parts && grid_fits(items * pl.max_parts, kWaves * 64) &&
-         (long long)a.n_seqs * a.max_q_len <= (1LL << 40) / a.n_head &&
+  const Plan pl = plan_of(p, a);
+  for (int i = 0; i < pl.n; ++i) {
+    const Launch& l = pl.at[i];
+    if (pairs > (1LL << 40) / l.tiles || pairs * l.tiles > (1LL << 40) / l.max_parts ||
+        !grid_fits(pairs * l.tiles * l.max_parts, kWaves * 64))
+      return false;
+  }
+  return (long long)a.n_seqs * a.max_q_len <= (1LL << 40) / a.n_head &&
          grid_fits(join_blocks(a), 256);
 }
 
@@ -986,26 +1404,33 @@ hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, ch
   ka.r = a.n_head / p->n_kv_head;
   while ((1 << ka.bs_log2) < p->block_size) ++ka.bs_log2;
   ka.num_blocks = p->num_blocks;
-  ka.cols = pl.cols;
-  ka.tiles = pl.tiles;
-  ka.part_keys = pl.part_keys;
-  ka.max_parts = pl.max_parts;
-  if (pl.max_parts > 1) {
-    ka.o_part = reinterpret_cast<float*>(ws);
-    ka.ml_part = reinterpret_cast<float2*>(ka.o_part + part_rows(a, pl) * p->head_dim);
-  }
   ka.err = p->err;
-  const unsigned blocks = (unsigned)((long long)a.n_seqs * p->n_kv_head * pl.tiles * pl.max_parts);
-  if (a.q_dtype == PKV_F32) attend_dt<PKV_F32>(ka, p->head_dim, pl, blocks, stream);
-  else if (a.q_dtype == PKV_F16) attend_dt<PKV_F16>(ka, p->head_dim, pl, blocks, stream);
-  else attend_dt<PKV_BF16>(ka, p->head_dim, pl, blocks, stream);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || pl.max_parts == 1) return e;
-  const unsigned jb = (unsigned)join_blocks(a);
-  if (p->head_dim == 64) q4_join_kernel<64><<<jb, 256, 0, stream>>>(ka);
-  else if (p->head_dim == 128) q4_join_kernel<128><<<jb, 256, 0, stream>>>(ka);
-  else q4_join_kernel<256><<<jb, 256, 0, stream>>>(ka);
-  return hipGetLastError();
+  ka.o_part = reinterpret_cast<float*>(ws);
+  ka.ml_part = reinterpret_cast<float2*>(ka.o_part + part_places(a, pl) * p->head_dim);
+  for (int i = 0; i < pl.n; ++i) {
+    const Launch& l = pl.at[i];
+    ka.min_cols = l.min_cols;
+    ka.max_cols = l.max_cols;
+    ka.cols = l.cols;
+    ka.tiles = l.tiles;
+    ka.part_keys = l.part_keys;
+    ka.max_parts = l.max_parts;
+    ka.seq_rows = l.seq_rows;
+    const unsigned blocks = (unsigned)((long long)a.n_seqs * p->n_kv_head * l.tiles * l.max_parts);
+    if (a.q_dtype == PKV_F32) attend_dt<PKV_F32>(ka, p->head_dim, l, blocks, stream);
+    else if (a.q_dtype == PKV_F16) attend_dt<PKV_F16>(ka, p->head_dim, l, blocks, stream);
+    else attend_dt<PKV_BF16>(ka, p->head_dim, l, blocks, stream);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (l.max_parts == 1) continue;
+    const unsigned jb = (unsigned)join_blocks(a);
+    if (p->head_dim == 64) q4_join_kernel<64><<<jb, 256, 0, stream>>>(ka);
+    else if (p->head_dim == 128) q4_join_kernel<128><<<jb, 256, 0, stream>>>(ka);
+    else q4_join_kernel<256><<<jb, 256, 0, stream>>>(ka);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace pkv

@@ -713,7 +713,7 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
  * pkv_compact, pkv_pool_check.  The others return PKV_ERR_UNSUPPORTED.
  *
  * What is held: 32 neighbouring channels of a token's row in one kv head are a
- * group.  With its elements x (NaN taken as 0, others limited to +-65504), m =
+ * group.  With its elements x (NaN taken as 0, others limited to +-65024), m =
  * f16(min x) and s = f16((max x - m) / 15), the subtraction and the division in f32,
  * an element is held as c = (x - m) / s in 64 bits, rounded to nearest even and
  * limited to 0 .. 15 (0 where s is 0), and stands for m + s c.

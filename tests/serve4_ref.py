@@ -4,7 +4,7 @@ written from their definitions.  Only the tests use them."""
 import numpy as np
 
 GROUP = 32
-F16_MAX = 65504.0
+LIMIT = 65024.0  # m + 15 s stays in the f16 range
 
 
 def f16(x):
@@ -16,7 +16,7 @@ def f16(x):
 def quantize(x):
     """(codes, m, s) of rows x (..., hd): codes as x, m and s (..., hd / 32)."""
     x = np.asarray(x, np.float64)
-    x = np.clip(np.where(np.isnan(x), 0.0, x), -F16_MAX, F16_MAX)
+    x = np.clip(np.where(np.isnan(x), 0.0, x), -LIMIT, LIMIT)
     y = x.reshape(*x.shape[:-1], -1, GROUP)
     m = f16(y.min(-1))
     top = y.max(-1).astype(np.float32)
@@ -70,15 +70,16 @@ def chunk_bytes(k, c, m, s, bs):
 
 def attention(q, keys, values, n_rows, scale, key_terms=None, value_terms=None):
     """Rows q (m, H, hd), the last m of n tokens with keys, values (n, kv, hd): (out,
-    A, B): the result, sum_k p |v| and the largest sum_d |q| |k| of the row, from
-    which bounds of f32 arithmetic are made; key_terms, value_terms: in the place of
-    |k| and |v| where these are added up from terms that may cancel."""
+    A, B, C): the result, sum_k p |v|, the largest sum_d |q| |k| of the row and the
+    root of the largest sum_d (q k)^2, from which bounds are made; key_terms,
+    value_terms: in the place of |k| and |v| in A and B where these are added up from
+    terms that may cancel."""
     key_terms = np.abs(keys) if key_terms is None else key_terms
     value_terms = np.abs(values) if value_terms is None else value_terms
     m, h, hd = q.shape
     n, kv, _ = keys.shape
     out, a = np.zeros((m, h, hd)), np.zeros((m, h, hd))
-    b = np.zeros((m, h))
+    b, c = np.zeros((2, m, h))
     for i in range(m):
         seen = n - m + i + 1
         if seen <= 0:
@@ -90,20 +91,25 @@ def attention(q, keys, values, n_rows, scale, key_terms=None, value_terms=None):
             w /= w.sum()
             out[i, j], a[i, j] = w @ vv, w @ value_terms[:seen, j * kv // h]
             b[i, j] = abs(scale) * (key_terms[:seen, j * kv // h] @ np.abs(q[i, j])).max()
-    return out, a, b
+            c[i, j] = abs(scale) * np.sqrt((kk ** 2 @ q[i, j] ** 2).max())
+    return out, a, b, c
 
 
-def tolerance(out, a, b, n, hd, weight_step, out_step):
+def tolerance(out, a, b, c, n, hd, weight_step, out_step, key_step=0.0, value_step=0.0):
     """Largest error of attention whose scores and sums are held in f32.
 
     A score is off by at most (hd + 16) 2^-23 of sum |q| |k| (a product and a sum
     each rounded, the sums in any order and perhaps truncated), and its exponent's
     argument and the exponential by 2^-20 more; two of them enter a weight (its
-    own and the denominator's).  A weight rounded before its product is off by
-    weight_step, sums over n keys by n 2^-23; the result is rounded once, by
-    out_step (half a step of its type)."""
+    own and the denominator's).  Keys that are rounded first, by key_step (half a step)
+    each and independently, move a score by key_step / sqrt(3) of the root of sum
+    (q k)^2 as a standard deviation, of which six are allowed (exceeded once in 5e8).
+    A weight rounded before its product is off by weight_step, a value by value_step, sums
+    over n keys by n 2^-23; the result is rounded once, by out_step (half a step
+    of its type)."""
     ds = (hd + 16) * 2.0 ** -23 * b[..., None] + 2.0 ** -20
-    rel = np.expm1(2 * ds) + weight_step + (n + 64) * 2.0 ** -23
+    ds = ds + 6 * key_step / np.sqrt(3.0) * c[..., None]
+    rel = np.expm1(2 * ds) + weight_step + value_step + (n + 64) * 2.0 ** -23
     return a * rel * (1 + out_step) + np.abs(out) * out_step + 2.0 ** -24
 
 
