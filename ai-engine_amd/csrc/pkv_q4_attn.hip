@@ -906,12 +906,17 @@ struct CT {
   static constexpr int NI = (K_ITEMS + V_ITEMS + 255) / 256;
   static constexpr int GS = G < 4 ? G : 4;          // groups of a V item's channels
   static constexpr int SM = 8 * G * 8;              // bytes of a tile's scales
-  static constexpr int STAGE = kTile * KP + HD * VP + 2 * SM + 16;
+  static constexpr int STAGE = kTile * KP + HD * VP + 2 * SM;
 };
 
-// Codes 4 bits apart in 16-bit halves as f16 numbers: hi: they are in bits 4 .. 7.
-__device__ __forceinline__ f16x2 code_pair(uint32_t w, bool hi) {
-  const f16x2 x = __builtin_bit_cast(f16x2, (w & (hi ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u);
+// Codes 4 bits apart in 16-bit halves as f16 numbers; hi: they are in bits 4 .. 7.  (w &
+// mask) | 1024.0 is 1024 + c or 1024 + 16 c; the constants are kept in registers so
+// that this is one instruction.
+struct CodeMasks {
+  uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;
+};
+__device__ __forceinline__ f16x2 code_pair(const CodeMasks& k, uint32_t w, bool hi) {
+  const f16x2 x = __builtin_bit_cast(f16x2, (w & (hi ? k.hi : k.lo)) | k.one);
   const f16x2 a = {(_Float16)1024.0f, (_Float16)1024.0f}, b = {(_Float16)64.0f, (_Float16)64.0f};
   const f16x2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
   return hi ? x * by - b : x - a;
@@ -927,7 +932,7 @@ __device__ __forceinline__ float half_max(float x) {  // over a lane and the one
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(kWaves * 64)
-    __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : HD == 128 ? 2 : 1))) q4_chunk_kernel(Q4KArgs ka) {
+    __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : HD == 128 ? (DT == PKV_BF16 ? 3 : 2) : 1))) q4_chunk_kernel(Q4KArgs ka) {
   using L = Q4Layout<HD>;
   using C = CT<HD>;
   constexpr int G = C::G, T = C::T, NS = HD / 16, ND = HD / 32;
@@ -997,59 +1002,80 @@ __global__ void __launch_bounds__(kWaves * 64)
   const char* kh = ka.k + (size_t)it.g * L::chunk(bs);
   const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
   const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
-  constexpr int SG = C::GS * 2;
-  struct Raw {
-    uint32_t code[4], s[SG], m[SG];
-    bool in;
-  };
-  Raw raw[C::NI];
-  // item j of this thread: of K (i, group, quad) or V (word, i, quad), wave-uniformly
-  auto kind = [&](int j) { return (tid + 256 * j) < C::K_ITEMS ? 0 : (tid + 256 * j) < C::K_ITEMS + C::V_ITEMS ? 1 : 2; };
-  auto load = [&](int k0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < C::NI; ++j) {
-      const int idx = tid + 256 * j;
-      Raw& r = raw[j];
-      const int k = __builtin_amdgcn_readfirstlane(kind(j));
-      if (k == 2) continue;
-      const int x = k == 0 ? idx : idx - C::K_ITEMS;
-      const int quad = k == 0 ? x / (4 * G) : x / (16 * C::VW);
-      const int key = k0 + 4 * quad;
-      int id = -1;
-      if (key < it.k1) {
-        id = table[key >> ka.bs_log2];
-        if ((unsigned)id >= (unsigned)ka.num_blocks) {
-          atomicOr(ka.err, PKV_EBIT_BLOCK);
-          id = -1;
-        }
-      }
-      r.in = id >= 0;
-      const int at = key & (bs - 1);
-      if (k == 0) {
-        const int i = x / G % 4, g = x % G;
-        const char* p = kh + (size_t)max(id, 0) * blk_stride;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          r.code[e] = *reinterpret_cast<const uint32_t*>(p + L::k_word(at + e, i, g));
-        load_words<8>(p + L::s_at(bs, at, g), *reinterpret_cast<uint32_t(*)[2]>(r.s));
-        load_words<8>(p + L::m_at(bs, at, g), *reinterpret_cast<uint32_t(*)[2]>(r.m));
-      } else {
-        const int i = x / C::VW % 16, w = x % C::VW;
-        const char* p = vh + (size_t)max(id, 0) * blk_stride;
-        const char* c = p + L::v_bytes(bs, at, i) + 4 * w;
-        if constexpr (T == 4) {
-          load_words<8>(c, *reinterpret_cast<uint32_t(*)[2]>(r.code));
-        } else if constexpr (T == 8) {
-          load_words<16>(c, r.code);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            r.code[e] = *reinterpret_cast<const uint32_t*>(c + e * (T / 2));
-        }
-        load_words<C::GS * 8>(p + L::s_at(bs, at, 4 * w), r.s);
-        load_words<C::GS * 8>(p + L::m_at(bs, at, 4 * w), r.m);
+  CodeMasks masks;
+  asm("" : "+v"(masks.lo), "+v"(masks.hi), "+v"(masks.one));
+
+  // block ids, 64 blocks' parts of 16 keys at a time: lane n has the n-th from `from` on
+  // (-1 outside the pool and from the last key on)
+  int from = it.k0, ids = 0;
+  auto fetch = [&]() {
+    const long long key = (long long)from + 16 * lane;
+    ids = -1;
+    if (key < it.k1) {
+      ids = table[key >> ka.bs_log2];
+      if ((unsigned)ids >= (unsigned)ka.num_blocks) {
+        atomicOr(ka.err, PKV_EBIT_BLOCK);
+        ids = -1;
       }
     }
+  };
+  fetch();
+
+  constexpr int SG = C::GS * 2;
+  uint32_t code[C::NI][4], sc[C::NI][SG], of[C::NI][SG];
+  // Item j of this thread, alike for a wave: 0 of K (i, group, quad), 1 of V (word, i,
+  // quad), 2 none.  The quads of a wave's items lie in one half of the tile but for
+  // keys of 64 channels.
+  auto kind = [&](int j) {
+    const int x = wave * 64 + 256 * j;
+    return x < C::K_ITEMS ? 0 : x < C::K_ITEMS + C::V_ITEMS ? 1 : 2;
+  };
+  auto k_quad = [&](int x) { return x / (4 * G); };
+  auto v_quad = [&](int x) { return x / (16 * C::VW); };
+  auto load = [&](int k0) __attribute__((always_inline)) {  // (steps of kTile from k0 = it.k0 on)
+    if (k0 - from >= 64 * 16) {
+      from = k0;
+      fetch();
+    }
+    const int n = (k0 - from) / 16;
+    const int id0 = max(readlane_i(ids, n), 0), id1 = max(readlane_i(ids, n + 1), 0);
+#pragma unroll
+    for (int j = 0; j < C::NI; ++j) {
+      const int idx = tid + 256 * j, k = kind(j);
+      if (k == 2) continue;
+      const int x = k == 0 ? idx : idx - C::K_ITEMS;
+      const int quad = k == 0 ? k_quad(x) : v_quad(x);
+      const int at = (k0 + 4 * quad) & (bs - 1);
+      const int id = (HD == 64 && k == 0 ? quad >> 2 : __builtin_amdgcn_readfirstlane(quad >> 2))
+                         ? id1 : id0;
+      const char* p = (k == 0 ? kh : vh) + (size_t)id * blk_stride;
+      if (k == 0) {
+        const int i = x / G % 4, g = x % G;
+        const char* c = p + (uint32_t)L::k_word(at, i, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) code[j][e] = *reinterpret_cast<const uint32_t*>(c + e * 16 * G);
+        const char* sm = p + (uint32_t)L::s_at(bs, at, g);
+        const uint2 y = *reinterpret_cast<const uint2*>(sm);
+        const uint2 z = *reinterpret_cast<const uint2*>(sm + bs * G * 2);
+        sc[j][0] = y.x, sc[j][1] = y.y, of[j][0] = z.x, of[j][1] = z.y;
+      } else {
+        const int i = x / C::VW % 16, w = x % C::VW;
+        const char* c = p + (uint32_t)(L::v_bytes(bs, at, i) + 4 * w);
+        if constexpr (T == 4) {
+          const uint2 y = *reinterpret_cast<const uint2*>(c);
+          code[j][0] = y.x, code[j][1] = y.y;
+        } else if constexpr (T == 8) {
+          load_words<16>(c, code[j]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) code[j][e] = *reinterpret_cast<const uint32_t*>(c + e * (T / 2));
+        }
+        const char* sm = p + (uint32_t)L::s_at(bs, at, 4 * w);
+        load_words<C::GS * 8>(sm, sc[j]);
+        load_words<C::GS * 8>(sm + bs * G * 2, of[j]);
+      }
+    }
+    return (readlane_i(ids, n) >= 0 ? 1 : 0) | (readlane_i(ids, n + 1) >= 0 ? 2 : 0);
   };
   auto store = [&](int b) __attribute__((always_inline)) {
     char* kl = lds + b * C::STAGE;
@@ -1057,27 +1083,25 @@ __global__ void __launch_bounds__(kWaves * 64)
     char* sl = vl + HD * C::VP;
 #pragma unroll
     for (int j = 0; j < C::NI; ++j) {
-      const int idx = tid + 256 * j;
-      const Raw& r = raw[j];
-      const int k = __builtin_amdgcn_readfirstlane(kind(j));
+      const int idx = tid + 256 * j, k = kind(j);
       if (k == 2) continue;
       const int x = k == 0 ? idx : idx - C::K_ITEMS;
-      const int quad = k == 0 ? x / (4 * G) : x / (16 * C::VW);
       if (k == 0) {
-        const int i = x / G % 4, g = x % G;
+        const int i = x / G % 4, g = x % G, quad = k_quad(x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           u32x4 y;
           if constexpr (EXACT) {
             uint32_t w[4];
-            k_pairs(r.code[e], w);
+            k_pairs(code[j][e], w);
             y = u32x4{w[0], w[1], w[2], w[3]};
           } else {
-            const f16x2 s2 = __builtin_bit_cast(f16x2, r.s[e / 2]), m2 = __builtin_bit_cast(f16x2, r.m[e / 2]);
+            const f16x2 s2 = __builtin_bit_cast(f16x2, sc[j][e / 2]);
+            const f16x2 m2 = __builtin_bit_cast(f16x2, of[j][e / 2]);
             const f16x2 s = {s2[e % 2], s2[e % 2]}, m = {m2[e % 2], m2[e % 2]};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const f16x2 v = code_pair(c & 2 ? r.code[e] >> 8 : r.code[e], c & 1) * s + m;
+              const f16x2 v = code_pair(masks, c & 2 ? code[j][e] >> 8 : code[j][e], c & 1) * s + m;
               y[c] = __builtin_bit_cast(uint32_t, v);
             }
           }
@@ -1085,16 +1109,13 @@ __global__ void __launch_bounds__(kWaves * 64)
         }
         if constexpr (EXACT) {
           if (i == 0) {
-            *reinterpret_cast<uint2*>(sl + (quad * G + g) * 8) = uint2{r.s[0], r.s[1]};
-            *reinterpret_cast<uint2*>(sl + C::SM + (quad * G + g) * 8) = uint2{r.m[0], r.m[1]};
+            *reinterpret_cast<uint2*>(sl + (quad * G + g) * 8) = uint2{sc[j][0], sc[j][1]};
+            *reinterpret_cast<uint2*>(sl + C::SM + (quad * G + g) * 8) = uint2{of[j][0], of[j][1]};
           }
         }
-        // whether the tile's two blocks are in the pool
-        if (i == 0 && g == 0 && quad % 4 == 0)
-          *reinterpret_cast<int*>(sl + 2 * C::SM + quad) = r.in;
       } else {
         // channel i + 16 t: quad 4 s + 2 b + h at (s, h, b)
-        const int i = x / C::VW % 16, w = x % C::VW;
+        const int i = x / C::VW % 16, w = x % C::VW, quad = v_quad(x);
         const int pos = (quad >> 2) * 32 + (quad & 1) * 16 + ((quad >> 1) & 1) * 8;
         constexpr int TC = T < 8 ? T : 8;
 #pragma unroll
@@ -1103,12 +1124,12 @@ __global__ void __launch_bounds__(kWaves * 64)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t pair;
-            if constexpr (T == 4) pair = r.code[e];
-            else pair = __builtin_amdgcn_perm(r.code[2 * e + 1], r.code[2 * e],
+            if constexpr (T == 4) pair = code[j][e];
+            else pair = __builtin_amdgcn_perm(code[j][2 * e + 1], code[j][2 * e],
                                               t & 4 ? 0x07060302u : 0x05040100u);
-            const f16x2 s = __builtin_bit_cast(f16x2, r.s[t / 2 * 2 + e]);
-            const f16x2 m = __builtin_bit_cast(f16x2, r.m[t / 2 * 2 + e]);
-            const f16x2 v = code_pair(t & 2 ? pair >> 8 : pair, t & 1) * s + m;
+            const f16x2 s = __builtin_bit_cast(f16x2, sc[j][t / 2 * 2 + e]);
+            const f16x2 m = __builtin_bit_cast(f16x2, of[j][t / 2 * 2 + e]);
+            const f16x2 v = code_pair(masks, t & 2 ? pair >> 8 : pair, t & 1) * s + m;
             y[e] = __builtin_bit_cast(uint32_t, v);
           }
           *reinterpret_cast<uint2*>(vl + (i + 16 * (t + 8 * w)) * C::VP + pos) = uint2{y[0], y[1]};
@@ -1124,9 +1145,9 @@ __global__ void __launch_bounds__(kWaves * 64)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
-  load(it.k0);
+  int in = load(it.k0);  // bit h: the block of the tile's half h is in the pool
   store(0);
-  load(it.k0 + kTile);
+  int in_next = load(it.k0 + kTile);
   __syncthreads();
   int b = 0;
   for (int k0 = it.k0; k0 < it.k1; k0 += kTile, b ^= 1) {
@@ -1166,12 +1187,10 @@ __global__ void __launch_bounds__(kWaves * 64)
         for (int i = 0; i < NS; ++i)
           x = mfma32(ld16(kl + cl * C::KP + i * 32 + half * 16), qf[i], x);
       }
-      const int in0 = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(sl + 2 * C::SM));
-      const int in1 = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(sl + 2 * C::SM + 4));
-      if (k0 + kTile > all || !in0 || !in1) {
+      if (k0 + kTile > all || in != 3) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (k0 + 8 * (i / 4) + 4 * half + i % 4 >= min(lim, it.k1) || !(i < 8 ? in0 : in1))
+          if (k0 + 8 * (i / 4) + 4 * half + i % 4 >= min(lim, it.k1) || !(in >> (i / 8) & 1))
             x[i] = -INFINITY;
       }
       float mx = x[0];
@@ -1195,15 +1214,18 @@ __global__ void __launch_bounds__(kWaves * 64)
       for (int i = 0; i < 16; ++i) x[i] = fast_exp2(fmaf(x[i], f, -ref));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        l += x[2 * e];
-        l += x[2 * e + 1];
         if constexpr (EXACT) {
           uint32_t hi, lo;
           split_half(x[2 * e], x[2 * e + 1], hi, lo);
           pf[0][e / 4][e % 4] = hi;
           pf[1][e / 4][e % 4] = lo;
-        } else {
-          pf[0][e / 4][e % 4] = pack_half(x[2 * e], x[2 * e + 1]);
+          l += x[2 * e];
+          l += x[2 * e + 1];
+        } else {  // the sum of what enters the product
+          const uint32_t w = pack_half(x[2 * e], x[2 * e + 1]);
+          const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+          pf[0][e / 4][e % 4] = w;
+          l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), one, l, false);
         }
       }
 #pragma unroll
@@ -1216,7 +1238,8 @@ __global__ void __launch_bounds__(kWaves * 64)
         }
     }
     store(b ^ 1);
-    load(k0 + 2 * kTile);
+    in = in_next;
+    in_next = load(k0 + 2 * kTile);
     __syncthreads();
   }
 
