@@ -45,6 +45,7 @@ struct Q4KArgs {
   int tiles;       // workgroups that a sequence's and kv head's columns take at most
   int part_keys;   // keys of a part, a multiple of kWaves * kStep
   int max_parts;
+  int join_rows;   // rows of a sequence that the join goes through
   int seq_rows;    // rows of a sequence in the partial results; 0: they are at the row's place
   float* o_part;   // [row][head][part][hd]
   float2* ml_part; // [row][head][part] (reference, sum)
@@ -112,19 +113,22 @@ __device__ __forceinline__ bool item_of(const Q4KArgs& ka, Item& it) {
   return true;
 }
 
-// N bytes (a multiple of 4) of consecutive words.
-template <int N>
+// N bytes (a multiple of 4) of consecutive words.  ONCE: nothing else of the launch reads
+// them, so the caches need not keep them.
+template <int N, bool ONCE = false>
 __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[N / 4]) {
   if constexpr (N == 4) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   } else if constexpr (N == 8) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    w[0] = x.x;
-    w[1] = x.y;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2* q = reinterpret_cast<const u32x2*>(p);
+    const u32x2 x = ONCE ? __builtin_nontemporal_load(q) : *q;
+    w[0] = x[0];
+    w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N / 16; ++i) {
-      const u32x4 x = ld16(p + 16 * i);
+      const u32x4 x = ONCE ? ld16_stream(p + 16 * i) : ld16(p + 16 * i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
     }
@@ -284,6 +288,38 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
     return x;
   };
 
+  // ---- the first step's keys and values, under way while the queries are taken ----
+  const int bs = 1 << ka.bs_log2;
+  const size_t blk_stride = (size_t)ka.kvh * L::chunk(bs);
+  const char* kh = ka.k + (size_t)it.g * L::chunk(bs);
+  const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
+  const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
+  const int s_off = bs * (HD / 2) + (kq * G + gp) * 8, m_off = s_off + bs * G * 2;
+  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (n16 * bs + kq * 4) * (T / 2);
+
+  struct KV {
+    uint32_t code[HD / 32], s[2], m[2];
+  };
+  auto load = [&](const char* base, int id, int key, bool keys, KV& t) {
+    const int at = key & (bs - 1);
+    const char* p = base + (size_t)max(id, 0) * blk_stride;
+    load_words<HD / 8, true>(p + at * (keys ? HD / 2 : T / 2) + (keys ? k_off : v_off), t.code);
+    load_words<8, true>(p + at * (G * 2) + s_off, t.s);
+    load_words<8, true>(p + at * (G * 2) + m_off, t.m);
+  };
+
+  constexpr int stride = kWaves * kStep;
+  int key = it.k0 + wave * kStep;
+  int ids = ids_of(ka, table, key, it.k1), left = 32;
+  int id[2] = {readlane_i(ids, 0), readlane_i(ids, 1)};
+  KV kt[2], vt[2];
+  if (key < it.k1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load(kh, id[j], key + 16 * j, true, kt[j]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load(vh, id[j], key + 16 * j, false, vt[j]);
+  }
+
   // ---- the columns' queries ----
   uint32_t qf[NT][NP][G][4];   // right operand: channels 32 g + 8 kq + e where g is gp
   float qs[NT], f[NT];         // sum of the group; a score is f times what the products give
@@ -325,25 +361,6 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   }
 
   // ---- the steps ----
-  const int bs = 1 << ka.bs_log2;
-  const size_t blk_stride = (size_t)ka.kvh * L::chunk(bs);
-  const char* kh = ka.k + (size_t)it.g * L::chunk(bs);
-  const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
-  const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
-  const int s_off = bs * (HD / 2) + (kq * G + gp) * 8, m_off = s_off + bs * G * 2;
-  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (n16 * bs + kq * 4) * (T / 2);
-
-  struct KV {
-    uint32_t code[HD / 32], s[2], m[2];
-  };
-  auto load = [&](const char* base, int id, int key, bool keys, KV& t) {
-    const int at = key & (bs - 1);
-    const char* p = base + (size_t)max(id, 0) * blk_stride;
-    load_words<HD / 8>(p + at * (keys ? HD / 2 : T / 2) + (keys ? k_off : v_off), t.code);
-    load_words<8>(p + at * (G * 2) + s_off, t.s);
-    load_words<8>(p + at * (G * 2) + m_off, t.m);
-  };
-
   f32x4 o[NT][T];   // row (c, g) = 4 kq + i: channel n16 + 16 t
   float ref[NT], l[NT], om[NT];
 #pragma unroll
@@ -354,18 +371,6 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
     for (int t = 0; t < T; ++t) o[c][t] = f32x4{0, 0, 0, 0};
   }
   float top = 14.0f;
-
-  constexpr int stride = kWaves * kStep;
-  int key = it.k0 + wave * kStep;
-  int ids = ids_of(ka, table, key, it.k1), left = 32;
-  int id[2] = {readlane_i(ids, 0), readlane_i(ids, 1)};
-  KV kt[2], vt[2];
-  if (key < it.k1) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) load(kh, id[j], key + 16 * j, true, kt[j]);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) load(vh, id[j], key + 16 * j, false, vt[j]);
-  }
   for (; key < it.k1; key += stride) {
     const bool masked = key + kStep > it.all || (id[0] | id[1]) < 0;
     const bool in[2] = {id[0] >= 0, id[1] >= 0};
@@ -1271,14 +1276,14 @@ __global__ void __launch_bounds__(kWaves * 64)
 // Joins the parts of a query row and head: one wave each.
 template <int HD>
 __global__ void __launch_bounds__(256) q4_join_kernel(Q4KArgs ka) {
-  constexpr int PER = HD / 64;
+  constexpr int PER = HD / 64, kAtOnce = 8;  // (kAtOnce divides 64)
   const Q4Args& a = ka.a;
   const int lane = threadIdx.x & 63;
   long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int h = (int)(u % a.n_head);
   u /= a.n_head;
-  const int i = (int)(u % a.max_q_len);
-  u /= a.max_q_len;
+  const int i = (int)(u % ka.join_rows);
+  u /= ka.join_rows;
   if (u >= a.n_seqs) return;
   int q0, rows, ctx, end;
   if (!sequence(ka, (int)u, false, q0, rows, ctx) || i >= rows || rows * ka.r < ka.min_cols ||
@@ -1295,13 +1300,28 @@ __global__ void __launch_bounds__(256) q4_join_kernel(Q4KArgs ka) {
   for (int p = lane; p < parts; p += 64) m = fmaxf(m, ml[p].x);
   m = row_group_max(row_max16(m));
   float l = 0.0f, x[PER] = {};
-  for (int p = 0; p < parts; ++p) {
-    const float2 t = ml[p];
-    const float by = fast_exp2(t.x - m);
-    l = fmaf(t.y, by, l);
+  for (int from = 0; from < parts; from += 64) {
+    float by = 0.0f;  // lane n: weight of part from + n
+    if (from + lane < parts) {
+      const float2 t = ml[from + lane];
+      by = fast_exp2(t.x - m);
+      l = fmaf(t.y, by, l);
+    }
+    for (int p = from; p < min(from + 64, parts); p += kAtOnce) {
+      float y[kAtOnce][PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = fmaf(o[(size_t)p * HD + j], by, x[j]);
+      for (int e = 0; e < kAtOnce; ++e)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) y[e][j] = o[(size_t)min(p + e, parts - 1) * HD + j];
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        const float w = lane_of(by, p - from + e);  // 0 behind the last part
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = fmaf(y[e][j], w, x[j]);
+      }
+    }
   }
+  l = swap32_sum(swap16_sum(row_sum16(l)));
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
   for (int j = 0; j < PER; ++j) put(a.out, a.out_dtype, at * HD + lane * PER + j, x[j] * inv);
@@ -1392,8 +1412,8 @@ void attend_dt(const Q4KArgs& ka, int hd, const Launch& l, unsigned blocks, hipS
   else attend<DT, 64>(ka, l, blocks, stream);
 }
 
-long long join_blocks(const Q4Args& a) {
-  return ((long long)a.n_seqs * a.max_q_len * a.n_head + 3) / 4;
+long long join_blocks(const Q4Args& a, int rows) {
+  return ((long long)a.n_seqs * rows * a.n_head + 3) / 4;
 }
 
 }  // namespace
@@ -1413,7 +1433,7 @@ bool q4_fits(const pkv_pool* p, const Q4Args& a) {
       return false;
   }
   return (long long)a.n_seqs * a.max_q_len <= (1LL << 40) / a.n_head &&
-         grid_fits(join_blocks(a), 256);
+         grid_fits(join_blocks(a, a.max_q_len), 256);
 }
 
 hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, char* ws,
@@ -1439,6 +1459,7 @@ hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, ch
     ka.part_keys = l.part_keys;
     ka.max_parts = l.max_parts;
     ka.seq_rows = l.seq_rows;
+    ka.join_rows = std::min(a.max_q_len, l.max_cols / ka.r);
     const unsigned blocks = (unsigned)((long long)a.n_seqs * p->n_kv_head * l.tiles * l.max_parts);
     if (a.q_dtype == PKV_F32) attend_dt<PKV_F32>(ka, p->head_dim, l, blocks, stream);
     else if (a.q_dtype == PKV_F16) attend_dt<PKV_F16>(ka, p->head_dim, l, blocks, stream);
@@ -1446,7 +1467,7 @@ hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, ch
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (l.max_parts == 1) continue;
-    const unsigned jb = (unsigned)join_blocks(a);
+    const unsigned jb = (unsigned)join_blocks(a, ka.join_rows);
     if (p->head_dim == 64) q4_join_kernel<64><<<jb, 256, 0, stream>>>(ka);
     else if (p->head_dim == 128) q4_join_kernel<128><<<jb, 256, 0, stream>>>(ka);
     else q4_join_kernel<256><<<jb, 256, 0, stream>>>(ka);
