@@ -47,9 +47,11 @@ __device__ __forceinline__ float quad_max(float x) {
   return fmaxf(x, quad<0x4E>(x));
 }
 
-// Codes of this lane's eight elements, and the group's m and s.
-__device__ __forceinline__ void quantize8(const float (&x)[8], int (&c)[8], _Float16& m,
-                                          _Float16& s) {
+// Codes of this lane's eight elements, nibble e of the result, and the group's m and s.
+// In f32, (x - m) times the reciprocal of s is within 2^-18 of the quotient below 16
+// (three roundings of 2^-24 and the reciprocal's 2^-23), so the codes are those of 64
+// bits unless it is as close to the middle between two of them; then 64 bits decide.
+__device__ __forceinline__ uint32_t quantize8(const float (&x)[8], _Float16& m, _Float16& s) {
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) {
@@ -60,76 +62,114 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], int (&c)[8], _Flo
   hi = quad_max(hi);
   m = (_Float16)lo;
   s = (_Float16)__fdiv_rn(__fsub_rn(hi, (float)m), 15.0f);
-  const double md = (double)m, sd = (double)s;
+  if (!(s > (_Float16)0.0f)) return 0;
+  const float mf = (float)m, inv = __builtin_amdgcn_rcpf((float)s);
+  uint32_t w = 0;
+  float near = 1.0f;  // least distance from a middle
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double y = s > (_Float16)0.0f ? rint(((double)x[e] - md) / sd) : 0.0;
-    c[e] = (int)fmin(fmax(y, 0.0), 15.0);
+    const float y = __builtin_amdgcn_fmed3f((x[e] - mf) * inv, 0.0f, 15.0f);
+    near = fminf(near, fabsf(__builtin_amdgcn_fractf(y) - 0.5f));
+    w |= (uint32_t)__builtin_rintf(y) << (4 * e);
   }
+  if (near < 0x1p-15f) {
+    const double md = (double)m, sd = (double)s;
+    w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      w |= (uint32_t)fmin(fmax(rint(((double)x[e] - md) / sd), 0.0), 15.0) << (4 * e);
+  }
+  return w;
 }
 
-// HD / 8 lanes a row (token, kv head): eight channels each, of K and of V.
+// Where a workgroup's tokens go: HD / 8 lanes a row, kRows<HD> tokens of one kv head,
+// because neighbouring tokens share the cache lines of a block's codes, scales and
+// offsets, and another workgroup's part of a line is written from another XCD.
+template <int HD>
+constexpr int kRows = kQ4Threads * 8 / HD;
+
+// The slot of a token, -1: none.
+__device__ __forceinline__ int slot_of(const int32_t* slots, long long tok, long long n,
+                                       long long n_slots, bool reporter, uint32_t* err) {
+  const int slot = tok < n ? slots[tok] : -1;
+  if (slot < n_slots) return slot;
+  if (reporter) atomicOr(err, PKV_EBIT_SLOT);
+  return -1;
+}
+
+// Words of a row of codes in LDS, padded so that 16 rows' 16-byte reads meet no bank twice.
+template <int HD>
+constexpr int kRowWords = HD / 8 + 4;
+
 template <int DT, int HD>
 __global__ void __launch_bounds__(kQ4Threads)
     q4_append_kernel(char* kp, char* vp, const char* k, const char* v, long long k_stride,
-                     long long v_stride, const int32_t* __restrict__ slots, long long rows,
-                     int kvh, int bs_log2, long long n_slots, uint32_t* err) {
+                     long long v_stride, const int32_t* __restrict__ slots, int n, int kvh,
+                     int bs_log2, long long n_slots, uint32_t* err) {
   using L = Q4Layout<HD>;
-  constexpr int LANES = HD / 8, E = DT == PKV_F32 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) uint8_t codes[kQ4Threads * 8];  // [row][i][t]
+  constexpr int LANES = HD / 8, E = DT == PKV_F32 ? 4 : 2, T = L::T;
+  // V codes [row][lane % 2][lane / 2]: channel 8 lane + e is (i, t) = (8 (lane % 2) + e, lane / 2)
+  __shared__ __attribute__((aligned(16))) uint32_t codes[kRows<HD>][kRowWords<HD>];
   const int bs = 1 << bs_log2;
+  const int h = blockIdx.x % kvh;
+  const long long tok0 = (long long)(blockIdx.x / kvh) * kRows<HD>;
   const int lane = threadIdx.x % LANES, local = threadIdx.x / LANES;
-  const long long r = (long long)blockIdx.x * (kQ4Threads / LANES) + local;
-  const long long tok = r / kvh;
-  const int h = (int)(r - tok * kvh);
-  int slot = r < rows ? slots[tok] : -1;
-  if (slot >= n_slots) {
-    if (lane == 0 && h == 0) atomicOr(err, PKV_EBIT_SLOT);
-    slot = -1;
-  }
-  const bool live = slot >= 0;
-  const int at = live ? slot & (bs - 1) : 0;
-  const size_t chunk = ((size_t)(live ? slot >> bs_log2 : 0) * kvh + h) * L::chunk(bs);
-  uint8_t* mine = codes + local * HD;
-  if (live) {
-    float x[8];
-    int c[8];
+  // a row of V codes is written by threads of their own order, tokens fastest
+  constexpr int W = T >= 8 ? T / 8 : 1;  // words of a column (HD 64: two columns' halves)
+  const int wl = threadIdx.x / W % kRows<HD>, col = threadIdx.x / (W * kRows<HD>);
+  const int slot = slot_of(slots, tok0 + local, n, n_slots, lane == 0 && h == 0, err);
+  const int wslot = slot_of(slots, tok0 + wl, n, n_slots, false, err);
+  if (slot >= 0) {
+    const long long tok = tok0 + local;
+    const size_t from = (size_t)h * HD + lane * 8;
+    float x[8], y[8];
+    load8<DT>(k + ((size_t)tok * k_stride + from) * E, x);
+    load8<DT>(v + ((size_t)tok * v_stride + from) * E, y);
     _Float16 m, s;
-    const int g = lane / 4, i = lane % 4;
-    load8<DT>(k + ((size_t)tok * k_stride + (size_t)h * HD + lane * 8) * E, x);
-    quantize8(x, c, m, s);
-    uint32_t w = 0;
+    const int g = lane / 4, i = lane % 4, at = slot & (bs - 1);
+    const size_t chunk = ((size_t)(slot >> bs_log2) * kvh + h) * L::chunk(bs);
+    uint32_t c = quantize8(x, m, s), w = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w |= (uint32_t)c[e] << q4_k_bit(e);
+    for (int e = 0; e < 8; ++e) w |= (c >> (4 * e) & 15) << q4_k_bit(e);
     char* o = kp + chunk;
     *reinterpret_cast<uint32_t*>(o + L::k_word(at, i, g)) = w;
     if (i == 0) {
       *reinterpret_cast<_Float16*>(o + L::s_at(bs, at, g)) = s;
       *reinterpret_cast<_Float16*>(o + L::m_at(bs, at, g)) = m;
     }
-    load8<DT>(v + ((size_t)tok * v_stride + (size_t)h * HD + lane * 8) * E, x);
-    quantize8(x, c, m, s);
+    codes[local][(lane & 1) * T + lane / 2] = quantize8(y, m, s);
     o = vp + chunk;
     if (i == 0) {
       *reinterpret_cast<_Float16*>(o + L::s_at(bs, at, g)) = s;
       *reinterpret_cast<_Float16*>(o + L::m_at(bs, at, g)) = m;
     }
-    // channel 8 lane + e is (i, t) = (8 (lane % 2) + e, lane / 2)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine[(8 * (lane & 1) + e) * L::T + lane / 2] = (uint8_t)c[e];
   }
   __syncthreads();
-  if (!live) return;
-  uint32_t w = 0;  // codes 8 lane .. of [i][t]
+  if (wslot < 0) return;
+  char* o = vp + ((size_t)(wslot >> bs_log2) * kvh + h) * L::chunk(bs);
+  const int at = wslot & (bs - 1);
+  if constexpr (HD == 64) {  // columns 2 col, 2 col + 1
+    const u32x4 x = *reinterpret_cast<const u32x4*>(&codes[wl][(col / 4) * T]);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= (uint32_t)mine[lane * 8 + e] << (4 * e);
-  char* o = vp + chunk;
-  if constexpr (HD == 64) {  // two columns of four
-    *reinterpret_cast<uint16_t*>(o + L::v_bytes(bs, at, 2 * lane)) = (uint16_t)w;
-    *reinterpret_cast<uint16_t*>(o + L::v_bytes(bs, at, 2 * lane + 1)) = (uint16_t)(w >> 16);
+    for (int j = 0; j < 2; ++j) {
+      const int i = 2 * col + j;
+      uint32_t w = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w |= (x[t] >> (4 * (i & 7)) & 15) << (4 * t);
+      *reinterpret_cast<uint16_t*>(o + L::v_bytes(bs, at, i)) = (uint16_t)w;
+    }
   } else {
-    constexpr int PER = L::T / 8;  // words of a column
-    *reinterpret_cast<uint32_t*>(o + L::v_bytes(bs, at, lane / PER) + 4 * (lane % PER)) = w;
+    const int word = threadIdx.x % W;
+    const uint32_t* c = &codes[wl][(col / 8) * T + 8 * word];
+    const u32x4 x0 = *reinterpret_cast<const u32x4*>(c);
+    const u32x4 x1 = *reinterpret_cast<const u32x4*>(c + 4);
+    uint32_t w = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      w |= (x0[t] >> (4 * (col & 7)) & 15) << (4 * t);
+      w |= (x1[t] >> (4 * (col & 7)) & 15) << (4 * t + 16);
+    }
+    *reinterpret_cast<uint32_t*>(o + L::v_bytes(bs, at, col) + 4 * word) = w;
   }
 }
 
@@ -152,41 +192,66 @@ __device__ __forceinline__ void store8(char* at, const float (&x)[8]) {
 template <int DT, int HD>
 __global__ void __launch_bounds__(kQ4Threads)
     q4_gather_kernel(const char* __restrict__ kp, const char* __restrict__ vp, char* __restrict__ ok,
-                     char* __restrict__ ov, const int32_t* __restrict__ slots, long long rows,
-                     int kvh, int bs_log2, long long n_slots, uint32_t* err) {
+                     char* __restrict__ ov, const int32_t* __restrict__ slots, int n, int kvh,
+                     int bs_log2, long long n_slots, uint32_t* err) {
   using L = Q4Layout<HD>;
-  constexpr int LANES = HD / 8, E = DT == PKV_F32 ? 4 : 2;
+  constexpr int LANES = HD / 8, E = DT == PKV_F32 ? 4 : 2, T = L::T;
+  constexpr int W = T >= 8 ? T / 8 : 1;
+  // V codes: words [row][word of a column][column] (HD 64: 16 bits a column)
+  __shared__ __attribute__((aligned(16))) uint32_t codes[kRows<HD>][kRowWords<HD>];
   const int bs = 1 << bs_log2;
-  const int lane = threadIdx.x % LANES;
-  const long long r = (long long)blockIdx.x * (kQ4Threads / LANES) + threadIdx.x / LANES;
-  if (r >= rows) return;
-  const long long tok = r / kvh;
-  const int h = (int)(r - tok * kvh);
-  int slot = slots[tok];
-  if (slot >= n_slots) {
-    if (lane == 0 && h == 0) atomicOr(err, PKV_EBIT_SLOT);
-    slot = -1;
+  const int h = blockIdx.x % kvh;
+  const long long tok0 = (long long)(blockIdx.x / kvh) * kRows<HD>;
+  const int lane = threadIdx.x % LANES, local = threadIdx.x / LANES;
+  const int wl = threadIdx.x / W % kRows<HD>, col = threadIdx.x / (W * kRows<HD>);
+  const int slot = slot_of(slots, tok0 + local, n, n_slots, lane == 0 && h == 0, err);
+  const int wslot = slot_of(slots, tok0 + wl, n, n_slots, false, err);
+  if (wslot >= 0) {
+    const char* o = vp + ((size_t)(wslot >> bs_log2) * kvh + h) * L::chunk(bs);
+    const int at = wslot & (bs - 1);
+    if constexpr (HD == 64) {
+      codes[wl][col] = *reinterpret_cast<const uint16_t*>(o + L::v_bytes(bs, at, 2 * col)) |
+                       *reinterpret_cast<const uint16_t*>(o + L::v_bytes(bs, at, 2 * col + 1)) << 16;
+    } else {
+      const int word = threadIdx.x % W;
+      codes[wl][16 * word + col] =
+          *reinterpret_cast<const uint32_t*>(o + L::v_bytes(bs, at, col) + 4 * word);
+    }
   }
-  float x[8] = {}, y[8] = {};
+  const int at = slot & (bs - 1), g = lane / 4, i = lane % 4, t = lane / 2;
+  float x[8] = {}, y[8] = {}, s = 0.0f, m = 0.0f;
   if (slot >= 0) {
-    const int at = slot & (bs - 1), g = lane / 4, i = lane % 4, t = lane / 2;
     const size_t chunk = ((size_t)(slot >> bs_log2) * kvh + h) * L::chunk(bs);
     const char* o = kp + chunk;
     const uint32_t w = *reinterpret_cast<const uint32_t*>(o + L::k_word(at, i, g));
-    float s = *reinterpret_cast<const _Float16*>(o + L::s_at(bs, at, g));
-    float m = *reinterpret_cast<const _Float16*>(o + L::m_at(bs, at, g));
+    s = *reinterpret_cast<const _Float16*>(o + L::s_at(bs, at, g));
+    m = *reinterpret_cast<const _Float16*>(o + L::m_at(bs, at, g));
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)((w >> q4_k_bit(e)) & 15), m);
     o = vp + chunk;
     s = *reinterpret_cast<const _Float16*>(o + L::s_at(bs, at, g));
     m = *reinterpret_cast<const _Float16*>(o + L::m_at(bs, at, g));
+  }
+  __syncthreads();
+  if (tok0 + local >= n) return;
+  if (slot >= 0) {
+    if constexpr (HD == 64) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(&codes[local][4 * (lane & 1)]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint8_t b = o[L::v_bytes(bs, at, 8 * (lane & 1) + e) + t / 2];
-      y[e] = fmaf(s, (float)((b >> (4 * (t & 1))) & 15), m);
+      for (int e = 0; e < 8; ++e)
+        y[e] = fmaf(s, (float)((w[e / 2] >> (16 * (e % 2) + 4 * t)) & 15), m);
+    } else {
+      const uint32_t* c = &codes[local][16 * (t / 8) + 8 * (lane & 1)];
+      const u32x4 w0 = *reinterpret_cast<const u32x4*>(c);
+      const u32x4 w1 = *reinterpret_cast<const u32x4*>(c + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = fmaf(s, (float)((w0[e] >> (4 * (t & 7))) & 15), m);
+        y[4 + e] = fmaf(s, (float)((w1[e] >> (4 * (t & 7))) & 15), m);
+      }
     }
   }
-  const size_t off = ((size_t)r * HD + lane * 8) * E;
+  const size_t off = (((size_t)(tok0 + local) * kvh + h) * HD + lane * 8) * E;
   store8<DT>(ok + off, x);
   store8<DT>(ov + off, y);
 }
@@ -198,8 +263,8 @@ int log2_of(int x) {
 }
 
 long long q4_blocks(const pkv_pool* p, int n) {
-  const long long per = kQ4Threads / (p->head_dim / 8);
-  return ((long long)n * p->n_kv_head + per - 1) / per;
+  const int per = kQ4Threads * 8 / p->head_dim;
+  return ((long long)n + per - 1) / per * p->n_kv_head;
 }
 
 template <int DT, int HD>
@@ -207,7 +272,7 @@ hipError_t append(const pkv_pool* p, int layer, const void* k, const void* v, lo
                   long long vs, const int32_t* slots, int n, hipStream_t stream) {
   q4_append_kernel<DT, HD><<<(unsigned)q4_blocks(p, n), kQ4Threads, 0, stream>>>(
       p->layer_k(layer), p->layer_v(layer), static_cast<const char*>(k),
-      static_cast<const char*>(v), ks, vs, slots, (long long)n * p->n_kv_head, p->n_kv_head,
+      static_cast<const char*>(v), ks, vs, slots, n, p->n_kv_head,
       log2_of(p->block_size), (long long)p->num_blocks * p->block_size, p->err);
   return hipGetLastError();
 }
@@ -217,7 +282,7 @@ hipError_t gather(const pkv_pool* p, int layer, const int32_t* slots, int n, voi
                   hipStream_t stream) {
   q4_gather_kernel<DT, HD><<<(unsigned)q4_blocks(p, n), kQ4Threads, 0, stream>>>(
       p->layer_k(layer), p->layer_v(layer), static_cast<char*>(ok), static_cast<char*>(ov), slots,
-      (long long)n * p->n_kv_head, p->n_kv_head, log2_of(p->block_size),
+      n, p->n_kv_head, log2_of(p->block_size),
       (long long)p->num_blocks * p->block_size, p->err);
   return hipGetLastError();
 }
