@@ -33,7 +33,6 @@ struct PT {
   static constexpr int VP = DT == PKV_F32 ? RB : RB + 32; // of V rows
   static constexpr int STAGE = KEYS * (KP + VP);
   static constexpr int CH = RB / 16;                      // 16-byte chunks of a row
-  static constexpr int NL = KEYS * CH / (kWaves * 64);    // chunks a thread loads, of K and of V
   static constexpr int WPE = RB >= 512 ? 1 : 3;           // waves per SIMD that registers are for
 };
 
@@ -65,14 +64,33 @@ __device__ __forceinline__ float pair_add(uint32_t w, float x) {
   }
 }
 
-template <int DT, int HD>
+// Four neighbouring channels of the output, times inv.
+template <int DT>
+__device__ __forceinline__ void put4(const PromptArgs& a, size_t e, const float (&x)[4], float inv) {
+  const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+  if (DT == PKV_F32 || a.out_dtype == PKV_F32)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + e) = f32x4{y[0], y[1], y[2], y[3]};
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + e) =
+        uint2{cvt_pk16<DT == PKV_BF16 ? PKV_BF16 : PKV_F16>(y[0], y[1]),
+              cvt_pk16<DT == PKV_BF16 ? PKV_BF16 : PKV_F16>(y[2], y[3])};
+}
+
+// SPLIT: the four waves have one unit, and every fourth tile of its keys each, with a
+// stage of LDS of their own; they join at the end.
+template <int DT, int HD, bool SPLIT>
 __global__ void __launch_bounds__(kWaves * 64)
-    __attribute__((amdgpu_waves_per_eu(PT<DT, HD>::WPE))) prompt_kernel(PromptArgs a, int max_groups) {
+    __attribute__((amdgpu_waves_per_eu(SPLIT ? 1 : PT<DT, HD>::WPE)))
+    prompt_kernel(PromptArgs a, int max_groups) {
   using C = PT<DT, HD>;
   constexpr int NS = HD / 16, ND = HD / 32;          // k-steps of Q K, 32-channel tiles of O
   constexpr int QR = DT == PKV_F32 ? HD / 8 : NS;    // 16-byte pieces of a lane's query
   constexpr bool F32 = DT == PKV_F32;
-  __shared__ __attribute__((aligned(16))) char lds[2 * C::STAGE];
+  constexpr int UNITS = SPLIT ? 1 : kWaves;          // of a workgroup
+  constexpr int LOADERS = SPLIT ? 64 : kWaves * 64;  // threads that a tile's loads are spread over
+  constexpr int NL = C::KEYS * C::CH / LOADERS;      // 16-byte pieces a thread loads, of K and of V
+  __shared__ __attribute__((aligned(16))) char lds[(SPLIT ? kWaves : 2) * C::STAGE];
+  __shared__ float sm_m[SPLIT ? kWaves : 1][kTok], sm_l[SPLIT ? kWaves : 1][kTok];
 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -83,7 +101,7 @@ __global__ void __launch_bounds__(kWaves * 64)
   const int lo = a.cu_lens[s], hi = a.cu_lens[s + 1];
   if (lo < 0 || hi > a.total || lo >= hi) return;
   const int len = hi - lo;
-  const int units = ((len - 1) / kTok + 1) * r, groups = (units + kWaves - 1) / kWaves;
+  const int units = ((len - 1) / kTok + 1) * r, groups = (units + UNITS - 1) / UNITS;
   const char* kp = static_cast<const char*>(a.k) + ((size_t)lo * a.k_stride + (size_t)g * HD) * C::E;
   const char* vp = static_cast<const char*>(a.v) + ((size_t)lo * a.v_stride + (size_t)g * HD) * C::E;
   const size_t kst = (size_t)a.k_stride * C::E, vst = (size_t)a.v_stride * C::E;
@@ -91,20 +109,20 @@ __global__ void __launch_bounds__(kWaves * 64)
   const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
 
   for (int grp = first; grp < groups; grp += max_groups) {
-    const int last_tile = (min(grp * kWaves + kWaves, units) - 1) / r;
+    const int last_tile = (min(grp * UNITS + UNITS, units) - 1) / r;
     const int n_keys = min(len, (last_tile + 1) * kTok);
     const int n_tiles = (n_keys + C::KEYS - 1) / C::KEYS;
 
     // ---- this wave's unit: tokens tb .. tb + 31 of a head; none if tb < 0 ----
-    const int un = grp * kWaves + wave;
+    const int un = grp * UNITS + (SPLIT ? 0 : wave);
     const int tb = un < units ? un / r * kTok : -1;
     const int head = g * r + (un < units ? un % r : 0);
 
     // A thread's pieces of a tile: rows row0 + RPT i of it, a 16-byte piece each.
-    constexpr int RPT = kWaves * 64 / C::CH;
-    const int row0 = tid / C::CH;
-    const uint32_t kb = 16 * (tid % C::CH);
-    u32x4 kr[C::NL], vr[C::NL];
+    constexpr int RPT = LOADERS / C::CH;
+    const int loader = SPLIT ? lane : tid, row0 = loader / C::CH;
+    const uint32_t kb = 16 * (loader % C::CH);
+    u32x4 kr[NL], vr[NL];
     // Buffer loads: rows behind the prompt, which may hold anything, come as 0.
     const uint32_t k_at = row0 * (uint32_t)kst + kb, v_at = row0 * (uint32_t)vst + kb;
     auto load = [&](int t) __attribute__((always_inline)) {
@@ -115,22 +133,22 @@ __global__ void __launch_bounds__(kWaves * 64)
       };
       const __amdgpu_buffer_rsrc_t ks = rows(kp, kst), vs = rows(vp, vst);
 #pragma unroll
-      for (int i = 0; i < C::NL; ++i) {
+      for (int i = 0; i < NL; ++i) {
         kr[i] = __builtin_amdgcn_raw_buffer_load_b128(ks, k_at, RPT * i * (uint32_t)kst, 0);
         vr[i] = __builtin_amdgcn_raw_buffer_load_b128(vs, v_at, RPT * i * (uint32_t)vst, 0);
       }
     };
     auto store = [&](int t) __attribute__((always_inline)) {
-      char* l = lds + (t & 1) * C::STAGE;
+      char* l = lds + (SPLIT ? wave : t & 1) * C::STAGE;
 #pragma unroll
-      for (int i = 0; i < C::NL; ++i) {
+      for (int i = 0; i < NL; ++i) {
         st16(l + (row0 + RPT * i) * C::KP + kb, kr[i]);
         st16(l + C::KEYS * C::KP + (row0 + RPT * i) * C::VP + kb, vr[i]);
       }
     };
 
     // ---- the queries: right operand ----
-    load(0);
+    load(SPLIT ? wave : 0);
     u32x4 qf[QR];
     {
       const int tok = min(max(tb, 0) + col, len - 1);
@@ -230,7 +248,59 @@ __global__ void __launch_bounds__(kWaves * 64)
       }
     };
 
-    __syncthreads();  // (the last group's tiles are read)
+    __syncthreads();  // (the last group's LDS is read)
+    if constexpr (SPLIT) {
+      for (int t = wave; t < n_tiles; t += kWaves) {
+        store(t);
+        load(t + kWaves);
+        // the wave's LDS operations are done in this order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const char* kl = lds + wave * C::STAGE;
+        step(kl, kl + C::KEYS * C::KP, t * C::KEYS == tb);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+      // ---- join ----
+      l = swap32_sum(l);
+      if (half == 0) {
+        sm_m[wave][col] = m;  // (the same in both halves)
+        sm_l[wave][col] = l;
+      }
+      __syncthreads();  // (tiles are read)
+      float* sums = reinterpret_cast<float*>(lds);  // [wave][d][i][lane]
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[((wave * ND + d) * 16 + i) * 64 + lane] = o[d][i];
+      __syncthreads();
+      float by[kWaves], top = -INFINITY;
+      l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sm_m[w][col]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        by[w] = w < n_tiles ? fast_exp2(sm_m[w][col] - top) : 0.0f;
+        l = fmaf(sm_l[w][col], by[w], l);
+      }
+      const int tok = tb + col;
+      if (tok >= len) continue;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {  // channels 32 d + 8 wave + 4 half ..
+        float y[4] = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          if (w < n_tiles)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              y[i] = fmaf(sums[((w * ND + d) * 16 + 4 * wave + i) * 64 + lane], by[w], y[i]);
+        put4<DT>(a, ((size_t)(lo + tok) * a.n_head + head) * HD + 32 * d + 8 * wave + 4 * half, y,
+                 1.0f / l);
+      }
+      continue;
+    }
     store(0);
     load(1);
     __syncthreads();
@@ -253,31 +323,39 @@ __global__ void __launch_bounds__(kWaves * 64)
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const size_t e = at + 32 * d + 8 * i;
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = o[d][4 * i + j] * inv;
-        if (F32 || a.out_dtype == PKV_F32) {
-          *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + e) = f32x4{y[0], y[1], y[2], y[3]};
-        } else {
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + e) =
-              uint2{cvt_pk16<DT>(y[0], y[1]), cvt_pk16<DT>(y[2], y[3])};
-        }
+        const float y[4] = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        put4<DT>(a, at + 32 * d + 8 * i, y, inv);
       }
   }
 }
 
+long long units_of(const PromptArgs& a) {
+  return (long long)((std::min(a.max_len, a.total) + kTok - 1) / kTok) * (a.n_head / a.n_kv_head);
+}
+// Whether the waves of a workgroup share a unit: with so few units that the longest
+// prompt's last ones take the time.  Not sharing and sharing took, us:
+//   f32    512 units 74, 38    1024  76, 72    1624  31, 22    3248 101, 102   6496 187, 233
+//   bf16   512 units 18, 14    1024  32, 26    2048  59, 72    2048 (short) 15, 19
+// (f32 with 256 channels has no room for it.)
+bool split_of(const PromptArgs& a) {
+  return !(a.dtype == PKV_F32 && a.head_dim == 256) &&
+         units_of(a) * a.n_seqs * a.n_kv_head <= (a.dtype == PKV_F32 ? 2048 : 1024);
+}
 long long max_groups_of(const PromptArgs& a) {
-  const long long units =
-      (long long)((std::min(a.max_len, a.total) + kTok - 1) / kTok) * (a.n_head / a.n_kv_head);
-  return (units + kWaves - 1) / kWaves;
+  return split_of(a) ? units_of(a) : (units_of(a) + kWaves - 1) / kWaves;
 }
 
 template <int DT, int HD>
 hipError_t run(const PromptArgs& a, hipStream_t stream) {
   const long long groups = max_groups_of(a);
-  prompt_kernel<DT, HD><<<(unsigned)(groups * a.n_seqs * a.n_kv_head), kWaves * 64, 0, stream>>>(
-      a, (int)groups);
+  const unsigned blocks = (unsigned)(groups * a.n_seqs * a.n_kv_head);
+  if constexpr (DT != PKV_F32 || HD != 256) {
+    if (split_of(a)) {
+      prompt_kernel<DT, HD, true><<<blocks, kWaves * 64, 0, stream>>>(a, (int)groups);
+      return hipGetLastError();
+    }
+  }
+  prompt_kernel<DT, HD, false><<<blocks, kWaves * 64, 0, stream>>>(a, (int)groups);
   return hipGetLastError();
 }
 

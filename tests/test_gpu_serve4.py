@@ -418,6 +418,15 @@ def test_longer_prompts(gpu, dt, h, kv, hd, lens):
     prompt_check(pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=1), cu, xs, dt, hd ** -0.5)
 
 
+@pytest.mark.parametrize("dt,hd", [("f32", 64), ("f32", 128), ("f32", 256), ("f16", 64), ("f16", 256),
+                                   ("bf16", 128), ("bf16", 256)])
+def test_many_prompts(gpu, dt, hd):
+    """More tiles and heads than fill the GPU twice: waves have a unit each."""
+    lens = [1, 97, 32, 33, 0, 64, 65, 5] + np.random.default_rng(hd).integers(1, 97, 40).tolist()
+    q, k, v, cu, xs = prompt_case(gpu, 25, dt, 14, 2, hd, lens, packed=True)
+    prompt_check(pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=97), cu, xs, dt, hd ** -0.5)
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("by,scale", [(20.0, 0.125), (1e-3, 0.125), (1.0, -0.3), (1.0, 0.0)])
 def test_prompts_of_large_and_small_values(gpu, dt, by, scale):
