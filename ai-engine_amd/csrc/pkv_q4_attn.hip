@@ -262,7 +262,7 @@ __device__ __forceinline__ float new_ref(float ref, float m, float top, bool les
 template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   using L = Q4Layout<HD>;
-  constexpr int G = L::G, T = L::T, NP = DT == PKV_F32 ? 2 : 1, E = DT == PKV_F32 ? 4 : 2;
+  constexpr int G = L::G, T = L::T, E = 2;
   constexpr int C = 16 / G;  // query columns of a tile
   __shared__ float sm_m[kWaves][NT * C], sm_l[kWaves][NT * C];
   __shared__ float sm_o[kWaves][NT][8][64];
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   }
 
   // ---- the columns' queries ----
-  uint32_t qf[NT][NP][G][4];   // right operand: channels 32 g + 8 kq + e where g is gp
+  uint32_t qf[NT][G][4];   // right operand: channels 32 g + 8 kq + e where g is gp
   float qs[NT], f[NT];         // sum of the group; a score is f times what the products give
   int lim[NT];                 // a column's keys
 #pragma unroll
@@ -350,13 +350,9 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const float by = (e & 2) ? 0.0625f : 1.0f;  // these codes are 16 times larger
-      uint32_t w[2];
-      if constexpr (NP == 2) split_half(x[e] * by, x[e + 1] * by, w[0], w[1]);
-      else w[0] = pack_half(x[e] * by, x[e + 1] * by);
+      const uint32_t w = pack_half(x[e] * by, x[e + 1] * by);
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int g = 0; g < G; ++g) qf[c][p][g][e / 2] = g == gp ? w[p] : 0u;
+      for (int g = 0; g < G; ++g) qf[c][g][e / 2] = g == gp ? w : 0u;
     }
   }
 
@@ -385,9 +381,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
         uint32_t kf[4];
         k_pairs(kt[j].code[g], kf);
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-          for (int p = 0; p < NP; ++p) d[c] = mfma16(kf, qf[c][p][g], d[c]);
+        for (int c = 0; c < NT; ++c) d[c] = mfma16(kf, qf[c][g], d[c]);
       }
 #pragma unroll
       for (int c = 0; c < NT; ++c)
@@ -551,12 +545,17 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 
 // ---- many columns ------------------------------------------------------------
 // Tiles of 16 query columns: a product per group, scaled and added up in the lane; the
-// offsets' products are one v_mfma_f32_16x16x4_f32 (its four k are groups).  DT: type of
-// q.  NT: tiles.
+// offsets' products are one v_mfma_f32_16x16x4_f32 (its four k are groups).  f32 queries
+// have all their calls here, with keys and values as f32 on f32 instructions, which
+// take eight times as long: in the f16 ones, products below 2^-24 of the largest of
+// eight lose bits, always downwards, which after offsets and codes have cancelled was
+// 2^-15 of a result over 2000 keys (now 2^-21; 64 sequences of 4096 keys, 8 kv heads of
+// 128 and 32 heads take 210 us, 75 in f16 parts).  DT: type of q.  NT: tiles.
 template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   using L = Q4Layout<HD>;
-  constexpr int G = L::G, T = L::T, NP = DT == PKV_F32 ? 2 : 1, E = DT == PKV_F32 ? 4 : 2;
+  constexpr int G = L::G, T = L::T, E = DT == PKV_F32 ? 4 : 2;
+  constexpr bool F32 = DT == PKV_F32;
   constexpr int GM = (G + 3) / 4;  // products of four groups' offsets
   __shared__ float sm_m[kWaves][NT * 16], sm_l[kWaves][NT * 16];
   __shared__ float sm_o[2][NT * 16 * HD];
@@ -567,7 +566,9 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, kq = lane >> 4, n16 = lane & 15;
 
-  uint32_t qf[NT][NP][G][4];   // right operand: column n16, channels 32 g + 8 kq + e
+  // right operand: column n16, channels 32 g + 8 kq + e
+  uint32_t qf[F32 ? 1 : NT][G][4];
+  float qx[F32 ? NT : 1][G][8];
   float qs[NT][GM];            // sum of group 4 b + kq
   float f[NT];
   int lim[NT];
@@ -590,8 +591,8 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
       }
     }
     big = row_group_max(big);
-    const int ex = big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
-    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - ex), 0x1p-126f);
+    const int ex = !F32 && big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
+    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, (F32 ? 0 : 24) - ex), 0x1p-126f);
 #pragma unroll
     for (int b = 0; b < GM; ++b) qs[c][b] = 0.0f;
 #pragma unroll
@@ -602,15 +603,14 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
         x[g][e] = ldexpf(a.scale < 0.0f ? -x[g][e] : x[g][e], ex);
         sum += x[g][e];
       }
-      sum = swap32_sum(swap16_sum(sum)) * 0x1p-24f;
+      sum = swap32_sum(swap16_sum(sum)) * (F32 ? 1.0f : 0x1p-24f);
       if (kq == g % 4) qs[c][g / 4] = sum;
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float by = (e & 2) ? 0.0625f : 1.0f;
-        if constexpr (NP == 2)
-          split_half(x[g][e] * by, x[g][e + 1] * by, qf[c][0][g][e / 2], qf[c][1][g][e / 2]);
-        else
-          qf[c][0][g][e / 2] = pack_half(x[g][e] * by, x[g][e + 1] * by);
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (F32) qx[c][g][e] = x[g][e];
+        else if (e % 2 == 0)
+          qf[c][g][e / 2] = pack_half(x[g][e] * ((e & 2) ? 0.0625f : 1.0f),
+                                      x[g][e + 1] * ((e & 2) ? 0.0625f : 1.0f));
       }
     }
   }
@@ -622,32 +622,38 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
   const int s_off = bs * (HD / 2) + kq * G * 8;
   const int k_off = (n16 * 4 + kq) * G * 4, v_off = (n16 * bs + kq * 4) * (T / 2);
+  const int quad_off = bs * (HD / 2) + (n16 >> 2) * G * 8;
   // offsets: key n16 of group kq (and kq + 4); tokens 4 kq .. of group n16
   const int km_off = bs * (HD / 2) + bs * G * 2 + ((n16 >> 2) * G + kq % G) * 8 + (n16 & 3) * 2;
   const int vm_off = bs * (HD / 2) + bs * G * 2 + (kq * G + n16 % G) * 8;
 
-  struct KTile {
-    uint32_t code[HD / 32], s[2 * G];
+  struct KTile {  // s: of tokens 4 kq .., for f32 queries of the four that n16 is among
+    uint32_t code[HD / 32], s[2 * G], all_m[F32 ? 2 * G : 1];
     _Float16 m[GM];
   };
   struct VTile {
-    uint32_t code[HD / 32], s[2 * G], m[2];
+    uint32_t code[HD / 32], s[2 * G], m[F32 ? 2 * G : 2];  // (m: of group n16 or all)
   };
   auto load_k = [&](int id, int key, KTile& t) {
     const int at = key & (bs - 1);
     const char* p = kh + (size_t)max(id, 0) * blk_stride;
     load_words<HD / 8>(p + at * (HD / 2) + k_off, t.code);
-    load_words<G * 8>(p + at * (G * 2) + s_off, t.s);
+    if constexpr (F32) {
+      load_words<G * 8>(p + at * (G * 2) + quad_off, t.s);
+      load_words<G * 8>(p + at * (G * 2) + quad_off + bs * G * 2, t.all_m);
+    } else {
+      load_words<G * 8>(p + at * (G * 2) + s_off, t.s);
 #pragma unroll
-    for (int b = 0; b < GM; ++b)
-      t.m[b] = *reinterpret_cast<const _Float16*>(p + at * (G * 2) + km_off + 32 * b);
+      for (int b = 0; b < GM; ++b)
+        t.m[b] = *reinterpret_cast<const _Float16*>(p + at * (G * 2) + km_off + 32 * b);
+    }
   };
   auto load_v = [&](int id, int key, VTile& t) {
     const int at = key & (bs - 1);
     const char* p = vh + (size_t)max(id, 0) * blk_stride;
     load_words<HD / 8>(p + at * (T / 2) + v_off, t.code);
     load_words<G * 8>(p + at * (G * 2) + s_off, t.s);
-    load_words<8>(p + at * (G * 2) + vm_off, t.m);
+    load_words<F32 ? G * 8 : 8>(p + at * (G * 2) + (F32 ? s_off + bs * G * 2 : vm_off), t.m);
   };
 
   f32x4 o[NT][T], om[NT];  // row 4 kq + i: channel n16 + 16 t; offsets' sum of group n16
@@ -685,20 +691,33 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
       for (int c = 0; c < NT; ++c) {
         acc[c] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < GM; ++b)
+        for (int b = 0; b < (F32 ? 0 : GM); ++b)
           acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kt[j].m[b], qs[c][b], acc[c], 0, 0, 0);
       }
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        uint32_t kf[4];
-        k_pairs(kt[j].code[g], kf);
+        if constexpr (F32) {
+          const uint32_t ws = n16 & 2 ? kt[j].s[2 * g + 1] : kt[j].s[2 * g];
+          const uint32_t wm = n16 & 2 ? kt[j].all_m[2 * g + 1] : kt[j].all_m[2 * g];
+          const float ks = n16 & 1 ? half_of(ws, 1) : half_of(ws, 0);
+          const float km = n16 & 1 ? half_of(wm, 1) : half_of(wm, 0);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          f32x4 d = mfma16(kf, qf[c][0][g], f32x4{0, 0, 0, 0});
-          if constexpr (NP == 2) d = mfma16(kf, qf[c][1][g], d);
+          for (int e = 0; e < 8; ++e) {
+            const float k = fmaf(ks, (float)(kt[j].code[g] >> q4_k_bit(e) & 15), km);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            acc[c][i] = fmaf(half_of(kt[j].s[2 * g + i / 2], i % 2), d[i], acc[c][i]);
+            for (int c = 0; c < NT; ++c)
+              acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(k, qx[c][g][e], acc[c], 0, 0, 0);
+          }
+        } else {
+          uint32_t kf[4];
+          k_pairs(kt[j].code[g], kf);
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            const f32x4 d = mfma16(kf, qf[c][g], f32x4{0, 0, 0, 0});
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[c][i] = fmaf(half_of(kt[j].s[2 * g + i / 2], i % 2), d[i], acc[c][i]);
+          }
         }
       }
 #pragma unroll
@@ -732,7 +751,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 2 * G; ++e) sw |= vt[j].s[e];
-    const bool big = sw & 0x40004000u;
+    const bool big = !F32 && sw & 0x40004000u;
     float mx[NT];
     bool far = top > 1.0f && big;
 #pragma unroll
@@ -755,55 +774,76 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float b = lane_of(by, 4 * kq + i);
-          om[c][i] *= b;
+          if constexpr (!F32) om[c][i] *= b;
 #pragma unroll
           for (int t = 0; t < T; ++t) o[c][t][i] *= b;
         }
       }
     }
-    uint32_t mf[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mf[e] = n16 < G ? vt[e / 2].m[e % 2] : 0u;
     float p[NT][2][4];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      uint32_t pf[2][4];
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           p[c][j][i] = fast_exp2(fmaf(x[c][j][i], f[c], -ref[c]));
           l[c] += p[c][j][i];
         }
+    if constexpr (F32) {
+      // token 4 kq + i's nibbles of channels n16 + 16 t follow those of i - 1
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          split_half(p[c][j][2 * e], p[c][j][2 * e + 1], pf[0][2 * j + e], pf[1][2 * j + e]);
-      }
-      om[c] = mfma16(pf[0], mf, om[c]);
-      om[c] = mfma16(pf[1], mf, om[c]);
-    }
-    uint32_t pair[2][2][T / 4];
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) v_pairs<T>(vt[j].code, pair[j]);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      uint32_t wf[NT][2][4];
+          for (int t = 0; t < T; ++t) {
+            const int g = t / 2, at = i * T + t;
+            const float code = (float)(vt[j].code[at / 8] >> (4 * (at % 8)) & 15);
+            const float v = fmaf(half_of(vt[j].s[2 * g + i / 2], i % 2), code,
+                                 half_of(vt[j].m[2 * g + i / 2], i % 2));
 #pragma unroll
-      for (int c = 0; c < NT; ++c)
+            for (int c = 0; c < NT; ++c)
+              o[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[c][j][i], v, o[c][t], 0, 0, 0);
+          }
+    } else {
+      uint32_t mf[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mf[e] = n16 < G ? vt[e / 2].m[e % 2] : 0u;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        uint32_t pf[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            split_scaled(p[c][j][2 * e], p[c][j][2 * e + 1], vt[j].s[2 * g + e],
-                         wf[c][0][2 * j + e], wf[c][1][2 * j + e]);
+            split_half(p[c][j][2 * e], p[c][j][2 * e + 1], pf[0][2 * j + e], pf[1][2 * j + e]);
+        om[c] = mfma16(pf[0], mf, om[c]);
+        om[c] = mfma16(pf[1], mf, om[c]);
+      }
+      uint32_t pair[2][2][T / 4];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t vf[4];
-        v_frag<T>(pair, 2 * g + b, vf);
+      for (int j = 0; j < 2; ++j) v_pairs<T>(vt[j].code, pair[j]);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        uint32_t wf[NT][2][4];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) o[c][2 * g + b] = mfma16(wf[c][q], vf, o[c][2 * g + b]);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              split_scaled(p[c][j][2 * e], p[c][j][2 * e + 1], vt[j].s[2 * g + e],
+                           wf[c][0][2 * j + e], wf[c][1][2 * j + e]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t vf[4];
+          v_frag<T>(pair, 2 * g + b, vf);
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) o[c][2 * g + b] = mfma16(wf[c][q], vf, o[c][2 * g + b]);
+        }
       }
     }
   }
@@ -818,7 +858,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
     }
     // offsets: group g of row 4 kq + i is in lane 16 kq + g
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = 0; g < (F32 ? 0 : G); ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float m = lane_of(om[c][i], 16 * kq + g);
@@ -1368,7 +1408,7 @@ Plan plan_of(const pkv_pool* p, const Q4Args& a) {
   Plan pl{};
   const int c = 16 / (p->head_dim / 32);  // query columns of a tile for few
   const long long cols = (long long)a.max_q_len * (a.n_head / p->n_kv_head);
-  if (cols <= 2 * c) {
+  if (cols <= 2 * c && a.q_dtype != PKV_F32) {
     const int nt = cols > c ? 2 : 1;
     pl.at[pl.n++] = launch_of(p, a, kFew, nt, 0, INT32_MAX, nt * c);
   } else if (cols <= 32 || a.q_dtype == PKV_F32) {
@@ -1398,14 +1438,13 @@ size_t part_places(const Q4Args& a, const Plan& pl) {
 template <int DT, int HD>
 void attend(const Q4KArgs& ka, const Launch& l, unsigned blocks, hipStream_t stream) {
   constexpr int T = kWaves * 64;
-  if (l.kind == kFew) {
-    if (l.nt == 1) q4_few_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
-    else q4_few_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
-  } else if (l.kind == kMany) {
+  if (l.kind == kMany) {
     if (l.nt == 1) q4_many_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
     else if constexpr (HD <= 128) q4_many_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
   } else if constexpr (DT != PKV_F32) {
-    q4_chunk_kernel<DT, HD><<<blocks, T, 0, stream>>>(ka);
+    if (l.kind == kChunk) q4_chunk_kernel<DT, HD><<<blocks, T, 0, stream>>>(ka);
+    else if (l.nt == 1) q4_few_kernel<DT, HD, 1><<<blocks, T, 0, stream>>>(ka);
+    else q4_few_kernel<DT, HD, 2><<<blocks, T, 0, stream>>>(ka);
   }
 }
 
