@@ -287,6 +287,34 @@ def test_attention_of_chunks(gpu, dt, h, kv, hd):
     c.check(c.run(max_q_len=300))
 
 
+@pytest.mark.parametrize("dt,h,kv,hd,bs", [("bf16", 32, 8, 128, 64), ("f16", 32, 4, 64, 256),
+                                           ("f16", 16, 8, 256, 32), ("bf16", 14, 2, 64, 128),
+                                           ("f32", 32, 8, 128, 256), ("bf16", 200, 1, 64, 16)])
+def test_attention_of_chunks_in_blocks(gpu, dt, h, kv, hd, bs):
+    c = Case(gpu, 8 * h + hd, dt, h, kv, hd, bs, [300, 64, 1, 65, 1500, 0, 33], [40, 64, 1, 9, 33, 0, 33])
+    out = c.run()
+    c.cache.check()
+    c.check(out)
+
+
+@pytest.mark.parametrize("h,kv,hd,rows", [(32, 8, 64, 1), (32, 8, 128, 1), (16, 8, 256, 1), (32, 8, 128, 9)])
+def test_f32_attention_is_f32(gpu, h, kv, hd, rows):
+    """Offsets and codes of values cancel, all the more over many keys: what is lost before
+    they do shows.  Scores are below 16 here, where half a step is 2^-21; one sums up hd
+    products, whose roundings add up at random to 2^-21 sqrt(hd / 3) at most, 2^-17.7
+    for 256: weights, and so results in norm, are off by that."""
+    n = 2000
+    c = Case(gpu, h + hd, "f32", h, kv, hd, 16, [n], [rows])
+    k, v = c.rng.normal(size=(2, c.cache.num_blocks * 16, kv, hd))
+    k, kx = typed(k.astype(np.float32), "f32", gpu)
+    v, vx = typed(v.astype(np.float32), "f32", gpu)
+    c.pool.q4_append(k, v, torch.arange(len(k), dtype=torch.int32, device=gpu))
+    c.take(kx, vx)
+    want = ref.attention(c.qx, *c.rows(0)[0], rows, c.scale, *c.rows(0)[1])[0]
+    off = host(c.run()).reshape(want.shape) - want
+    assert np.linalg.norm(off) <= 2.0 ** -17.7 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("dt,h,kv,hd,bs", [("bf16", 32, 8, 128, 16), ("f16", 32, 4, 64, 256),
                                            ("f32", 14, 2, 64, 32), ("bf16", 16, 8, 256, 16)])
 def test_attention_of_long_contexts(gpu, dt, h, kv, hd, bs):
