@@ -108,12 +108,16 @@ class BlockAllocator:
 # ---------------------------------------------------------------------------
 # device pool
 # ---------------------------------------------------------------------------
+_DTYPES: dict = {}  # torch's dtypes, once torch is needed
+
+
 def pkv_dtype(t) -> int:
-    import torch
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t not in m:
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if t not in _DTYPES:
         raise TypeError(f"unsupported dtype {t}")
-    return m[t]
+    return _DTYPES[t]
 
 
 def torch_dtype(d: int):
@@ -406,14 +410,14 @@ def _rows_view(t, name: str, device, dtype, heads, head_dim):
         raise ValueError(f"{name} must be a tensor on {device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        raise ValueError(f"{name} must be (tokens, {heads}, {head_dim}), got {tuple(t.shape)}")
-    row, stride, e = heads * head_dim, t.stride(0), t.element_size()
-    if (t.stride(2) != 1 and head_dim > 1) or (t.stride(1) != head_dim and heads > 1) or \
-            t.data_ptr() % 16 or (t.shape[0] > 1 and (stride < row or stride * e % 16)):
-        t = t.clone(memory_format=torch.contiguous_format)
-        stride = row
-    return t, (stride if t.shape[0] > 1 else row)
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name} must be (tokens, {heads}, {head_dim}), got {tuple(shape)}")
+    row, (stride, head_step, step) = heads * head_dim, t.stride()
+    if (step != 1 and head_dim > 1) or (head_step != head_dim and heads > 1) or \
+            t.data_ptr() % 16 or (shape[0] > 1 and (stride < row or stride * t.itemsize % 16)):
+        t, stride = t.clone(memory_format=torch.contiguous_format), row
+    return t, (stride if shape[0] > 1 else row)
 
 
 def _attn_out(out, rows: int, width: int, dtype, out_dtype, device):
@@ -468,8 +472,8 @@ def prompt_attention(q, k, v, cu_lens, max_len: int | None = None, scale: float 
         vv, vs = _rows_view(v, "v", dev, q.dtype, kvh, hd)
         out = _attn_out(out, total, H * hd, q.dtype, out_dtype, dev)
         check(lib().pkv_prompt_attention(
-            _dev_ptr(qq), _dev_ptr(kk), _dev_ptr(vv), pkv_dtype(q.dtype), qs, ks, vs,
-            _dev_ptr(out), pkv_dtype(out.dtype), _dev_ptr(cu), n, total, max(int(max_len), 1), H,
+            qq.data_ptr(), kk.data_ptr(), vv.data_ptr(), pkv_dtype(q.dtype), qs, ks, vs,
+            out.data_ptr(), pkv_dtype(out.dtype), cu.data_ptr(), n, total, max(int(max_len), 1), H,
             kvh, hd, float(scale), s), None)
     return out
 
@@ -506,36 +510,33 @@ def adjust_logits(logits, tokens=None, cu_tokens=None, prompt_lens=None, repetit
     if mask is None and mask_rows is not None:
         raise ValueError("mask_rows without mask")
 
-    def dev_arr(t, name, dtype, shape=None):
-        return None if t is None else _device_tensor(t, name, dev, dtype, shape)
-
     s, ctx = _run_on(stream, dev, (logits, out, tokens, cu_tokens, prompt_lens, repetition, presence,
                                    frequency, bias_tokens, bias_values, cu_bias, mask, mask_rows))
     with ctx:
-        tok = dev_arr(tokens, "tokens", i32)
-        cut = dev_arr(cu_tokens, "cu_tokens", i32, (B + 1,))
-        pl = dev_arr(prompt_lens, "prompt_lens", i32, (B,))
-        rep = dev_arr(repetition, "repetition", f32, (B,))
-        pres = dev_arr(presence, "presence", f32, (B,))
-        freq = dev_arr(frequency, "frequency", f32, (B,))
-        bt = dev_arr(bias_tokens, "bias_tokens", i32)
-        bv = dev_arr(bias_values, "bias_values", f32, None if bt is None else bt.shape)
-        cb = dev_arr(cu_bias, "cu_bias", i32, (B + 1,))
-        mk = dev_arr(mask, "mask", i32)
-        mr = dev_arr(mask_rows, "mask_rows", i32, (B,))
-        if mk is not None and mk.dim() != 2:
-            raise ValueError("mask must be (masks, words)")
+        row, ends, held, at = (B,), (B + 1,), [], []
+        for t, name, dtype, shape in (
+                (tokens, "tokens", i32, None), (cu_tokens, "cu_tokens", i32, ends),
+                (prompt_lens, "prompt_lens", i32, row), (repetition, "repetition", f32, row),
+                (presence, "presence", f32, row), (frequency, "frequency", f32, row),
+                (bias_tokens, "bias_tokens", i32, None), (bias_values, "bias_values", f32,
+                                                          getattr(bias_tokens, "shape", None)),
+                (cu_bias, "cu_bias", i32, ends), (mask, "mask", i32, None),
+                (mask_rows, "mask_rows", i32, row)):
+            if t is not None:
+                t = _device_tensor(t, name, dev, dtype, shape)
+                held.append(t)  # (copies live until the launch is queued)
+            at.append(None if t is None else t.data_ptr())
+        masks, words = (0, 0)
+        if mask is not None:
+            if mask.dim() != 2:
+                raise ValueError("mask must be (masks, words)")
+            masks, words = mask.shape
         if out is None:
             out = torch.empty((B, V), dtype=logits.dtype, device=dev)
-
-        def at(t):
-            return None if t is None else _dev_ptr(t)
-
         check(lib().pkv_adjust_logits(
-            _dev_ptr(logits), _dev_ptr(out), pkv_dtype(logits.dtype), logits.stride(0),
-            out.stride(0), B, V, at(tok), at(cut), 0 if tok is None else tok.numel(), at(pl),
-            at(rep), at(pres), at(freq), at(bt), at(bv), at(cb), 0 if bt is None else bt.numel(),
-            at(mk), 0 if mk is None else mk.shape[0], 0 if mk is None else mk.shape[1], at(mr), s),
+            logits.data_ptr(), out.data_ptr(), pkv_dtype(logits.dtype), logits.stride(0),
+            out.stride(0), B, V, at[0], at[1], 0 if tokens is None else tokens.numel(), *at[2:9],
+            0 if bias_tokens is None else bias_tokens.numel(), at[9], masks, words, at[10], s),
             None)
     return out
 
@@ -1186,8 +1187,8 @@ class KvPool:
             sm = _i32_on(slot_mapping, c.device)
             if sm.numel() != k.shape[0] or v.shape[0] != k.shape[0]:
                 raise ValueError("slot_mapping / k / v lengths differ")
-            check(lib().pkv_q4_append(self._h, self.layer_index, _dev_ptr(kk), _dev_ptr(vv),
-                                      pkv_dtype(k.dtype), ks, vs, _dev_ptr(sm), sm.numel(), s),
+            check(lib().pkv_q4_append(self._h, self.layer_index, kk.data_ptr(), vv.data_ptr(),
+                                      pkv_dtype(k.dtype), ks, vs, sm.data_ptr(), sm.numel(), s),
                   self._h)
 
     def q4_gather(self, slot_mapping, out_dtype=None, stream=None):
@@ -1203,8 +1204,8 @@ class KvPool:
             ok = torch.empty((sm.numel(), c.n_kv_head, c.head_dim),
                              dtype=out_dtype or torch.float32, device=c.device)
             ov = torch.empty_like(ok)
-            check(lib().pkv_q4_gather(self._h, self.layer_index, _dev_ptr(sm), sm.numel(),
-                                      _dev_ptr(ok), _dev_ptr(ov), pkv_dtype(ok.dtype), s), self._h)
+            check(lib().pkv_q4_gather(self._h, self.layer_index, sm.data_ptr(), sm.numel(),
+                                      ok.data_ptr(), ov.data_ptr(), pkv_dtype(ok.dtype), s), self._h)
         return ok, ov
 
     def q4_attention(self, q, block_tables, context_lens, cu_q_lens=None,
@@ -1257,10 +1258,10 @@ class KvPool:
                                                 int(max_context_len), H)
             ws = _workspace(need, c.device) if need else None
             check(lib().pkv_q4_attention(
-                self._h, self.layer_index, _dev_ptr(qq), pkv_dtype(q.dtype), qs, _dev_ptr(out),
-                pkv_dtype(out.dtype), _dev_ptr(cu) if cu is not None else None, _dev_ptr(cl),
-                _dev_ptr(bt), bt.shape[1], n, rows, int(max_q_len), int(max_context_len), H,
-                float(scale), _dev_ptr(ws) if need else None, need, s), self._h)
+                self._h, self.layer_index, qq.data_ptr(), pkv_dtype(q.dtype), qs, out.data_ptr(),
+                pkv_dtype(out.dtype), cu.data_ptr() if cu is not None else None, cl.data_ptr(),
+                bt.data_ptr(), bt.shape[1], n, rows, int(max_q_len), int(max_context_len), H,
+                float(scale), ws.data_ptr() if need else None, need, s), self._h)
         return out
 
     def _check_rows(self, t, name: str) -> None:
