@@ -1,10 +1,17 @@
 // pkv_logits.hip -- penalties, biases and masks on logits before a token is chosen
 // (gfx950).
 //
-// A workgroup has a slice of one request's row.  It first counts the request's tokens
-// that fall into the slice in LDS (integers, so in any order), and finds the last
-// bias entry of each token there; then every logit of the slice is read, changed
-// and written once.
+// A workgroup has a slice of one request's row: two or one 16 bytes of logits a thread,
+// 16,384 or 8192 tokens of 16 bits (with biases the tables in LDS are two).  It counts the
+// request's tokens that fall into the slice (integers, so in any order), marks the ones
+// seen by a bit, and finds the last bias entry of each token; a thread then computes the
+// logits of its own that have a bit one after another, and writes all of them once.
+//
+// Bound by the histories: each slice goes through the whole of its request's.  128 rows of
+// 128,256 bf16 logits with histories up to 8000 take 27 us, 13.4 (the copy rate) without
+// any.  With slices of 4096 and every logit computed in place, so that a wave of 512
+// went through the division for a few of them, they took 34; a list of the changed
+// tokens made by a shared counter, 42.
 #include "pkv_device.h"
 #include "pkv_internal.h"
 

@@ -11,6 +11,10 @@ C ABI in include/pagedkv.h:
                                 (attention.rs:11-28,100-136, transformer.rs:271-292)
   KvPool.prefill_attention      prefill_seq's attention (transformer.rs:139-196)
 
+and, without a counterpart there, a cache held in 4 bits (dtype Q4: KvPool.q4_append,
+q4_gather, q4_attention), prompt_attention over rows that no pool holds yet, and
+adjust_logits before a token is chosen.
+
 torch tensors are used only as device memory and for the current stream.
 """
 from __future__ import annotations
