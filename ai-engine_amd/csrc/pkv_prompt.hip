@@ -101,7 +101,12 @@ __global__ void __launch_bounds__(kWaves * 64)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int pairs = a.n_seqs * a.n_kv_head, r = a.n_head / a.n_kv_head;
   // longest first: groups of units by their place in a prompt of max_len, from the end
-  const int pair = blockIdx.x % pairs, first = max_groups - 1 - (int)(blockIdx.x / pairs);
+  const int place = blockIdx.x / pairs, first = max_groups - 1 - place;
+  // Workgroups go to the 8 XCDs in turn, so a pair would stay on one, good for its keys
+  // in that cache, but prompts differ in length: unless every XCD has each prompt by
+  // its heads, pairs move on from place to place (16 prompts, 2 kv heads: 186 and 121 us;
+  // one prompt, where nothing is gained: 110 and 117).
+  const int pair = (int)((blockIdx.x + (a.n_kv_head % 8 && a.n_seqs > 1 ? (unsigned)place : 0u)) % pairs);
   const int s = pair / a.n_kv_head, g = pair % a.n_kv_head;
   const int lo = a.cu_lens[s], hi = a.cu_lens[s + 1];
   if (lo < 0 || hi > a.total || lo >= hi) return;
@@ -339,12 +344,15 @@ long long units_of(const PromptArgs& a) {
 }
 // Whether the waves of a workgroup share a unit: with so few units that the longest
 // prompt's last ones take the time.  Not sharing and sharing took, us:
-//   f32    512 units 74, 38    1024  76, 72    1624  31, 22    3248 101, 102   6496 187, 233
-//   bf16   512 units 18, 14    1024  32, 26    2048  59, 72    2048 (short) 15, 19
+//   f32, 64 channels     1624 units 31, 18    3248  100, 59    6496 122, 136
+//   f32, 128             512 units 74, 38     1024  76, 71     3648  86, 104   4032  537, 684
+//   16 bits, 128         512 units 18, 14     1024  32, 26     2048  56, 65
+//   16 bits, 64          2016 units 38, 36    2048 (of 500 tokens) 15, 19
 // (f32 with 256 channels has no room for it.)
 bool split_of(const PromptArgs& a) {
-  return !(a.dtype == PKV_F32 && a.head_dim == 256) &&
-         units_of(a) * a.n_seqs * a.n_kv_head <= (a.dtype == PKV_F32 ? 2048 : 1024);
+  const __int128 units = (__int128)units_of(a) * a.n_seqs * a.n_kv_head;
+  if (a.dtype == PKV_F32) return a.head_dim <= 128 && units <= 4096 * 64 / a.head_dim;
+  return units <= 1024;
 }
 long long max_groups_of(const PromptArgs& a) {
   return split_of(a) ? units_of(a) : (units_of(a) + kWaves - 1) / kWaves;

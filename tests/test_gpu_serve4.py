@@ -450,7 +450,7 @@ def test_longer_prompts(gpu, dt, h, kv, hd, lens):
                                    ("bf16", 128), ("bf16", 256)])
 def test_many_prompts(gpu, dt, hd):
     """More tiles and heads than fill the GPU twice: waves have a unit each."""
-    lens = [1, 97, 32, 33, 0, 64, 65, 5] + np.random.default_rng(hd).integers(1, 97, 40).tolist()
+    lens = [1, 97, 32, 33, 0, 64, 65, 5] + np.random.default_rng(hd).integers(1, 97, 90).tolist()
     q, k, v, cu, xs = prompt_case(gpu, 25, dt, 14, 2, hd, lens, packed=True)
     prompt_check(pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=97), cu, xs, dt, hd ** -0.5)
 
