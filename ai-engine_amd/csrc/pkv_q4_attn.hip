@@ -4,10 +4,14 @@
 //   q . k = sum_g s_g (q_g . c_g) + m_g sum(q_g)
 // and the values' sum
 //   o_g = sum_k (p_k s_kg) c_k + sum_k p_k m_kg,
-// so both products run on the matrix cores over the codes themselves.  A code's four
-// bits in the low bits of an f16 are the number c 2^-24, and in the next four 16 c
-// 2^-24 (subnormals, which v_mfma_f32_16x16x32_f16 takes exactly): one mask makes
-// two of them, a second one the next two, and nothing is converted.
+// so both products run on the matrix cores over the codes themselves, as f16 numbers
+// that two instructions make of two codes.  As f16 subnormals, bits masked out of the
+// words, they need only one, and v_mfma_f32_16x16x32_f16 takes them exactly.  But it aligns
+// eight products by their operands' exponents, subnormals counting as 2^-14, and
+// drops bits, downwards, that a normal number would keep: up to 2^-13 of the largest
+// weight (of 1 in c) each.  In the values' sum, where offsets and codes cancel, that was 2^-15 of
+// results over 2000 keys; for the keys of a decode it is 2^-15 of a query's largest
+// element in a score, below what rounding results to 16 bits costs, and kept.
 //
 // A column is a query row of a chunk and one of the heads of a kv head's group.  A
 // wave takes 32 keys a step: two tiles S^T = K Q^T of 16 keys, whose lanes then hold
@@ -186,13 +190,30 @@ __device__ __forceinline__ void put(void* out, int dt, size_t i, float x) {
   else static_cast<uint16_t*>(out)[i] = (uint16_t)f32_to_bf16_bits(x);
 }
 
-// Four words of a K code word: its channels 2 e, 2 e + 1 as f16 pairs.
-__device__ __forceinline__ void k_pairs(uint32_t w, uint32_t (&f)[4]) {
-  const uint32_t w8 = w >> 8;
-  f[0] = w & 0x000f000fu;
-  f[1] = w & 0x00f000f0u;
-  f[2] = w8 & 0x000f000fu;
-  f[3] = w8 & 0x00f000f0u;
+// Codes 4 bits apart in 16-bit halves as f16 numbers; hi: they are in bits 4 .. 7.  (w &
+// mask) | 1024.0 is 1024 + c or 1024 + 16 c, and one packed instruction makes c of it; the
+// constants are kept in registers so that the first is one instruction too.
+struct CodeMasks {
+  uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;
+  __device__ __forceinline__ CodeMasks() { asm("" : "+v"(lo), "+v"(hi), "+v"(one)); }
+};
+__device__ __forceinline__ f16x2 code_pair(const CodeMasks& k, uint32_t w, bool hi) {
+  const f16x2 x = __builtin_bit_cast(f16x2, (w & (hi ? k.hi : k.lo)) | k.one);
+  const f16x2 a = {(_Float16)1024.0f, (_Float16)1024.0f}, b = {(_Float16)64.0f, (_Float16)64.0f};
+  const f16x2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
+  return hi ? x * by - b : x - a;
+}
+
+// Four words of a K code word: its channels 2 e, 2 e + 1 as f16 pairs; or as subnormals, c
+// 2^-24 of even e and 16 c 2^-24 of odd ones.
+__device__ __forceinline__ void k_subnormals(uint32_t w, uint32_t (&f)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = (e & 2 ? w >> 8 : w) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+__device__ __forceinline__ void k_pairs(const CodeMasks& k, uint32_t w, uint32_t (&f)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    f[e] = __builtin_bit_cast(uint32_t, code_pair(k, e & 2 ? w >> 8 : w, e & 1));
 }
 
 // V codes of a lane's four tokens (T / 2 bytes each): for channels 4 h .. 4 h + 3 of the
@@ -216,14 +237,14 @@ __device__ __forceinline__ void v_pairs(const uint32_t (&code)[T / 2], uint32_t 
 }
 // Right operand of channels i + 16 t from the pairs of both 16-token tiles.
 template <int T>
-__device__ __forceinline__ void v_frag(const uint32_t (&pair)[2][2][T / 4], int t,
-                                       uint32_t (&f)[4]) {
+__device__ __forceinline__ void v_frag(const CodeMasks& k, const uint32_t (&pair)[2][2][T / 4],
+                                       int t, uint32_t (&f)[4]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t w = pair[j][e][t / 4];
-      f[2 * j + e] = ((t & 2) ? w >> 8 : w) & ((t & 1) ? 0x00f000f0u : 0x000f000fu);
+      f[2 * j + e] = __builtin_bit_cast(uint32_t, code_pair(k, t & 2 ? w >> 8 : w, t & 1));
     }
 }
 
@@ -263,7 +284,8 @@ __device__ __forceinline__ float new_ref(float ref, float m, float top, bool les
 //
 // Bound by the reads of codes, scales and offsets, each once and past the caches (6.5
 // TB/s for blocks anywhere, 5.7 through them): 256 sequences of 512 .. 4096 keys, 8 kv
-// heads of 128 and 32 heads, 158 us, 48 of 12 .. 32 thousand 239, 5.0 and 5.3 TB/s.  A few
+// heads of 128 and 32 heads, 162 us, 48 of 12 .. 32 thousand 247, 4.8 and 5.1 TB/s (values'
+// codes as subnormals, see above: 157 and 238).  A few
 // sequences are a chain of waits (lengths, ids, keys and values, the join): 8 of
 // 600 .. 9000, heads of 64, 16.9 us and 4.0 for the join.
 template <int DT, int HD, int NT>
@@ -374,6 +396,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
     for (int t = 0; t < T; ++t) o[c][t] = f32x4{0, 0, 0, 0};
   }
   float top = 14.0f;
+  const CodeMasks masks;
   for (; key < it.k1; key += stride) {
     const bool masked = key + kStep > it.all || (id[0] | id[1]) < 0;
     const bool in[2] = {id[0] >= 0, id[1] >= 0};
@@ -386,7 +409,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         uint32_t kf[4];
-        k_pairs(kt[j].code[g], kf);
+        k_subnormals(kt[j].code[g], kf);
 #pragma unroll
         for (int c = 0; c < NT; ++c) d[c] = mfma16(kf, qf[c][g], d[c]);
       }
@@ -477,7 +500,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       uint32_t vf[4];
-      v_frag<T>(pair, t, vf);
+      v_frag<T>(masks, pair, t, vf);
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -518,8 +541,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
       if constexpr (HD == 64) y = o[c][e / 2][2 * (e % 2) + e / 4];
       else if constexpr (HD == 128) y = o[c][e][e / 2];
       else y = (kq & 1) ? o[c][8 + e][e / 2] : o[c][e][e / 2];
-      const float by = (HD == 64 ? e / 2 : e) % 2 ? 0x1p20f : 0x1p24f;
-      sm_o[wave][c][e][lane] = fmaf(y, by, lane_of(om[c], qc * G + t / 2));
+      sm_o[wave][c][e][lane] = y + lane_of(om[c], qc * G + t / 2);
     }
   __syncthreads();
   for (int j = threadIdx.x; j < NT * 512; j += kWaves * 64) {
@@ -554,10 +576,9 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 // Tiles of 16 query columns: a product per group, scaled and added up in the lane; the
 // offsets' products are one v_mfma_f32_16x16x4_f32 (its four k are groups).  f32 queries
 // have all their calls here, with keys and values as f32 on f32 instructions, which
-// take eight times as long: in the f16 ones, products below 2^-24 of the largest of
-// eight lose bits, always downwards, which after offsets and codes have cancelled was
-// 2^-15 of a result over 2000 keys (now 2^-21; 64 sequences of 4096 keys, 8 kv heads of
-// 128 and 32 heads take 210 us, 75 in f16 parts).  DT: type of q.  NT: tiles.
+// take eight times as long: in two f16 parts queries and weights would be off by 2^-22, and
+// sums by what the f16 ones drop of small products.  64 sequences of 4096 keys, 8 kv heads of 128, 32
+// heads, f32: 209 us.  DT: type of q.  NT: tiles.
 template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   using L = Q4Layout<HD>;
@@ -599,7 +620,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
     }
     big = row_group_max(big);
     const int ex = !F32 && big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;
-    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, (F32 ? 0 : 24) - ex), 0x1p-126f);
+    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, -ex), 0x1p-126f);
 #pragma unroll
     for (int b = 0; b < GM; ++b) qs[c][b] = 0.0f;
 #pragma unroll
@@ -610,14 +631,13 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
         x[g][e] = ldexpf(a.scale < 0.0f ? -x[g][e] : x[g][e], ex);
         sum += x[g][e];
       }
-      sum = swap32_sum(swap16_sum(sum)) * (F32 ? 1.0f : 0x1p-24f);
+      sum = swap32_sum(swap16_sum(sum));
       if (kq == g % 4) qs[c][g / 4] = sum;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (F32) qx[c][g][e] = x[g][e];
         else if (e % 2 == 0)
-          qf[c][g][e / 2] = pack_half(x[g][e] * ((e & 2) ? 0.0625f : 1.0f),
-                                      x[g][e + 1] * ((e & 2) ? 0.0625f : 1.0f));
+          qf[c][g][e / 2] = pack_half(x[g][e], x[g][e + 1]);
       }
     }
   }
@@ -674,6 +694,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
     for (int t = 0; t < T; ++t) o[c][t] = f32x4{0, 0, 0, 0};
   }
   float top = 14.0f;
+  const CodeMasks masks;
 
   constexpr int stride = kWaves * kStep;
   int key = it.k0 + wave * kStep;
@@ -717,7 +738,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
           }
         } else {
           uint32_t kf[4];
-          k_pairs(kt[j].code[g], kf);
+          k_pairs(masks, kt[j].code[g], kf);
 #pragma unroll
           for (int c = 0; c < NT; ++c) {
             const f32x4 d = mfma16(kf, qf[c][g], f32x4{0, 0, 0, 0});
@@ -845,7 +866,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           uint32_t vf[4];
-          v_frag<T>(pair, 2 * g + b, vf);
+          v_frag<T>(masks, pair, 2 * g + b, vf);
 #pragma unroll
           for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -869,8 +890,8 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float m = lane_of(om[c][i], 16 * kq + g);
-        o[c][2 * g][i] = fmaf(o[c][2 * g][i], 0x1p24f, m);
-        o[c][2 * g + 1][i] = fmaf(o[c][2 * g + 1][i], 0x1p20f, m);
+        o[c][2 * g][i] += m;
+        o[c][2 * g + 1][i] += m;
       }
   }
   __syncthreads();
@@ -966,18 +987,6 @@ struct CT {
   static constexpr int STAGE = kTile * KP + HD * VP + 2 * SM;
 };
 
-// Codes 4 bits apart in 16-bit halves as f16 numbers; hi: they are in bits 4 .. 7.  (w &
-// mask) | 1024.0 is 1024 + c or 1024 + 16 c; the constants are kept in registers so
-// that this is one instruction.
-struct CodeMasks {
-  uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;
-};
-__device__ __forceinline__ f16x2 code_pair(const CodeMasks& k, uint32_t w, bool hi) {
-  const f16x2 x = __builtin_bit_cast(f16x2, (w & (hi ? k.hi : k.lo)) | k.one);
-  const f16x2 a = {(_Float16)1024.0f, (_Float16)1024.0f}, b = {(_Float16)64.0f, (_Float16)64.0f};
-  const f16x2 by = {(_Float16)0.0625f, (_Float16)0.0625f};
-  return hi ? x * by - b : x - a;
-}
 __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -1030,16 +1039,13 @@ __global__ void __launch_bounds__(kWaves * 64)
     }
     big = half_max(big);
     const int ex = big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;  // below 2^14
-    f = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, (EXACT ? 24 : 0) - ex), 0x1p-126f);
+    f = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, -ex), 0x1p-126f);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[i][e] = ldexpf(a.scale < 0.0f ? -x[i][e] : x[i][e], ex);
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float by = EXACT && (e & 2) ? 0.0625f : 1.0f;  // (these codes are 16 times larger)
-        qf[i][e / 2] = pack_half(x[i][e] * by, x[i][e + 1] * by);
-      }
+      for (int e = 0; e < 8; e += 2) qf[i][e / 2] = pack_half(x[i][e], x[i][e + 1]);
     }
     if constexpr (EXACT) {  // sums of groups 2 j + half
 #pragma unroll
@@ -1047,7 +1053,7 @@ __global__ void __launch_bounds__(kWaves * 64)
         float t = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) t += x[2 * g][e] + x[2 * g + 1][e];
-        t = swap32_sum(t) * 0x1p-24f;
+        t = swap32_sum(t);
         if (half == g % 2) qs[g / 2] = t;
       }
     }
@@ -1059,8 +1065,7 @@ __global__ void __launch_bounds__(kWaves * 64)
   const char* kh = ka.k + (size_t)it.g * L::chunk(bs);
   const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
   const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
-  CodeMasks masks;
-  asm("" : "+v"(masks.lo), "+v"(masks.hi), "+v"(masks.one));
+  const CodeMasks masks;
 
   // block ids, 64 blocks' parts of 16 keys at a time: lane n has the n-th from `from` on
   // (-1 outside the pool and from the last key on)
@@ -1150,7 +1155,7 @@ __global__ void __launch_bounds__(kWaves * 64)
           u32x4 y;
           if constexpr (EXACT) {
             uint32_t w[4];
-            k_pairs(code[j][e], w);
+            k_pairs(masks, code[j][e], w);
             y = u32x4{w[0], w[1], w[2], w[3]};
           } else {
             const f16x2 s2 = __builtin_bit_cast(f16x2, sc[j][e / 2]);

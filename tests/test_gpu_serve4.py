@@ -297,22 +297,38 @@ def test_attention_of_chunks_in_blocks(gpu, dt, h, kv, hd, bs):
     c.check(out)
 
 
+def normal_rows(gpu, dt, h, kv, hd, rows):
+    """A sequence of 2000 normal keys and values, its result, and the plain one's."""
+    c = Case(gpu, h + hd, dt, h, kv, hd, 16, [2000], [rows])
+    k, v = c.rng.normal(size=(2, c.cache.num_blocks * 16, kv, hd))
+    k, kx = typed(k.astype(np.float32), dt, gpu)
+    v, vx = typed(v.astype(np.float32), dt, gpu)
+    c.pool.q4_append(k, v, torch.arange(len(k), dtype=torch.int32, device=gpu))
+    c.take(kx, vx)
+    want = ref.attention(c.qx, *c.rows(0)[0], rows, c.scale, *c.rows(0)[1])[0]
+    return host(c.run(out_dtype=torch.float32)).reshape(want.shape), want
+
+
 @pytest.mark.parametrize("h,kv,hd,rows", [(32, 8, 64, 1), (32, 8, 128, 1), (16, 8, 256, 1), (32, 8, 128, 9)])
 def test_f32_attention_is_f32(gpu, h, kv, hd, rows):
     """Offsets and codes of values cancel, all the more over many keys: what is lost before
     they do shows.  Scores are below 16 here, where half a step is 2^-21; one sums up hd
     products, whose roundings add up at random to 2^-21 sqrt(hd / 3) at most, 2^-17.7
     for 256: weights, and so results in norm, are off by that."""
-    n = 2000
-    c = Case(gpu, h + hd, "f32", h, kv, hd, 16, [n], [rows])
-    k, v = c.rng.normal(size=(2, c.cache.num_blocks * 16, kv, hd))
-    k, kx = typed(k.astype(np.float32), "f32", gpu)
-    v, vx = typed(v.astype(np.float32), "f32", gpu)
-    c.pool.q4_append(k, v, torch.arange(len(k), dtype=torch.int32, device=gpu))
-    c.take(kx, vx)
-    want = ref.attention(c.qx, *c.rows(0)[0], rows, c.scale, *c.rows(0)[1])[0]
-    off = host(c.run()).reshape(want.shape) - want
-    assert np.linalg.norm(off) <= 2.0 ** -17.7 * np.linalg.norm(want)
+    got, want = normal_rows(gpu, "f32", h, kv, hd, rows)
+    assert np.linalg.norm(got - want) <= 2.0 ** -17.7 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("h,kv,hd,rows", [(32, 8, 64, 1), (32, 8, 128, 1), (16, 8, 256, 1), (32, 8, 128, 3)])
+def test_f32_results_of_16_bit_queries(gpu, dt, h, kv, hd, rows):
+    """Nothing is rounded to 16 bits but weights, in two parts (2^-22).  The matrix
+    instructions keep a product of a code as a subnormal to 2^-13 of the largest of eight
+    query elements, 2^-12 here, which takes bits of elements below 1/4, a fifth of them: at random
+    2^-12 sqrt(hd / 5 / 12) steps of the keys, of 0.3, times the scale, 2^-16.7 at any
+    hd (0.3 2^-12 / sqrt(60)): what weights, and results in norm, are off by."""
+    got, want = normal_rows(gpu, dt, h, kv, hd, rows)
+    assert np.linalg.norm(got - want) <= 2.0 ** -16 * np.linalg.norm(want)
 
 
 @pytest.mark.parametrize("dt,h,kv,hd,bs", [("bf16", 32, 8, 128, 16), ("f16", 32, 4, 64, 256),
