@@ -158,9 +158,11 @@ __global__ void __launch_bounds__(kQ4Threads)
   const int h = blockIdx.x % kvh;
   const uint32_t tok0 = blockIdx.x / kvh * kRows<HD>, left = n - tok0;  // left: 1 or more
   const uint32_t lane = threadIdx.x % LANES, local = threadIdx.x / LANES;
-  // a row of V codes is written by threads of their own order, tokens fastest
+  // V codes are written by threads in the order of their bytes
   constexpr int W = T >= 8 ? T / 8 : 1;  // words of a column (HD 64: two columns' halves)
-  const uint32_t wl = threadIdx.x / W % kRows<HD>, col = threadIdx.x / (W * kRows<HD>);
+  constexpr uint32_t COLS = HD == 64 ? 8 : 16;
+  const uint32_t wl = (threadIdx.x / W & 3) | threadIdx.x / (4 * W * COLS) << 2;
+  const uint32_t col = threadIdx.x / (4 * W) % COLS;
   const int slot = slot_of(slots + tok0, local < left, local, n_slots, lane == 0 && h == 0, err);
   const int wslot = slot_of(slots + tok0, wl < left, wl, n_slots, false, err);
   const size_t blk_bytes = (size_t)kvh * L::chunk(bs), head_at = (size_t)h * L::chunk(bs);
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kQ4Threads)
       uint32_t w = 0;
 #pragma unroll
       for (int t = 3; t >= 0; --t) w = w << 4 | __builtin_amdgcn_ubfe(x[t], 4 * (i & 7), 4);
-      *reinterpret_cast<uint16_t*>(o + L::v_bytes(bs, at, i)) = (uint16_t)w;
+      *reinterpret_cast<uint16_t*>(o + L::v_bytes(at, i)) = (uint16_t)w;
     }
   } else {
     const int word = threadIdx.x % W;
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(kQ4Threads)
 #pragma unroll
     for (int t = 7; t >= 0; --t)
       w = w << 4 | __builtin_amdgcn_ubfe(t < 4 ? x0[t % 4] : x1[t % 4], 4 * (col & 7), 4);
-    *reinterpret_cast<uint32_t*>(o + L::v_bytes(bs, at, col) + 4 * word) = w;
+    *reinterpret_cast<uint32_t*>(o + L::v_bytes(at, col) + 4 * word) = w;
   }
 }
 
@@ -251,19 +253,21 @@ __global__ void __launch_bounds__(kQ4Threads)
   const int h = blockIdx.x % kvh;
   const uint32_t tok0 = blockIdx.x / kvh * kRows<HD>, left = n - tok0;  // left: 1 or more
   const uint32_t lane = threadIdx.x % LANES, local = threadIdx.x / LANES;
-  const uint32_t wl = threadIdx.x / W % kRows<HD>, col = threadIdx.x / (W * kRows<HD>);
+  constexpr uint32_t COLS = HD == 64 ? 8 : 16;
+  const uint32_t wl = (threadIdx.x / W & 3) | threadIdx.x / (4 * W * COLS) << 2;
+  const uint32_t col = threadIdx.x / (4 * W) % COLS;
   const int slot = slot_of(slots + tok0, local < left, local, n_slots, lane == 0 && h == 0, err);
   const int wslot = slot_of(slots + tok0, wl < left, wl, n_slots, false, err);
   if (wslot >= 0) {
     const char* o = vp + ((size_t)(wslot >> bs_log2) * kvh + h) * L::chunk(bs);
     const int at = wslot & (bs - 1);
     if constexpr (HD == 64) {
-      codes[wl][col] = *reinterpret_cast<const uint16_t*>(o + L::v_bytes(bs, at, 2 * col)) |
-                       *reinterpret_cast<const uint16_t*>(o + L::v_bytes(bs, at, 2 * col + 1)) << 16;
+      codes[wl][col] = *reinterpret_cast<const uint16_t*>(o + L::v_bytes(at, 2 * col)) |
+                       *reinterpret_cast<const uint16_t*>(o + L::v_bytes(at, 2 * col + 1)) << 16;
     } else {
       const int word = threadIdx.x % W;
       codes[wl][16 * word + col] =
-          *reinterpret_cast<const uint32_t*>(o + L::v_bytes(bs, at, col) + 4 * word);
+          *reinterpret_cast<const uint32_t*>(o + L::v_bytes(at, col) + 4 * word);
     }
   }
   const int at = slot & (bs - 1), g = lane / 4, i = lane % 4, t = lane / 2;

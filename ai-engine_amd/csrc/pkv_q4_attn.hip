@@ -284,7 +284,7 @@ __device__ __forceinline__ float new_ref(float ref, float m, float top, bool les
 //
 // Bound by the reads of codes, scales and offsets, each once and past the caches (6.5
 // TB/s for blocks anywhere, 5.7 through them): 256 sequences of 512 .. 4096 keys, 8 kv
-// heads of 128 and 32 heads, 162 us, 48 of 12 .. 32 thousand 247, 4.8 and 5.1 TB/s (values'
+// heads of 128 and 32 heads, 161 us, 48 of 12 .. 32 thousand 244, 4.9 and 5.2 TB/s (values'
 // codes as subnormals, see above: 157 and 238).  A few
 // sequences are a chain of waits (lengths, ids, keys and values, the join): 8 of
 // 600 .. 9000, heads of 64, 16.9 us and 4.0 for the join.
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
   const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
   const int s_off = bs * (HD / 2) + (kq * G + gp) * 8, m_off = s_off + bs * G * 2;
-  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (n16 * bs + kq * 4) * (T / 2);
+  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (kq * 16 + n16) * (2 * T);
 
   struct KV {
     uint32_t code[HD / 32], s[2], m[2];
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   auto load = [&](const char* base, int id, int key, bool keys, KV& t) {
     const int at = key & (bs - 1);
     const char* p = base + (size_t)max(id, 0) * blk_stride;
-    load_words<HD / 8, true>(p + at * (keys ? HD / 2 : T / 2) + (keys ? k_off : v_off), t.code);
+    load_words<HD / 8, true>(p + at * (HD / 2) + (keys ? k_off : v_off), t.code);
     load_words<8, true>(p + at * (G * 2) + s_off, t.s);
     load_words<8, true>(p + at * (G * 2) + m_off, t.m);
   };
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   const char* vh = ka.v + (size_t)it.g * L::chunk(bs);
   const int32_t* table = a.block_tables + (size_t)it.s * a.max_blocks_per_seq;
   const int s_off = bs * (HD / 2) + kq * G * 8;
-  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (n16 * bs + kq * 4) * (T / 2);
+  const int k_off = (n16 * 4 + kq) * G * 4, v_off = (kq * 16 + n16) * (2 * T);
   const int quad_off = bs * (HD / 2) + (n16 >> 2) * G * 8;
   // offsets: key n16 of group kq (and kq + 4); tokens 4 kq .. of group n16
   const int km_off = bs * (HD / 2) + bs * G * 2 + ((n16 >> 2) * G + kq % G) * 8 + (n16 & 3) * 2;
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   auto load_v = [&](int id, int key, VTile& t) {
     const int at = key & (bs - 1);
     const char* p = vh + (size_t)max(id, 0) * blk_stride;
-    load_words<HD / 8>(p + at * (T / 2) + v_off, t.code);
+    load_words<HD / 8>(p + at * (HD / 2) + v_off, t.code);
     load_words<G * 8>(p + at * (G * 2) + s_off, t.s);
     load_words<F32 ? G * 8 : 8>(p + at * (G * 2) + (F32 ? s_off + bs * G * 2 : vm_off), t.m);
   };
@@ -1122,7 +1122,7 @@ __global__ void __launch_bounds__(kWaves * 64)
         sc[j][0] = y.x, sc[j][1] = y.y, of[j][0] = z.x, of[j][1] = z.y;
       } else {
         const int i = x / C::VW % 16, w = x % C::VW;
-        const char* c = p + (uint32_t)(L::v_bytes(bs, at, i) + 4 * w);
+        const char* c = p + (uint32_t)(L::v_bytes(at, i) + 4 * w);
         if constexpr (T == 4) {
           const uint2 y = *reinterpret_cast<const uint2*>(c);
           code[j][0] = y.x, code[j][1] = y.y;

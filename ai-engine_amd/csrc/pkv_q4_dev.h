@@ -16,8 +16,8 @@ struct Q4Layout {
   static __device__ __forceinline__ int k_word(int tok, int i, int g) {
     return ((tok * 4 + i) * G + g) * 4;
   }
-  static __device__ __forceinline__ int v_bytes(int bs, int tok, int i) {
-    return (i * bs + tok) * (T / 2);
+  static __device__ __forceinline__ int v_bytes(int tok, int i) {
+    return (((tok >> 2) * 16 + i) * 4 + (tok & 3)) * (T / 2);
   }
   static __device__ __forceinline__ int s_at(int bs, int tok, int g) {
     return bs * (HD / 2) + (((tok >> 2) * G + g) * 4 + (tok & 3)) * 2;

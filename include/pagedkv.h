@@ -723,8 +723,8 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
  * a chunk being bs * hd * 5 / 8 bytes:
  *   K  codes  [bs][4][G] 32-bit words: word (token, i, g) has channels 32 g + 8 i
  *             + e, e = 0 .. 7, in bits 4 (e / 2 + 4 (e % 2)) on
- *   V  codes  [16][bs][T / 2] bytes: (i, token) has channels i + 16 t, t = 0 .. T - 1,
- *             in bits 4 t on
+ *   V  codes  [bs / 4][16][4][T / 2] bytes: (token / 4, i, token % 4) has channels i + 16 t,
+ *             t = 0 .. T - 1, in bits 4 t on
  *   both then s and m, each [bs / 4][G][4] f16 (token / 4, group, token % 4)
  * so that a token's bytes are its own: rows are written without reading others. */
 

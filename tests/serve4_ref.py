@@ -60,7 +60,7 @@ def chunk_bytes(k, c, m, s, bs):
         for i in range(16):
             for j in range(t):
                 w[i, :, j // 2] |= (c[:, i + 16 * j] << (4 * (j % 2))).astype(np.uint8)
-        words = w.reshape(-1)
+        words = w.reshape(16, bs // 4, 4, t // 2).transpose(1, 0, 2, 3).reshape(-1)
 
     def quads(x):
         return x.reshape(bs // 4, 4, g).transpose(0, 2, 1).astype(np.float16).reshape(-1).view(np.uint8)

@@ -56,8 +56,8 @@ def test_reference_chunk_layout_is_the_headers():
     rest = b[bs * hd // 2:].view(np.float16)
     assert rest[(7 // 4 * 2 + 1) * 4 + 7 % 4] == s[7, 1] and rest[bs * 2 + (7 // 4 * 2 + 1) * 4 + 3] == m[7, 1]
     b = ref.chunk_bytes(False, c, m, s, bs)
-    v = b[:bs * hd // 2].reshape(16, bs, 2)
-    assert v[5, 9, 1] >> 4 == c[9, 5 + 16 * 3]
+    v = b[:bs * hd // 2].reshape(bs // 4, 16, 4, 2)
+    assert v[9 // 4, 5, 9 % 4, 1] >> 4 == c[9, 5 + 16 * 3]
     assert b[bs * hd // 2:].view(np.float16)[bs * 2 + (7 // 4 * 2 + 1) * 4 + 3] == m[7, 1]
 
 
