@@ -778,7 +778,8 @@ int pkv_q4_attention(pkv_pool* pool, int layer, const void* q, int q_dtype,
 /* Causal attention of whole prompts over their own rows, packed: token i of prompt s
  * is row cu_lens[s] + i and attends tokens 0 .. i of its prompt; out_h = sum_j
  * softmax_j(scale q_h . k_j) v_j, f32 accumulation and softmax (for 16-bit types the
- * weights are rounded to them before the second product).
+ * weights are rounded to them before the second product).  Tokens behind i may hold
+ * anything, NaN and infinities too.
  *  q: token t at q + t * q_token_stride elements, [n_head][head_dim]; k, v likewise,
  *      [n_kv_head][head_dim]; all in dtype (PKV_F32, PKV_F16 or PKV_BF16), 16-byte
  *      aligned, strides multiples of 16 bytes that hold a row, at most 2^24.  Query head h reads kv head

@@ -1,0 +1,45 @@
+"""Serving from a cache held in 4 bits at its edges."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import pagedkv
+import serve4_ref as ref
+from test_gpu_serve4 import HALF, PROMPT_WEIGHT, host, i32, prompt_case
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# packed prompt attention
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dt,hd", [("f32", 64), ("f32", 128), ("f32", 256), ("f16", 64), ("f16", 128),
+                                   ("bf16", 64), ("bf16", 128), ("bf16", 256)])
+@pytest.mark.parametrize("others", [0, 150])
+def test_prompts_see_nothing_behind_a_token(gpu, dt, hd, others):
+    """Values that are not finite reach their own token and later ones only, in their own
+    channels: a weight of 0 behind a token is no product.  A key's NaN reaches all of them.
+    (150 more prompts: waves have units of their own.)"""
+    lens = [3, 70, 33, 128, 1] + [64] * others
+    q, k, v, cu, (qx, kx, vx) = prompt_case(gpu, 26, dt, 8, 2, hd, lens)
+    for s, at, ch, x in [(0, 2, 0, math.nan), (1, 40, 5, math.inf), (1, 69, hd - 1, -math.inf),
+                         (1, 12, 17, math.nan), (2, 32, 3, math.nan), (3, 0, 9, math.inf),
+                         (3, 95, 33, math.nan), (3, 96, 33, math.inf), (4, 0, 2, math.nan)]:
+        v[cu[s] + at, 1, ch] = x
+        vx[cu[s] + at, 1, ch] = x
+    for s, at in [(1, 50), (2, 31), (3, 100)]:
+        k[cu[s] + at, 0, 1] = math.nan
+        kx[cu[s] + at, 0, 1] = math.nan
+    got = host(pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=128)).reshape(-1, 8, hd)
+    for a, b in zip(cu[:6], cu[1:]):
+        with np.errstate(invalid="ignore"):
+            want, *abc = ref.attention(qx[a:b], kx[a:b], vx[a:b], b - a, hd ** -0.5)
+        odd = ~np.isfinite(want)
+        assert np.array_equal(got[a:b][odd], want[odd], equal_nan=True)
+        kv = [np.where(np.isfinite(x[a:b]), x[a:b], 0.0) for x in (kx, vx)]
+        _, *abc = ref.attention(qx[a:b], *kv, b - a, hd ** -0.5)
+        tol = ref.tolerance(np.where(odd, 0.0, want), *abc, b - a, hd, PROMPT_WEIGHT[dt], HALF[dt])
+        err = np.abs(np.where(odd, 0.0, got[a:b] - np.where(odd, 0.0, want)))
+        assert np.all(err <= tol), (a, b, float((err / tol).max()))
