@@ -436,8 +436,12 @@ bool split_of(const PromptArgs& a) {
   if (a.dtype == PKV_F32) return a.head_dim <= 128 && units <= 4096 * 64 / a.head_dim;
   return units <= 1024;
 }
+// Groups that a prompt's kv heads have workgroups for: the bound's, or what one launch
+// takes of them (workgroups then have several in turn).
 long long max_groups_of(const PromptArgs& a) {
-  return split_of(a) ? units_of(a) : (units_of(a) + kWaves - 1) / kWaves;
+  const long long groups = split_of(a) ? units_of(a) : (units_of(a) + kWaves - 1) / kWaves;
+  const long long most = 0xFFFFFFFFLL / (kWaves * 64) / ((long long)a.n_seqs * a.n_kv_head);
+  return std::max(std::min(groups, most), 1LL);
 }
 
 template <int DT, int HD>
@@ -467,7 +471,6 @@ bool prompt_fits(const PromptArgs& a) {
   const long long pairs = (long long)a.n_seqs * a.n_kv_head;
   return pairs <= INT32_MAX &&
          ((long long)a.total / kTok + 1) * (a.n_head / a.n_kv_head) <= INT32_MAX / 2 &&
-         max_groups_of(a) <= (1LL << 40) / pairs &&
          grid_fits(max_groups_of(a) * pairs, kWaves * 64);
 }
 

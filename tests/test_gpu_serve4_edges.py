@@ -7,7 +7,7 @@ import torch
 
 import pagedkv
 import serve4_ref as ref
-from test_gpu_serve4 import HALF, PROMPT_WEIGHT, host, i32, prompt_case
+from test_gpu_serve4 import HALF, PROMPT_WEIGHT, host, i32, prompt_case, prompt_check
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,12 @@ def test_prompts_see_nothing_behind_a_token(gpu, dt, hd, others):
         tol = ref.tolerance(np.where(odd, 0.0, want), *abc, b - a, hd, PROMPT_WEIGHT[dt], HALF[dt])
         err = np.abs(np.where(odd, 0.0, got[a:b] - np.where(odd, 0.0, want)))
         assert np.all(err <= tol), (a, b, float((err / tol).max()))
+
+
+def test_many_short_prompts_beside_a_bound_far_above_them(gpu):
+    """Without max_len and with offsets on the device the bound is all rows: more
+    workgroups than a launch has, of which each then takes several shares."""
+    lens = [1] * 4000 + [700, 90] + [2] * 3700
+    q, k, v, cu, xs = prompt_case(gpu, 28, "f16", 32, 32, 64, lens)
+    out = pagedkv.prompt_attention(q, k, v, i32(cu, gpu))
+    prompt_check(out, cu[3990:4020], xs, "f16", 0.125)
