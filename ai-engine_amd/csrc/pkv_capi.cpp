@@ -1604,7 +1604,7 @@ size_t pkv_q4_workspace_bytes(const pkv_pool* p, int n_seqs, int total_q, int ma
   pkv::Q4Args a{};
   a.n_seqs = n_seqs;
   a.total_q = total_q;
-  a.max_q_len = max_q_len;
+  a.max_q_len = std::min(max_q_len, total_q);
   a.max_context_len = max_context_len;
   a.n_head = n_head;
   a.q_dtype = PKV_F32;
@@ -1653,6 +1653,7 @@ int pkv_q4_attention(pkv_pool* p, int layer, const void* q, int q_dtype,
   if (overlap({out, rows_bytes(row, row, out_dtype, total_q)},
               {q, rows_bytes(q_token_stride, row, q_dtype, total_q)}))
     return fail(p, PKV_ERR_INVALID, "q4_attention: out overlaps q");
+  max_q_len = std::min(max_q_len, total_q);  // (a chunk of more rows than there are is left out)
   pkv::Q4Args a{q, q_dtype, q_token_stride, out, out_dtype, cu_q_lens, context_lens, block_tables,
                 max_blocks_per_seq, n_seqs, total_q, max_q_len, max_context_len, n_head, scale};
   if (!pkv::q4_fits(p, a))

@@ -1472,6 +1472,10 @@ void attend_dt(const Q4KArgs& ka, int hd, const Launch& l, unsigned blocks, hipS
   else attend<DT, 64>(ka, l, blocks, stream);
 }
 
+// Rows of a sequence that a launch may have parts of.
+int join_rows(const pkv_pool* p, const Q4Args& a, const Launch& l) {
+  return std::min(a.max_q_len, l.max_cols / (a.n_head / p->n_kv_head));
+}
 long long join_blocks(const Q4Args& a, int rows) {
   return ((long long)a.n_seqs * rows * a.n_head + 3) / 4;
 }
@@ -1491,9 +1495,12 @@ bool q4_fits(const pkv_pool* p, const Q4Args& a) {
     if (pairs > (1LL << 40) / l.tiles || pairs * l.tiles > (1LL << 40) / l.max_parts ||
         !grid_fits(pairs * l.tiles * l.max_parts, kWaves * 64))
       return false;
+    const int rows = join_rows(p, a, l);
+    if (l.max_parts > 1 && ((long long)a.n_seqs * rows > (1LL << 40) / a.n_head ||
+                            !grid_fits(join_blocks(a, rows), 256)))
+      return false;
   }
-  return (long long)a.n_seqs * a.max_q_len <= (1LL << 40) / a.n_head &&
-         grid_fits(join_blocks(a, a.max_q_len), 256);
+  return true;
 }
 
 hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, char* ws,
@@ -1519,7 +1526,7 @@ hipError_t launch_q4_attention(const pkv_pool* p, int layer, const Q4Args& a, ch
     ka.part_keys = l.part_keys;
     ka.max_parts = l.max_parts;
     ka.seq_rows = l.seq_rows;
-    ka.join_rows = std::min(a.max_q_len, l.max_cols / ka.r);
+    ka.join_rows = join_rows(p, a, l);
     const unsigned blocks = (unsigned)((long long)a.n_seqs * p->n_kv_head * l.tiles * l.max_parts);
     if (a.q_dtype == PKV_F32) attend_dt<PKV_F32>(ka, p->head_dim, l, blocks, stream);
     else if (a.q_dtype == PKV_F16) attend_dt<PKV_F16>(ka, p->head_dim, l, blocks, stream);

@@ -764,6 +764,9 @@ int pkv_q4_gather(pkv_pool* pool, int layer, const int32_t* slot_mapping, int n,
  *      length, or rows outside [0, total_q) is left out: its rows are as they
  *      were, as are rows of no sequence, and pkv_pool_check() reports it.  Keys of
  *      block ids outside the pool are not attended, and reported.
+ *      A launch of 2^32 work-items is refused (PKV_ERR_UNSUPPORTED): 256 for each part of
+ *      the keys (256 keys or more), sequence, kv head and 128 columns of max_q_len (total_q at
+ *      most) times n_head / n_kv_head; 16 columns for f32 queries.
  *  n_head / n_kv_head: any integer.  scale finite.
  * Workspace: 16-byte aligned, of at least pkv_q4_workspace_bytes (0: none needed). */
 size_t pkv_q4_workspace_bytes(const pkv_pool* pool, int n_seqs, int total_q, int max_q_len,

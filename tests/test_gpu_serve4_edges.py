@@ -7,7 +7,7 @@ import torch
 
 import pagedkv
 import serve4_ref as ref
-from test_gpu_serve4 import HALF, PROMPT_WEIGHT, host, i32, prompt_case, prompt_check
+from test_gpu_serve4 import HALF, PROMPT_WEIGHT, Case, host, i32, prompt_case, prompt_check
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,33 @@ def test_many_short_prompts_beside_a_bound_far_above_them(gpu):
     q, k, v, cu, xs = prompt_case(gpu, 28, "f16", 32, 32, 64, lens)
     out = pagedkv.prompt_attention(q, k, v, i32(cu, gpu))
     prompt_check(out, cu[3990:4020], xs, "f16", 0.125)
+
+
+# ---------------------------------------------------------------------------
+# attention over the pool
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_single_tokens_beside_a_long_chunk(gpu, dt):
+    """The bound of a chunk is one of every sequence: what the launches are made of is
+    far below sequences times it."""
+    n, m = 2048, 1100
+    rng = np.random.default_rng(41)
+    ctx, q_lens = rng.integers(1, 20, n).tolist(), [1] * n
+    ctx[100], q_lens[100] = m + 3, m
+    ctx[n - 1], q_lens[n - 1] = 37, 30
+    c = Case(gpu, 41, dt, 32, 8, 64, 16, ctx, q_lens)
+    out = c.run()
+    c.cache.check()
+    some = [0, 1, 99, 101, 102, 1999, n - 2, n - 1]
+    c.check(out, skip=set(range(n)) - set(some) - {100})
+    # without a bound on the host
+    again = c.pool.q4_attention(c.q, i32(c.tables, gpu), i32(c.ctx, gpu), cu_q_lens=i32(c.cu, gpu))
+    c.cache.check()
+    c.check(again, skip=set(range(n)) - set(some))
+
+
+def test_bounds_may_be_far_above_the_rows(gpu):
+    c = Case(gpu, 42, "bf16", 8, 2, 64, 16, [40, 5], [30, 1])
+    for most in (31, 1 << 20, 1 << 30):
+        c.check(c.run(max_q_len=most))
+    c.check(c.run(max_q_len=1 << 30, max_context_len=1 << 20))
