@@ -1410,12 +1410,14 @@ Launch launch_of(const pkv_pool* p, const Q4Args& a, Kind kind, int nt, int min_
   // most: with 2048 workgroups wanted and no limit, and with these, 64 sequences of 4096
   // keys took 107 and 92 us, 8 of 600 .. 9000 23.6 and 21.3, one of 32,000 24 and 21,
   // 48 of 12 .. 32 thousand 252 and 247, but 32 of 500 .. 16,000 79 and 85.  A part is
-  // worth its join from 256 keys on, for 128 columns from 1024.
+  // worth its join from 256 keys on, for 128 columns from 1024.  Chunks, whose rows' partial
+  // results would take gigabytes, have no such limit: f32, without and with it, 16 of
+  // 64 rows over 500 .. 16,000 keys took 1643 and 1581 us, 8 of 128 over 8192 1439 and 1479.
   const long long want = std::max(1LL, 768 / std::max(items, 1LL));
   const int unit = kWaves * kStep;
   long long keys = (a.max_context_len + want - 1) / want;
   keys = std::max(kind == kChunk ? 1024LL : 256LL, (keys + unit - 1) / unit * unit);
-  if (kind != kChunk) keys = std::min(keys, 4096LL);
+  if (most <= 32) keys = std::min(keys, 4096LL);
   l.part_keys = (int)keys;
   l.max_parts = (int)((a.max_context_len + keys - 1) / keys);
   return l;

@@ -82,3 +82,26 @@ def test_bounds_may_be_far_above_the_rows(gpu):
     for most in (31, 1 << 20, 1 << 30):
         c.check(c.run(max_q_len=most))
     c.check(c.run(max_q_len=1 << 30, max_context_len=1 << 20))
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+def test_scratch_of_chunks_is_small(gpu, kind):
+    """A call's scratch holds partial results of single tokens' and short contexts' parts,
+    not of every row of long chunks."""
+    cache = pagedkv.PagedKvCache(1, 1, 16, 8, 128, pagedkv.Q4)
+    size = pagedkv.lib().pkv_q4_workspace_bytes
+    if kind == 0:  # 12 chunks, 1200 rows: one row of a sequence may have parts, 8 of them (96
+        # workgroups without, 768 wanted)
+        assert size(cache.handle, 12, 1200, 600, 8200, 64) <= 12 * 64 * 8 * 130 * 4
+    else:  # 255 single tokens and 8192 rows: two rows of a sequence, 32 parts
+        assert size(cache.handle, 256, 8447, 8192, 131072, 32) <= 256 * 2 * 32 * 32 * 130 * 4
+
+
+@pytest.mark.parametrize("h,kv,hd", [(8, 2, 128), (4, 2, 64), (4, 4, 256)])
+def test_f32_chunks_over_long_contexts(gpu, h, kv, hd):
+    """Chunks of f32 queries that fill the GPU go through all keys in one part, past the
+    4096 whose block ids a wave has at once."""
+    c = Case(gpu, 44, "f32", h, kv, hd, 16, [9003] + [40] * 30, [40] * 31)
+    out = c.run(max_q_len=800)
+    c.cache.check()
+    c.check(out, skip=range(2, 31))
