@@ -6,12 +6,13 @@
 //   o_g = sum_k (p_k s_kg) c_k + sum_k p_k m_kg,
 // so both products run on the matrix cores over the codes themselves, as f16 numbers
 // that two instructions make of two codes.  As f16 subnormals, bits masked out of the
-// words, they need only one, and v_mfma_f32_16x16x32_f16 takes them exactly.  But it aligns
+// words, they need fewer, and v_mfma_f32_16x16x32_f16 takes them exactly.  But it aligns
 // eight products by their operands' exponents, subnormals counting as 2^-14, and
-// drops bits, downwards, that a normal number would keep: up to 2^-13 of the largest
-// weight (of 1 in c) each.  In the values' sum, where offsets and codes cancel, that was 2^-15 of
-// results over 2000 keys; for the keys of a decode it is 2^-15 of a query's largest
-// element in a score, below what rounding results to 16 bits costs, and kept.
+// drops bits, downwards, that a normal number would keep: of codes as c 2^-24 up to 2^-13 of the
+// largest weight (of 1 in c) each.  In the values' sum, where offsets and codes cancel, that
+// was 2^-15 of results over 2000 keys.  Keys' codes of single tokens are c 2^-20, which leaves
+// 2^-17 of the largest of eight query elements, times the step s: as exact as normal
+// numbers where one channel in 32 is 64 times the others (2^-20 of results in norm; c 2^-24: 2^-16).
 //
 // A column is a query row of a chunk and one of the heads of a kv head's group.  A
 // wave takes 32 keys a step: two tiles S^T = K Q^T of 16 keys, whose lanes then hold
@@ -204,11 +205,11 @@ __device__ __forceinline__ f16x2 code_pair(const CodeMasks& k, uint32_t w, bool 
   return hi ? x * by - b : x - a;
 }
 
-// Four words of a K code word: its channels 2 e, 2 e + 1 as f16 pairs; or as subnormals, c
-// 2^-24 of even e and 16 c 2^-24 of odd ones.
+// Four words of a K code word: its channels 2 e, 2 e + 1 as f16 pairs; or as subnormals,
+// c 2^-20.
 __device__ __forceinline__ void k_subnormals(uint32_t w, uint32_t (&f)[4]) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = (e & 2 ? w >> 8 : w) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
+  for (int e = 0; e < 4; ++e) f[e] = (e ? w >> 4 * (e - 1) : w << 4) & 0x00f000f0u;
 }
 __device__ __forceinline__ void k_pairs(const CodeMasks& k, uint32_t w, uint32_t (&f)[4]) {
 #pragma unroll
@@ -284,8 +285,9 @@ __device__ __forceinline__ float new_ref(float ref, float m, float top, bool les
 //
 // Bound by the reads of codes, scales and offsets, each once and past the caches (6.5
 // TB/s for blocks anywhere, 5.7 through them): 256 sequences of 512 .. 4096 keys, 8 kv
-// heads of 128 and 32 heads, 161 us, 48 of 12 .. 32 thousand 244, 4.9 and 5.2 TB/s (values'
-// codes as subnormals, see above: 157 and 238).  A few
+// heads of 128 and 32 heads, 164 us, 48 of 12 .. 32 thousand 250, 4.8 and 5.1 TB/s.  Of the
+// codes' forms above, keys' as c 2^-24 took 1.5 % less and as normal numbers 2.5 % more, values'
+// as subnormals 2.5 % less.  A few
 // sequences are a chain of waits (lengths, ids, keys and values, the join): 8 of
 // 600 .. 9000, heads of 64, 16.9 us and 4.0 for the join.
 template <int DT, int HD, int NT>
@@ -369,17 +371,16 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
     }
     big = col_max(row_group_max(big));
     const int ex = big > 0.0f ? 14 - __builtin_amdgcn_frexp_expf(big) : 0;  // below 2^14
-    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 24 - ex), 0x1p-126f);
+    f[c] = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, 20 - ex), 0x1p-126f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       x[e] = ldexpf(a.scale < 0.0f ? -x[e] : x[e], ex);
       sum += x[e];
     }
-    qs[c] = swap32_sum(swap16_sum(sum)) * 0x1p-24f;
+    qs[c] = swap32_sum(swap16_sum(sum)) * 0x1p-20f;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float by = (e & 2) ? 0.0625f : 1.0f;  // these codes are 16 times larger
-      const uint32_t w = pack_half(x[e] * by, x[e + 1] * by);
+      const uint32_t w = pack_half(x[e], x[e + 1]);
 #pragma unroll
       for (int g = 0; g < G; ++g) qf[c][g][e / 2] = g == gp ? w : 0u;
     }

@@ -747,8 +747,10 @@ int pkv_q4_gather(pkv_pool* pool, int layer, const int32_t* slot_mapping, int n,
 /* Attention over a 4-bit pool: out_h = sum_k softmax_k(scale q_h . k) v_k over the
  * values that the row's keys stand for, f32 accumulation and softmax.  f32 queries are
  * f32 throughout.  With 16-bit queries weights enter the second product in 22 bits;
- * in calls with a chunk of more than 32 columns (rows times heads of a kv head) values,
- * and for bf16 queries also keys and weights, may be rounded to f16.
+ * for up to 1024 / head_dim columns (rows times heads of a kv head) a product of a query element
+ * and a code c is kept to 2^-17 of the largest of eight such elements;
+ * in calls with a chunk of more than 32 columns values, and for bf16 queries also keys and
+ * weights, may be rounded to f16.
  *  q: token i at q + i * q_token_stride elements, [n_head][head_dim] in q_dtype
  *      (PKV_F32, PKV_F16 or PKV_BF16); 16-byte aligned, the stride at least n_head *
  *      head_dim, at most 2^24 and a multiple of 16 bytes.  Elements beyond 2^100 in magnitude, or

@@ -7,7 +7,7 @@ import torch
 
 import pagedkv
 import serve4_ref as ref
-from test_gpu_serve4 import HALF, PROMPT_WEIGHT, Case, host, i32, prompt_case, prompt_check
+from test_gpu_serve4 import HALF, PROMPT_WEIGHT, Case, host, i32, prompt_case, prompt_check, typed
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,26 @@ def test_f32_chunks_over_long_contexts(gpu, h, kv, hd):
     out = c.run(max_q_len=800)
     c.cache.check()
     c.check(out, skip=range(2, 31))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("h,kv,hd", [(32, 8, 64), (32, 8, 128), (16, 8, 256)])
+def test_queries_with_far_out_channels(gpu, dt, h, kv, hd):
+    """One channel of each group 64 times the others.  Scores have a deviation of some 2.5,
+    so scale q is at most 2.5 / sqrt(groups) there.  Products with codes are kept to 2^-17 of
+    the largest of eight: the seven beside that channel are off by 2^-17 sqrt(7 / 12) of it at
+    random, times a step of the keys, 0.3, and 2.5 over all groups: 2^-17.8 in a score.
+    Values' sums of 2000 keys, of which some four matter, lose 2^-20: 2^-17 in norm."""
+    c = Case(gpu, h + hd, dt, h, kv, hd, 16, [2000], [1], scale=2.5 / 64 / math.sqrt(hd // 32))
+    k, v = c.rng.normal(size=(2, c.cache.num_blocks * 16, kv, hd))
+    k, kx = typed(k.astype(np.float32), dt, gpu)
+    v, vx = typed(v.astype(np.float32), dt, gpu)
+    c.pool.q4_append(k, v, torch.arange(len(k), dtype=torch.int32, device=gpu))
+    c.take(kx, vx)
+    q = c.rng.normal(size=(1, h, hd))
+    q[..., ::32] *= 64.0
+    c.q, c.qx = typed(q, dt, gpu)
+    want = ref.attention(c.qx, *c.rows(0)[0], 1, c.scale, *c.rows(0)[1])[0]
+    got = host(c.run(out_dtype=torch.float32)).reshape(want.shape)
+    off = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert off <= 2.0 ** -17, math.log2(off)
