@@ -32,6 +32,8 @@ namespace {
 
 constexpr int kWaves = 4;                  // of a workgroup; they take the steps in turn
 constexpr int kStep = 32;                  // keys of a wave's step
+constexpr int kIdSteps = 32;               // steps that a wave has the block ids of at once
+constexpr int kFewKeys = kIdSteps * kWaves * kStep;  // keys of a part at most, for few columns
 constexpr float kNone = -3.0e38f;          // reference of a column without keys
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -285,7 +287,7 @@ __device__ __forceinline__ float new_ref(float ref, float m, float top, bool les
 //
 // Bound by the reads of codes, scales and offsets, each once and past the caches (6.5
 // TB/s for blocks anywhere, 5.7 through them): 256 sequences of 512 .. 4096 keys, 8 kv
-// heads of 128 and 32 heads, 164 us, 48 of 12 .. 32 thousand 250, 4.8 and 5.1 TB/s.  Of the
+// heads of 128 and 32 heads, 163 us, 48 of 12 .. 32 thousand 249, 4.8 and 5.1 TB/s.  Of the
 // codes' forms above, keys' as c 2^-24 took 1.5 % less and as normal numbers 2.5 % more, values'
 // as subnormals 2.5 % less.  A few
 // sequences are a chain of waits (lengths, ids, keys and values, the join): 8 of
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 
   constexpr int stride = kWaves * kStep;
   int key = it.k0 + wave * kStep;
-  int ids = ids_of(ka, table, key, it.k1), left = 32;
+  const int ids = ids_of(ka, table, key, it.k1);  // (of all steps: parts are kFewKeys at most)
   int id[2] = {readlane_i(ids, 0), readlane_i(ids, 1)};
   KV kt[2], vt[2];
   if (key < it.k1) {
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
   }
   float top = 14.0f;
   const CodeMasks masks;
-  for (; key < it.k1; key += stride) {
+  for (int step = 1; key < it.k1; key += stride, ++step) {
     const bool masked = key + kStep > it.all || (id[0] | id[1]) < 0;
     const bool in[2] = {id[0] >= 0, id[1] >= 0};
     float x[NT][2][4];
@@ -422,16 +424,12 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
                                     half_of(kt[j].m[i / 2], i % 2) * qs[c]));
     }
     // the next step's keys
-    if (--left == 0) {
-      ids = ids_of(ka, table, key + stride, it.k1);
-      left = 32;
-    }
     const int next = key + stride;
     const bool more = next < it.k1;
     if (more) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        id[j] = readlane_i(ids, 2 * (32 - left) + j);
+        id[j] = readlane_i(ids, 2 * step + j);
         load(kh, id[j], next + 16 * j, true, kt[j]);
       }
     }
@@ -699,7 +697,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
 
   constexpr int stride = kWaves * kStep;
   int key = it.k0 + wave * kStep;
-  int ids = ids_of(ka, table, key, it.k1), left = 32;
+  int ids = ids_of(ka, table, key, it.k1), left = kIdSteps;
   int id[2] = {readlane_i(ids, 0), readlane_i(ids, 1)};
   KTile kt[2];
   VTile vt[2];
@@ -756,13 +754,13 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
     }
     if (--left == 0) {
       ids = ids_of(ka, table, key + stride, it.k1);
-      left = 32;
+      left = kIdSteps;
     }
     const int next = key + stride;
     if (next < it.k1) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        id[j] = readlane_i(ids, 2 * (32 - left) + j);
+        id[j] = readlane_i(ids, 2 * (kIdSteps - left) + j);
         load_k(id[j], next + 16 * j, kt[j]);
       }
     }
@@ -1418,7 +1416,7 @@ Launch launch_of(const pkv_pool* p, const Q4Args& a, Kind kind, int nt, int min_
   const int unit = kWaves * kStep;
   long long keys = (a.max_context_len + want - 1) / want;
   keys = std::max(kind == kChunk ? 1024LL : 256LL, (keys + unit - 1) / unit * unit);
-  if (most <= 32) keys = std::min(keys, 4096LL);
+  if (most <= 32) keys = std::min(keys, (long long)kFewKeys);
   l.part_keys = (int)keys;
   l.max_parts = (int)((a.max_context_len + keys - 1) / keys);
   return l;
