@@ -7,7 +7,7 @@ import torch
 
 import pagedkv
 import serve4_ref as ref
-from test_gpu_serve4 import HALF, PROMPT_WEIGHT, Case, host, i32, prompt_case, prompt_check, typed
+from test_gpu_serve4 import HALF, PROMPT_WEIGHT, TD, Case, host, i32, prompt_case, prompt_check, typed
 
 pytestmark = pytest.mark.gpu
 
@@ -43,6 +43,23 @@ def test_prompts_see_nothing_behind_a_token(gpu, dt, hd, others):
         tol = ref.tolerance(np.where(odd, 0.0, want), *abc, b - a, hd, PROMPT_WEIGHT[dt], HALF[dt])
         err = np.abs(np.where(odd, 0.0, got[a:b] - np.where(odd, 0.0, want)))
         assert np.all(err <= tol), (a, b, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dt,h,kv,hd", [("bf16", 16, 8, 128), ("f16", 32, 2, 64), ("f32", 40, 2, 256),
+                                        ("f32", 32, 2, 128), ("bf16", 16, 2, 256)])
+def test_longer_prompts_of_waves_with_units_of_their_own(gpu, dt, h, kv, hd):
+    """Hundreds of keys a unit, groups of units that a workgroup takes one after another
+    because the bound is too small, and rows of no prompt that hold anything."""
+    lens, lead, tail = [700, 513, 1, 330, 0, 645], 5, 9
+    lens = lens + [97] * (60 if dt == "f32" else 20)
+    q, k, v, cu, xs = prompt_case(gpu, 27, dt, h, kv, hd, lens, lead, tail)
+    for x in (q, k, v):
+        x[:lead], x[-tail:] = math.nan, math.inf
+    for max_len in (700, 400):
+        out = torch.full((q.shape[0], h * hd), 7.0, dtype=TD[dt], device=gpu)
+        pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=max_len, out=out)
+        prompt_check(out, cu[:9], xs, dt, hd ** -0.5)
+        assert torch.all(out[:lead] == 7) and torch.all(out[-tail:] == 7)
 
 
 def test_many_short_prompts_beside_a_bound_far_above_them(gpu):
@@ -128,3 +145,11 @@ def test_queries_with_far_out_channels(gpu, dt, h, kv, hd):
     got = host(c.run(out_dtype=torch.float32)).reshape(want.shape)
     off = np.linalg.norm(got - want) / np.linalg.norm(want)
     assert off <= 2.0 ** -17, math.log2(off)
+
+
+@pytest.mark.parametrize("dt,h,kv,hd", [("bf16", 8, 2, 128), ("f16", 7, 1, 64), ("f32", 8, 2, 64)])
+def test_more_parts_than_lanes(gpu, dt, h, kv, hd):
+    """A sequence in 66 parts and more: the join goes through them 64 at a time."""
+    c = Case(gpu, 43, dt, h, kv, hd, 16, [20001, 17000, 5])
+    c.check(c.run())
+    c.check(c.run(max_context_len=1 << 20))
