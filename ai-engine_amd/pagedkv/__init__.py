@@ -271,7 +271,8 @@ _HERE = contextlib.nullcontext()
 def _run_on(stream, device, tensors):
     """(raw stream to launch on, context in which to allocate and launch).
     Another stream than the current one first waits for the work queued on the
-    current one, and the tensors' memory is not reused before it has run."""
+    current one, and the tensors' memory is not reused before it has run.  What is
+    no tensor on the device is passed over (the call's own checks name it)."""
     import torch
     if stream is None and torch.cuda.current_device() == device.index:
         # the handle alone: a Stream object costs 2 us of a 10 us call
@@ -283,7 +284,7 @@ def _run_on(stream, device, tensors):
         raise ValueError(f"stream must be on {device}")
     stream.wait_stream(cur)
     for t in tensors:
-        if t is not None:
+        if isinstance(t, torch.Tensor) and t.device == device:
             t.record_stream(stream)
     return _stream_ptr(stream), torch.cuda.stream(stream)
 

@@ -153,3 +153,29 @@ def test_more_parts_than_lanes(gpu, dt, h, kv, hd):
     c = Case(gpu, 43, dt, h, kv, hd, 16, [20001, 17000, 5])
     c.check(c.run())
     c.check(c.run(max_context_len=1 << 20))
+
+
+# ---------------------------------------------------------------------------
+# streams
+# ---------------------------------------------------------------------------
+def test_another_stream_changes_no_refusal(gpu):
+    side = torch.cuda.Stream()
+    x = torch.zeros((2, 100), device=gpu)
+    toks, cu, cpu = i32([1, 2], gpu), i32([0, 1, 2], gpu), torch.tensor([0, 1, 2], dtype=torch.int32)
+    rows = torch.zeros((4, 2, 64), device=gpu, dtype=torch.float16)
+    pool = pagedkv.PagedKvCache(1, 2, 16, 2, 64, pagedkv.Q4).layer(0)
+    for s in (None, side):
+        for bad in (cpu, [0, 1, 2]):
+            with pytest.raises(ValueError, match="cu_tokens must be a tensor on"):
+                pagedkv.adjust_logits(x, tokens=toks, cu_tokens=bad, stream=s)
+        with pytest.raises(ValueError, match="out must be"):
+            pagedkv.adjust_logits(x, out=x.cpu(), stream=s)
+        with pytest.raises(ValueError, match="k must be a tensor on"):
+            pagedkv.prompt_attention(rows, rows.cpu(), rows, [0, 4], stream=s)
+        with pytest.raises(ValueError, match="out must be"):
+            pagedkv.prompt_attention(rows, rows, rows, [0, 4], out=torch.zeros((4, 128)), stream=s)
+        with pytest.raises(ValueError, match="v must be a tensor on"):
+            pool.q4_append(rows, rows.cpu(), [0, 1, 2, 3], stream=s)
+    got = pagedkv.adjust_logits(x, tokens=toks, cu_tokens=cu, stream=side)
+    side.synchronize()
+    assert not got.any()
