@@ -716,7 +716,8 @@ int pkv_verify_drafts(const void* target_logits, int target_dtype, long long tar
  * group.  With its elements x (NaN taken as 0, others limited to +-65024), m =
  * f16(min x) and s = f16((max x - m) / 15), the subtraction and the division in f32,
  * an element is held as c = (x - m) / s in 64 bits, rounded to nearest even and
- * limited to 0 .. 15 (0 where s is 0), and stands for m + s c.
+ * limited to 0 .. 15, and stands for m + s c.  Where s is not positive c is 0; s is
+ * negative, and held so, where m rounds above max x.
  *
  * Layout: block_size a power of two in [16, 256], bs; hd = head_dim, G = hd / 32
  * groups, T = hd / 16.  One layer's K (or V) is [num_blocks][n_kv_head][chunk],

@@ -13,6 +13,26 @@ pytestmark = pytest.mark.gpu
 
 
 # ---------------------------------------------------------------------------
+# rows into the pool
+# ---------------------------------------------------------------------------
+def test_groups_whose_offset_rounds_above_them(gpu):
+    """f16(0.3) is above 0.3: the step is negative, and codes are 0."""
+    x = np.full((16, 1, 64), np.float32(0.3), np.float64)
+    x[:, 0, 32:] += np.arange(32) * 1e-6
+    k, x = typed(x, "f32", gpu)
+    c, m, s = ref.quantize(x)
+    assert np.all(m > x.max()) and np.all(s < 0) and not c.any()
+    cache = pagedkv.PagedKvCache(1, 1, 16, 1, 64, pagedkv.Q4)
+    slots = i32(np.arange(16), gpu)
+    cache.layer(0).q4_append(k, k, slots)
+    for which in (pagedkv.K, pagedkv.V):
+        want = ref.chunk_bytes(which == pagedkv.K, c[:, 0], m[:, 0], s[:, 0], 16)
+        assert np.array_equal(cache.read_bytes(0, which).reshape(-1), want)
+    for o in cache.layer(0).q4_gather(slots):
+        assert np.array_equal(host(o), np.broadcast_to(m[..., :1], o.shape))
+
+
+# ---------------------------------------------------------------------------
 # packed prompt attention
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dt,hd", [("f32", 64), ("f32", 128), ("f32", 256), ("f16", 64), ("f16", 128),
