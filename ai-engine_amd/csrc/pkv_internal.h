@@ -22,8 +22,8 @@ struct pkv_pool {
   int head_dim = 0;
   int dtype = 0;
   int device = 0;
-  size_t elem_bytes = 0;
-  size_t row_bytes = 0;    // one (slot, kv head) row: head_dim * elem_bytes
+  size_t elem_bytes = 0;   // (PKV_Q4: 0)
+  size_t row_bytes = 0;    // one (slot, kv head) row: head_dim * elem_bytes, or q4_row_bytes
   size_t block_bytes = 0;  // one block of one layer's K (or V)
   size_t layer_bytes = 0;  // one layer's K (or V): num_blocks * block_bytes
   char* base = nullptr;    // device slab

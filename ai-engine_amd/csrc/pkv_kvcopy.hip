@@ -7,8 +7,9 @@
 // All of them are HBM-bound streams of 16-byte vectors: every thread moves
 // whole 16-byte chunks, consecutive lanes touch consecutive chunks, and each
 // thread issues all of its loads before its stores so that several requests
-// are in flight per lane.  Rows are head_dim * elem_bytes >= 128 bytes, so a
-// token row is always a whole number of 16-byte chunks.
+// are in flight per lane.  Rows of F32, F16 and BF16 pools are head_dim * elem_bytes
+// >= 128 bytes, so a token row is always a whole number of 16-byte chunks; pools of
+// PKV_Q4, whose rows are 40 bytes and more, are moved by blocks of 16 rows at least.
 #include <algorithm>
 
 #include "pkv_device.h"

@@ -9,7 +9,8 @@
 //
 // Bound by the histories: each slice goes through the whole of its request's.  128 rows of
 // 128,256 bf16 logits with histories up to 8000 take 27 us, 13.4 (the copy rate) without
-// any.  With slices of 4096 and every logit computed in place, so that a wave of 512
+// any; some 60 % of the cycles are vector instructions, the rest the waits of four rounds
+// of workgroups.  With slices of 4096 and every logit computed in place, so that a wave of 512
 // went through the division for a few of them, they took 34; a list of the changed
 // tokens made by a shared counter, 42.
 #include "pkv_device.h"

@@ -6,10 +6,10 @@
 // wherever they are stored.
 //
 // Both directions move bytes: rows of 2 or 4 bytes an element and a pool of 5 bits, each
-// once.  60,001 tokens of 8 heads of 128 in f16 take 90 us to store and 50 to read
-// back (3.6 and 6.5 TB/s; a large copy moves 5.0).  The store spends 70 of them on some 340
-// vector instructions a wave of 1024 elements; with 64-bit divisions throughout, and
-// 2 tokens of 8 heads a workgroup, it took 150.
+// once.  60,001 tokens of 8 heads of 128 in f16 take 85 us to store and 48 to read
+// back (3.8 and 6.7 TB/s; a large copy moves 5.0), 126 one after the other.  The store spends
+// 83 % of its cycles on some 360 vector instructions a wave of 1024 elements; with 64-bit
+// divisions throughout, and 2 tokens of 8 heads a workgroup, it took 150.
 #include <algorithm>
 
 #include "pkv_internal.h"

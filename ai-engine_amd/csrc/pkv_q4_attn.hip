@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kWaves * 64) q4_few_kernel(Q4KArgs ka) {
 // have all their calls here, with keys and values as f32 on f32 instructions, which
 // take eight times as long: in two f16 parts queries and weights would be off by 2^-22, and
 // sums by what the f16 ones drop of small products.  64 sequences of 4096 keys, 8 kv heads of 128, 32
-// heads, f32: 209 us.  DT: type of q.  NT: tiles.
+// heads, f32: 207 us.  DT: type of q.  NT: tiles.
 template <int DT, int HD, int NT>
 __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
   using L = Q4Layout<HD>;
@@ -966,9 +966,11 @@ __global__ void __launch_bounds__(kWaves * 64) q4_many_kernel(Q4KArgs ka) {
 // and the offsets' products are f32 ones, and weights are two f16.
 //
 // Bound by vector instructions: for a tile of 32 keys a wave needs 512 cycles of matrix
-// ones and, for codes to f16, exp2, maximum and sums, some 850 of vector ones.  8
-// sequences of 256 rows over 4096 keys, 8 kv heads of 128 and 64 heads: bf16 387 us, 0.69
-// PFLOP/s, f16 551.
+// ones and, for codes to f16, exp2, maximum and sums, some 760 of vector ones.  8
+// sequences of 256 rows over 4096 keys, 8 kv heads of 128 and 64 heads: bf16 372 us, 0.72
+// PFLOP/s, f16 517.  Ragged chunks leave CUs idle at the end, since keys are not split once
+// there are 768 workgroups: 12 chunks of up to 200 rows over 500 to 8000 keys have
+// instructions in 45 % of the cycles (27 vector, 18 matrix).  bf16 with 128 channels spills seven registers.
 constexpr int kTile = 32;
 constexpr float kTau = 8.0f;  // weights are at most 2^8 of their reference
 
