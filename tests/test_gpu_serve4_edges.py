@@ -52,17 +52,22 @@ def test_prompts_see_nothing_behind_a_token(gpu, dt, hd, others):
     for s, at in [(1, 50), (2, 31), (3, 100)]:
         k[cu[s] + at, 0, 1] = math.nan
         kx[cu[s] + at, 0, 1] = math.nan
-    got = host(pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=128)).reshape(-1, 8, hd)
+    results = []
+    for out_dt in {dt, "f32"}:
+        out = pagedkv.prompt_attention(q, k, v, i32(cu, gpu), max_len=128, out_dtype=TD[out_dt])
+        results.append((out_dt, host(out).reshape(-1, 8, hd)))
     for a, b in zip(cu[:6], cu[1:]):
         with np.errstate(invalid="ignore"):
             want, *abc = ref.attention(qx[a:b], kx[a:b], vx[a:b], b - a, hd ** -0.5)
         odd = ~np.isfinite(want)
-        assert np.array_equal(got[a:b][odd], want[odd], equal_nan=True)
         kv = [np.where(np.isfinite(x[a:b]), x[a:b], 0.0) for x in (kx, vx)]
         _, *abc = ref.attention(qx[a:b], *kv, b - a, hd ** -0.5)
-        tol = ref.tolerance(np.where(odd, 0.0, want), *abc, b - a, hd, PROMPT_WEIGHT[dt], HALF[dt])
-        err = np.abs(np.where(odd, 0.0, got[a:b] - np.where(odd, 0.0, want)))
-        assert np.all(err <= tol), (a, b, float((err / tol).max()))
+        for out_dt, got in results:
+            assert np.array_equal(got[a:b][odd], want[odd], equal_nan=True)
+            tol = ref.tolerance(np.where(odd, 0.0, want), *abc, b - a, hd, PROMPT_WEIGHT[dt],
+                                HALF[out_dt])
+            err = np.abs(np.where(odd, 0.0, got[a:b]) - np.where(odd, 0.0, want))
+            assert np.all(err <= tol), (out_dt, a, b, float((err / tol).max()))
 
 
 @pytest.mark.parametrize("dt,h,kv,hd", [("bf16", 16, 8, 128), ("f16", 32, 2, 64), ("f32", 40, 2, 256),
